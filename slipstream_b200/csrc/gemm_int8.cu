@@ -1,0 +1,540 @@
+// Matrix product of 8-bit integers on the 5th-generation tensor cores of sm_100a:
+//   Y[m, n] = (sum_k X[m, k] * W[n, k]) * x_scale[m] * w_scale[n] (+ bias[n])
+// X: activations, one row and one scale a token; W: weights, one row and one scale an output feature; both int8 and K-major.
+// The sum is exact: products and additions are 32-bit integers (tcgen05.mma kind::i8; 127^2 K < 2^31 up to K = 133,143), so a
+// result does not depend on how K is cut, on the kernel or on what else is in the batch.  What follows is float32: the sum is
+// converted (one rounding from 2^24 on), multiplied by the token's scale, then by the feature's, then the bias is added, and
+// the result is rounded once to the output type.  The gated form pairs the features of a feed-forward's gate and up matrices
+// (stacked in runs of 64 rows each) and writes silu(gate) * up.
+//
+// A row's stage in shared memory is 128 bytes, 128 elements of K, under the 128-byte swizzle; an instruction takes 32 of them.
+//
+// Every wait on an mbarrier is bounded: after WAIT_LIMIT polls the kernel sets SS_ERR_WAIT_LIMIT in the error word, stops
+// waiting everywhere, waits for its copies in flight, frees its tensor memory and returns.
+//
+// Tensor memory is taken BEHIND griddepcontrol.wait, and the kernel behind is let go only when it has been taken: a kernel
+// that takes it before the kernel in front is through, or lets a kernel start that may take it first, can wait for a block
+// that waits for it.
+
+#include <cuda.h>
+
+#include "tc5.cuh"
+
+#define I8_BM 128
+#define I8_BK 128       // K elements, and bytes of a row, in a stage
+#define I8_THREADS 192
+
+struct Int8Args {
+    const float* x_scale;  // [tokens]
+    const float* w_scale;  // [features]
+    const void* bias;      // [features] or null
+    void* out;             // [tokens][ldc]
+    int* err;
+    int64_t ldc;
+    int tokens, features, K;
+    int out_features;      // columns written: features, or the gated form's (at most features / 2)
+    int out_f32, bias_f32, gated;
+    int bn;                // few tokens: the tokens of a tile; many tokens: the features of a tile
+    int stages, slices;
+};
+
+__device__ __forceinline__ void i8_load(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(k), "r"(row) : "memory");
+}
+// weights that are read once a step: the first to leave L2 again
+__device__ __forceinline__ void i8_load_once(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+        ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(k), "r"(row), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: D signed 32-bit, A and B signed 8-bit, both K-major.
+__device__ __forceinline__ uint32_t i8_idesc(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// One wait for a copy of this block that is still in flight after a wait gave up (its own limit, blind to the flag).
+__device__ __forceinline__ void i8_drain(uint64_t* bar, uint32_t parity) {
+    volatile int none = 0;
+    (void)mbar_wait(bar, parity, &none);
+}
+
+__device__ __forceinline__ float i8_bias(const Int8Args& g, int f) {
+    return g.bias_f32 ? ((const float*)g.bias)[f] : to_float(((const bf16*)g.bias)[f]);
+}
+// The sum as a result: in this order everywhere, no fused multiply-add, so that both kernels give the same bits.
+__device__ __forceinline__ float i8_value(int sum, float xs, float ws, float bias) {
+    return __fadd_rn(__fmul_rn(__fmul_rn((float)sum, xs), ws), bias);
+}
+__device__ __forceinline__ float i8_gate(const Int8Args& g, float gate, float up) {
+    return g.out_f32 ? silu_mul<false>(gate, up) : silu_mul<true>(gate, up);
+}
+
+// Four neighbouring outputs of a token.
+__device__ __forceinline__ void i8_store4(const Int8Args& g, int token, int f, const float (&v)[4]) {
+    const int64_t at = (int64_t)token * g.ldc + f;
+    if (f + 4 <= g.out_features && (g.ldc & 3) == 0) {
+        if (g.out_f32) {
+            *reinterpret_cast<float4*>((float*)g.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+            uint2 packed;
+            packed.x = *reinterpret_cast<const uint32_t*>(&lo);
+            packed.y = *reinterpret_cast<const uint32_t*>(&hi);
+            *reinterpret_cast<uint2*>((bf16*)g.out + at) = packed;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (f + e >= g.out_features) break;
+        if (g.out_f32) ((float*)g.out)[at + e] = v[e];
+        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(v[e]);
+    }
+}
+
+__device__ __forceinline__ int4 i8_ld_cluster(const int* local, uint32_t rank) {
+    uint32_t addr = s_addr(local), remote;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
+    return v;
+}
+
+// ---------------------------------------------------------------- few tokens: the weights' bytes are the work
+//
+// The weights are the instruction's A (their rows fill its 128 lanes), the tokens its B (bn of them, a multiple of 16 up to
+// 256).  A block forms a tile of 128 features x bn tokens over one slice of K; the 1 to 8 slices of a tile are a thread-block
+// cluster along grid.z, whose blocks leave their sums in shared memory and add up the token columns rank, rank + slices, ...
+// of all of them.  Warp 0 (one lane) fetches, warp 1 issues the products, warps 2 to 5 write the result out.
+__global__ void __launch_bounds__(I8_THREADS)
+gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Int8Args g) {
+    extern __shared__ unsigned char smem_raw[];
+    const int bn = g.bn, stages = g.stages, n_sl = g.slices;
+    const int w_bytes = I8_BM * I8_BK, stage_bytes = w_bytes + bn * I8_BK;
+    unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);
+    uint64_t* empty = full + stages;
+    uint64_t* acc_ready = empty + stages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_ready + 1);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* xs_s = reinterpret_cast<float*>(full) + 64;  // [256], behind the barriers
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t0 = blockIdx.x * bn, f0 = blockIdx.y * I8_BM;  // first token, first feature
+    const int k_total = (g.K + I8_BK - 1) / I8_BK;
+    const int per = (k_total + n_sl - 1) / n_sl;
+    const int k_begin = blockIdx.z * per, k_iters = max(0, min(k_total, k_begin + per) - k_begin);
+    const int ahead = min(stages, k_iters);
+    const uint32_t tmem_cols = bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256;
+    const uint64_t once = l2_evict_first_policy();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(acc_ready, 1);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
+        for (int it = 0; it < ahead; ++it) {
+            mbar_expect_tx(&full[it], stage_bytes);
+            i8_load_once(tiles + it * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[it], once);
+        }
+    }
+    // nor do the scales and the bias of the four features (gated: four pairs) that a lane writes out
+    const int half = g.gated ? lane >> 4 : 0, fl = g.gated ? (lane & 15) * 4 : lane * 4;
+    float ws[4], bs[4], ws2[4], bs2[4];
+    if (warp >= 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int f = f0 + fl + e, f2 = f + 64;
+            ws[e] = f < g.features ? __ldg(g.w_scale + f) : 0.f;
+            bs[e] = g.bias && f < g.features ? i8_bias(g, f) : 0.f;
+            ws2[e] = g.gated && f2 < g.features ? __ldg(g.w_scale + f2) : 0.f;
+            bs2[e] = g.gated && g.bias && f2 < g.features ? i8_bias(g, f2) : 0.f;
+        }
+    }
+    pdl_wait();
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)), "r"(tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    } else if (threadIdx.x == 0) {
+        for (int it = 0; it < ahead; ++it)
+            i8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[it]);
+    } else if (warp >= 2) {
+        for (int i = threadIdx.x - 64; i < bn; i += 128) xs_s[i] = t0 + i < g.tokens ? __ldg(g.x_scale + t0 + i) : 0.f;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_launch_dependents();
+    const uint32_t tmem_acc = *tmem_slot;
+    int* sums = reinterpret_cast<int*>(tiles);  // [bn][128], over the ring when all its stages have been used
+
+    if (warp == 0 && lane == 0) {
+        int it = ahead;
+        for (; it < k_iters; ++it) {
+            const int s = it % stages;
+            if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, gave_up)) break;
+            mbar_expect_tx(&full[s], stage_bytes);
+            i8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[s], once);
+            i8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[s]);
+        }
+        if (*gave_up)
+            for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
+    } else if (warp == 1) {
+        const uint32_t idesc = i8_idesc(I8_BM, bn);
+        for (int it = 0; it < k_iters; ++it) {
+            const int s = it % stages;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / stages) & 1, gave_up))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            unsigned char* w_tile = tiles + s * stage_bytes;
+            const uint64_t w_desc = smem_desc(w_tile), x_desc = smem_desc(w_tile + w_bytes);
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < I8_BK / 32; ++kk)  // 32 bytes further along the swizzled row
+                    umma_i8(tmem_acc, w_desc + (uint64_t)(kk * 2), x_desc + (uint64_t)(kk * 2), idesc, (it | kk) != 0);
+                umma_commit(&empty[s]);
+            }
+            __syncwarp();
+        }
+        if (elect_one()) umma_commit(acc_ready);
+        __syncwarp();
+    } else if (warp >= 2) {
+        const int quarter = warp & 3;  // warp w reads lanes 32 * (w % 4) .. + 31 of the accumulator
+        if (k_iters > 0) mbar_wait(acc_ready, 0, gave_up);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int c = 0; c < bn; c += 16) {
+            uint32_t r[16];
+            if (k_iters > 0) {
+                tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + c, r);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) r[j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(c + j) * I8_BM + quarter * 32 + lane] = (int)r[j];
+        }
+        if (n_sl == 1) asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+    if (n_sl > 1) cluster_sync_all();  // every block's sums lie in its shared memory
+    if (warp >= 2) {
+        const int rank = n_sl > 1 ? (int)cluster_rank() : 0, q = warp & 3;
+        const int live = min(bn, g.tokens - t0);
+        // a warp takes a token column (gated: two) at a time, a lane four features of it
+        const int lanes_of = g.gated ? 2 : 1;
+        for (int i = q * lanes_of + half;; i += 4 * lanes_of) {
+            const int c = rank + i * n_sl;
+            if (c >= live) break;
+            int4 a = make_int4(0, 0, 0, 0), b = a;
+            for (int s = 0; s < n_sl; ++s) {
+                const int* from = sums + c * I8_BM + fl;
+                const int4 v = n_sl > 1 ? i8_ld_cluster(from, (uint32_t)s) : *reinterpret_cast<const int4*>(from);
+                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+                if (g.gated) {
+                    const int4 u = n_sl > 1 ? i8_ld_cluster(from + 64, (uint32_t)s) : *reinterpret_cast<const int4*>(from + 64);
+                    b.x += u.x; b.y += u.y; b.z += u.z; b.w += u.w;
+                }
+            }
+            const float xs = xs_s[c];
+            float v[4] = {i8_value(a.x, xs, ws[0], bs[0]), i8_value(a.y, xs, ws[1], bs[1]),
+                          i8_value(a.z, xs, ws[2], bs[2]), i8_value(a.w, xs, ws[3], bs[3])};
+            if (g.gated) {
+                const float u[4] = {i8_value(b.x, xs, ws2[0], bs2[0]), i8_value(b.y, xs, ws2[1], bs2[1]),
+                                    i8_value(b.z, xs, ws2[2], bs2[2]), i8_value(b.w, xs, ws2[3], bs2[3])};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = i8_gate(g, v[e], u[e]);
+                i8_store4(g, t0 + c, f0 / 2 + fl, v);
+            } else {
+                i8_store4(g, t0 + c, f0 + fl, v);
+            }
+        }
+    }
+    if (n_sl > 1) cluster_sync_before_exit();  // nobody leaves while its sums are still being read
+    if (*gave_up && threadIdx.x == 0) atomicOr(g.err, SS_ERR_WAIT_LIMIT);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(tmem_cols));
+    }
+}
+
+// ---------------------------------------------------------------- many tokens: the tensor cores are the work
+//
+// A persistent kernel on pairs of SMs (tcgen05.mma.cta_group::2).  A pair walks over tiles of 256 tokens x bn features, token
+// tiles fastest.  Block r of the pair fetches tokens r * 128 .. of the tile and half of its features' weights; the leader
+// (block 0) issues the products, which leave the tokens of block r in block r's tensor memory.  The accumulator is
+// double-buffered (2 x 256 columns): the four epilogue warps of each block write a tile out while the next one is formed.
+//   full[s]      in the leader: the bytes of both blocks' copies;     empty[s]     in each block: the products have read the stage
+//   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all eight epilogue warps are
+#define I8_PAIR_STAGES 6
+#define I8_MAX_BN 256
+
+__device__ __forceinline__ uint32_t i8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
+
+__device__ __forceinline__ void i8_load_pair(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(s_addr(dst)), "l"(map), "r"(i8_leader(bar)), "r"(k), "r"(row) : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void i8_commit_pair(uint64_t* bar) {  // arrives at `bar` in both blocks of the pair
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(s_addr(bar)), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ void i8_arrive_leader(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(i8_leader(bar)) : "memory");
+}
+
+// 16 neighbouring outputs of a token.
+__device__ __forceinline__ void i8_store16(const Int8Args& g, int token, int f, const float (&v)[16]) {
+    const int64_t at = (int64_t)token * g.ldc + f;
+    if (f + 16 <= g.out_features && (g.ldc & 7) == 0) {
+        if (g.out_f32) {
+            float4* dst = reinterpret_cast<float4*>((float*)g.out + at);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+            uint32_t p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                p[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            uint4* dst = reinterpret_cast<uint4*>((bf16*)g.out + at);
+            dst[0] = make_uint4(p[0], p[1], p[2], p[3]);
+            dst[1] = make_uint4(p[4], p[5], p[6], p[7]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        if (f + e >= g.out_features) break;
+        if (g.out_f32) ((float*)g.out)[at + e] = v[e];
+        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(v[e]);
+    }
+}
+// 16 sums of a token, features f .. f + 15, as values
+__device__ __forceinline__ void i8_values16(const Int8Args& g, const uint32_t (&r)[16], float xs, int f, float (&v)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const bool in = f + e < g.features;
+        v[e] = i8_value((int)r[e], xs, in ? __ldg(g.w_scale + f + e) : 0.f, g.bias && in ? i8_bias(g, f + e) : 0.f);
+    }
+}
+
+__global__ void __launch_bounds__(I8_THREADS)
+gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Int8Args g) {
+    constexpr int X_BYTES = I8_BM * I8_BK, W_BYTES = I8_BM * I8_BK, STAGES = I8_PAIR_STAGES;  // this block's halves
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + STAGES * (X_BYTES + W_BYTES));
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();  // 0: the leader
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int bn = g.bn;  // a multiple of 32
+    const int n_m = (g.tokens + 2 * I8_BM - 1) / (2 * I8_BM), n_tiles = n_m * ((g.features + bn - 1) / bn);
+    const int k_iters = (g.K + I8_BK - 1) / I8_BK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    if (warp == 1) {  // the same warp of both blocks allocates all 512 columns of the pair
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();  // both blocks' barriers exist before either signals the other's
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_launch_dependents();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int it = 0;
+        bool ok = true;
+        const int bytes = 2 * (X_BYTES + (bn / 2) * I8_BK);
+        for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+            const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * (bn / 2);
+            for (int k = 0; k < k_iters; ++k, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, gave_up)) { ok = false; break; }
+                if (rank == 0) mbar_expect_tx(&full[s], bytes);
+                unsigned char* x_tile = tiles + s * (X_BYTES + W_BYTES);
+                i8_load_pair(x_tile, &map_x, k * I8_BK, m0, &full[s]);
+                i8_load_pair(x_tile + X_BYTES, &map_w, k * I8_BK, n0, &full[s]);
+            }
+        }
+        if (*gave_up && rank == 0)
+            for (int back = max(0, it - STAGES); back < it; ++back) i8_drain(&full[back % STAGES], (back / STAGES) & 1);
+    } else if (warp == 1 && rank == 0) {
+        const uint32_t idesc = i8_idesc(2 * I8_BM, bn);
+        int it = 0, j = 0;
+        bool ok = true;
+        for (int t = pair; t < n_tiles && ok; t += n_pairs, ++j) {
+            const int buf = j & 1;
+            if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1, gave_up))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = 0; k < k_iters; ++k, ++it) {
+                const int s = it % STAGES;
+                if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / STAGES) & 1, gave_up))) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                unsigned char* x_tile = tiles + s * (X_BYTES + W_BYTES);
+                const uint64_t x_desc = smem_desc(x_tile), w_desc = smem_desc(x_tile + X_BYTES);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < I8_BK / 32; ++kk)
+                        umma_i8_pair(tmem + buf * I8_MAX_BN, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, (k | kk) != 0);
+                    i8_commit_pair(&empty[s]);
+                }
+                __syncwarp();
+            }
+            if (elect_one()) i8_commit_pair(&acc_full[buf]);
+            __syncwarp();
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3;
+        int j = 0;
+        for (int t = pair; t < n_tiles; t += n_pairs, ++j) {
+            const int buf = j & 1, n0 = (t / n_m) * bn;
+            const int m = (t % n_m) * 2 * I8_BM + rank * I8_BM + quarter * 32 + lane;
+            const float xs = m < g.tokens ? __ldg(g.x_scale + m) : 0.f;
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * I8_MAX_BN;
+            if (!g.gated) {
+#pragma unroll 1
+                for (int c = 0; c < bn; c += 16) {
+                    uint32_t r[16];
+                    float v[16];
+                    tmem_ld16(acc + c, r);
+                    if (m >= g.tokens || n0 + c >= g.features) continue;
+                    i8_values16(g, r, xs, n0 + c, v);
+                    i8_store16(g, m, n0 + c, v);
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < bn / 2; c += 16) {
+                    const int gc = (c / 64) * 128 + (c % 64);
+                    uint32_t gr[16], ur[16];
+                    float v[16], u[16];
+                    tmem_ld16(acc + gc, gr);
+                    tmem_ld16(acc + gc + 64, ur);
+                    if (m >= g.tokens || n0 + gc >= g.features) continue;
+                    i8_values16(g, gr, xs, n0 + gc, v);
+                    i8_values16(g, ur, xs, n0 + gc + 64, u);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = i8_gate(g, v[e], u[e]);
+                    i8_store16(g, m, n0 / 2 + c, v);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) i8_arrive_leader(&acc_empty[buf]);
+        }
+    }
+    if (*gave_up && threadIdx.x == 0) atomicOr(g.err, SS_ERR_WAIT_LIMIT);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();  // neither block leaves (or frees tensor memory) while the other may still signal it
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+typedef CUresult (*I8Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// int8 matrix [rows, K] with row stride ld bytes; box = 128 x box_rows.
+static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows) {
+    static I8Encode enc = nullptr;
+    if (!enc) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            return -2001;
+        enc = (I8Encode)p;
+    }
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {I8_BK, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -2002;
+}
+
+#define I8_SMEM_MAX 232448  // 227 KB
+#define I8_SMEM_REST 2560   // alignment, barriers, the tokens' scales
+
+// x [tokens, K] and w [features, K] int8 with row strides ldx, ldw (multiples of 16 bytes, bases on 16 bytes), K <= 133,143.
+// gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
+// many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `two` blocks an SM wanted (0, 1).
+// many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
+extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
+                            const void* bias, int bias_f32, void* out, int64_t ldc, int out_f32, int tokens, int features, int K,
+                            int gated, int out_features, int many, int bn, int slices, int two, int* err, cudaStream_t stream) {
+    if (tokens <= 0 || features <= 0) return 0;
+    if (K <= 0 || K > 133143 || ldx % 16 || ldw % 16 || ldx < K || ldw < K) return -2003;
+    if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return -2004;
+    if (gated ? (features % 128 || out_features > features / 2) : out_features != features) return -2005;
+    if (bn < 16 || bn > I8_MAX_BN || bn % (many ? 32 : 16) || (many && gated && bn % 128) || (!many && (slices < 1 || slices > 8))) return -2006;
+    Int8Args g = {};
+    g.x_scale = x_scale; g.w_scale = w_scale; g.bias = bias; g.out = out; g.err = err; g.ldc = ldc;
+    g.tokens = tokens; g.features = features; g.K = K; g.out_features = out_features;
+    g.out_f32 = out_f32; g.bias_f32 = bias_f32; g.gated = gated; g.bn = bn; g.slices = slices;
+    CUtensorMap map_x, map_w;
+    if (many) {
+        if (int rc = i8_map(&map_x, x, tokens, K, ldx, I8_BM)) return rc;
+        if (int rc = i8_map(&map_w, w, features, K, ldw, bn / 2)) return rc;
+        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST;
+        static SsPerDevice opted;
+        if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, smem, opted)) return rc;
+        const int64_t n_tiles = (int64_t)((tokens + 255) / 256) * ((features + bn - 1) / bn);
+        const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
+        ss_launch_cluster_x(gemm_int8_many_kernel, dim3(2 * pairs), dim3(I8_THREADS), smem, stream, 2, map_x, map_w, g);
+        return SS_LAUNCH_CHECK();
+    }
+    if (int rc = i8_map(&map_x, x, tokens, K, ldx, bn)) return rc;
+    if (int rc = i8_map(&map_w, w, features, K, ldw, I8_BM)) return rc;
+    static SsPerDevice opted;
+    if (int rc = ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return rc;
+    const int stage = I8_BM * I8_BK + bn * I8_BK;
+    const int room = two ? I8_SMEM_MAX / 2 - 1024 : I8_SMEM_MAX;
+    int stages = (room - I8_SMEM_REST) / stage;
+    const int needed = (bn * I8_BM * 4 + stage - 1) / stage;  // the ring also holds the sums
+    stages = stages < needed ? needed : stages > 12 ? 12 : stages;
+    g.stages = stages;
+    const int smem = stages * stage + I8_SMEM_REST;
+    if (smem > I8_SMEM_MAX) return -2007;
+    const dim3 grid((tokens + bn - 1) / bn, (features + I8_BM - 1) / I8_BM, slices);
+    if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, stream, slices, map_w, map_x, g);
+    else ss_launch(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, stream, map_w, map_x, g);
+    return SS_LAUNCH_CHECK();
+}

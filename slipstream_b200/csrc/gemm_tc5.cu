@@ -49,11 +49,6 @@ __device__ __forceinline__ void tma_load_2d_once(void* dst, const CUtensorMap* m
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
         ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(c0), "r"(c1), "l"(policy) : "memory");
 }
-__device__ __forceinline__ uint64_t l2_evict_first_policy() {
-    uint64_t policy;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    return policy;
-}
 
 #define TC_HC_MAX 4  // most hyper-connected streams a product writes into itself
 

@@ -1,0 +1,422 @@
+// Rows of 8-bit integers with one float32 scale each: how activations and weights become such rows, and back.
+//
+// A row v becomes q and s with q * s near v: a = max |v|, s = a / 127, q = rint(v * (127 / a)), ties to even, so -127 <= q <= 127
+// and the largest element keeps its value.  A row of zeros has s = 0.  A row that holds an infinity or NaN has s = NaN and q = 0:
+// all that is formed from it is NaN, as it would be without the rounding.  The maximum is taken over the bits of |v| as unsigned
+// integers, which order like the values and put NaN on top.
+//
+// Rows of q start on 16 bytes (their stride is a multiple of 16); what lies between a row's end and the next row is not written.
+//
+// All three kernels are bound by memory: a row is read once, into registers, and its results are written from there.
+
+#include "common.cuh"
+
+namespace {
+
+constexpr uint32_t INF_BITS = 0x7f800000u;
+constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: behind the sum with it, a float's low byte is the rounded integer's
+
+// Four elements from memory: one load of 16 (float32) or 8 bytes (bfloat16) where rows are aligned for it, else one by one,
+// the `left` that there are.
+template <bool ALIGNED>
+__device__ __forceinline__ void load4(const float* p, int left, float (&v)[4]) {
+    if (ALIGNED && left >= 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? p[e] : 0.f;
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void load4(const bf16* p, int left, float (&v)[4]) {
+    if (ALIGNED && left >= 4) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xffff0000u);
+        v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xffff0000u);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? to_float(p[e]) : 0.f;
+}
+
+__device__ __forceinline__ uint32_t top_of(uint32_t top, const float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    return top;
+}
+
+// What a row's largest magnitude (its bits) makes of it.
+struct RowScale {
+    float scale, inverse, before;  // q = rint((v * before) * inverse)
+    uint32_t keep;                 // 0: the row's values are written as zeros
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+    RowScale r;
+    const float a = __uint_as_float(top);
+    const bool fine = top < INF_BITS && top > 0;
+    r.before = a < 0x1p-100f ? 0x1p64f : 1.f;  // 127 / a stays finite (and the product with `before` is exact)
+    r.inverse = fine ? __fdiv_rn(127.f, a * r.before) : 0.f;
+    r.scale = top < INF_BITS ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu);
+    r.keep = fine ? 0xffffffffu : 0u;
+    return r;
+}
+__device__ __forceinline__ uint32_t quantize4(const float (&v)[4], const RowScale& r) {
+    uint32_t b[4];
+    if (r.before == 1.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e], r.inverse), MAGIC));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e] * r.before, r.inverse), MAGIC));
+    }
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & r.keep;
+}
+__device__ __forceinline__ void store4(int8_t* q, int left, uint32_t word) {
+    if (left >= 4) {
+        *reinterpret_cast<uint32_t*>(q) = word;
+        return;
+    }
+    for (int e = 0; e < left; ++e) q[e] = (int8_t)(word >> (8 * e));
+}
+
+// The block's largest `top` and the sum of its `sum`, with one barrier; every thread gets both.  The order of the additions
+// depends on the number of threads alone.
+__device__ __forceinline__ void block_top_sum(uint32_t& top, float& sum, uint32_t* tops, float* sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    top = __reduce_max_sync(0xffffffffu, top);
+    sum = warp_sum(sum);
+    if (lane == 0) { tops[warp] = top; sums[warp] = sum; }
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+    sum = warp_sum(lane < warps ? sums[lane] : 0.f);
+}
+
+// Threads of a block at most where NG vectors of a row stay in a thread's registers.
+template <int NG>
+constexpr int most_threads() { return NG == 0 || NG > 2 ? 512 : 1024; }
+
+// ---------------------------------------------------------------- rows to int8
+//
+// A block per row.  NG vectors of 16 bytes a thread stay in registers as they came; NG = 0: rows of any width, read twice.
+template <typename T>
+struct RawVec {
+    static constexpr int G = 16 / (int)sizeof(T);
+    uint4 raw;
+    template <bool ALIGNED>
+    __device__ __forceinline__ void load(const T* p, int left) {
+        if (ALIGNED && left >= G) {
+            raw = *reinterpret_cast<const uint4*>(p);
+            return;
+        }
+        T t[G];
+#pragma unroll
+        for (int e = 0; e < G; ++e) t[e] = e < left ? p[e] : from_float<T>(0.f);
+        if constexpr (G == 4) {
+            raw = make_uint4(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3]));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)__bfloat16_as_ushort(t[2 * e]) | (uint32_t)__bfloat16_as_ushort(t[2 * e + 1]) << 16;
+            raw = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w; }
+    // bits of the largest magnitude so far: of float32 values, or of bfloat16 values in both halves of the word
+    __device__ __forceinline__ uint32_t top(uint32_t t) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t = G == 4 ? max(t, word(i) & 0x7fffffffu) : __vmaxu2(t, word(i) & 0x7fff7fffu);
+        return t;
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t t) { return G == 4 ? t : max(t << 16, t & 0xffff0000u); }
+    __device__ __forceinline__ void four(int i, float (&v)[4]) const {  // elements 4 i .. 4 i + 3
+        if constexpr (G == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(word(e));
+        } else {
+            v[0] = __uint_as_float(word(2 * i) << 16); v[1] = __uint_as_float(word(2 * i) & 0xffff0000u);
+            v[2] = __uint_as_float(word(2 * i + 1) << 16); v[3] = __uint_as_float(word(2 * i + 1) & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ void quantize(int8_t* q, int left, const RowScale& r) const {
+        float v[4];
+        if constexpr (G == 8) {
+            uint2 w;
+            four(0, v); w.x = quantize4(v, r);
+            four(1, v); w.y = quantize4(v, r);
+            if (left >= 8) {
+                *reinterpret_cast<uint2*>(q) = w;
+            } else {
+                store4(q, left, w.x);
+                store4(q + 4, left - 4, w.y);
+            }
+        } else {
+            four(0, v);
+            store4(q, left, quantize4(v, r));
+        }
+    }
+};
+
+template <typename T, bool ALIGNED, int NG>
+__global__ void __launch_bounds__(most_threads<NG>())
+quantize_rows_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales,
+                     int width, int early) {
+    using Vec = RawVec<T>;
+    constexpr int G = Vec::G;
+    __shared__ uint32_t tops[32];
+    __shared__ float sums[32];
+    if (early) pdl_launch_dependents();
+    pdl_wait();
+    const T* row = x + (int64_t)blockIdx.x * stride;
+    int8_t* out = q + (int64_t)blockIdx.x * q_stride;
+    Vec v[NG ? NG : 1];
+    uint32_t top = 0;
+    float none = 0.f;
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * blockDim.x) * G;
+            v[i].template load<ALIGNED>(row + j, width - j);
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) top = v[i].top(top);
+    } else {
+        for (int j = threadIdx.x * G; j < width; j += blockDim.x * G) {
+            v[0].template load<ALIGNED>(row + j, width - j);
+            top = v[0].top(top);
+        }
+    }
+    top = Vec::top_bits(top);
+    block_top_sum(top, none, tops, sums);
+    const RowScale r = row_scale(top);
+    if (threadIdx.x == 0) scales[blockIdx.x] = r.scale;
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * blockDim.x) * G;
+            if (j < width) v[i].quantize(out + j, width - j, r);
+        }
+    } else {
+        for (int j = threadIdx.x * G; j < width; j += blockDim.x * G) {
+            v[0].template load<ALIGNED>(row + j, width - j);
+            v[0].quantize(out + j, width - j, r);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- add + RMS norm to int8
+//
+// x = residual + delta, written to residual_out (if there is one); v = x / sqrt(mean(x^2) + eps) * w, as int8 rows.  The norm's
+// factor is the same for the whole row, so q is that of x * w, and the factor enters the scale alone: the squares' sum and the
+// largest |x * w| are found in one pass with one barrier, and v is never rounded to fewer than its 24 bits.
+//
+// A block per row; NG groups of four elements a thread stay in registers; NG = 0: rows of any width, read twice.
+template <typename T, bool ALIGNED, int NG>
+__global__ void __launch_bounds__(most_threads<NG>())
+add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, float* residual_out, const void* __restrict__ weight,
+                        int w_f32, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int width, float eps) {
+    // few rows: the weights do not depend on the kernels in front and are on the way before those are through
+    constexpr bool EARLY_W = NG == 1 || NG == 2;
+    __shared__ uint32_t tops[32];
+    __shared__ float sums[32];
+    pdl_launch_dependents();
+    float w[EARLY_W ? NG : 1][4], v[NG ? NG : 1][4];
+    auto load_w = [&](int j, float (&to)[4]) {
+        if (w_f32) load4<ALIGNED>((const float*)weight + j, width - j, to);
+        else load4<ALIGNED>((const bf16*)weight + j, width - j, to);
+    };
+    if constexpr (EARLY_W) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) load_w((threadIdx.x + i * blockDim.x) * 4, w[i]);
+    }
+    pdl_wait();
+    const int64_t at = (int64_t)blockIdx.x * width;
+    const float* row = residual + at;
+    int8_t* out = q + (int64_t)blockIdx.x * q_stride;
+    uint32_t top = 0;
+    float ss = 0.f;
+    auto load_x = [&](int j, bool add, float (&x)[4]) {
+        load4<ALIGNED>(row + j, width - j, x);
+        if (add) {
+            float d[4];
+            load4<ALIGNED>(delta + at + j, width - j, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __fadd_rn(x[e], d[e]);
+        }
+    };
+    auto store_x = [&](int j, const float (&x)[4]) {
+        float* to = residual_out + at + j;
+        if (ALIGNED && j + 4 <= width) {
+            *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < width) to[e] = x[e];
+        }
+    };
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) load_x((threadIdx.x + i * blockDim.x) * 4, delta != nullptr, v[i]);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * blockDim.x) * 4;
+            if (residual_out && j < width) store_x(j, v[i]);
+            float (&wi)[4] = w[EARLY_W ? i : 0];
+            if constexpr (!EARLY_W) load_w(j, wi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ss = fmaf(v[i][e], v[i][e], ss);
+                v[i][e] *= wi[e];
+            }
+            top = top_of(top, v[i]);
+        }
+    } else {
+        for (int j = threadIdx.x * 4; j < width; j += blockDim.x * 4) {
+            load_x(j, delta != nullptr, v[0]);
+            if (residual_out) store_x(j, v[0]);
+            load_w(j, w[0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ss = fmaf(v[0][e], v[0][e], ss);
+                v[0][e] *= w[0][e];
+            }
+            top = top_of(top, v[0]);
+        }
+    }
+    block_top_sum(top, ss, tops, sums);
+    RowScale r = row_scale(top);
+    const float rstd = 1.0f / sqrtf(ss / (float)width + eps);
+    if (threadIdx.x == 0) scales[blockIdx.x] = __fdiv_rn(__uint_as_float(top) * rstd, 127.f);
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * blockDim.x) * 4;
+            if (j < width) store4(out + j, width - j, quantize4(v[i], r));
+        }
+    } else {
+        // the sum again: from residual_out where it was written (by this thread), else formed once more
+        if (residual_out) row = residual_out + at;
+        for (int j = threadIdx.x * 4; j < width; j += blockDim.x * 4) {
+            load_x(j, delta != nullptr && !residual_out, v[0]);
+            load_w(j, w[0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[0][e] *= w[0][e];
+            store4(out + j, width - j, quantize4(v[0], r));
+        }
+    }
+}
+
+// ---------------------------------------------------------------- int8 rows to values
+//
+// y = q * s, rounded once.  A block per row; eight (bfloat16) or four (float32) elements a thread and step where the output's
+// rows start on 16 bytes, else one.
+template <typename T, bool ALIGNED>
+__global__ void dequantize_rows_kernel(const int8_t* __restrict__ q, int64_t q_stride, const float* __restrict__ scales,
+                                       T* __restrict__ y, int width) {
+    constexpr int G = ALIGNED ? 16 / (int)sizeof(T) : 1;
+    pdl_launch_dependents();
+    pdl_wait();
+    const float s = scales[blockIdx.x];
+    const int8_t* row = q + (int64_t)blockIdx.x * q_stride;
+    T* out = y + (int64_t)blockIdx.x * width;
+    for (int j = threadIdx.x * G; j < width; j += blockDim.x * G) {
+        if constexpr (!ALIGNED) {
+            out[j] = from_float<T>((float)row[j] * s);
+        } else {
+            uint32_t words[G / 4];
+            if constexpr (G == 8) *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(row + j);
+            else words[0] = *reinterpret_cast<const uint32_t*>(row + j);
+            T v[G];
+#pragma unroll
+            for (int e = 0; e < G; ++e) v[e] = from_float<T>((float)(int8_t)(words[e / 4] >> (8 * (e & 3))) * s);
+            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+// How a row of `groups` vectors or groups is dealt out: NG a thread (0: the row is read twice) and the threads of a block.  Up to
+// two rows an SM leave SMs to spare, so a row gets as many threads as a block holds; many rows run in blocks of up to 256
+// threads where that suffices, several of them on an SM.
+struct RowShape { int ng, threads; };
+inline RowShape row_shape(int groups, int64_t rows) {
+    const int sizes[8] = {1, 2, 3, 4, 6, 8, 10, 0};
+    const bool few = rows <= 2 * (int64_t)ss_sm_count();
+    for (int pass = few ? 1 : 0; pass < 2; ++pass)
+        for (int i = 0; i < 7; ++i) {
+            const int threads = ((groups + sizes[i] - 1) / sizes[i] + 31) / 32 * 32;
+            if (threads <= (pass == 0 ? 256 : sizes[i] > 2 ? 512 : 1024)) return {sizes[i], threads};
+        }
+    return {0, 512};
+}
+#define ROW_SHAPES(CASE) switch (shape.ng) { CASE(0); CASE(1); CASE(2); CASE(3); CASE(4); CASE(6); CASE(8); CASE(10); }
+
+template <typename T, bool ALIGNED>
+int launch_quantize(const void* x, int64_t stride, int8_t* q, int64_t q_stride, float* scales, int rows, int width, int early,
+                    cudaStream_t stream) {
+    constexpr int G = RawVec<T>::G;
+    const RowShape shape = row_shape((width + G - 1) / G, rows);
+#define QUANT(NG) case NG: ss_launch(quantize_rows_kernel<T, ALIGNED, NG>, dim3(rows), dim3(shape.threads), 0, stream, (const T*)x, stride, q, q_stride, scales, width, early); break
+    ROW_SHAPES(QUANT)
+#undef QUANT
+    return SS_LAUNCH_CHECK();
+}
+
+template <typename T, bool ALIGNED>
+int launch_norm(const float* residual, const void* delta, float* residual_out, const void* weight, int w_f32, int8_t* q,
+                int64_t q_stride, float* scales, int rows, int width, float eps, cudaStream_t stream) {
+    const RowShape shape = row_shape((width + 3) / 4, rows);
+#define NORM(NG) case NG: ss_launch(add_rmsnorm_int8_kernel<T, ALIGNED, NG>, dim3(rows), dim3(shape.threads), 0, stream, residual, (const T*)delta, residual_out, weight, w_f32, q, q_stride, scales, width, eps); break
+    ROW_SHAPES(NORM)
+#undef NORM
+    return SS_LAUNCH_CHECK();
+}
+
+inline bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+// x [rows, width] with row stride `stride` (elements).  early: the kernel behind may start at once; it may then have read
+// what it takes for constant before q is written, so only for q that it does not take for that (weights are).
+extern "C" int ss_quantize_rows_int8(const void* x, int64_t stride, int8_t* q, int64_t q_stride, float* scales, int rows, int width,
+                                     int dtype, int early, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
+    if (dtype == SS_BF16)
+        return on16(x) && stride % 8 == 0 ? launch_quantize<bf16, true>(x, stride, q, q_stride, scales, rows, width, early, stream)
+                                                          : launch_quantize<bf16, false>(x, stride, q, q_stride, scales, rows, width, early, stream);
+    return on16(x) && stride % 4 == 0 ? launch_quantize<float, true>(x, stride, q, q_stride, scales, rows, width, early, stream)
+                                      : launch_quantize<float, false>(x, stride, q, q_stride, scales, rows, width, early, stream);
+}
+
+// residual, delta (or null) and residual_out (or null; may be residual) [rows, width], contiguous.
+extern "C" int ss_add_rmsnorm_int8(const float* residual, const void* delta, float* residual_out, const void* weight, int w_f32,
+                                   int8_t* q, int64_t q_stride, float* scales, int rows, int width, float eps, int delta_dtype,
+                                   cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
+    const bool aligned = width % 4 == 0 && on16(residual) && on16(delta) && on16(residual_out) && on16(weight);
+    if (delta_dtype == SS_BF16)
+        return aligned ? launch_norm<bf16, true>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream)
+                       : launch_norm<bf16, false>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream);
+    return aligned ? launch_norm<float, true>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream)
+                   : launch_norm<float, false>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream);
+}
+
+// y [rows, width], contiguous.
+extern "C" int ss_dequantize_rows_int8(const int8_t* q, int64_t q_stride, const float* scales, void* y, int rows, int width, int dtype,
+                                       cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
+    const int g = dtype == SS_BF16 ? 8 : 4;
+    const bool aligned = on16(y) && width % g == 0;
+    int threads = (width / (aligned ? g : 1) + 31) / 32 * 32;
+    threads = threads < 32 ? 32 : threads > 256 ? 256 : threads;
+#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows), dim3(threads), 0, stream, q, q_stride, scales, (T*)y, width)
+    if (dtype == SS_BF16) { if (aligned) DEQ(bf16, true); else DEQ(bf16, false); }
+    else { if (aligned) DEQ(float, true); else DEQ(float, false); }
+#undef DEQ
+    return SS_LAUNCH_CHECK();
+}

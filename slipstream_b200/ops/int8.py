@@ -1,0 +1,228 @@
+"""Rows of 8-bit integers: the norm that ends in them, products of them, and how values become them and back.
+
+A row of int8 values comes with one float32 scale and stands for ``values * scale``.  Activations are such rows (a scale per
+token), and so are the weights of a product (a scale per output feature).  A product of both is exact in 32-bit integers; the
+scales are applied to the sum.  ``quantize_rows_int8`` is symmetric and has no zero point: the largest magnitude of a row becomes
+127 (or -127), a row of zeros has the scale 0, and a row that holds an infinity or NaN has the scale NaN, so that what is formed
+from it is NaN.
+
+Rows of values start on 16 bytes: their stride is a multiple of 16, whatever their width.  ``int8_rows_like`` makes such rows,
+and every function here that returns int8 rows uses it.
+
+Weights are taken for constant, as in the other products of this package: `linear_int8` may read them before the kernels in
+front of it are through.  `quantize_rows_int8` therefore keeps the kernels behind it waiting unless it is told
+(``activations=True``) that its rows will not be a product's weights.
+"""
+
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from .functions import KernelError, _check, _code, _need, _ptr, _stream, error_word, gemm_library, ops_library, sm_count
+
+RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
+MAX_K = 133143  # 127^2 K stays below 2^31
+_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
+
+
+class Int8Rows:
+    """``values`` int8 [N, K], whose rows start on 16 bytes, and ``scales`` float32 [N]: row n stands for
+    ``values[n] * scales[n]``."""
+
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
+        self.values = values
+        self.scales = scales
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def nbytes(self) -> int:
+        """Bytes a pass over the rows reads (without what pads them)."""
+        return self.values.numel() + 4 * self.scales.numel()
+
+    def dequantize(self, dtype: torch.dtype) -> torch.Tensor:
+        return dequantize_rows_int8(self, dtype)
+
+
+def int8_rows_like(rows: int, width: int, device: torch.device) -> Int8Rows:
+    """Int8 rows with nothing in them yet."""
+    stride = (width + 15) & -16
+    values = torch.empty_strided((rows, width), (stride, 1), dtype=_I8, device=device)
+    return Int8Rows(values, torch.empty(rows, dtype=_F32, device=device))
+
+
+def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int]:
+    """(rows, width, stride) of int8 rows that the kernels take."""
+    if not isinstance(r, Int8Rows):
+        raise KernelError(f"{what} must be Int8Rows, not {type(r).__name__}")
+    v, s = r.values, r.scales
+    if v.dim() != 2 or v.dtype != _I8 or not v.is_cuda:
+        raise KernelError(f"{what}: the values must be a two-dimensional int8 CUDA tensor, got {v.dtype} {tuple(v.shape)} on {v.device}")
+    n, k = v.shape
+    if s.dtype != _F32 or not s.is_cuda or s.numel() != n or not s.is_contiguous():
+        raise KernelError(f"{what}: the scales must be {n} contiguous float32 numbers on the device")
+    stride = v.stride(0) if n > 1 else (k + 15) & -16
+    if n and k and (v.stride(1) != 1 and k > 1 or stride % 16 or stride < k or v.data_ptr() % 16):
+        raise KernelError(f"{what}: rows must be contiguous and start on 16 bytes (a stride that is a multiple of 16), got strides {v.stride()}")
+    return n, k, stride
+
+
+def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Rows:
+    """The rows of ``x`` (float32 or bfloat16 [N, K], any row stride) as int8 rows: ``a = max |x_n|``, ``scale = a / 127``,
+    ``q = rint(x * (127 / a))``, ties to even.  Tokens of activations, or output features of a weight.
+
+    ``activations``: the rows are a product's activations, not its weights, and the kernel behind may start early."""
+    if not x.is_cuda or x.dim() != 2:
+        raise KernelError(f"x must be a two-dimensional CUDA tensor, got {tuple(x.shape)} on {x.device}")
+    n, k = x.shape
+    if k < 1:
+        raise KernelError("rows without elements have no scale")
+    if k > 1 and x.stride(1) != 1:
+        raise KernelError(f"the rows of x must be contiguous, got strides {x.stride()}")
+    out = int8_rows_like(n, k, x.device)
+    if n == 0:
+        return out
+    _check(ops_library().ss_quantize_rows_int8(x.data_ptr(), x.stride(0), out.values.data_ptr(), (k + 15) & -16, out.scales.data_ptr(),
+                                               n, k, _code(x.dtype), activations, _stream()), "quantize_rows_int8")
+    return out
+
+
+def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
+    """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once."""
+    n, k, stride = _need_rows(rows, "rows")
+    out = torch.empty((n, k), dtype=dtype, device=rows.values.device)
+    code = _code(dtype)
+    if n and k:
+        _check(ops_library().ss_dequantize_rows_int8(rows.values.data_ptr(), stride, rows.scales.data_ptr(), out.data_ptr(), n, k, code,
+                                                     _stream()), "dequantize_rows_int8")
+    return out
+
+
+def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
+                     residual_out: torch.Tensor | None = None) -> Int8Rows:
+    """``add_rmsnorm`` that ends in int8 rows: ``residual`` (float32 [N, H]) += ``delta`` (float32 or bfloat16, or None), and
+    ``x / sqrt(mean(x^2) + eps) * weight`` of the new stream, formed in float32, as int8 rows.
+
+    ``residual_out`` (float32 [N, H]) gets the new stream instead, and ``residual`` stays as it is.  ``weight`` is bfloat16 or
+    float32."""
+    _need(residual, _F32, "residual")
+    if residual.dim() != 2:
+        raise KernelError(f"residual must be [tokens, features], got {tuple(residual.shape)}")
+    n, h = residual.shape
+    if h < 1:
+        raise KernelError("rows without elements have no norm")
+    code = 1
+    if delta is not None:
+        _need(delta, None, "delta")
+        code = _code(delta.dtype)
+        if delta.shape != residual.shape:
+            raise KernelError(f"delta {tuple(delta.shape)} does not match residual {tuple(residual.shape)}")
+    _need(weight, None, "norm weight")
+    if weight.numel() != h or weight.dtype not in (_BF16, _F32):
+        raise KernelError("norm weight has the wrong size or dtype")
+    if residual_out is not None:
+        _need(residual_out, _F32, "residual_out")
+        if residual_out.shape != residual.shape:
+            raise KernelError(f"residual_out {tuple(residual_out.shape)} does not match residual {tuple(residual.shape)}")
+        to = residual_out.data_ptr()
+    else:
+        to = residual.data_ptr() if delta is not None else None
+    out = int8_rows_like(n, h, residual.device)
+    if n == 0:
+        return out
+    _check(ops_library().ss_add_rmsnorm_int8(residual.data_ptr(), _ptr(delta), to, weight.data_ptr(), weight.dtype == _F32,
+                                             out.values.data_ptr(), (h + 15) & -16, out.scales.data_ptr(), n, h, float(eps), code,
+                                             _stream()), "add_rmsnorm_int8")
+    return out
+
+
+# --------------------------------------------------------------------------- products
+
+@functools.lru_cache(maxsize=None)
+def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False) -> tuple[int, int, int, int]:
+    """(many, tile, K slices, two) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
+    (tokens of the first, features of the second), and for the first the slices of K and whether two blocks share an SM."""
+    k_iters = (k + 127) // 128
+    if tokens <= 256:
+        tile = max(16, (tokens + 15) // 16 * 16)
+        tiles = (features + 127) // 128
+        slices = max(1, min(8, k_iters, sms // tiles)) if tiles < sms else 1
+        return 0, tile, slices, int(tile <= 32)
+    return 1, 256, 1, 0
+
+
+def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype: torch.dtype, gated: bool, columns: int | None,
+             plan: tuple[int, int, int, int] | None, what: str) -> torch.Tensor:
+    tokens, k, ldx = _need_rows(x, "x")
+    features, k_w, ldw = _need_rows(weight, "weight")
+    if k_w != k:
+        raise KernelError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
+    if not 1 <= k <= MAX_K:
+        raise KernelError(f"an int8 product takes 1 to {MAX_K} elements of K, not {k}")
+    if gated:
+        if features % (2 * RUN):
+            raise KernelError(f"gate and up rows alternate in runs of {RUN}: {features} rows are no multiple of {2 * RUN}")
+        columns = features // 2 if columns is None else columns
+        if not 0 <= columns <= features // 2:
+            raise KernelError(f"{columns} features asked of {features // 2}")
+    else:
+        columns = features
+    out = torch.empty((tokens, columns), dtype=out_dtype, device=x.values.device)
+    out_f32 = 1 - _code(out_dtype)
+    bias_f32 = 0
+    if bias is not None:
+        _need(bias, None, "bias")
+        if bias.numel() != features or bias.dtype not in (_BF16, _F32):
+            raise KernelError("bias has the wrong size or dtype")
+        bias_f32 = int(bias.dtype == _F32)
+    if tokens == 0 or columns == 0:
+        return out
+    many, tile, slices, two = plan or int8_plan(tokens, features, k, sm_count(out.device), gated)
+    _check(gemm_library().ss_gemm_int8(x.values.data_ptr(), ldx, x.scales.data_ptr(), weight.values.data_ptr(), ldw, weight.scales.data_ptr(),
+                                       _ptr(bias), bias_f32, out.data_ptr(), columns, out_f32, tokens, features, k, gated, columns,
+                                       many, tile, slices, two, error_word(out.device).data_ptr(), _stream()), what)
+    return out
+
+
+def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
+                plan: tuple[int, int, int, int] | None = None) -> torch.Tensor:
+    """``x @ weight.T + bias`` for int8 rows: ``x`` [tokens, K] with a scale a token, ``weight`` [features, K] with a scale a
+    feature.  The sum over K is exact (32-bit integers); it is multiplied by both scales and the bias (bfloat16 or float32
+    [features]) is added in float32, and the result is rounded once to ``out_dtype`` (bfloat16 or float32)."""
+    return _product(x, weight, bias, out_dtype, False, None, plan, "linear_int8")
+
+
+def gate_up_swiglu_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
+                        features: int | None = None, plan: tuple[int, int, int, int] | None = None) -> torch.Tensor:
+    """``silu(gate(x)) * up(x)`` for int8 rows, the products as in `linear_int8`, the unit formed in float32 in the product's
+    epilogue and rounded once.  The rows of ``weight`` (and of ``bias``) alternate ``RUN`` gate and ``RUN`` up features
+    (`stack_gate_up`); ``features``: how many of the weight's pairs are real (those behind them pad the last run)."""
+    return _product(x, weight, bias, out_dtype, True, features, plan, "gate_up_swiglu_int8")
+
+
+def stack_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """The rows of ``gate`` and ``up`` (matrices or vectors of I rows) in alternating runs of ``RUN``, the last run padded with
+    zeros: the layout of `gate_up_swiglu_int8`, for weights before they are rounded and for biases."""
+    if gate.shape != up.shape:
+        raise KernelError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} differ")
+    rows, rest = gate.shape[0], gate.shape[1:]
+    runs = -(-rows // RUN)
+    stacked = gate.new_zeros((runs, 2, RUN, *rest))
+    for i, t in enumerate((gate, up)):
+        padded = t.new_zeros((runs * RUN, *rest))
+        padded[:rows] = t
+        stacked[:, i] = padded.reshape(runs, RUN, *rest)
+    return stacked.reshape(2 * runs * RUN, *rest)
+
+
+__all__ = ["Int8Rows", "int8_rows_like", "quantize_rows_int8", "dequantize_rows_int8", "add_rmsnorm_int8", "linear_int8",
+           "gate_up_swiglu_int8", "stack_gate_up", "int8_plan"]
