@@ -77,10 +77,10 @@ __device__ __forceinline__ float i8_gate(const Int8Args& g, float gate, float up
     return g.out_f32 ? silu_mul<false>(gate, up) : silu_mul<true>(gate, up);
 }
 
-// Four neighbouring outputs of a token.
-__device__ __forceinline__ void i8_store4(const Int8Args& g, int token, int f, const float (&v)[4]) {
+// Four outputs of a token, `apart` features from one another.
+__device__ __forceinline__ void i8_store4(const Int8Args& g, int token, int f, int apart, const float (&v)[4]) {
     const int64_t at = (int64_t)token * g.ldc + f;
-    if (f + 4 <= g.out_features && (g.ldc & 3) == 0) {
+    if (apart == 1 && f + 4 <= g.out_features) {
         if (g.out_f32) {
             *reinterpret_cast<float4*>((float*)g.out + at) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
@@ -94,18 +94,41 @@ __device__ __forceinline__ void i8_store4(const Int8Args& g, int token, int f, c
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (f + e >= g.out_features) break;
-        if (g.out_f32) ((float*)g.out)[at + e] = v[e];
-        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(v[e]);
+        if (f + e * apart >= g.out_features) break;
+        if (g.out_f32) ((float*)g.out)[at + e * apart] = v[e];
+        else ((bf16*)g.out)[at + e * apart] = __float2bfloat16_rn(v[e]);
     }
 }
 
-__device__ __forceinline__ int4 i8_ld_cluster(const int* local, uint32_t rank) {
-    uint32_t addr = s_addr(local), remote;
-    int4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
-    return v;
+// Four sums of a token's column, `apart` features from one another, out of the shared memory of all blocks of the cluster.
+__device__ __forceinline__ void i8_add_slices(const int* column, int fl, int apart, int n_sl, int (&sum)[4]) {
+    if (n_sl == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = column[fl + e * apart];
+        return;
+    }
+    int part[8][4];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        if (s < n_sl) {
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(column + fl)), "r"(s));
+            if (apart == 1) {
+                asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(part[s][0]), "=r"(part[s][1]), "=r"(part[s][2]), "=r"(part[s][3]) : "r"(remote) : "memory");
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[s][e]) : "r"(remote + 4 * e * apart) : "memory");
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[s][e] = 0;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        sum[e] = ((part[0][e] + part[1][e]) + (part[2][e] + part[3][e])) + ((part[4][e] + part[5][e]) + (part[6][e] + part[7][e]));
 }
 
 // ---------------------------------------------------------------- few tokens: the weights' bytes are the work
@@ -148,13 +171,15 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             i8_load_once(tiles + it * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[it], once);
         }
     }
-    // nor do the scales and the bias of the four features (gated: four pairs) that a lane writes out
-    const int half = g.gated ? lane >> 4 : 0, fl = g.gated ? (lane & 15) * 4 : lane * 4;
+    // nor do the scales and the bias of the four features (gated: four pairs) that a lane writes out: neighbours, or, where
+    // the output's rows do not start on four elements, one of each quarter of the tile
+    const int half = g.gated ? lane >> 4 : 0, of = g.gated ? lane & 15 : lane;
+    const int apart = (g.ldc & 3) == 0 ? 1 : g.gated ? 16 : 32, fl = apart == 1 ? of * 4 : of;
     float ws[4], bs[4], ws2[4], bs2[4];
     if (warp >= 2) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int f = f0 + fl + e, f2 = f + 64;
+            const int f = f0 + fl + e * apart, f2 = f + 64;
             ws[e] = f < g.features ? __ldg(g.w_scale + f) : 0.f;
             bs[e] = g.bias && f < g.features ? i8_bias(g, f) : 0.f;
             ws2[e] = g.gated && f2 < g.features ? __ldg(g.w_scale + f2) : 0.f;
@@ -228,32 +253,34 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (warp >= 2) {
         const int rank = n_sl > 1 ? (int)cluster_rank() : 0, q = warp & 3;
         const int live = min(bn, g.tokens - t0);
-        // a warp takes a token column (gated: two) at a time, a lane four features of it
-        const int lanes_of = g.gated ? 2 : 1;
-        for (int i = q * lanes_of + half;; i += 4 * lanes_of) {
-            const int c = rank + i * n_sl;
-            if (c >= live) break;
-            int4 a = make_int4(0, 0, 0, 0), b = a;
-            for (int s = 0; s < n_sl; ++s) {
-                const int* from = sums + c * I8_BM + fl;
-                const int4 v = n_sl > 1 ? i8_ld_cluster(from, (uint32_t)s) : *reinterpret_cast<const int4*>(from);
-                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-                if (g.gated) {
-                    const int4 u = n_sl > 1 ? i8_ld_cluster(from + 64, (uint32_t)s) : *reinterpret_cast<const int4*>(from + 64);
-                    b.x += u.x; b.y += u.y; b.z += u.z; b.w += u.w;
-                }
-            }
-            const float xs = xs_s[c];
-            float v[4] = {i8_value(a.x, xs, ws[0], bs[0]), i8_value(a.y, xs, ws[1], bs[1]),
-                          i8_value(a.z, xs, ws[2], bs[2]), i8_value(a.w, xs, ws[3], bs[3])};
+        // a warp takes two token columns (gated: each of its halves two) at a time, a lane four features of them; all loads of
+        // both columns are on the way before the first is added
+        const int step = g.gated ? 8 : 4;
+        for (int i = g.gated ? 2 * q + half : q;; i += 2 * step) {
+            const int c0 = rank + i * n_sl, c1 = c0 + step * n_sl;
+            if (c0 >= live) break;
+            int s0[4], s1[4];
+            i8_add_slices(sums + c0 * I8_BM, fl, apart, n_sl, s0);
+            if (c1 < live) i8_add_slices(sums + c1 * I8_BM, fl, apart, n_sl, s1);
+            int u0[4], u1[4];
             if (g.gated) {
-                const float u[4] = {i8_value(b.x, xs, ws2[0], bs2[0]), i8_value(b.y, xs, ws2[1], bs2[1]),
-                                    i8_value(b.z, xs, ws2[2], bs2[2]), i8_value(b.w, xs, ws2[3], bs2[3])};
+                i8_add_slices(sums + c0 * I8_BM + 64, fl, apart, n_sl, u0);
+                if (c1 < live) i8_add_slices(sums + c1 * I8_BM + 64, fl, apart, n_sl, u1);
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = i8_gate(g, v[e], u[e]);
-                i8_store4(g, t0 + c, f0 / 2 + fl, v);
-            } else {
-                i8_store4(g, t0 + c, f0 + fl, v);
+            for (int p = 0; p < 2; ++p) {
+                const int c = p ? c1 : c0;
+                if (c >= live) break;
+                const int (&a)[4] = p ? s1 : s0;
+                const int (&b)[4] = p ? u1 : u0;
+                const float xs = xs_s[c];
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = i8_value(a[e], xs, ws[e], bs[e]);
+                    if (g.gated) v[e] = i8_gate(g, v[e], i8_value(b[e], xs, ws2[e], bs2[e]));
+                }
+                i8_store4(g, t0 + c, (g.gated ? f0 / 2 : f0) + fl, apart, v);
             }
         }
     }
@@ -272,11 +299,12 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 // A persistent kernel on pairs of SMs (tcgen05.mma.cta_group::2).  A pair walks over tiles of 256 tokens x bn features, token
 // tiles fastest.  Block r of the pair fetches tokens r * 128 .. of the tile and half of its features' weights; the leader
 // (block 0) issues the products, which leave the tokens of block r in block r's tensor memory.  The accumulator is
-// double-buffered (2 x 256 columns): the four epilogue warps of each block write a tile out while the next one is formed.
+// double-buffered (2 x 256 columns): the eight epilogue warps of each block write a tile out while the next one is formed.
 //   full[s]      in the leader: the bytes of both blocks' copies;     empty[s]     in each block: the products have read the stage
-//   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all eight epilogue warps are
+//   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all sixteen epilogue warps are
 #define I8_PAIR_STAGES 6
 #define I8_MAX_BN 256
+#define I8_MANY_THREADS 320  // producer, issuer, eight epilogue warps
 
 __device__ __forceinline__ uint32_t i8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
 
@@ -299,44 +327,59 @@ __device__ __forceinline__ void i8_arrive_leader(uint64_t* bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(i8_leader(bar)) : "memory");
 }
 
-// 16 neighbouring outputs of a token.
-__device__ __forceinline__ void i8_store16(const Int8Args& g, int token, int f, const float (&v)[16]) {
+__device__ __forceinline__ void i8_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+// 32 sums of a token as values, in place; ws and bs: the features' scales and biases, in shared memory.
+__device__ __forceinline__ void i8_values32(uint32_t (&r)[32], float xs, const float* ws, const float* bs) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+        const float4 w = *reinterpret_cast<const float4*>(ws + e), b = *reinterpret_cast<const float4*>(bs + e);
+        r[e] = __float_as_uint(i8_value((int)r[e], xs, w.x, b.x));
+        r[e + 1] = __float_as_uint(i8_value((int)r[e + 1], xs, w.y, b.y));
+        r[e + 2] = __float_as_uint(i8_value((int)r[e + 2], xs, w.z, b.z));
+        r[e + 3] = __float_as_uint(i8_value((int)r[e + 3], xs, w.w, b.w));
+    }
+}
+// 32 neighbouring outputs of a token.
+__device__ __forceinline__ void i8_store32(const Int8Args& g, int token, int f, const uint32_t (&r)[32]) {
     const int64_t at = (int64_t)token * g.ldc + f;
-    if (f + 16 <= g.out_features && (g.ldc & 7) == 0) {
+    if (f + 32 <= g.out_features && (g.ldc & 7) == 0) {
         if (g.out_f32) {
-            float4* dst = reinterpret_cast<float4*>((float*)g.out + at);
+            uint4* dst = reinterpret_cast<uint4*>((float*)g.out + at);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            for (int q = 0; q < 8; ++q) dst[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
         } else {
-            uint32_t p[8];
+            uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+            for (int e = 0; e < 16; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
                 p[e] = *reinterpret_cast<const uint32_t*>(&h);
             }
             uint4* dst = reinterpret_cast<uint4*>((bf16*)g.out + at);
-            dst[0] = make_uint4(p[0], p[1], p[2], p[3]);
-            dst[1] = make_uint4(p[4], p[5], p[6], p[7]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]);
         }
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < 32; ++e) {
         if (f + e >= g.out_features) break;
-        if (g.out_f32) ((float*)g.out)[at + e] = v[e];
-        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(v[e]);
-    }
-}
-// 16 sums of a token, features f .. f + 15, as values
-__device__ __forceinline__ void i8_values16(const Int8Args& g, const uint32_t (&r)[16], float xs, int f, float (&v)[16]) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const bool in = f + e < g.features;
-        v[e] = i8_value((int)r[e], xs, in ? __ldg(g.w_scale + f + e) : 0.f, g.bias && in ? i8_bias(g, f + e) : 0.f);
+        if (g.out_f32) ((float*)g.out)[at + e] = __uint_as_float(r[e]);
+        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(__uint_as_float(r[e]));
     }
 }
 
-__global__ void __launch_bounds__(I8_THREADS)
+__global__ void __launch_bounds__(I8_MANY_THREADS)
 gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Int8Args g) {
     constexpr int X_BYTES = I8_BM * I8_BK, W_BYTES = I8_BM * I8_BK, STAGES = I8_PAIR_STAGES;  // this block's halves
     extern __shared__ unsigned char smem_raw[];
@@ -347,6 +390,8 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* ws_s = reinterpret_cast<float*>(full) + 64;  // [2][256] scales and [2][256] biases of a tile's features
+    float* bs_s = ws_s + 2 * I8_MAX_BN;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();  // 0: the leader
@@ -357,7 +402,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 16); }
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -415,39 +460,48 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             __syncwarp();
         }
     } else if (warp >= 2) {
-        const int quarter = warp & 3;
+        // warps 2 to 5 write out the first half of a tile's columns, warps 6 to 9 the second, each its quarter of the rows
+        const int quarter = warp & 3, half = (warp - 2) >> 2, col = threadIdx.x - 64;
+        const int cols = (bn / 2 + 31) / 32 * 32;
         int j = 0;
         for (int t = pair; t < n_tiles; t += n_pairs, ++j) {
             const int buf = j & 1, n0 = (t / n_m) * bn;
             const int m = (t % n_m) * 2 * I8_BM + rank * I8_BM + quarter * 32 + lane;
+            float* ws = ws_s + buf * I8_MAX_BN;
+            float* bs = bs_s + buf * I8_MAX_BN;
+            const bool in = col < bn && n0 + col < g.features;
+            ws[col] = in ? __ldg(g.w_scale + n0 + col) : 0.f;
+            bs[col] = in && g.bias ? i8_bias(g, n0 + col) : 0.f;
             const float xs = m < g.tokens ? __ldg(g.x_scale + m) : 0.f;
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up))) break;
+            // (a buffer is written again two tiles later, behind the barrier that every warp reaches when it is through with it)
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
+            const bool formed = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * I8_MAX_BN;
-            if (!g.gated) {
+            if (!formed) {
+            } else if (!g.gated) {
 #pragma unroll 1
-                for (int c = 0; c < bn; c += 16) {
-                    uint32_t r[16];
-                    float v[16];
-                    tmem_ld16(acc + c, r);
+                for (int c = half * cols; c < min(bn, (half + 1) * cols); c += 32) {
+                    uint32_t r[32];
+                    i8_tmem_ld32(acc + c, r);
                     if (m >= g.tokens || n0 + c >= g.features) continue;
-                    i8_values16(g, r, xs, n0 + c, v);
-                    i8_store16(g, m, n0 + c, v);
+                    i8_values32(r, xs, ws + c, bs + c);
+                    i8_store32(g, m, n0 + c, r);
                 }
             } else {
 #pragma unroll 1
-                for (int c = 0; c < bn / 2; c += 16) {
+                for (int c = half * 32; c < bn / 2; c += 64) {  // outputs
                     const int gc = (c / 64) * 128 + (c % 64);
-                    uint32_t gr[16], ur[16];
-                    float v[16], u[16];
-                    tmem_ld16(acc + gc, gr);
-                    tmem_ld16(acc + gc + 64, ur);
+                    uint32_t r[32], u[32];
+                    i8_tmem_ld32(acc + gc, r);
+                    i8_tmem_ld32(acc + gc + 64, u);
                     if (m >= g.tokens || n0 + gc >= g.features) continue;
-                    i8_values16(g, gr, xs, n0 + gc, v);
-                    i8_values16(g, ur, xs, n0 + gc + 64, u);
+                    i8_values32(r, xs, ws + gc, bs + gc);
+                    i8_values32(u, xs, ws + gc + 64, bs + gc + 64);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = i8_gate(g, v[e], u[e]);
-                    i8_store16(g, m, n0 / 2 + c, v);
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(i8_gate(g, __uint_as_float(r[e]), __uint_as_float(u[e])));
+                    i8_store32(g, m, n0 / 2 + c, r);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -513,12 +567,12 @@ extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, co
     if (many) {
         if (int rc = i8_map(&map_x, x, tokens, K, ldx, I8_BM)) return rc;
         if (int rc = i8_map(&map_w, w, features, K, ldw, bn / 2)) return rc;
-        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST;
+        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST + 4 * I8_MAX_BN * 4;
         static SsPerDevice opted;
         if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, smem, opted)) return rc;
         const int64_t n_tiles = (int64_t)((tokens + 255) / 256) * ((features + bn - 1) / bn);
         const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-        ss_launch_cluster_x(gemm_int8_many_kernel, dim3(2 * pairs), dim3(I8_THREADS), smem, stream, 2, map_x, map_w, g);
+        ss_launch_cluster_x(gemm_int8_many_kernel, dim3(2 * pairs), dim3(I8_MANY_THREADS), smem, stream, 2, map_x, map_w, g);
         return SS_LAUNCH_CHECK();
     }
     if (int rc = i8_map(&map_x, x, tokens, K, ldx, bn)) return rc;
