@@ -23,6 +23,7 @@
 #define I8_BM 128
 #define I8_BK 128       // K elements, and bytes of a row, in a stage
 #define I8_THREADS 192
+#define I8_MAX_BN 256
 
 struct Int8Args {
     const float* x_scale;  // [tokens]
@@ -100,43 +101,25 @@ __device__ __forceinline__ void i8_store4(const Int8Args& g, int token, int f, i
     }
 }
 
-// Four sums of a token's column, `apart` features from one another, out of the shared memory of all blocks of the cluster.
-__device__ __forceinline__ void i8_add_slices(const int* column, int fl, int apart, int n_sl, int (&sum)[4]) {
-    if (n_sl == 1) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = column[fl + e * apart];
-        return;
-    }
-    int part[8][4];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        if (s < n_sl) {
-            uint32_t remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(column + fl)), "r"(s));
-            if (apart == 1) {
-                asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(part[s][0]), "=r"(part[s][1]), "=r"(part[s][2]), "=r"(part[s][3]) : "r"(remote) : "memory");
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[s][e]) : "r"(remote + 4 * e * apart) : "memory");
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) part[s][e] = 0;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        sum[e] = ((part[0][e] + part[1][e]) + (part[2][e] + part[3][e])) + ((part[4][e] + part[5][e]) + (part[6][e] + part[7][e]));
+// sum at `to` in the shared memory of block `rank` of the cluster += v; four bytes of the transaction that `bar` there counts
+__device__ __forceinline__ void i8_add_remote(uint32_t to, uint32_t bar, int v) {
+    asm volatile("red.async.relaxed.cluster.shared::cluster.mbarrier::complete_tx::bytes.add.s32 [%0], %1, [%2];"
+                 ::"r"(to), "r"(v), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t i8_remote(const void* p, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(p)), "r"(rank));
+    return remote;
 }
 
 // ---------------------------------------------------------------- few tokens: the weights' bytes are the work
 //
 // The weights are the instruction's A (their rows fill its 128 lanes), the tokens its B (bn of them, a multiple of 16 up to
-// 256).  A block forms a tile of 128 features x bn tokens over one slice of K; the 1 to 8 slices of a tile are a thread-block
-// cluster along grid.z, whose blocks leave their sums in shared memory and add up the token columns rank, rank + slices, ...
-// of all of them.  Warp 0 (one lane) fetches, warp 1 issues the products, warps 2 to 5 write the result out.
+// 256).  A block forms a tile of 128 features x bn tokens over one slice of K.  The 1 to 8 slices of a tile are a thread-block
+// cluster along grid.z: token column c belongs to block c % slices, and every block adds its sums of the column into that
+// block's shared memory from its registers (red.async; whole numbers, so in any order), which counts the bytes on a barrier of its
+// own.  No block waits for another but for these sums.  Warp 0 (one lane) fetches, warp 1 issues the products, warps 2 to 5
+// write the result out.
 __global__ void __launch_bounds__(I8_THREADS)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Int8Args g) {
     extern __shared__ unsigned char smem_raw[];
@@ -146,75 +129,75 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);
     uint64_t* empty = full + stages;
     uint64_t* acc_ready = empty + stages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_ready + 1);
+    uint64_t* sums_ready = acc_ready + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_ready + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* xs_s = reinterpret_cast<float*>(full) + 64;  // [256], behind the barriers
+    // [own columns][128]: of a cluster's block behind the scales; alone over the ring, when all its stages have been used
+    int* sums = n_sl > 1 ? reinterpret_cast<int*>(xs_s + I8_MAX_BN) : reinterpret_cast<int*>(tiles);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t0 = blockIdx.x * bn, f0 = blockIdx.y * I8_BM;  // first token, first feature
+    const int live = min(bn, g.tokens - t0);                   // columns that hold tokens
+    const int rank = n_sl > 1 ? (int)cluster_rank() : 0;
+    const int mine = live > rank ? (live - 1 - rank) / n_sl + 1 : 0;  // columns rank, rank + slices, ...
     const int k_total = (g.K + I8_BK - 1) / I8_BK;
     const int per = (k_total + n_sl - 1) / n_sl;
     const int k_begin = blockIdx.z * per, k_iters = max(0, min(k_total, k_begin + per) - k_begin);
+    const int senders = (k_total + per - 1) / per;  // blocks that have any K
     const int ahead = min(stages, k_iters);
     const uint32_t tmem_cols = bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256;
-    const uint64_t once = l2_evict_first_policy();
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(acc_ready, 1);
+        mbar_init(sums_ready, 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (n_sl > 1) mbar_expect_tx(sums_ready, (uint32_t)(senders * mine * I8_BM * 4));
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
+        const uint64_t once = l2_evict_first_policy();
         for (int it = 0; it < ahead; ++it) {
             mbar_expect_tx(&full[it], stage_bytes);
             i8_load_once(tiles + it * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[it], once);
         }
+    } else if (warp >= 2 && n_sl > 1) {
+        for (int i = threadIdx.x - 64; i < mine * (I8_BM / 4); i += 128) reinterpret_cast<int4*>(sums)[i] = make_int4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    // nor do the scales and the bias of the four features (gated: four pairs) that a lane writes out: neighbours, or, where
-    // the output's rows do not start on four elements, one of each quarter of the tile
-    const int half = g.gated ? lane >> 4 : 0, of = g.gated ? lane & 15 : lane;
-    const int apart = (g.ldc & 3) == 0 ? 1 : g.gated ? 16 : 32, fl = apart == 1 ? of * 4 : of;
-    float ws[4], bs[4], ws2[4], bs2[4];
-    if (warp >= 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int f = f0 + fl + e * apart, f2 = f + 64;
-            ws[e] = f < g.features ? __ldg(g.w_scale + f) : 0.f;
-            bs[e] = g.bias && f < g.features ? i8_bias(g, f) : 0.f;
-            ws2[e] = g.gated && f2 < g.features ? __ldg(g.w_scale + f2) : 0.f;
-            bs2[e] = g.gated && g.bias && f2 < g.features ? i8_bias(g, f2) : 0.f;
+    __syncthreads();
+    if (n_sl > 1) {
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this block's sums are zero and its barriers stand
+        if (warp < 2) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t once = l2_evict_first_policy();
+            pdl_wait();
+            for (int it = 0; it < ahead; ++it)
+                i8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[it]);
+            int it = ahead;
+            for (; it < k_iters; ++it) {
+                const int s = it % stages;
+                if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, gave_up)) break;
+                mbar_expect_tx(&full[s], stage_bytes);
+                i8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[s], once);
+                i8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[s]);
+            }
+            if (*gave_up)
+                for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
         }
-    }
-    pdl_wait();
-    if (warp == 1) {
+        __syncwarp();
+    } else if (warp == 1) {
+        pdl_wait();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)), "r"(tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    } else if (threadIdx.x == 0) {
-        for (int it = 0; it < ahead; ++it)
-            i8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[it]);
-    } else if (warp >= 2) {
-        for (int i = threadIdx.x - 64; i < bn; i += 128) xs_s[i] = t0 + i < g.tokens ? __ldg(g.x_scale + t0 + i) : 0.f;
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    pdl_launch_dependents();
-    const uint32_t tmem_acc = *tmem_slot;
-    int* sums = reinterpret_cast<int*>(tiles);  // [bn][128], over the ring when all its stages have been used
-
-    if (warp == 0 && lane == 0) {
-        int it = ahead;
-        for (; it < k_iters; ++it) {
-            const int s = it % stages;
-            if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, gave_up)) break;
-            mbar_expect_tx(&full[s], stage_bytes);
-            i8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[s], once);
-            i8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[s]);
-        }
-        if (*gave_up)
-            for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
-    } else if (warp == 1) {
+        pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        asm volatile("bar.arrive 2, 160;" ::: "memory");  // the epilogue warps read the slot behind it
+        const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
         const uint32_t idesc = i8_idesc(I8_BM, bn);
         for (int it = 0; it < k_iters; ++it) {
             const int s = it % stages;
@@ -232,64 +215,78 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
         if (elect_one()) umma_commit(acc_ready);
         __syncwarp();
-    } else if (warp >= 2) {
-        const int quarter = warp & 3;  // warp w reads lanes 32 * (w % 4) .. + 31 of the accumulator
-        if (k_iters > 0) mbar_wait(acc_ready, 0, gave_up);
+    } else {
+        // nor do the scales and the bias of the four features (gated: four pairs) depend on the kernels in front that a lane writes
+        // out: neighbours, or, where the output's rows do not start on four elements, one of each quarter of the tile
+        const int quarter = warp & 3;
+        const int half = g.gated ? lane >> 4 : 0, of = g.gated ? lane & 15 : lane;
+        const int apart = (g.ldc & 3) == 0 ? 1 : g.gated ? 16 : 32, fl = apart == 1 ? of * 4 : of;
+        float ws[4], bs[4], ws2[4], bs2[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int f = f0 + fl + e * apart, f2 = f + 64;
+            ws[e] = f < g.features ? __ldg(g.w_scale + f) : 0.f;
+            bs[e] = g.bias && f < g.features ? i8_bias(g, f) : 0.f;
+            ws2[e] = g.gated && f2 < g.features ? __ldg(g.w_scale + f2) : 0.f;
+            bs2[e] = g.gated && g.bias && f2 < g.features ? i8_bias(g, f2) : 0.f;
+        }
+        if (n_sl > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        pdl_wait();  // the output may still be in use by the kernels in front, which also wrote the tokens' scales
+        for (int i = threadIdx.x - 64; i < live; i += 128) xs_s[i] = __ldg(g.x_scale + t0 + i);
+        asm volatile("bar.sync 2, 160;" ::: "memory");  // the scales are there, and the tensor memory's address
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int c = 0; c < bn; c += 16) {
-            uint32_t r[16];
+        const uint32_t acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(quarter * 32) << 16);
+        bool ok = mbar_wait(acc_ready, 0, gave_up);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (n_sl == 1) {
+            for (int c = 0; c < live; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(acc + c, r);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[(c + j) * I8_BM + quarter * 32 + lane] = (int)r[j];
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        } else {
             if (k_iters > 0) {
-                tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + c, r);
-            } else {
+                int owner = 0, at = 0;  // of column c: block c % slices, its column c / slices
+                for (int c = 0; c < live; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(acc + c, r);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = 0u;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sums[(c + j) * I8_BM + quarter * 32 + lane] = (int)r[j];
-        }
-        if (n_sl == 1) asm volatile("bar.sync 1, 128;" ::: "memory");
-    }
-    if (n_sl > 1) cluster_sync_all();  // every block's sums lie in its shared memory
-    if (warp >= 2) {
-        const int rank = n_sl > 1 ? (int)cluster_rank() : 0, q = warp & 3;
-        const int live = min(bn, g.tokens - t0);
-        // a warp takes two token columns (gated: each of its halves two) at a time, a lane four features of them; all loads of
-        // both columns are on the way before the first is added
-        const int step = g.gated ? 8 : 4;
-        for (int i = g.gated ? 2 * q + half : q;; i += 2 * step) {
-            const int c0 = rank + i * n_sl, c1 = c0 + step * n_sl;
-            if (c0 >= live) break;
-            int s0[4], s1[4];
-            i8_add_slices(sums + c0 * I8_BM, fl, apart, n_sl, s0);
-            if (c1 < live) i8_add_slices(sums + c1 * I8_BM, fl, apart, n_sl, s1);
-            int u0[4], u1[4];
-            if (g.gated) {
-                i8_add_slices(sums + c0 * I8_BM + 64, fl, apart, n_sl, u0);
-                if (c1 < live) i8_add_slices(sums + c1 * I8_BM + 64, fl, apart, n_sl, u1);
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int c = p ? c1 : c0;
-                if (c >= live) break;
-                const int (&a)[4] = p ? s1 : s0;
-                const int (&b)[4] = p ? u1 : u0;
-                const float xs = xs_s[c];
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = i8_value(a[e], xs, ws[e], bs[e]);
-                    if (g.gated) v[e] = i8_gate(g, v[e], i8_value(b[e], xs, ws2[e], bs2[e]));
+                    for (int j = 0; j < 16; ++j) {
+                        if (c + j < live)
+                            i8_add_remote(i8_remote(sums + at * I8_BM + quarter * 32 + lane, owner), i8_remote(sums_ready, owner), (int)r[j]);
+                        if (++owner == n_sl) { owner = 0; ++at; }
+                    }
                 }
-                i8_store4(g, t0 + c, (g.gated ? f0 / 2 : f0) + fl, apart, v);
             }
+            ok = mbar_wait(sums_ready, 0, gave_up) && ok;
+        }
+        // a warp takes a token column (gated: each of its halves one) at a time, a lane four features of it
+        for (int i = g.gated ? 2 * quarter + half : quarter; i < mine; i += g.gated ? 8 : 4) {
+            const int c = rank + i * n_sl;
+            const int* from = sums + i * I8_BM + fl;
+            const float xs = xs_s[c];
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = i8_value(from[e * apart], xs, ws[e], bs[e]);
+                if (g.gated) v[e] = i8_gate(g, v[e], i8_value(from[e * apart + 64], xs, ws2[e], bs2[e]));
+            }
+            i8_store4(g, t0 + c, (g.gated ? f0 / 2 : f0) + fl, apart, v);
         }
     }
-    if (n_sl > 1) cluster_sync_before_exit();  // nobody leaves while its sums are still being read
+    if (n_sl > 1) {  // nobody leaves while sums may still be on their way to it, whatever gave up
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+    }
     if (*gave_up && threadIdx.x == 0) atomicOr(g.err, SS_ERR_WAIT_LIMIT);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(tmem_cols));
     }
 }
@@ -303,7 +300,6 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 //   full[s]      in the leader: the bytes of both blocks' copies;     empty[s]     in each block: the products have read the stage
 //   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all sixteen epilogue warps are
 #define I8_PAIR_STAGES 6
-#define I8_MAX_BN 256
 #define I8_MANY_THREADS 320  // producer, issuer, eight epilogue warps
 
 __device__ __forceinline__ uint32_t i8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
@@ -350,32 +346,51 @@ __device__ __forceinline__ void i8_values32(uint32_t (&r)[32], float xs, const f
         r[e + 3] = __float_as_uint(i8_value((int)r[e + 3], xs, w.w, b.w));
     }
 }
-// 32 neighbouring outputs of a token.
-__device__ __forceinline__ void i8_store32(const Int8Args& g, int token, int f, const uint32_t (&r)[32]) {
-    const int64_t at = (int64_t)token * g.ldc + f;
-    if (f + 32 <= g.out_features && (g.ldc & 7) == 0) {
-        if (g.out_f32) {
-            uint4* dst = reinterpret_cast<uint4*>((float*)g.out + at);
+// A warp's 32 tokens x 32 outputs, a token a thread, through 2 KB of shared memory of the warp's own, so that it writes whole
+// 64-byte runs of a row instead of 16 bytes of 32 rows at a time (2,048 x 3,584 x 9,472: <TIME>).  Rows of 64 bytes lie in `stage`
+// with their four 16-byte pieces turned by (row / 2) % 4, which keeps both directions free of bank conflicts.
+__device__ __forceinline__ void i8_write_run(const Int8Args& g, unsigned char* stage, const uint32_t (&w)[16], int m0, int f, int width) {
+    const int lane = threadIdx.x & 31, size = g.out_f32 ? 4 : 2;
+    __syncwarp();
 #pragma unroll
-            for (int q = 0; q < 8; ++q) dst[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-        } else {
-            uint32_t p[16];
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    __syncwarp();
+    unsigned char* out = (unsigned char*)g.out;
+    if (f + width <= g.out_features && ((g.ldc * size) & 15) == 0) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-                p[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            uint4* dst = reinterpret_cast<uint4*>((bf16*)g.out + at);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), q = lane & 3;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
+            if (m0 + r < g.tokens) *reinterpret_cast<uint4*>(out + ((int64_t)(m0 + r) * g.ldc + f) * size + q * 16) = v;
         }
-        return;
+    } else {
+        for (int i = lane; i < 32 * width; i += 32) {
+            const int r = i / width, c = i - r * width, at = c * size;
+            const unsigned char* from = stage + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15);
+            if (m0 + r >= g.tokens || f + c >= g.out_features) continue;
+            const int64_t to = (int64_t)(m0 + r) * g.ldc + f + c;
+            if (g.out_f32) ((uint32_t*)out)[to] = *reinterpret_cast<const uint32_t*>(from);
+            else ((uint16_t*)out)[to] = *reinterpret_cast<const uint16_t*>(from);
+        }
     }
+}
+__device__ __forceinline__ void i8_write32(const Int8Args& g, unsigned char* stage, const uint32_t (&r)[32], int m0, int f) {
+    uint32_t w[16];
+    if (g.out_f32) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        if (f + e >= g.out_features) break;
-        if (g.out_f32) ((float*)g.out)[at + e] = __uint_as_float(r[e]);
-        else ((bf16*)g.out)[at + e] = __float2bfloat16_rn(__uint_as_float(r[e]));
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = r[16 * h + e];
+            i8_write_run(g, stage, w, m0, f + 16 * h, 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        i8_write_run(g, stage, w, m0, f, 32);
     }
 }
 
@@ -392,6 +407,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* ws_s = reinterpret_cast<float*>(full) + 64;  // [2][256] scales and [2][256] biases of a tile's features
     float* bs_s = ws_s + 2 * I8_MAX_BN;
+    unsigned char* runs = reinterpret_cast<unsigned char*>(bs_s + 2 * I8_MAX_BN);  // 2 KB for each epilogue warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();  // 0: the leader
@@ -406,24 +422,38 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();  // both blocks' barriers exist before either signals the other's
+    const int first = min(STAGES, pair < n_tiles ? k_iters : 0);  // stages of the first tile that are fetched ahead
+    const int bytes = 2 * (X_BYTES + (bn / 2) * I8_BK);
+    if (threadIdx.x == 0) {
+        // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
+        for (int k = 0; k < first; ++k) {
+            if (rank == 0) mbar_expect_tx(&full[k], bytes);
+            i8_load_pair(tiles + k * (X_BYTES + W_BYTES) + X_BYTES, &map_w, k * I8_BK, (pair / n_m) * bn + rank * (bn / 2), &full[k]);
+        }
+    }
     pdl_wait();
     if (warp == 1) {  // the same warp of both blocks allocates all 512 columns of the pair
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
+    } else if (threadIdx.x == 0) {
+        for (int k = 0; k < first; ++k)
+            i8_load_pair(tiles + k * (X_BYTES + W_BYTES), &map_x, k * I8_BK, (pair % n_m) * 2 * I8_BM + rank * I8_BM, &full[k]);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();  // both blocks' barriers exist before either signals the other's
+    cluster_sync_all();  // the tensor memory of both blocks has been taken
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    pdl_launch_dependents();
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0 && lane == 0) {
         int it = 0;
         bool ok = true;
-        const int bytes = 2 * (X_BYTES + (bn / 2) * I8_BK);
         for (int t = pair; t < n_tiles && ok; t += n_pairs) {
             const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * (bn / 2);
             for (int k = 0; k < k_iters; ++k, ++it) {
+                if (it < first) continue;
                 const int s = it % STAGES;
                 if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, gave_up)) { ok = false; break; }
                 if (rank == 0) mbar_expect_tx(&full[s], bytes);
@@ -463,6 +493,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         // warps 2 to 5 write out the first half of a tile's columns, warps 6 to 9 the second, each its quarter of the rows
         const int quarter = warp & 3, half = (warp - 2) >> 2, col = threadIdx.x - 64;
         const int cols = (bn / 2 + 31) / 32 * 32;
+        unsigned char* stage = runs + (warp - 2) * 2048;
         int j = 0;
         for (int t = pair; t < n_tiles; t += n_pairs, ++j) {
             const int buf = j & 1, n0 = (t / n_m) * bn;
@@ -485,9 +516,8 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 for (int c = half * cols; c < min(bn, (half + 1) * cols); c += 32) {
                     uint32_t r[32];
                     i8_tmem_ld32(acc + c, r);
-                    if (m >= g.tokens || n0 + c >= g.features) continue;
                     i8_values32(r, xs, ws + c, bs + c);
-                    i8_store32(g, m, n0 + c, r);
+                    i8_write32(g, stage, r, m - lane, n0 + c);
                 }
             } else {
 #pragma unroll 1
@@ -496,12 +526,11 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     uint32_t r[32], u[32];
                     i8_tmem_ld32(acc + gc, r);
                     i8_tmem_ld32(acc + gc + 64, u);
-                    if (m >= g.tokens || n0 + gc >= g.features) continue;
                     i8_values32(r, xs, ws + gc, bs + gc);
                     i8_values32(u, xs, ws + gc + 64, bs + gc + 64);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(i8_gate(g, __uint_as_float(r[e]), __uint_as_float(u[e])));
-                    i8_store32(g, m, n0 / 2 + c, r);
+                    i8_write32(g, stage, r, m - lane, n0 / 2 + c);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -545,20 +574,20 @@ static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
 }
 
 #define I8_SMEM_MAX 232448  // 227 KB
-#define I8_SMEM_REST 2560   // alignment, barriers, the tokens' scales
+#define I8_SMEM_REST 2560   // alignment, barriers, scales
 
 // x [tokens, K] and w [features, K] int8 with row strides ldx, ldw (multiples of 16 bytes, bases on 16 bytes), K <= 133,143.
 // gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
-// many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `two` blocks an SM wanted (0, 1).
+// many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for.
 // many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
 extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
                             const void* bias, int bias_f32, void* out, int64_t ldc, int out_f32, int tokens, int features, int K,
-                            int gated, int out_features, int many, int bn, int slices, int two, int* err, cudaStream_t stream) {
+                            int gated, int out_features, int many, int bn, int slices, int per_sm, int* err, cudaStream_t stream) {
     if (tokens <= 0 || features <= 0) return 0;
     if (K <= 0 || K > 133143 || ldx % 16 || ldw % 16 || ldx < K || ldw < K) return -2003;
     if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return -2004;
     if (gated ? (features % 128 || out_features > features / 2) : out_features != features) return -2005;
-    if (bn < 16 || bn > I8_MAX_BN || bn % (many ? 32 : 16) || (many && gated && bn % 128) || (!many && (slices < 1 || slices > 8))) return -2006;
+    if (bn < 16 || bn > I8_MAX_BN || bn % (many ? 32 : 16) || (many && gated && bn % 128) || (!many && (slices < 1 || slices > 8 || per_sm < 1 || per_sm > 4))) return -2006;
     Int8Args g = {};
     g.x_scale = x_scale; g.w_scale = w_scale; g.bias = bias; g.out = out; g.err = err; g.ldc = ldc;
     g.tokens = tokens; g.features = features; g.K = K; g.out_features = out_features;
@@ -567,7 +596,7 @@ extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, co
     if (many) {
         if (int rc = i8_map(&map_x, x, tokens, K, ldx, I8_BM)) return rc;
         if (int rc = i8_map(&map_w, w, features, K, ldw, bn / 2)) return rc;
-        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST + 4 * I8_MAX_BN * 4;
+        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
         static SsPerDevice opted;
         if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, smem, opted)) return rc;
         const int64_t n_tiles = (int64_t)((tokens + 255) / 256) * ((features + bn - 1) / bn);
@@ -580,12 +609,13 @@ extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, co
     static SsPerDevice opted;
     if (int rc = ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return rc;
     const int stage = I8_BM * I8_BK + bn * I8_BK;
-    const int room = two ? I8_SMEM_MAX / 2 - 1024 : I8_SMEM_MAX;
-    int stages = (room - I8_SMEM_REST) / stage;
-    const int needed = (bn * I8_BM * 4 + stage - 1) / stage;  // the ring also holds the sums
+    const int rest = I8_SMEM_REST + (slices > 1 ? (bn + slices - 1) / slices * I8_BM * 4 : 0);  // a cluster's blocks: the columns they own
+    const int room = per_sm > 1 ? 233472 / per_sm - 1024 : I8_SMEM_MAX;  // (228 KB an SM, 1 KB of it a block's own)
+    int stages = (room - rest) / stage;
+    const int needed = slices > 1 ? 2 : (bn * I8_BM * 4 + stage - 1) / stage;  // alone, the ring also holds the sums
     stages = stages < needed ? needed : stages > 12 ? 12 : stages;
     g.stages = stages;
-    const int smem = stages * stage + I8_SMEM_REST;
+    const int smem = stages * stage + rest;
     if (smem > I8_SMEM_MAX) return -2007;
     const dim3 grid((tokens + bn - 1) / bn, (features + I8_BM - 1) / I8_BM, slices);
     if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, stream, slices, map_w, map_x, g);

@@ -149,15 +149,15 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
 
 @functools.lru_cache(maxsize=None)
 def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False) -> tuple[int, int, int, int]:
-    """(many, tile, K slices, two) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
-    (tokens of the first, features of the second), and for the first the slices of K and whether two blocks share an SM."""
+    """(many, tile, K slices, blocks an SM) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
+    (tokens of the first, features of the second), and for the first the slices of K and how many blocks an SM the ring is sized for."""
     k_iters = (k + 127) // 128
     if tokens <= 256:
         tile = max(16, (tokens + 15) // 16 * 16)
         tiles = (features + 127) // 128
         slices = max(1, min(8, k_iters, sms // tiles)) if tiles < sms else 1
-        return 0, tile, slices, int(tile <= 32)
-    return 1, 256, 1, 0
+        return 0, tile, slices, 2 if tile <= 32 else 1
+    return 1, 256, 1, 1
 
 
 def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype: torch.dtype, gated: bool, columns: int | None,
@@ -186,10 +186,10 @@ def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype
         bias_f32 = int(bias.dtype == _F32)
     if tokens == 0 or columns == 0:
         return out
-    many, tile, slices, two = plan or int8_plan(tokens, features, k, sm_count(out.device), gated)
+    many, tile, slices, per_sm = plan or int8_plan(tokens, features, k, sm_count(out.device), gated)
     _check(gemm_library().ss_gemm_int8(x.values.data_ptr(), ldx, x.scales.data_ptr(), weight.values.data_ptr(), ldw, weight.scales.data_ptr(),
                                        _ptr(bias), bias_f32, out.data_ptr(), columns, out_f32, tokens, features, k, gated, columns,
-                                       many, tile, slices, two, error_word(out.device).data_ptr(), _stream()), what)
+                                       many, tile, slices, per_sm, error_word(out.device).data_ptr(), _stream()), what)
     return out
 
 

@@ -185,8 +185,8 @@ def test_linear(tokens, k, features):
 
 def plans(tokens, k, gated):
     few = max(16, min(256, (tokens + 15) // 16 * 16))
-    out = [(0, tile, slices, two) for tile in {16, 32, 48, few, 128, 256} for slices in (1, 2, 5, 8) for two in (0, 1) if tile <= 2 * few]
-    return out + [(1, tile, 1, 0) for tile in ((128, 256) if gated else (32, 96, 128, 224, 256))]
+    out = [(0, tile, slices, per_sm) for tile in {16, 32, 48, few, 128, 256} for slices in (1, 2, 5, 8) for per_sm in (1, 2, 4) if tile <= 2 * few]
+    return out + [(1, tile, 1, 1) for tile in ((128, 256) if gated else (32, 96, 128, 224, 256))]
 
 
 @pytest.mark.parametrize("tokens, k, features", [(1, 200, 130), (19, 1500, 515), (150, 3584, 700), (515, 900, 1024)])
@@ -393,8 +393,8 @@ def test_refusals():
                  lambda: o.linear_int8(good, w, torch.zeros(127, device=DEV)), lambda: o.linear_int8(good, w, torch.zeros(128, device=DEV).half()),
                  lambda: o.linear_int8(good, w, None, torch.float16), lambda: o.gate_up_swiglu_int8(good, good),
                  lambda: o.gate_up_swiglu_int8(good, w, features=65), lambda: o.stack_gate_up(x, x[:2]),
-                 lambda: o.linear_int8(good, w, plan=(0, 24, 1, 0)), lambda: o.linear_int8(good, w, plan=(0, 16, 9, 0)),
-                 lambda: o.linear_int8(good, w, plan=(1, 48, 1, 0)), lambda: o.gate_up_swiglu_int8(good, w, plan=(1, 96, 1, 0))):
+                 lambda: o.linear_int8(good, w, plan=(0, 24, 1, 1)), lambda: o.linear_int8(good, w, plan=(0, 16, 9, 1)),
+                 lambda: o.linear_int8(good, w, plan=(1, 48, 1, 1)), lambda: o.gate_up_swiglu_int8(good, w, plan=(1, 96, 1, 1))):
         with pytest.raises(err):
             call()
     assert o.linear_int8(o.quantize_rows_int8(torch.empty(0, 64, device=DEV)), w).shape == (0, 128)
