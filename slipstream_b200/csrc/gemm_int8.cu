@@ -178,13 +178,16 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             pdl_wait();
             for (int it = 0; it < ahead; ++it)
                 i8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[it]);
-            int it = ahead;
+            // (a stage's number and its parity are counted, not divided out: the loops of this thread and of the issuer are what a
+            // step takes where its products are small)
+            int it = ahead, s = 0;
+            uint32_t parity = 0;
             for (; it < k_iters; ++it) {
-                const int s = it % stages;
-                if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, gave_up)) break;
+                if (!mbar_wait(&empty[s], parity, gave_up)) break;
                 mbar_expect_tx(&full[s], stage_bytes);
                 i8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[s], once);
                 i8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[s]);
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
             if (*gave_up)
                 for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
@@ -199,12 +202,14 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         asm volatile("bar.arrive 2, 160;" ::: "memory");  // the epilogue warps read the slot behind it
         const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
         const uint32_t idesc = i8_idesc(I8_BM, bn);
+        const uint64_t w_first = smem_desc(tiles), x_first = smem_desc(tiles + w_bytes);
+        const uint32_t stage_step = (uint32_t)stage_bytes >> 4;  // of a descriptor's address
+        int s = 0;
+        uint32_t parity = 0;
         for (int it = 0; it < k_iters; ++it) {
-            const int s = it % stages;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / stages) & 1, gave_up))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], parity, gave_up))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            unsigned char* w_tile = tiles + s * stage_bytes;
-            const uint64_t w_desc = smem_desc(w_tile), x_desc = smem_desc(w_tile + w_bytes);
+            const uint64_t w_desc = w_first + s * stage_step, x_desc = x_first + s * stage_step;
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < I8_BK / 32; ++kk)  // 32 bytes further along the swizzled row
@@ -212,6 +217,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 umma_commit(&empty[s]);
             }
             __syncwarp();
+            if (++s == stages) { s = 0; parity ^= 1; }
         }
         if (elect_one()) umma_commit(acc_ready);
         __syncwarp();
@@ -299,7 +305,6 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 // double-buffered (2 x 256 columns): the eight epilogue warps of each block write a tile out while the next one is formed.
 //   full[s]      in the leader: the bytes of both blocks' copies;     empty[s]     in each block: the products have read the stage
 //   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all sixteen epilogue warps are
-#define I8_PAIR_STAGES 6
 #define I8_MANY_THREADS 320  // producer, issuer, eight epilogue warps
 
 __device__ __forceinline__ uint32_t i8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
@@ -396,12 +401,13 @@ __device__ __forceinline__ void i8_write32(const Int8Args& g, unsigned char* sta
 
 __global__ void __launch_bounds__(I8_MANY_THREADS)
 gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Int8Args g) {
-    constexpr int X_BYTES = I8_BM * I8_BK, W_BYTES = I8_BM * I8_BK, STAGES = I8_PAIR_STAGES;  // this block's halves
+    constexpr int X_BYTES = I8_BM * I8_BK;
+    const int stages = g.stages, stage_bytes = X_BYTES + g.bn / 2 * I8_BK;  // this block's halves
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + STAGES * (X_BYTES + W_BYTES));
-    uint64_t* empty = full + STAGES;
-    uint64_t* acc_full = empty + STAGES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);
+    uint64_t* empty = full + stages;
+    uint64_t* acc_full = empty + stages;
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -417,20 +423,20 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const int k_iters = (g.K + I8_BK - 1) / I8_BK;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 16); }
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // both blocks' barriers exist before either signals the other's
-    const int first = min(STAGES, pair < n_tiles ? k_iters : 0);  // stages of the first tile that are fetched ahead
+    const int first = min(stages, pair < n_tiles ? k_iters : 0);  // stages of the first tile that are fetched ahead
     const int bytes = 2 * (X_BYTES + (bn / 2) * I8_BK);
     if (threadIdx.x == 0) {
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
         for (int k = 0; k < first; ++k) {
             if (rank == 0) mbar_expect_tx(&full[k], bytes);
-            i8_load_pair(tiles + k * (X_BYTES + W_BYTES) + X_BYTES, &map_w, k * I8_BK, (pair / n_m) * bn + rank * (bn / 2), &full[k]);
+            i8_load_pair(tiles + k * stage_bytes + X_BYTES, &map_w, k * I8_BK, (pair / n_m) * bn + rank * (bn / 2), &full[k]);
         }
     }
     pdl_wait();
@@ -440,7 +446,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
     } else if (threadIdx.x == 0) {
         for (int k = 0; k < first; ++k)
-            i8_load_pair(tiles + k * (X_BYTES + W_BYTES), &map_x, k * I8_BK, (pair % n_m) * 2 * I8_BM + rank * I8_BM, &full[k]);
+            i8_load_pair(tiles + k * stage_bytes, &map_x, k * I8_BK, (pair % n_m) * 2 * I8_BM + rank * I8_BM, &full[k]);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // the tensor memory of both blocks has been taken
@@ -448,43 +454,48 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0 && lane == 0) {
-        int it = 0;
+        int it = 0, s = 0;
+        uint32_t parity = 1;  // of the round before the first: the stages are free
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += n_pairs) {
             const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * (bn / 2);
             for (int k = 0; k < k_iters; ++k, ++it) {
-                if (it < first) continue;
-                const int s = it % STAGES;
-                if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, gave_up)) { ok = false; break; }
-                if (rank == 0) mbar_expect_tx(&full[s], bytes);
-                unsigned char* x_tile = tiles + s * (X_BYTES + W_BYTES);
-                i8_load_pair(x_tile, &map_x, k * I8_BK, m0, &full[s]);
-                i8_load_pair(x_tile + X_BYTES, &map_w, k * I8_BK, n0, &full[s]);
+                if (it >= first) {
+                    if (!mbar_wait(&empty[s], parity, gave_up)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(&full[s], bytes);
+                    unsigned char* x_tile = tiles + s * stage_bytes;
+                    i8_load_pair(x_tile, &map_x, k * I8_BK, m0, &full[s]);
+                    i8_load_pair(x_tile + X_BYTES, &map_w, k * I8_BK, n0, &full[s]);
+                }
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
         }
         if (*gave_up && rank == 0)
-            for (int back = max(0, it - STAGES); back < it; ++back) i8_drain(&full[back % STAGES], (back / STAGES) & 1);
+            for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
     } else if (warp == 1 && rank == 0) {
         const uint32_t idesc = i8_idesc(2 * I8_BM, bn);
-        int it = 0, j = 0;
+        const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + X_BYTES);
+        const uint32_t stage_step = (uint32_t)stage_bytes >> 4;  // of a descriptor's address
+        int j = 0, s = 0;
+        uint32_t parity = 0;
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += n_pairs, ++j) {
             const int buf = j & 1;
             if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1, gave_up))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int k = 0; k < k_iters; ++k, ++it) {
-                const int s = it % STAGES;
-                if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / STAGES) & 1, gave_up))) { ok = false; break; }
+            const uint32_t acc = tmem + buf * I8_MAX_BN;
+            for (int k = 0; k < k_iters; ++k) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&full[s], parity, gave_up))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                unsigned char* x_tile = tiles + s * (X_BYTES + W_BYTES);
-                const uint64_t x_desc = smem_desc(x_tile), w_desc = smem_desc(x_tile + X_BYTES);
+                const uint64_t x_desc = x_first + s * stage_step, w_desc = w_first + s * stage_step;
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < I8_BK / 32; ++kk)
-                        umma_i8_pair(tmem + buf * I8_MAX_BN, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, (k | kk) != 0);
+                        umma_i8_pair(acc, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, (k | kk) != 0);
                     i8_commit_pair(&empty[s]);
                 }
                 __syncwarp();
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
             if (elect_one()) i8_commit_pair(&acc_full[buf]);
             __syncwarp();
@@ -596,9 +607,13 @@ extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, co
     if (many) {
         if (int rc = i8_map(&map_x, x, tokens, K, ldx, I8_BM)) return rc;
         if (int rc = i8_map(&map_w, w, features, K, ldw, bn / 2)) return rc;
-        constexpr int smem = I8_PAIR_STAGES * 2 * I8_BM * I8_BK + I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
+        constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
+        const int stage = I8_BM * I8_BK + bn / 2 * I8_BK;
+        g.stages = (I8_SMEM_MAX - rest) / stage;
+        g.stages = g.stages > 12 ? 12 : g.stages;
+        const int smem = g.stages * stage + rest;
         static SsPerDevice opted;
-        if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, smem, opted)) return rc;
+        if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, I8_SMEM_MAX, opted)) return rc;
         const int64_t n_tiles = (int64_t)((tokens + 255) / 256) * ((features + bn - 1) / bn);
         const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
         ss_launch_cluster_x(gemm_int8_many_kernel, dim3(2 * pairs), dim3(I8_MANY_THREADS), smem, stream, 2, map_x, map_w, g);
