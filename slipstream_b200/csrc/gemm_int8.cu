@@ -37,6 +37,7 @@ struct Int8Args {
     int out_f32, bias_f32, gated;
     int bn;                // few tokens: the tokens of a tile; many tokens: the features of a tile
     int stages, slices;
+    int wide_copies;        // many tokens: the two steps of a stage come in one copy (K is a multiple of 128)
 };
 
 __device__ __forceinline__ void i8_load(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
@@ -314,6 +315,22 @@ __device__ __forceinline__ void i8_load_pair(void* dst, const CUtensorMap* map, 
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(s_addr(dst)), "l"(map), "r"(i8_leader(bar)), "r"(k), "r"(row) : "memory");
 }
+// two steps of K in one copy: the map's third coordinate counts steps
+__device__ __forceinline__ void i8_load_pair_steps(void* dst, const CUtensorMap* map, int step, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(s_addr(dst)), "l"(map), "r"(i8_leader(bar)), "r"(0), "r"(row), "r"(step) : "memory");
+}
+// `rows` rows of the steps of K of stage k, as [step][row][128 bytes]
+template <int STEPS>
+__device__ __forceinline__ void i8_load_stage(unsigned char* dst, const CUtensorMap* map, bool wide, int k, int row, int rows, uint64_t* bar) {
+    if (STEPS == 2 && wide) {
+        i8_load_pair_steps(dst, map, 2 * k, row, bar);
+        return;
+    }
+    i8_load_pair(dst, map, STEPS * k * I8_BK, row, bar);
+    if (STEPS == 2) i8_load_pair(dst + rows * I8_BK, map, (2 * k + 1) * I8_BK, row, bar);
+}
 __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -399,10 +416,11 @@ __device__ __forceinline__ void i8_write32(const Int8Args& g, unsigned char* sta
     }
 }
 
+template <int STEPS>
 __global__ void __launch_bounds__(I8_MANY_THREADS)
 gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Int8Args g) {
-    constexpr int X_BYTES = I8_BM * I8_BK;
-    const int stages = g.stages, stage_bytes = X_BYTES + g.bn / 2 * I8_BK;  // this block's halves
+    constexpr int x_bytes = STEPS * I8_BM * I8_BK;
+    const int w_rows = g.bn / 2, stages = g.stages, stage_bytes = x_bytes + STEPS * w_rows * I8_BK;  // this block's halves
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);
@@ -420,7 +438,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const int bn = g.bn;  // a multiple of 32
     const int n_m = (g.tokens + 2 * I8_BM - 1) / (2 * I8_BM), n_tiles = n_m * ((g.features + bn - 1) / bn);
-    const int k_iters = (g.K + I8_BK - 1) / I8_BK;
+    const int k_steps = (g.K + I8_BK - 1) / I8_BK, k_iters = (k_steps + STEPS - 1) / STEPS;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -431,12 +449,12 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // both blocks' barriers exist before either signals the other's
     const int first = min(stages, pair < n_tiles ? k_iters : 0);  // stages of the first tile that are fetched ahead
-    const int bytes = 2 * (X_BYTES + (bn / 2) * I8_BK);
+    const int bytes = 2 * stage_bytes;  // of both blocks
     if (threadIdx.x == 0) {
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
         for (int k = 0; k < first; ++k) {
             if (rank == 0) mbar_expect_tx(&full[k], bytes);
-            i8_load_pair(tiles + k * stage_bytes + X_BYTES, &map_w, k * I8_BK, (pair / n_m) * bn + rank * (bn / 2), &full[k]);
+            i8_load_stage<STEPS>(tiles + k * stage_bytes + x_bytes, &map_w, g.wide_copies, k, (pair / n_m) * bn + rank * w_rows, w_rows, &full[k]);
         }
     }
     pdl_wait();
@@ -446,7 +464,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
     } else if (threadIdx.x == 0) {
         for (int k = 0; k < first; ++k)
-            i8_load_pair(tiles + k * stage_bytes, &map_x, k * I8_BK, (pair % n_m) * 2 * I8_BM + rank * I8_BM, &full[k]);
+            i8_load_stage<STEPS>(tiles + k * stage_bytes, &map_x, g.wide_copies, k, (pair % n_m) * 2 * I8_BM + rank * I8_BM, I8_BM, &full[k]);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // the tensor memory of both blocks has been taken
@@ -458,14 +476,14 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         uint32_t parity = 1;  // of the round before the first: the stages are free
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-            const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * (bn / 2);
+            const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * w_rows;
             for (int k = 0; k < k_iters; ++k, ++it) {
                 if (it >= first) {
                     if (!mbar_wait(&empty[s], parity, gave_up)) { ok = false; break; }
                     if (rank == 0) mbar_expect_tx(&full[s], bytes);
                     unsigned char* x_tile = tiles + s * stage_bytes;
-                    i8_load_pair(x_tile, &map_x, k * I8_BK, m0, &full[s]);
-                    i8_load_pair(x_tile + X_BYTES, &map_w, k * I8_BK, n0, &full[s]);
+                    i8_load_stage<STEPS>(x_tile, &map_x, g.wide_copies, k, m0, I8_BM, &full[s]);
+                    i8_load_stage<STEPS>(x_tile + x_bytes, &map_w, g.wide_copies, k, n0, w_rows, &full[s]);
                 }
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
@@ -474,8 +492,9 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
     } else if (warp == 1 && rank == 0) {
         const uint32_t idesc = i8_idesc(2 * I8_BM, bn);
-        const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + X_BYTES);
+        const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + x_bytes);
         const uint32_t stage_step = (uint32_t)stage_bytes >> 4;  // of a descriptor's address
+        const uint32_t w_step = (uint32_t)(w_rows * I8_BK) >> 4;
         int j = 0, s = 0;
         uint32_t parity = 0;
         bool ok = true;
@@ -492,6 +511,11 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 #pragma unroll
                     for (int kk = 0; kk < I8_BK / 32; ++kk)
                         umma_i8_pair(acc, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, (k | kk) != 0);
+                    if (STEPS == 2 && 2 * k + 1 < k_steps) {
+#pragma unroll
+                        for (int kk = 0; kk < I8_BK / 32; ++kk)
+                            umma_i8_pair(acc, x_desc + (uint64_t)(I8_BM * I8_BK / 16 + kk * 2), w_desc + (uint64_t)(w_step + kk * 2), idesc, 1);
+                    }
                     i8_commit_pair(&empty[s]);
                 }
                 __syncwarp();
@@ -564,8 +588,9 @@ typedef CUresult (*I8Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// int8 matrix [rows, K] with row stride ld bytes; box = 128 x box_rows.
-static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows) {
+// int8 matrix [rows, K] with row stride ld bytes; box = 128 x box_rows, or, with `steps` (K a multiple of 128), two steps of K:
+// the matrix as [K / 128][rows][128], box = 128 x box_rows x 2.
+static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, bool steps = false) {
     static I8Encode enc = nullptr;
     if (!enc) {
         void* p = nullptr;
@@ -574,11 +599,11 @@ static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
             return -2001;
         enc = (I8Encode)p;
     }
-    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld};
-    cuuint32_t box[2] = {I8_BK, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+    cuuint64_t dims[3] = {(cuuint64_t)(steps ? I8_BK : K), (cuuint64_t)rows, (cuuint64_t)(K / I8_BK)};
+    cuuint64_t strides[2] = {(cuuint64_t)ld, I8_BK};
+    cuuint32_t box[3] = {I8_BK, (cuuint32_t)box_rows, 2};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, steps ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : -2002;
@@ -586,6 +611,23 @@ static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
 
 #define I8_SMEM_MAX 232448  // 227 KB
 #define I8_SMEM_REST 2560   // alignment, barriers, scales
+
+template <int STEPS>
+static int launch_many(const void* x, int64_t ldx, const void* w, int64_t ldw, Int8Args& g, cudaStream_t stream) {
+    CUtensorMap map_x, map_w;
+    g.wide_copies = STEPS == 2 && g.K % I8_BK == 0;
+    if (int rc = i8_map(&map_x, x, g.tokens, g.K, ldx, I8_BM, g.wide_copies)) return rc;
+    if (int rc = i8_map(&map_w, w, g.features, g.K, ldw, g.bn / 2, g.wide_copies)) return rc;
+    static SsPerDevice opted;
+    if (int rc = ss_opt_in_smem(gemm_int8_many_kernel<STEPS>, I8_SMEM_MAX, opted)) return rc;
+    constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
+    const int stage = STEPS * (I8_BM + g.bn / 2) * I8_BK;
+    g.stages = (I8_SMEM_MAX - rest) / stage;
+    const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + g.bn - 1) / g.bn);
+    const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
+    ss_launch_cluster_x(gemm_int8_many_kernel<STEPS>, dim3(2 * pairs), dim3(I8_MANY_THREADS), g.stages * stage + rest, stream, 2, map_x, map_w, g);
+    return SS_LAUNCH_CHECK();
+}
 
 // x [tokens, K] and w [features, K] int8 with row strides ldx, ldw (multiples of 16 bytes, bases on 16 bytes), K <= 133,143.
 // gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
@@ -605,19 +647,7 @@ extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, co
     g.out_f32 = out_f32; g.bias_f32 = bias_f32; g.gated = gated; g.bn = bn; g.slices = slices;
     CUtensorMap map_x, map_w;
     if (many) {
-        if (int rc = i8_map(&map_x, x, tokens, K, ldx, I8_BM)) return rc;
-        if (int rc = i8_map(&map_w, w, features, K, ldw, bn / 2)) return rc;
-        constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
-        const int stage = I8_BM * I8_BK + bn / 2 * I8_BK;
-        g.stages = (I8_SMEM_MAX - rest) / stage;
-        g.stages = g.stages > 12 ? 12 : g.stages;
-        const int smem = g.stages * stage + rest;
-        static SsPerDevice opted;
-        if (int rc = ss_opt_in_smem(gemm_int8_many_kernel, I8_SMEM_MAX, opted)) return rc;
-        const int64_t n_tiles = (int64_t)((tokens + 255) / 256) * ((features + bn - 1) / bn);
-        const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-        ss_launch_cluster_x(gemm_int8_many_kernel, dim3(2 * pairs), dim3(I8_MANY_THREADS), smem, stream, 2, map_x, map_w, g);
-        return SS_LAUNCH_CHECK();
+        return bn <= 192 ? launch_many<2>(x, ldx, w, ldw, g, stream) : launch_many<1>(x, ldx, w, ldw, g, stream);
     }
     if (int rc = i8_map(&map_x, x, tokens, K, ldx, bn)) return rc;
     if (int rc = i8_map(&map_w, w, features, K, ldw, I8_BM)) return rc;
