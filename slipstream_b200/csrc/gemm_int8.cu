@@ -609,15 +609,41 @@ static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
     return r == CUDA_SUCCESS ? 0 : -2002;
 }
 
-#define I8_SMEM_MAX 232448  // 227 KB
+#define I8_SMEM_MAX 232448  // 227 KB of a block
+#define I8_SMEM_SM 233472   // 228 KB of an SM, 1 KB of it each block's own
 #define I8_SMEM_REST 2560   // alignment, barriers, scales
 
+// How many clusters of `n` blocks of the kernel for few tokens run at the same time where the ring is sized for `per_sm` blocks an
+// SM (n = 1: blocks).
+extern "C" int ss_gemm_int8_resident(int n, int per_sm) {
+    static SsPerDevice opted;
+    if (n < 1 || n > 8 || per_sm < 1 || ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return 0;
+    return ss_resident_clusters(gemm_int8_few_kernel, I8_THREADS, per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX, n);
+}
+
+// The arguments of a product as one record: a call through ctypes takes 2.0 us for 22 arguments and 0.6 us for the address of a
+// packed record.
+struct Int8Call {
+    const void* x;  // [tokens, K] int8, row stride ldx
+    int64_t ldx;
+    const float* x_scale;
+    const void* w;  // [features, K] int8, row stride ldw
+    int64_t ldw;
+    const float* w_scale;
+    const void* bias;
+    int64_t bias_f32;
+    void* out;  // [tokens, ldc]
+    int64_t ldc, out_f32, tokens, features, K, gated, out_features, many, bn, slices, per_sm;
+    int* err;
+    cudaStream_t stream;
+};
+
 template <int STEPS>
-static int launch_many(const void* x, int64_t ldx, const void* w, int64_t ldw, Int8Args& g, cudaStream_t stream) {
+static int launch_many(const Int8Call& c, Int8Args& g) {
     CUtensorMap map_x, map_w;
     g.wide_copies = STEPS == 2 && g.K % I8_BK == 0;
-    if (int rc = i8_map(&map_x, x, g.tokens, g.K, ldx, I8_BM, g.wide_copies)) return rc;
-    if (int rc = i8_map(&map_w, w, g.features, g.K, ldw, g.bn / 2, g.wide_copies)) return rc;
+    if (int rc = i8_map(&map_x, c.x, g.tokens, g.K, c.ldx, I8_BM, g.wide_copies)) return rc;
+    if (int rc = i8_map(&map_w, c.w, g.features, g.K, c.ldw, g.bn / 2, g.wide_copies)) return rc;
     static SsPerDevice opted;
     if (int rc = ss_opt_in_smem(gemm_int8_many_kernel<STEPS>, I8_SMEM_MAX, opted)) return rc;
     constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
@@ -625,45 +651,44 @@ static int launch_many(const void* x, int64_t ldx, const void* w, int64_t ldw, I
     g.stages = (I8_SMEM_MAX - rest) / stage;
     const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + g.bn - 1) / g.bn);
     const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-    ss_launch_cluster_x(gemm_int8_many_kernel<STEPS>, dim3(2 * pairs), dim3(I8_MANY_THREADS), g.stages * stage + rest, stream, 2, map_x, map_w, g);
+    ss_launch_cluster_x(gemm_int8_many_kernel<STEPS>, dim3(2 * pairs), dim3(I8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
     return SS_LAUNCH_CHECK();
 }
 
-// x [tokens, K] and w [features, K] int8 with row strides ldx, ldw (multiples of 16 bytes, bases on 16 bytes), K <= 133,143.
+// Row strides are multiples of 16 bytes and bases stand on 16 bytes; K <= 133,143.
 // gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
 // many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for.
 // many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
-extern "C" int ss_gemm_int8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
-                            const void* bias, int bias_f32, void* out, int64_t ldc, int out_f32, int tokens, int features, int K,
-                            int gated, int out_features, int many, int bn, int slices, int per_sm, int* err, cudaStream_t stream) {
-    if (tokens <= 0 || features <= 0) return 0;
-    if (K <= 0 || K > 133143 || ldx % 16 || ldw % 16 || ldx < K || ldw < K) return -2003;
-    if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return -2004;
-    if (gated ? (features % 128 || out_features > features / 2) : out_features != features) return -2005;
-    if (bn < 16 || bn > I8_MAX_BN || bn % (many ? 32 : 16) || (many && gated && bn % 128) || (!many && (slices < 1 || slices > 8 || per_sm < 1 || per_sm > 4))) return -2006;
+extern "C" int ss_gemm_int8(const Int8Call* call) {
+    const Int8Call& c = *call;
+    if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
+    if (c.tokens > INT32_MAX - 256 || c.features > INT32_MAX - 256 || c.K <= 0 || c.K > 133143 || c.ldx % 16 || c.ldw % 16 || c.ldx < c.K || c.ldw < c.K) return -2003;
+    if (((uintptr_t)c.x & 15) || ((uintptr_t)c.w & 15) || ((uintptr_t)c.out & 15)) return -2004;
+    if (c.gated ? (c.features % 128 || c.out_features > c.features / 2) : c.out_features != c.features) return -2005;
+    const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;
+    if (bn < 16 || bn > I8_MAX_BN || bn % (c.many ? 32 : 16) || (c.many && c.gated && bn % 128)
+        || (!c.many && (slices < 1 || slices > 8 || per_sm < 1 || per_sm > 4 || (c.features + I8_BM - 1) / I8_BM > 65535))) return -2006;
     Int8Args g = {};
-    g.x_scale = x_scale; g.w_scale = w_scale; g.bias = bias; g.out = out; g.err = err; g.ldc = ldc;
-    g.tokens = tokens; g.features = features; g.K = K; g.out_features = out_features;
-    g.out_f32 = out_f32; g.bias_f32 = bias_f32; g.gated = gated; g.bn = bn; g.slices = slices;
+    g.x_scale = c.x_scale; g.w_scale = c.w_scale; g.bias = c.bias; g.out = c.out; g.err = c.err; g.ldc = c.ldc;
+    g.tokens = (int)c.tokens; g.features = (int)c.features; g.K = (int)c.K; g.out_features = (int)c.out_features;
+    g.out_f32 = (int)c.out_f32; g.bias_f32 = (int)c.bias_f32; g.gated = (int)c.gated; g.bn = bn; g.slices = slices;
+    if (c.many) return bn <= 192 ? launch_many<2>(c, g) : launch_many<1>(c, g);
     CUtensorMap map_x, map_w;
-    if (many) {
-        return bn <= 192 ? launch_many<2>(x, ldx, w, ldw, g, stream) : launch_many<1>(x, ldx, w, ldw, g, stream);
-    }
-    if (int rc = i8_map(&map_x, x, tokens, K, ldx, bn)) return rc;
-    if (int rc = i8_map(&map_w, w, features, K, ldw, I8_BM)) return rc;
+    if (int rc = i8_map(&map_x, c.x, g.tokens, g.K, c.ldx, bn)) return rc;
+    if (int rc = i8_map(&map_w, c.w, g.features, g.K, c.ldw, I8_BM)) return rc;
     static SsPerDevice opted;
     if (int rc = ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return rc;
     const int stage = I8_BM * I8_BK + bn * I8_BK;
     const int rest = I8_SMEM_REST + (slices > 1 ? (bn + slices - 1) / slices * I8_BM * 4 : 0);  // a cluster's blocks: the columns they own
-    const int room = per_sm > 1 ? 233472 / per_sm - 1024 : I8_SMEM_MAX;  // (228 KB an SM, 1 KB of it a block's own)
+    const int room = per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX;
     int stages = (room - rest) / stage;
     const int needed = slices > 1 ? 2 : (bn * I8_BM * 4 + stage - 1) / stage;  // alone, the ring also holds the sums
     stages = stages < needed ? needed : stages > 12 ? 12 : stages;
     g.stages = stages;
     const int smem = stages * stage + rest;
     if (smem > I8_SMEM_MAX) return -2007;
-    const dim3 grid((tokens + bn - 1) / bn, (features + I8_BM - 1) / I8_BM, slices);
-    if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, stream, slices, map_w, map_x, g);
-    else ss_launch(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, stream, map_w, map_x, g);
+    const dim3 grid((g.tokens + bn - 1) / bn, (g.features + I8_BM - 1) / I8_BM, slices);
+    if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, c.stream, slices, map_w, map_x, g);
+    else ss_launch(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, c.stream, map_w, map_x, g);
     return SS_LAUNCH_CHECK();
 }

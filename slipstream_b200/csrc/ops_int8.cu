@@ -378,44 +378,65 @@ inline bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// x [rows, width] with row stride `stride` (elements).  early: the kernel behind may start at once; it may then have read
-// what it takes for constant before q is written, so only for q that it does not take for that (weights are).
-extern "C" int ss_quantize_rows_int8(const void* x, int64_t stride, int8_t* q, int64_t q_stride, float* scales, int rows, int width,
-                                     int dtype, int early, cudaStream_t stream) {
-    if (rows <= 0) return 0;
-    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
-    if (dtype == SS_BF16)
-        return on16(x) && stride % 8 == 0 ? launch_quantize<bf16, true>(x, stride, q, q_stride, scales, rows, width, early, stream)
-                                                          : launch_quantize<bf16, false>(x, stride, q, q_stride, scales, rows, width, early, stream);
-    return on16(x) && stride % 4 == 0 ? launch_quantize<float, true>(x, stride, q, q_stride, scales, rows, width, early, stream)
-                                      : launch_quantize<float, false>(x, stride, q, q_stride, scales, rows, width, early, stream);
+// The arguments of a call as one record (a call through ctypes takes 0.1 us an argument).
+struct Int8RowsCall {
+    const void* x;  // quantize: [rows, width], row stride `stride` elements; dequantize: unused; norm: the stream, [rows, width]
+    int64_t stride;
+    int8_t* q;  // [rows, width], row stride q_stride
+    int64_t q_stride;
+    float* scales;
+    int64_t rows, width, dtype;  // of x; of the values; of delta
+    int64_t early;               // quantize, see below
+    void* y;                     // dequantize: [rows, width]; norm: residual_out or null (may be x)
+    const void* delta;           // norm: [rows, width] or null
+    const void* weight;
+    int64_t w_f32;
+    double eps;
+    cudaStream_t stream;
+};
+
+static int int8_rows_refused(const Int8RowsCall& c) {
+    return c.width <= 0 || c.width > INT32_MAX - 8 || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
 }
 
-// residual, delta (or null) and residual_out (or null; may be residual) [rows, width], contiguous.
-extern "C" int ss_add_rmsnorm_int8(const float* residual, const void* delta, float* residual_out, const void* weight, int w_f32,
-                                   int8_t* q, int64_t q_stride, float* scales, int rows, int width, float eps, int delta_dtype,
-                                   cudaStream_t stream) {
-    if (rows <= 0) return 0;
-    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
-    const bool aligned = width % 4 == 0 && on16(residual) && on16(delta) && on16(residual_out) && on16(weight);
-    if (delta_dtype == SS_BF16)
-        return aligned ? launch_norm<bf16, true>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream)
-                       : launch_norm<bf16, false>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream);
-    return aligned ? launch_norm<float, true>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream)
-                   : launch_norm<float, false>(residual, delta, residual_out, weight, w_f32, q, q_stride, scales, rows, width, eps, stream);
+// early: the kernel behind may start at once; it may then have read what it takes for constant before q is written, so only
+// for q that it does not take for that (weights are).
+extern "C" int ss_quantize_rows_int8(const Int8RowsCall* call) {
+    const Int8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = int8_rows_refused(c)) return rc;
+    const int rows = (int)c.rows, width = (int)c.width, early = (int)c.early;
+    if (c.dtype == SS_BF16)
+        return on16(c.x) && c.stride % 8 == 0 ? launch_quantize<bf16, true>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream)
+                                              : launch_quantize<bf16, false>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream);
+    return on16(c.x) && c.stride % 4 == 0 ? launch_quantize<float, true>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream)
+                                          : launch_quantize<float, false>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream);
 }
 
-// y [rows, width], contiguous.
-extern "C" int ss_dequantize_rows_int8(const int8_t* q, int64_t q_stride, const float* scales, void* y, int rows, int width, int dtype,
-                                       cudaStream_t stream) {
-    if (rows <= 0) return 0;
-    if (width <= 0 || q_stride % 16 || !on16(q)) return -2003;
-    const int g = dtype == SS_BF16 ? 8 : 4;
-    const bool aligned = on16(y) && width % g == 0;
+extern "C" int ss_add_rmsnorm_int8(const Int8RowsCall* call) {
+    const Int8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = int8_rows_refused(c)) return rc;
+    const int rows = (int)c.rows, width = (int)c.width, w_f32 = (int)c.w_f32;
+    const float* residual = (const float*)c.x;
+    const bool aligned = width % 4 == 0 && on16(c.x) && on16(c.delta) && on16(c.y) && on16(c.weight);
+    if (c.dtype == SS_BF16)
+        return aligned ? launch_norm<bf16, true>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream)
+                       : launch_norm<bf16, false>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream);
+    return aligned ? launch_norm<float, true>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream)
+                   : launch_norm<float, false>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream);
+}
+
+extern "C" int ss_dequantize_rows_int8(const Int8RowsCall* call) {
+    const Int8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = int8_rows_refused(c)) return rc;
+    const int rows = (int)c.rows, width = (int)c.width, g = c.dtype == SS_BF16 ? 8 : 4;
+    const bool aligned = on16(c.y) && width % g == 0;
     int threads = (width / (aligned ? g : 1) + 31) / 32 * 32;
     threads = threads < 32 ? 32 : threads > 256 ? 256 : threads;
-#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows), dim3(threads), 0, stream, q, q_stride, scales, (T*)y, width)
-    if (dtype == SS_BF16) { if (aligned) DEQ(bf16, true); else DEQ(bf16, false); }
+#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows), dim3(threads), 0, c.stream, c.q, c.q_stride, c.scales, (T*)c.y, width)
+    if (c.dtype == SS_BF16) { if (aligned) DEQ(bf16, true); else DEQ(bf16, false); }
     else { if (aligned) DEQ(float, true); else DEQ(float, false); }
 #undef DEQ
     return SS_LAUNCH_CHECK();

@@ -17,6 +17,7 @@ front of it are through.  `quantize_rows_int8` therefore keeps the kernels behin
 from __future__ import annotations
 
 import functools
+from struct import Struct
 
 import torch
 
@@ -25,6 +26,8 @@ from .functions import KernelError, _check, _code, _need, _ptr, _stream, error_w
 RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
 MAX_K = 133143  # 127^2 K stays below 2^31
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
+_ROWS_CALL = Struct("=13qdq").pack  # csrc/ops_int8.cu: Int8RowsCall
+_PRODUCT_CALL = Struct("=22q").pack  # csrc/gemm_int8.cu: Int8Call
 
 
 class Int8Rows:
@@ -55,9 +58,8 @@ class Int8Rows:
 
 def int8_rows_like(rows: int, width: int, device: torch.device) -> Int8Rows:
     """Int8 rows with nothing in them yet."""
-    stride = (width + 15) & -16
-    values = torch.empty_strided((rows, width), (stride, 1), dtype=_I8, device=device)
-    return Int8Rows(values, torch.empty(rows, dtype=_F32, device=device))
+    values = torch.empty_strided((rows, width), ((width + 15) & -16, 1), dtype=_I8, device=device)
+    return Int8Rows(values, torch.empty_strided((rows,), (1,), dtype=_F32, device=device))
 
 
 def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int]:
@@ -65,13 +67,15 @@ def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int]:
     if not isinstance(r, Int8Rows):
         raise KernelError(f"{what} must be Int8Rows, not {type(r).__name__}")
     v, s = r.values, r.scales
-    if v.dim() != 2 or v.dtype != _I8 or not v.is_cuda:
+    if v.dim() != 2 or v.dtype is not _I8 or not v.is_cuda:
         raise KernelError(f"{what}: the values must be a two-dimensional int8 CUDA tensor, got {v.dtype} {tuple(v.shape)} on {v.device}")
     n, k = v.shape
-    if s.dtype != _F32 or not s.is_cuda or s.numel() != n or not s.is_contiguous():
-        raise KernelError(f"{what}: the scales must be {n} contiguous float32 numbers on the device")
-    stride = v.stride(0) if n > 1 else (k + 15) & -16
-    if n and k and (v.stride(1) != 1 and k > 1 or stride % 16 or stride < k or v.data_ptr() % 16):
+    if s.dtype is not _F32 or s.numel() != n or not s.is_contiguous() or s.get_device() != v.get_device():
+        raise KernelError(f"{what}: the scales must be {n} contiguous float32 numbers beside the values")
+    stride, step = v.stride()
+    if n < 2:
+        stride = (k + 15) & -16
+    if n and k and (step != 1 and k > 1 or stride & 15 or stride < k or v.data_ptr() & 15):
         raise KernelError(f"{what}: rows must be contiguous and start on 16 bytes (a stride that is a multiple of 16), got strides {v.stride()}")
     return n, k, stride
 
@@ -86,24 +90,28 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     n, k = x.shape
     if k < 1:
         raise KernelError("rows without elements have no scale")
-    if k > 1 and x.stride(1) != 1:
+    stride, step = x.stride()
+    if k > 1 and step != 1:
         raise KernelError(f"the rows of x must be contiguous, got strides {x.stride()}")
+    code = _code(x.dtype)
     out = int8_rows_like(n, k, x.device)
-    if n == 0:
-        return out
-    _check(ops_library().ss_quantize_rows_int8(x.data_ptr(), x.stride(0), out.values.data_ptr(), (k + 15) & -16, out.scales.data_ptr(),
-                                               n, k, _code(x.dtype), activations, _stream()), "quantize_rows_int8")
+    if n:
+        _check(ops_library().ss_quantize_rows_int8(_ROWS_CALL(
+            x.data_ptr(), stride, out.values.data_ptr(), (k + 15) & -16, out.scales.data_ptr(), n, k, code, activations, 0, 0, 0, 0, 0.0,
+            _stream())), "quantize_rows_int8")
     return out
 
 
 def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
     """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once."""
     n, k, stride = _need_rows(rows, "rows")
-    out = torch.empty((n, k), dtype=dtype, device=rows.values.device)
     code = _code(dtype)
+    values = rows.values
+    out = torch.empty_strided((n, k), (k, 1), dtype=dtype, device=values.device)
     if n and k:
-        _check(ops_library().ss_dequantize_rows_int8(rows.values.data_ptr(), stride, rows.scales.data_ptr(), out.data_ptr(), n, k, code,
-                                                     _stream()), "dequantize_rows_int8")
+        _check(ops_library().ss_dequantize_rows_int8(_ROWS_CALL(
+            0, 0, values.data_ptr(), stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, _stream())),
+            "dequantize_rows_int8")
     return out
 
 
@@ -135,29 +143,100 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
             raise KernelError(f"residual_out {tuple(residual_out.shape)} does not match residual {tuple(residual.shape)}")
         to = residual_out.data_ptr()
     else:
-        to = residual.data_ptr() if delta is not None else None
+        to = residual.data_ptr() if delta is not None else 0
     out = int8_rows_like(n, h, residual.device)
-    if n == 0:
-        return out
-    _check(ops_library().ss_add_rmsnorm_int8(residual.data_ptr(), _ptr(delta), to, weight.data_ptr(), weight.dtype == _F32,
-                                             out.values.data_ptr(), (h + 15) & -16, out.scales.data_ptr(), n, h, float(eps), code,
-                                             _stream()), "add_rmsnorm_int8")
+    if n:
+        _check(ops_library().ss_add_rmsnorm_int8(_ROWS_CALL(
+            residual.data_ptr(), h, out.values.data_ptr(), (h + 15) & -16, out.scales.data_ptr(), n, h, code, 0, to, _ptr(delta) or 0,
+            weight.data_ptr(), weight.dtype is _F32, float(eps), _stream())), "add_rmsnorm_int8")
     return out
 
 
 # --------------------------------------------------------------------------- products
 
-@functools.lru_cache(maxsize=None)
-def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False) -> tuple[int, int, int, int]:
+class _Device:
+    """What the products ask of a device: its multiprocessors, where its error word is, and how many clusters of 1 to 8 blocks of
+    the kernel for few tokens it holds at the same time, with its ring sized for one block an SM and for two."""
+
+    def __init__(self, device: torch.device) -> None:
+        self.sms = sm_count(device)
+        self.error_ptr = error_word(device).data_ptr()  # (the word lives as long as the process)
+        lib = gemm_library()
+        self.resident = tuple(tuple(lib.ss_gemm_int8_resident(n, per) or self.sms * per // n for n in range(1, 9)) for per in (1, 2))
+
+
+_devices: dict[torch.device, _Device] = {}
+
+
+def _device(device: torch.device) -> _Device:
+    found = _devices.get(device)
+    if found is None:
+        with torch.cuda.device(device):
+            found = _devices[device] = _Device(device)
+    return found
+
+
+def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
+              resident: tuple[tuple[int, ...], tuple[int, ...]] | None = None) -> tuple[int, int, int, int]:
     """(many, tile, K slices, blocks an SM) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
-    (tokens of the first, features of the second), and for the first the slices of K and how many blocks an SM the ring is sized for."""
-    k_iters = (k + 127) // 128
-    if tokens <= 256:
-        tile = max(16, (tokens + 15) // 16 * 16)
-        tiles = (features + 127) // 128
-        slices = max(1, min(8, k_iters, sms // tiles)) if tiles < sms else 1
-        return 0, tile, slices, 2 if tile <= 32 else 1
-    return 1, 256, 1, 1
+    (tokens of the first, features of the second), and for the first the slices of K and how many blocks an SM the ring is sized
+    for.  ``resident``: clusters of 1 to 8 blocks that run at the same time, with the ring sized for one block an SM and for two.
+
+    The choice is the cheapest by an estimate of cycles whose constants are fitted to 4,220 measured products (1 to 4,096 tokens, the
+    projections of the 0.5B, 1.5B and 7B layer sizes, tiles and slices of all sizes).  What it takes is on average 2 % slower than the
+    fastest of them at the same sizes, and at worst 17 %; one tile for all tokens up to 256 and K in one slice, else tiles of 256 x 256,
+    would be 43 % slower."""
+    # what follows depends on the tokens in steps of 16 (their tiles) up to 640 and of 256 beyond: few plans for many counts
+    step = 16 if tokens <= 640 else 256
+    return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
+
+
+@functools.lru_cache(maxsize=None)
+def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -> tuple[int, int, int, int]:
+    if resident is None:
+        resident = tuple(tuple(sms * per // n for n in range(1, 9)) for per in (1, 2))
+    k_steps = (k + 127) // 128
+    best = None
+    for parts in range(1, 9) if tokens <= 640 else ():
+        tile = ((tokens + parts - 1) // parts + 15) // 16 * 16
+        if tile > 256 or (parts > 1 and tile <= 16):
+            continue
+        tiles = (features + 127) // 128 * ((tokens + tile - 1) // tile)
+        for slices in range(1, min(8, k_steps) + 1):
+            blocks = tiles * slices
+            if slices > 1 and blocks > 3 * sms:
+                break
+            if slices == 7:  # (clusters that fit worst into the GPU's processor clusters)
+                continue
+            for per in (1, 2) if tile <= 128 else (1,):
+                rest = 2560 + ((tile + slices - 1) // slices * 512 if slices > 1 else 0)
+                stages = max(2, min(12, ((232448 if per == 1 else 115712) - rest) // ((128 + tile) * 128)))
+                held = max(1, resident[per - 1][slices - 1]) * slices  # blocks that run at the same time
+                waves = (blocks + held - 1) // held
+                shared = max(1.0, min(float(per), blocks / sms))
+                # a step of K: the loops of the fetching and issuing threads; what an SM takes in; the ring's latency; the memory
+                cycles = max(330.0, shared * (128 + tile) * 128 / 56, 2470 / stages, min(blocks, held) * 16384 * 148 / (3070 * sms))
+                cost = 3870 + waves * ((k_steps + slices - 1) // slices * cycles + 465 + 17.4 * tile)
+                if slices > 1:
+                    cost += waves * (148 + 61 * tile * (slices - 1) / slices)
+                if waves > 1:
+                    cost += 4440
+                elif per == 2 and blocks <= (0.5 if slices == 1 else 0.45) * held:  # the kernel behind has room for its first stages
+                    cost -= 900
+                if best is None or cost < best[0]:
+                    best = (cost, (0, tile, slices, per))
+    if tokens > 64:
+        rows = (tokens + 255) // 256
+        for tile in ((128, 256) if gated else (32, 64, 96, 128, 160, 192, 224, 256)):
+            tiles = rows * ((features + tile - 1) // tile)
+            pairs = max(1, sms // 2)
+            rounds = (tiles + pairs - 1) // pairs
+            cycles = max(322.0 if tile <= 192 else 493.0, 2.43 * tile, (min(128, tokens) + tile / 2) * 128 / 60,
+                         min(tiles, pairs) * tile * 128 * 148 / (3070 * sms * min(rows, tiles, pairs)))
+            cost = 3840 + rounds * k_steps * cycles + 2120 + 18.6 * tile + (rounds - 1) * 1270 + (10.8 * tile if gated else 0)
+            if best is None or cost < best[0]:
+                best = (cost, (1, tile, 1, 1))
+    return best[1]
 
 
 def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype: torch.dtype, gated: bool, columns: int | None,
@@ -176,20 +255,24 @@ def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype
             raise KernelError(f"{columns} features asked of {features // 2}")
     else:
         columns = features
-    out = torch.empty((tokens, columns), dtype=out_dtype, device=x.values.device)
     out_f32 = 1 - _code(out_dtype)
-    bias_f32 = 0
+    bias_ptr = bias_f32 = 0
     if bias is not None:
         _need(bias, None, "bias")
         if bias.numel() != features or bias.dtype not in (_BF16, _F32):
             raise KernelError("bias has the wrong size or dtype")
-        bias_f32 = int(bias.dtype == _F32)
+        bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is _F32
+    device = x.values.device
+    if weight.values.device != device:
+        raise KernelError(f"x is on {device}, weight on {weight.values.device}")
+    out = torch.empty_strided((tokens, columns), (columns, 1), dtype=out_dtype, device=device)
     if tokens == 0 or columns == 0:
         return out
-    many, tile, slices, per_sm = plan or int8_plan(tokens, features, k, sm_count(out.device), gated)
-    _check(gemm_library().ss_gemm_int8(x.values.data_ptr(), ldx, x.scales.data_ptr(), weight.values.data_ptr(), ldw, weight.scales.data_ptr(),
-                                       _ptr(bias), bias_f32, out.data_ptr(), columns, out_f32, tokens, features, k, gated, columns,
-                                       many, tile, slices, per_sm, error_word(out.device).data_ptr(), _stream()), what)
+    d = _device(device)
+    many, tile, slices, per_sm = plan or int8_plan(tokens, features, k, d.sms, gated, d.resident)
+    _check(gemm_library().ss_gemm_int8(_PRODUCT_CALL(
+        x.values.data_ptr(), ldx, x.scales.data_ptr(), weight.values.data_ptr(), ldw, weight.scales.data_ptr(), bias_ptr, bias_f32,
+        out.data_ptr(), columns, out_f32, tokens, features, k, gated, columns, many, tile, slices, per_sm, d.error_ptr, _stream())), what)
     return out
 
 
