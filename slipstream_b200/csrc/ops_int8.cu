@@ -9,7 +9,25 @@
 //
 // All three kernels are bound by memory: a row is read once, into registers, and its results are written from there.
 
-#include "common.cuh"
+#include "tc5.cuh"
+
+// The arguments of a call as one record (a call through ctypes takes 0.1 us an argument).
+struct Int8RowsCall {
+    const void* x;  // quantize: [rows, width], row stride `stride` elements; dequantize: unused; norm: the stream, [rows, width]
+    int64_t stride;
+    int8_t* q;  // [rows, width], row stride q_stride
+    int64_t q_stride;
+    float* scales;
+    int64_t rows, width, dtype;  // of x; of the values; of delta
+    int64_t early;               // quantize, see below
+    void* y;                     // dequantize: [rows, width]; norm: residual_out or null (may be x)
+    const void* delta;           // norm: [rows, width] or null
+    const void* weight;
+    int64_t w_f32;
+    double eps;
+    int* err;
+    cudaStream_t stream;
+};
 
 namespace {
 
@@ -210,7 +228,11 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict
 // x = residual + delta, written to residual_out (if there is one); v = x / sqrt(mean(x^2) + eps) * w, as int8 rows.  The norm's
 // factor is the same for the whole row, so q is that of x * w, and the factor enters the scale alone: the squares' sum and the
 // largest |x * w| are found in one pass with one barrier, and v is never rounded to fewer than its 24 bits.
-//
+__device__ __forceinline__ float norm_scale(uint32_t top, float squares, int width, float eps) {
+    const float rstd = 1.0f / sqrtf(squares / (float)width + eps);
+    return top < INF_BITS ? __fdiv_rn(__uint_as_float(top) * rstd, 127.f) : __uint_as_float(0x7fffffffu);
+}
+
 // A block per row; NG groups of four elements a thread stay in registers; NG = 0: rows of any width, read twice.
 template <typename T, bool ALIGNED, int NG>
 __global__ void __launch_bounds__(most_threads<NG>())
@@ -285,9 +307,8 @@ add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, floa
         }
     }
     block_top_sum(top, ss, tops, sums);
-    RowScale r = row_scale(top);
-    const float rstd = 1.0f / sqrtf(ss / (float)width + eps);
-    if (threadIdx.x == 0) scales[blockIdx.x] = __fdiv_rn(__uint_as_float(top) * rstd, 127.f);
+    const RowScale r = row_scale(top);
+    if (threadIdx.x == 0) scales[blockIdx.x] = norm_scale(top, ss, width, eps);
     if constexpr (NG > 0) {
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -307,30 +328,218 @@ add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, floa
     }
 }
 
+// ---------------------------------------------------------------- many rows
+//
+// The same two operations for many wide rows: two or three blocks an SM, each taking rows blockIdx.x, + gridDim.x, ... through a ring
+// of `stages` rows in shared memory that one thread fills by bulk copies, so that the rows behind are on their way through the two
+// passes over this one (with registers alone DRAM was 40 % busy: too few warps fit beside what they hold).  A block's stage is free
+// when all its threads have read their part, behind the one barrier a row.  NG vectors a thread; rows of a multiple of 16 bytes that
+// start on 16 bytes.  Norm of 4,096 x 3,584 (bfloat16 branch): 29.4 us, 84 % of the measured copy rate, a block per row 35.0;
+// 2,048 x 8,192 33.3 and 44.7; rounding 2,048 x 18,944 (bfloat16) 20.8 and 22.0.  Rows below 16 KB stay with a block per row: a row's
+// chain of two passes and a barrier is about 1,500 cycles however narrow it is, and many small blocks hide more of them (norm of
+// 4,096 x 896: 10.5 us through a ring, 8.7 so; rounding 4,096 x 3,584: 10.5 and 9.8).
+constexpr int RING_THREADS = 256;
+constexpr int ring_blocks(int ng) { return ng <= 4 ? 3 : 2; }  // blocks an SM at most
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(s_addr(dst)), "l"(src), "r"(bytes), "r"(s_addr(bar)) : "memory");
+}
+struct RowRing {
+    unsigned char* rows;  // [stages][row_bytes]
+    uint64_t* full;
+    int* gave_up;
+    int stages, row_bytes;
+};
+// smem: the rows (16-byte aligned), then the barriers, then the flag
+__device__ __forceinline__ RowRing row_ring(unsigned char* smem, int stages, int row_bytes) {
+    RowRing r;
+    r.rows = smem;
+    r.full = reinterpret_cast<uint64_t*>(smem + stages * row_bytes);
+    r.gave_up = reinterpret_cast<int*>(r.full + stages);
+    r.stages = stages;
+    r.row_bytes = row_bytes;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&r.full[s], 1);
+        *r.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    return r;
+}
+
+// Behind a wait that gave up: the block does not end under its copies in flight, the last of the `issued` ones (each wait has its
+// own limit).
+__device__ __forceinline__ void drain_ring(const RowRing& r, int issued, int* err) {
+    if (!*(volatile int*)r.gave_up || threadIdx.x) return;
+    for (int i = max(0, issued - r.stages); i < issued; ++i) {
+        volatile int none = 0;
+        (void)mbar_wait(&r.full[i % r.stages], (i / r.stages) & 1, &none);
+    }
+    atomicOr(err, SS_ERR_WAIT_LIMIT);
+}
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(RING_THREADS, ring_blocks(NG))
+quantize_ring_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int rows,
+                     int width, int stages, int early, int* err) {
+    using Vec = RawVec<T>;
+    constexpr int G = Vec::G;
+    extern __shared__ __align__(128) unsigned char ring_smem[];
+    __shared__ uint32_t tops[2][RING_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bytes = width * (int)sizeof(T);
+    const RowRing ring = row_ring(ring_smem, stages, bytes);
+    if (early) pdl_launch_dependents();
+    pdl_wait();
+    auto fetch = [&](int64_t row, int s) {
+        mbar_expect_tx(&ring.full[s], bytes);
+        bulk_load(ring.rows + s * bytes, x + row * stride, bytes, &ring.full[s]);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages && blockIdx.x + (int64_t)s * gridDim.x < rows; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+    int s = 0, n = 0;
+    uint32_t parity = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
+        mbar_wait(&ring.full[s], parity, ring.gave_up);
+        const T* from = reinterpret_cast<const T*>(ring.rows + s * bytes);
+        Vec v[NG];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * G;
+            v[i].raw = j < width ? *reinterpret_cast<const uint4*>(from + j) : make_uint4(0, 0, 0, 0);
+            top = v[i].top(top);
+        }
+        top = __reduce_max_sync(0xffffffffu, Vec::top_bits(top));
+        if (lane == 0) tops[n & 1][warp] = top;  // (two sets: the next row's are written while slow warps still read these)
+        __syncthreads();
+        if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
+        top = __reduce_max_sync(0xffffffffu, lane < RING_THREADS / 32 ? tops[n & 1][lane] : 0u);
+        const RowScale r = row_scale(top);
+        if (threadIdx.x == 0) scales[row] = r.scale;
+        int8_t* out = q + row * q_stride;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * G;
+            if (j < width) v[i].quantize(out + j, width - j, r);
+        }
+        if (++s == stages) { s = 0; parity ^= 1; }
+    }
+    drain_ring(ring, n, err);  // (the block's rows are its copies, in order)
+}
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(RING_THREADS, ring_blocks(NG))
+add_rmsnorm_int8_ring_kernel(const float* residual, const T* __restrict__ delta, float* residual_out, const void* __restrict__ weight,
+                             int w_f32, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int rows, int width, float eps,
+                             int stages, int* err) {
+    extern __shared__ __align__(128) unsigned char ring_smem[];
+    __shared__ uint32_t tops[2][RING_THREADS / 32];
+    __shared__ float sums[2][RING_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int x_bytes = width * 4, d_bytes = delta ? width * (int)sizeof(T) : 0, bytes = x_bytes + d_bytes;
+    const RowRing ring = row_ring(ring_smem, stages, bytes);
+    pdl_launch_dependents();
+    float w[NG][4];  // for all rows of the block
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int j = (threadIdx.x + i * RING_THREADS) * 4;
+        if (w_f32) load4<true>((const float*)weight + j, width - j, w[i]);
+        else load4<true>((const bf16*)weight + j, width - j, w[i]);
+    }
+    pdl_wait();
+    auto fetch = [&](int64_t row, int s) {
+        mbar_expect_tx(&ring.full[s], bytes);
+        bulk_load(ring.rows + s * bytes, residual + row * width, x_bytes, &ring.full[s]);
+        if (d_bytes) bulk_load(ring.rows + s * bytes + x_bytes, delta + row * width, d_bytes, &ring.full[s]);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages && blockIdx.x + (int64_t)s * gridDim.x < rows; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+    int s = 0, n = 0;
+    uint32_t parity = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
+        mbar_wait(&ring.full[s], parity, ring.gave_up);
+        const float* from = reinterpret_cast<const float*>(ring.rows + s * bytes);
+        const T* from_d = reinterpret_cast<const T*>(ring.rows + s * bytes + x_bytes);
+        float v[NG][4], ss = 0.f;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * 4;
+            if (j < width) {
+                load4<true>(from + j, 4, v[i]);
+                if (d_bytes) {
+                    float d[4];
+                    load4<true>(from_d + j, 4, d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][e] = __fadd_rn(v[i][e], d[e]);
+                }
+                if (residual_out) *reinterpret_cast<float4*>(residual_out + row * width + j) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ss = fmaf(v[i][e], v[i][e], ss);
+                    v[i][e] *= w[i][e];
+                }
+                top = top_of(top, v[i]);
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        ss = warp_sum(ss);
+        if (lane == 0) { tops[n & 1][warp] = top; sums[n & 1][warp] = ss; }
+        __syncthreads();
+        if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
+        top = __reduce_max_sync(0xffffffffu, lane < RING_THREADS / 32 ? tops[n & 1][lane] : 0u);
+        ss = warp_sum(lane < RING_THREADS / 32 ? sums[n & 1][lane] : 0.f);
+        const RowScale r = row_scale(top);
+        if (threadIdx.x == 0) scales[row] = norm_scale(top, ss, width, eps);
+        int8_t* out = q + row * q_stride;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * 4;
+            if (j < width) *reinterpret_cast<uint32_t*>(out + j) = quantize4(v[i], r);
+        }
+        if (++s == stages) { s = 0; parity ^= 1; }
+    }
+    drain_ring(ring, n, err);  // (the block's rows are its copies, in order)
+}
+
 // ---------------------------------------------------------------- int8 rows to values
 //
-// y = q * s, rounded once.  A block per row; eight (bfloat16) or four (float32) elements a thread and step where the output's
-// rows start on 16 bytes, else one.
+// y = q * s, rounded once.  A row is cut into spans of groups (eight bfloat16 or four float32 elements, where the output's rows
+// start on 16 bytes, else one), a block each, four groups a thread, all loaded before the first is written.
+constexpr int DEQ_THREADS = 256, DEQ_GROUPS = 4;
+
 template <typename T, bool ALIGNED>
-__global__ void dequantize_rows_kernel(const int8_t* __restrict__ q, int64_t q_stride, const float* __restrict__ scales,
-                                       T* __restrict__ y, int width) {
+__global__ void __launch_bounds__(DEQ_THREADS)
+dequantize_rows_kernel(const int8_t* __restrict__ q, int64_t q_stride, const float* __restrict__ scales, T* __restrict__ y, int width,
+                       int spans) {
     constexpr int G = ALIGNED ? 16 / (int)sizeof(T) : 1;
     pdl_launch_dependents();
     pdl_wait();
-    const float s = scales[blockIdx.x];
-    const int8_t* row = q + (int64_t)blockIdx.x * q_stride;
-    T* out = y + (int64_t)blockIdx.x * width;
-    for (int j = threadIdx.x * G; j < width; j += blockDim.x * G) {
-        if constexpr (!ALIGNED) {
-            out[j] = from_float<T>((float)row[j] * s);
-        } else {
-            uint32_t words[G / 4];
-            if constexpr (G == 8) *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(row + j);
-            else words[0] = *reinterpret_cast<const uint32_t*>(row + j);
+    const int row = blockIdx.x / spans, first = (blockIdx.x - row * spans) * (int)(blockDim.x * DEQ_GROUPS) + threadIdx.x;
+    const float s = scales[row];
+    const int8_t* from = q + (int64_t)row * q_stride;
+    T* out = y + (int64_t)row * width;
+    uint32_t words[DEQ_GROUPS][2];
+#pragma unroll
+    for (int i = 0; i < DEQ_GROUPS; ++i) {
+        const int64_t j = (int64_t)(first + i * blockDim.x) * G;
+        if (j < width) {
+            if constexpr (G == 8) *reinterpret_cast<uint2*>(words[i]) = *reinterpret_cast<const uint2*>(from + j);
+            else if constexpr (G == 4) words[i][0] = *reinterpret_cast<const uint32_t*>(from + j);
+            else words[i][0] = (uint32_t)(uint8_t)from[j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < DEQ_GROUPS; ++i) {
+        const int64_t j = (int64_t)(first + i * blockDim.x) * G;
+        if (j < width) {
             T v[G];
 #pragma unroll
-            for (int e = 0; e < G; ++e) v[e] = from_float<T>((float)(int8_t)(words[e / 4] >> (8 * (e & 3))) * s);
-            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(v);
+            for (int e = 0; e < G; ++e) v[e] = from_float<T>((float)(int8_t)(words[i][e / 4] >> (8 * (e & 3))) * s);
+            if constexpr (ALIGNED) *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(v);
+            else out[j] = v[0];
         }
     }
 }
@@ -352,6 +561,53 @@ inline RowShape row_shape(int groups, int64_t rows) {
     return {0, 512};
 }
 #define ROW_SHAPES(CASE) switch (shape.ng) { CASE(0); CASE(1); CASE(2); CASE(3); CASE(4); CASE(6); CASE(8); CASE(10); }
+
+// The ring: blocks an SM, and stages of a block's ring (0: the rows are too few, too narrow or too wide).  Three rows in flight a
+// block where three blocks share an SM, else two at least; four rows a block at least.
+struct RingShape { int blocks, stages; };
+constexpr int RING_SMEM = 112 * 1024;  // of a block, two of which share an SM
+inline int ring_groups(int vectors) {
+    const int ng = (vectors + RING_THREADS - 1) / RING_THREADS;
+    return ng <= 4 ? ng : ng <= 6 ? 6 : ng <= 8 ? 8 : ng <= 10 ? 10 : 12;
+}
+inline RingShape ring_shape(int64_t rows, int64_t row_bytes, int vectors) {
+    if (row_bytes < 16384 || vectors > 12 * RING_THREADS || row_bytes % 16) return {0, 0};
+    for (int blocks = ring_blocks(ring_groups(vectors)); blocks >= 2; --blocks) {
+        const int64_t stages = (224 * 1024 / blocks - 2048) / (row_bytes + 8);
+        if (stages >= blocks && rows >= 4 * (int64_t)blocks * ss_sm_count()) return {blocks, (int)stages};
+    }
+    return {0, 0};
+}
+
+template <typename T>
+int launch_quantize_ring(const Int8RowsCall& c, RingShape shape) {
+    const int vectors = (int)((c.width * sizeof(T) + 15) / 16), blocks = shape.blocks * ss_sm_count(), stages = shape.stages;
+    const int smem = (int)(stages * (c.width * sizeof(T) + 8)) + 64;
+    int rc = 0;
+#define QUANT(NG) case NG: { \
+        static SsPerDevice opted; \
+        if ((rc = ss_opt_in_smem(quantize_ring_kernel<T, NG>, RING_SMEM, opted))) return rc; \
+        ss_launch(quantize_ring_kernel<T, NG>, dim3(blocks), dim3(RING_THREADS), smem, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, (int)c.rows, (int)c.width, stages, (int)c.early, c.err); \
+    } break
+    switch (ring_groups(vectors)) { QUANT(4); QUANT(6); QUANT(8); QUANT(10); QUANT(12); }
+#undef QUANT
+    return SS_LAUNCH_CHECK();
+}
+
+template <typename T>
+int launch_norm_ring(const Int8RowsCall& c, RingShape shape) {
+    const int vectors = (int)((c.width + 3) / 4), blocks = shape.blocks * ss_sm_count(), stages = shape.stages;
+    const int smem = (int)(stages * (c.width * (4 + (c.delta ? sizeof(T) : 0)) + 8)) + 64;
+    int rc = 0;
+#define NORM(NG) case NG: { \
+        static SsPerDevice opted; \
+        if ((rc = ss_opt_in_smem(add_rmsnorm_int8_ring_kernel<T, NG>, RING_SMEM, opted))) return rc; \
+        ss_launch(add_rmsnorm_int8_ring_kernel<T, NG>, dim3(blocks), dim3(RING_THREADS), smem, c.stream, (const float*)c.x, (const T*)c.delta, (float*)c.y, c.weight, (int)c.w_f32, c.q, c.q_stride, c.scales, (int)c.rows, (int)c.width, (float)c.eps, stages, c.err); \
+    } break
+    switch (ring_groups(vectors)) { NORM(2); NORM(3); NORM(4); NORM(6); NORM(8); NORM(10); NORM(12); }
+#undef NORM
+    return SS_LAUNCH_CHECK();
+}
 
 template <typename T, bool ALIGNED>
 int launch_quantize(const void* x, int64_t stride, int8_t* q, int64_t q_stride, float* scales, int rows, int width, int early,
@@ -378,23 +634,6 @@ inline bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// The arguments of a call as one record (a call through ctypes takes 0.1 us an argument).
-struct Int8RowsCall {
-    const void* x;  // quantize: [rows, width], row stride `stride` elements; dequantize: unused; norm: the stream, [rows, width]
-    int64_t stride;
-    int8_t* q;  // [rows, width], row stride q_stride
-    int64_t q_stride;
-    float* scales;
-    int64_t rows, width, dtype;  // of x; of the values; of delta
-    int64_t early;               // quantize, see below
-    void* y;                     // dequantize: [rows, width]; norm: residual_out or null (may be x)
-    const void* delta;           // norm: [rows, width] or null
-    const void* weight;
-    int64_t w_f32;
-    double eps;
-    cudaStream_t stream;
-};
-
 static int int8_rows_refused(const Int8RowsCall& c) {
     return c.width <= 0 || c.width > INT32_MAX - 8 || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
 }
@@ -406,6 +645,11 @@ extern "C" int ss_quantize_rows_int8(const Int8RowsCall* call) {
     if (c.rows <= 0) return 0;
     if (int rc = int8_rows_refused(c)) return rc;
     const int rows = (int)c.rows, width = (int)c.width, early = (int)c.early;
+    const int size = c.dtype == SS_BF16 ? 2 : 4;
+    if (on16(c.x) && c.stride * size % 16 == 0) {
+        const RingShape shape = ring_shape(c.rows, c.width * size, (int)((c.width * size + 15) / 16));
+        if (shape.blocks) return c.dtype == SS_BF16 ? launch_quantize_ring<bf16>(c, shape) : launch_quantize_ring<float>(c, shape);
+    }
     if (c.dtype == SS_BF16)
         return on16(c.x) && c.stride % 8 == 0 ? launch_quantize<bf16, true>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream)
                                               : launch_quantize<bf16, false>(c.x, c.stride, c.q, c.q_stride, c.scales, rows, width, early, c.stream);
@@ -420,6 +664,10 @@ extern "C" int ss_add_rmsnorm_int8(const Int8RowsCall* call) {
     const int rows = (int)c.rows, width = (int)c.width, w_f32 = (int)c.w_f32;
     const float* residual = (const float*)c.x;
     const bool aligned = width % 4 == 0 && on16(c.x) && on16(c.delta) && on16(c.y) && on16(c.weight);
+    if (aligned && (c.dtype != SS_BF16 || !c.delta || width % 8 == 0)) {
+        const RingShape shape = ring_shape(c.rows, c.width * (4 + (!c.delta ? 0 : c.dtype == SS_BF16 ? 2 : 4)), (width + 3) / 4);
+        if (shape.blocks) return c.dtype == SS_BF16 ? launch_norm_ring<bf16>(c, shape) : launch_norm_ring<float>(c, shape);
+    }
     if (c.dtype == SS_BF16)
         return aligned ? launch_norm<bf16, true>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream)
                        : launch_norm<bf16, false>(residual, c.delta, (float*)c.y, c.weight, w_f32, c.q, c.q_stride, c.scales, rows, width, (float)c.eps, c.stream);
@@ -433,9 +681,12 @@ extern "C" int ss_dequantize_rows_int8(const Int8RowsCall* call) {
     if (int rc = int8_rows_refused(c)) return rc;
     const int rows = (int)c.rows, width = (int)c.width, g = c.dtype == SS_BF16 ? 8 : 4;
     const bool aligned = on16(c.y) && width % g == 0;
-    int threads = (width / (aligned ? g : 1) + 31) / 32 * 32;
-    threads = threads < 32 ? 32 : threads > 256 ? 256 : threads;
-#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows), dim3(threads), 0, c.stream, c.q, c.q_stride, c.scales, (T*)c.y, width)
+    const int groups = (width + (aligned ? g : 1) - 1) / (aligned ? g : 1);
+    int threads = ((groups + DEQ_GROUPS - 1) / DEQ_GROUPS + 31) / 32 * 32;
+    threads = threads > DEQ_THREADS ? DEQ_THREADS : threads;
+    const int span = threads * DEQ_GROUPS, spans = (groups + span - 1) / span;
+    if (c.rows * spans > INT32_MAX) return -2003;
+#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows * spans), dim3(threads), 0, c.stream, c.q, c.q_stride, c.scales, (T*)c.y, width, spans)
     if (c.dtype == SS_BF16) { if (aligned) DEQ(bf16, true); else DEQ(bf16, false); }
     else { if (aligned) DEQ(float, true); else DEQ(float, false); }
 #undef DEQ

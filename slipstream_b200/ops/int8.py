@@ -26,7 +26,7 @@ from .functions import KernelError, _check, _code, _need, _ptr, _stream, error_w
 RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
 MAX_K = 133143  # 127^2 K stays below 2^31
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
-_ROWS_CALL = Struct("=13qdq").pack  # csrc/ops_int8.cu: Int8RowsCall
+_ROWS_CALL = Struct("=13qd2q").pack  # csrc/ops_int8.cu: Int8RowsCall
 _PRODUCT_CALL = Struct("=22q").pack  # csrc/gemm_int8.cu: Int8Call
 
 
@@ -98,7 +98,7 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     if n:
         _check(ops_library().ss_quantize_rows_int8(_ROWS_CALL(
             x.data_ptr(), stride, out.values.data_ptr(), (k + 15) & -16, out.scales.data_ptr(), n, k, code, activations, 0, 0, 0, 0, 0.0,
-            _stream())), "quantize_rows_int8")
+            error_word(x.device).data_ptr(), _stream())), "quantize_rows_int8")
     return out
 
 
@@ -110,7 +110,7 @@ def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty_strided((n, k), (k, 1), dtype=dtype, device=values.device)
     if n and k:
         _check(ops_library().ss_dequantize_rows_int8(_ROWS_CALL(
-            0, 0, values.data_ptr(), stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, _stream())),
+            0, 0, values.data_ptr(), stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, 0, _stream())),
             "dequantize_rows_int8")
     return out
 
@@ -148,7 +148,8 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
     if n:
         _check(ops_library().ss_add_rmsnorm_int8(_ROWS_CALL(
             residual.data_ptr(), h, out.values.data_ptr(), (h + 15) & -16, out.scales.data_ptr(), n, h, code, 0, to, _ptr(delta) or 0,
-            weight.data_ptr(), weight.dtype is _F32, float(eps), _stream())), "add_rmsnorm_int8")
+            weight.data_ptr(), weight.dtype is _F32, float(eps),
+            error_word(residual.device).data_ptr(), _stream())), "add_rmsnorm_int8")
     return out
 
 

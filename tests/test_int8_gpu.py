@@ -83,6 +83,26 @@ def test_quantize_rows(dtype, width):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width, pad", [(8, 0), (16, 8), (896, 0), (2048, 24), (3584, 0), (4100, 4), (5000, 3), (9736, 0), (12288, 0), (18944, 0), (24576, 0), (30000, 0)])
+def test_quantize_many_rows(dtype, width, pad):
+    """Rows enough for several a block, at widths on both sides of what the copies into shared memory take; a row of zeros, one of
+    infinities and one of NaN among them change no other."""
+    o = ops()
+    x = normal(gen(width), 1301 if width > 9000 else 2600, width + pad, dtype=dtype)[:, :width]
+    x[17], x[300], x[1184] = 0, float("inf"), float("nan")
+    got = o.quantize_rows_int8(x)
+    top = x.float().abs().amax(dim=1, keepdim=True)
+    q = (x.float() * (torch.full_like(top, 127.0) / top)).round()
+    fine = torch.ones(x.shape[0], dtype=torch.bool, device=DEV)
+    fine[[17, 300, 1184]] = False
+    assert torch.equal(got.values[fine], q[fine].to(torch.int8))
+    assert torch.equal(got.scales[fine], (top / torch.full_like(top, 127.0))[fine, 0])
+    assert not got.values[~fine].any() and got.scales[17] == 0 and torch.isnan(got.scales[[300, 1184]]).all()
+    assert torch.equal(o.dequantize_rows_int8(got, dtype)[fine], (got.values.float() * got.scales[:, None]).to(dtype)[fine])
+    o.check_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("width", [33, 3584, 50000])
 def test_quantize_rows_without_a_scale(dtype, width):
     x = normal(gen(1), 9, width, dtype=dtype)
@@ -148,6 +168,36 @@ def test_add_rmsnorm(dtype, w_dtype, width):
         again = o.add_rmsnorm_int8(residual, delta, weight, eps)  # in place
         assert torch.equal(residual, stream)
         assert torch.equal(again.values, got.values) and torch.equal(again.scales, got.scales)
+
+
+@pytest.mark.parametrize("dtype, w_dtype", [(BF16, BF16), (BF16, F32), (F32, F32), (None, BF16)])
+@pytest.mark.parametrize("width", [8, 64, 896, 1540, 3584, 4100, 5120, 8192, 12288, 16384])
+def test_add_rmsnorm_many_rows(dtype, w_dtype, width):
+    o, eps, n = ops(), 1e-6, 1301
+    g = gen(width)
+    residual = normal(g, n, width) * 3
+    delta = None if dtype is None else normal(g, n, width, dtype=dtype)
+    weight = (1 + 0.1 * normal(g, width)).to(w_dtype)
+    residual[17] = 0
+    if delta is not None:
+        delta[17] = 0
+    residual[300, 1], residual[1200, width - 1] = float("inf"), float("nan")
+    stream = residual if delta is None else residual + delta.float()
+    fine = torch.ones(n, dtype=torch.bool, device=DEV)
+    fine[[300, 1200]] = False
+    x = stream.to(F64)
+    v = x / (x.square().mean(dim=1, keepdim=True) + eps).sqrt() * weight.to(F64)
+    out = torch.full_like(residual, 7.0)
+    got = o.add_rmsnorm_int8(residual, delta, weight, eps, residual_out=out)
+    assert torch.equal(out[fine], stream[fine])
+    check_rows(o.Int8Rows(got.values[fine], got.scales[fine]), v[fine], 2.0 ** -17)
+    assert torch.isnan(got.scales[~fine]).all() and not got.values[~fine].any()
+    again = o.add_rmsnorm_int8(residual, delta, weight, eps)  # in place
+    assert torch.equal(residual[fine], stream[fine])
+    assert torch.equal(again.values, got.values) and torch.equal(again.scales[fine], got.scales[fine])
+    few = o.add_rmsnorm_int8(stream[fine][:40].contiguous(), None, weight, eps)  # a row's bytes do not depend on how many there are
+    assert torch.equal(few.values, got.values[fine][:40])
+    o.check_errors(torch.device(DEV))
 
 
 def test_add_rmsnorm_rows_without_a_scale():
