@@ -25,6 +25,7 @@ class ModelOptions:
     dtype: str | None = None  # bfloat16 | float32; None takes config.json's torch_dtype
     max_model_len: int | None = None  # None takes max_position_embeddings
     load_format: str = "safetensors"  # safetensors | random (weights drawn on the device)
+    quantization: str | None = None  # int8: the layers' projections in 8 bits, for architectures that have such layers
 
     def __post_init__(self) -> None:
         if self.dtype is not None and self.dtype not in ("bfloat16", "float32"):
@@ -33,6 +34,8 @@ class ModelOptions:
             raise ValueError("max_model_len must be >= 1")
         if self.load_format not in ("safetensors", "random"):
             raise ValueError(f"unknown load_format: {self.load_format}")
+        if self.quantization not in (None, "int8"):
+            raise ValueError(f"unknown quantization: {self.quantization} (int8)")
 
 
 ModelConfig = ModelOptions  # the reference's name for it (slipstream/core/config.py:25-57)
@@ -108,10 +111,10 @@ class EngineConfig:
                   max_model_len: int | None = None, load_format: str = "safetensors",
                   cache: CacheConfig | None = None, scheduler: SchedulerConfig | None = None,
                   parallel: ParallelConfig | None = None, seed: int = 0,
-                  use_cuda_graphs: bool = True) -> "EngineConfig":
+                  use_cuda_graphs: bool = True, quantization: str | None = None) -> "EngineConfig":
         return cls(
             model=ModelOptions(model_id=model_id, dtype=dtype, max_model_len=max_model_len,
-                               load_format=load_format),
+                               load_format=load_format, quantization=quantization),
             cache=cache if cache is not None else CacheConfig(),
             scheduler=scheduler if scheduler is not None else SchedulerConfig(),
             parallel=parallel if parallel is not None else ParallelConfig(),

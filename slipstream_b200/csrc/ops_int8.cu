@@ -98,8 +98,7 @@ __device__ __forceinline__ void store4(int8_t* q, int left, uint32_t word) {
     for (int e = 0; e < left; ++e) q[e] = (int8_t)(word >> (8 * e));
 }
 
-// The block's largest `top` and the sum of its `sum`, with one barrier; every thread gets both.  The order of the additions
-// depends on the number of threads alone.
+// The block's largest `top` and the sum of its `sum`, with one barrier; every thread gets both.
 __device__ __forceinline__ void block_top_sum(uint32_t& top, float& sum, uint32_t* tops, float* sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     top = __reduce_max_sync(0xffffffffu, top);
@@ -228,6 +227,38 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict
 // x = residual + delta, written to residual_out (if there is one); v = x / sqrt(mean(x^2) + eps) * w, as int8 rows.  The norm's
 // factor is the same for the whole row, so q is that of x * w, and the factor enters the scale alone: the squares' sum and the
 // largest |x * w| are found in one pass with one barrier, and v is never rounded to fewer than its 24 bits.
+// The squares' sum does not depend on how many rows there are, whatever shape the launch takes for them: the sums of 32 neighbouring
+// groups of four (a warp's, one group a lane) are formed first, then lane l adds sums l, l + 32, ... of the row, then the lanes.
+__device__ __forceinline__ float squares_of(const float (&v)[4]) {
+    return fmaf(v[3], v[3], fmaf(v[2], v[2], fmaf(v[1], v[1], v[0] * v[0])));
+}
+// The warp's sums of NG values a thread, sum i to sums[i * stride].  At every level half of the sums that are left go to the other
+// half of the lanes (P values in P + log2(32 / P) shuffles, not 5 P); a sum adds the same pairs as warp_sum does.
+template <int NG>
+__device__ __forceinline__ void warp_sums(const float (&part)[NG], float* sums, int stride) {
+    constexpr int P = NG == 1 ? 1 : NG == 2 ? 2 : NG <= 4 ? 4 : NG <= 8 ? 8 : 16, STEP = 32 / P;
+    const int lane = threadIdx.x & 31;
+    float a[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) a[i] = i < NG ? part[i] : 0.f;
+    int w = 16;
+#pragma unroll
+    for (int n = P / 2; n >= 1; n /= 2, w /= 2) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float send = lane & w ? a[i] : a[i + n], keep = lane & w ? a[i + n] : a[i];
+            a[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+        }
+    }
+#pragma unroll
+    for (; w >= 1; w /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], w);
+    if (lane % STEP == 0 && lane / STEP < NG) sums[lane / STEP * stride] = a[0];
+}
+__device__ __forceinline__ float sum_of_sums(const float* sums, int width) {
+    float total = 0.f;
+    for (int c = threadIdx.x & 31; c < (width + 127) / 128; c += 32) total += sums[c];
+    return warp_sum(total);
+}
 __device__ __forceinline__ float norm_scale(uint32_t top, float squares, int width, float eps) {
     const float rstd = 1.0f / sqrtf(squares / (float)width + eps);
     return top < INF_BITS ? __fdiv_rn(__uint_as_float(top) * rstd, 127.f) : __uint_as_float(0x7fffffffu);
@@ -241,9 +272,10 @@ add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, floa
     // few rows: the weights do not depend on the kernels in front and are on the way before those are through
     constexpr bool EARLY_W = NG == 1 || NG == 2;
     __shared__ uint32_t tops[32];
-    __shared__ float sums[32];
+    __shared__ float sums[NG ? 32 * NG : 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
-    float w[EARLY_W ? NG : 1][4], v[NG ? NG : 1][4];
+    float w[EARLY_W ? NG : 1][4], v[NG ? NG : 1][4], part[NG ? NG : 1];
     auto load_w = [&](int j, float (&to)[4]) {
         if (w_f32) load4<ALIGNED>((const float*)weight + j, width - j, to);
         else load4<ALIGNED>((const bf16*)weight + j, width - j, to);
@@ -286,13 +318,17 @@ add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, floa
             if (residual_out && j < width) store_x(j, v[i]);
             float (&wi)[4] = w[EARLY_W ? i : 0];
             if constexpr (!EARLY_W) load_w(j, wi);
+            part[i] = squares_of(v[i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                ss = fmaf(v[i][e], v[i][e], ss);
-                v[i][e] *= wi[e];
-            }
+            for (int e = 0; e < 4; ++e) v[i][e] *= wi[e];
             top = top_of(top, v[i]);
         }
+        warp_sums(part, sums + warp, blockDim.x >> 5);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+        top = __reduce_max_sync(0xffffffffu, lane < (blockDim.x >> 5) ? tops[lane] : 0u);
+        ss = sum_of_sums(sums, width);
     } else {
         for (int j = threadIdx.x * 4; j < width; j += blockDim.x * 4) {
             load_x(j, delta != nullptr, v[0]);
@@ -305,8 +341,8 @@ add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, floa
             }
             top = top_of(top, v[0]);
         }
+        block_top_sum(top, ss, tops, sums);
     }
-    block_top_sum(top, ss, tops, sums);
     const RowScale r = row_scale(top);
     if (threadIdx.x == 0) scales[blockIdx.x] = norm_scale(top, ss, width, eps);
     if constexpr (NG > 0) {
@@ -436,7 +472,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* __restrict__ delta,
                              int stages, int* err) {
     extern __shared__ __align__(128) unsigned char ring_smem[];
     __shared__ uint32_t tops[2][RING_THREADS / 32];
-    __shared__ float sums[2][RING_THREADS / 32];
+    __shared__ float sums[2][NG * RING_THREADS / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int x_bytes = width * 4, d_bytes = delta ? width * (int)sizeof(T) : 0, bytes = x_bytes + d_bytes;
     const RowRing ring = row_ring(ring_smem, stages, bytes);
@@ -462,7 +498,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* __restrict__ delta,
         mbar_wait(&ring.full[s], parity, ring.gave_up);
         const float* from = reinterpret_cast<const float*>(ring.rows + s * bytes);
         const T* from_d = reinterpret_cast<const T*>(ring.rows + s * bytes + x_bytes);
-        float v[NG][4], ss = 0.f;
+        float v[NG][4], part[NG];
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -476,21 +512,22 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* __restrict__ delta,
                     for (int e = 0; e < 4; ++e) v[i][e] = __fadd_rn(v[i][e], d[e]);
                 }
                 if (residual_out) *reinterpret_cast<float4*>(residual_out + row * width + j) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    ss = fmaf(v[i][e], v[i][e], ss);
-                    v[i][e] *= w[i][e];
-                }
-                top = top_of(top, v[i]);
+                for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
             }
+            part[i] = squares_of(v[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] *= w[i][e];
+            top = top_of(top, v[i]);
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        ss = warp_sum(ss);
-        if (lane == 0) { tops[n & 1][warp] = top; sums[n & 1][warp] = ss; }
+        warp_sums(part, sums[n & 1] + warp, RING_THREADS / 32);
+        if (lane == 0) tops[n & 1][warp] = top;
         __syncthreads();
         if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
         top = __reduce_max_sync(0xffffffffu, lane < RING_THREADS / 32 ? tops[n & 1][lane] : 0u);
-        ss = warp_sum(lane < RING_THREADS / 32 ? sums[n & 1][lane] : 0.f);
+        const float ss = sum_of_sums(sums[n & 1], width);
         const RowScale r = row_scale(top);
         if (threadIdx.x == 0) scales[row] = norm_scale(top, ss, width, eps);
         int8_t* out = q + row * q_stride;

@@ -114,7 +114,7 @@ class LLMEngine:
         self.runner = ModelRunner(
             m.model_id, dtype=m.dtype, page_size=c.block_size, num_pages=c.num_gpu_blocks,
             gpu_memory_utilization=c.gpu_memory_utilization, max_num_seqs=s.max_num_seqs,
-            max_model_len=m.max_model_len, load_format=m.load_format, seed=config.seed,
+            max_model_len=m.max_model_len, load_format=m.load_format, quantization=m.quantization, seed=config.seed,
             use_cuda_graphs=config.use_cuda_graphs,
             max_step_tokens=min(s.max_num_batched_tokens,
                                 s.prefill_chunk_size if s.enable_chunked_prefill else s.max_num_batched_tokens))
@@ -465,7 +465,7 @@ class LLM:
                  block_size: int = 16, num_gpu_blocks: int | None = None, gpu_memory_utilization: float = 0.9,
                  max_num_seqs: int = 256, max_num_batched_tokens: int = 8192, prefill_chunk_size: int = 256,
                  enable_chunked_prefill: bool = True, seed: int = 0, load_format: str = "safetensors",
-                 use_cuda_graphs: bool = True) -> None:
+                 use_cuda_graphs: bool = True, quantization: str | None = None) -> None:
         self.engine = LLMEngine(EngineConfig.for_model(
             model, dtype=dtype, max_model_len=max_model_len, load_format=load_format,
             cache=CacheConfig(block_size=block_size, gpu_memory_utilization=gpu_memory_utilization,
@@ -473,7 +473,7 @@ class LLM:
             scheduler=SchedulerConfig(max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens,
                                       enable_chunked_prefill=enable_chunked_prefill,
                                       prefill_chunk_size=prefill_chunk_size),
-            seed=seed, use_cuda_graphs=use_cuda_graphs))
+            seed=seed, use_cuda_graphs=use_cuda_graphs, quantization=quantization))
 
     def generate(self, prompts: list[str] | None = None, sampling_params: SamplingParams | list[SamplingParams] | None = None,
                  *, prompt_token_ids: list[list[int]] | None = None) -> list[RequestOutput]:

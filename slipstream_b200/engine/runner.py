@@ -38,12 +38,13 @@ class ModelRunner:
                  num_pages: "int | list[int] | None" = None, gpu_memory_utilization: float = 0.9,
                  max_num_seqs: int = 256, max_model_len: int | None = None, load_format: str = "safetensors",
                  seed: int = 0, device: str | torch.device = "cuda:0", use_cuda_graphs: bool = True,
-                 max_step_tokens: int | None = None) -> None:
+                 max_step_tokens: int | None = None, quantization: str | None = None) -> None:
         """``page_size``: tokens per page for cache groups whose mixers do not ask for a size of their own.
         ``num_pages``: pages of that size the cache should hold (groups with another page size get as many pages
         as hold the same tokens; a windowed group at most what ``max_num_seqs`` requests can keep of their windows
         when a step feeds up to ``max_step_tokens`` tokens of a request), or one count per cache group, or None
-        to size the pools from the free device memory."""
+        to size the pools from the free device memory.  ``quantization`` "int8": the layers' projections run in 8 bits
+        (``parts/int8.py``), their weights rounded here from the checkpoint's."""
         ops.require_cuda()
         self.device = torch.device(device)
         if self.device.type == "cuda":
@@ -58,7 +59,8 @@ class ModelRunner:
         self.page_size = page_size
         self.max_num_seqs = max_num_seqs
 
-        self.model = self.architecture.build(self.config)
+        self.quantization = quantization
+        self.model = self.architecture.build_model(self.config, quantization)
         specs = self.model.weight_specs()
         if load_format == "random":
             weights = random_weights_on_device(specs, self.runtime, seed)

@@ -24,6 +24,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
     p.add_argument("--max-model-len", type=int, default=None)
     p.add_argument("--load-format", choices=["safetensors", "random"], default="safetensors")
+    p.add_argument("--quantization", choices=["int8"], default=None,
+                   help="run the layers' projections in 8-bit integers (weights rounded at load, activations token by token)")
     p.add_argument("--seed", type=int, default=0, help="engine seed (random weights, unseeded requests)")
     # cache
     p.add_argument("--block-size", type=int, default=16)
@@ -88,7 +90,7 @@ def main(argv: list[str] | None = None) -> int:
               max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
               prefill_chunk_size=args.prefill_chunk_size,
               enable_chunked_prefill=not args.disable_chunked_prefill, seed=args.seed,
-              load_format=args.load_format)
+              load_format=args.load_format, quantization=args.quantization)
     if prompts_ids:
         outs = llm.generate(prompt_token_ids=prompts_ids, sampling_params=params)
     else:

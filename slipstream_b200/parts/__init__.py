@@ -9,6 +9,7 @@ from .differential import DifferentialAttention
 from .embedding import LMHead, SummedEmbedding, TokenEmbedding
 from .mlp import GELU_TANH, ActivatedFeedForward, GatedFeedForward, SwiGLUFeedForward
 from .experts import RoutedExperts
+from .int8 import Int8PagedAttention, Int8RMSNorm, Int8SwiGLUFeedForward
 from .norm import GroupRMSNorm, JoiningNorm, NormedBranch, RMSNorm, StreamRounding
 from .state_space import StateSpaceMixer
 from .recurrent import (ConvolvedInput, DecayedLinearAttention, GatedLinearRecurrenceMixer, GatedRecurrenceMixer,
@@ -25,4 +26,4 @@ __all__ = ["BLOCKS", "EMBEDDINGS", "HEADS", "Embedding", "Head", "FEED_FORWARDS"
            "StateSpaceMixer", "SummedEmbedding", "ActivatedFeedForward", "ConvolvedInput", "GatedRecurrenceMixer",
            "MatrixMemoryMixer", "LatentAttention", "ParallelBlock", "DecayedLinearAttention", "GatedLinearRecurrenceMixer",
            "ParallelMixers", "SandwichBlock", "DifferentialAttention", "GELU_TANH", "JoiningNorm", "NormedBranch",
-           "BandedRotaryEncoding"]
+           "BandedRotaryEncoding", "Int8PagedAttention", "Int8RMSNorm", "Int8SwiGLUFeedForward"]

@@ -346,6 +346,16 @@ class PagedAttention(Mixer):
         write into the decode kernel is off for it, since that kernel takes the projection output as it is."""
         return None
 
+    def project(self, x: torch.Tensor) -> torch.Tensor:
+        """The stacked projection of the layer's input."""
+        return ops.linear(x, self.qkv_weight, self.qkv_b)
+
+    def project_out(self, out: torch.Tensor, into: IntoNorm | None):
+        """The output projection of the concatenated heads, and the norm behind it where ``into`` asks for that."""
+        if into is not None:
+            return into.close(out, self.o_weight, self.o_b)
+        return ops.linear(out, self.o_weight, self.o_b)
+
     def _check_spread(self, layer: LayerBinding) -> None:
         if not layer.writes_cache:
             raise ValueError(f"{self.name}: a layer with keys and values of its own writes its pages")
@@ -354,7 +364,7 @@ class PagedAttention(Mixer):
 
     def forward(self, x: torch.Tensor, ctx, layer: LayerBinding, into: IntoNorm | None = None) -> torch.Tensor:
         meta = ctx.groups[layer.group]
-        qkv = ops.linear(x, self.qkv_weight, self.qkv_b)
+        qkv = self.project(x)
         plain_projection = type(self).after_projection is PagedAttention.after_projection
         if not plain_projection:
             self.after_projection(qkv, ctx)
@@ -414,6 +424,4 @@ class PagedAttention(Mixer):
         if self.rotate_values:
             ops.turn_heads(out, ctx.positions, self.value_inv_freq, self.num_heads, self.head_dim, self.value_dim,
                            interleaved=getattr(self.position_encoding, "interleaved", False), sign=-1.0)
-        if into is not None:
-            return into.close(out, self.o_weight, self.o_b)
-        return ops.linear(out, self.o_weight, self.o_b)
+        return self.project_out(out, into)

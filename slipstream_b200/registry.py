@@ -3,7 +3,8 @@
 ``config.json``'s ``architectures[0]`` (or a single ``architecture`` string) picks
 the entry; a folder without that key falls back on ``model_type`` (the reference dispatches on ``model_type`` alone,
 slipstream/models/loader.py:50-55).  Another architecture is added with
-``register_architecture(name, ConfigClass, builder, model_types=(...))``.
+``register_architecture(name, ConfigClass, builder, model_types=(...))``; a builder that takes ``quantization=`` names the values
+that it knows (``quantizations=("int8",)``).
 """
 
 from __future__ import annotations
@@ -19,18 +20,28 @@ from slipstream_b200.config.model_config import ConfigError, ModelConfigBase, Qw
 class Architecture:
     name: str
     config_class: type
-    build: Callable[[Any], Any]
+    build: Callable[..., Any]
     model_types: tuple[str, ...] = ()
+    quantizations: tuple[str, ...] = ()  # values of ``quantization=`` that ``build`` takes
+
+    def build_model(self, config: Any, quantization: str | None = None) -> Any:
+        """The model of ``config``, its layers in the given precision (None: that of the runtime)."""
+        if quantization is None:
+            return self.build(config)
+        if quantization not in self.quantizations:
+            known = ", ".join(self.quantizations) or "none"
+            raise ConfigError(f"{self.name} has no quantization {quantization!r} (known: {known})")
+        return self.build(config, quantization=quantization)
 
 
 _ARCHITECTURES: dict[str, Architecture] = {}
 
 
-def register_architecture(name: str, config_class: type, build: Callable[[Any], Any],
-                          model_types: tuple[str, ...] = ()) -> None:
+def register_architecture(name: str, config_class: type, build: Callable[..., Any],
+                          model_types: tuple[str, ...] = (), quantizations: tuple[str, ...] = ()) -> None:
     if name in _ARCHITECTURES:
         raise KeyError(f"architecture {name!r} is already registered")
-    _ARCHITECTURES[name] = Architecture(name, config_class, build, tuple(model_types))
+    _ARCHITECTURES[name] = Architecture(name, config_class, build, tuple(model_types), tuple(quantizations))
 
 
 def unregister_architecture(name: str) -> None:
@@ -86,7 +97,7 @@ def _register_builtin() -> None:
     from slipstream_b200.config.sazepel_config import SazepelConfig
     from slipstream_b200.models.sazepel import build_sazepel
 
-    register_architecture("Qwen2ForCausalLM", Qwen2Config, build_qwen2, model_types=("qwen2", "qwen"))
+    register_architecture("Qwen2ForCausalLM", Qwen2Config, build_qwen2, model_types=("qwen2", "qwen"), quantizations=("int8",))
     register_architecture("Fokedra", FokedraConfig, build_fokedra)
     register_architecture("Sarudra", SarudraConfig, build_sarudra)
     register_architecture("Bezutar", BezutarConfig, build_bezutar)

@@ -2,7 +2,7 @@
 
 Tolerances, from the formulas.  A row's scale is a / 127 in one float32 division: half a unit in the last place, 2^-24.  A value
 lands on the nearest step but for the rounding of v * (127 / a), two roundings of a number up to 127: at most 0.5 + 127 * 2^-23
-steps off.  The norm adds the error of its factor: a float32 sum of up to 2^17 squares in at most 110 additions a term (110 *
+steps off.  The norm adds the error of its factor: a float32 sum of squares in at most 110 additions a term (110 *
 2^-24 of the sum, half of it in the root) and six single roundings, below 2^-17 of a value.  The sums of products are whole
 numbers: what follows them is three float32 operations in a fixed order, so linear outputs are compared bit for bit.  The gated
 unit's exponential and division are off by a few 2^-22 in the approximate form that bfloat16 outputs take, far below that type's
@@ -195,8 +195,9 @@ def test_add_rmsnorm_many_rows(dtype, w_dtype, width):
     again = o.add_rmsnorm_int8(residual, delta, weight, eps)  # in place
     assert torch.equal(residual[fine], stream[fine])
     assert torch.equal(again.values, got.values) and torch.equal(again.scales[fine], got.scales[fine])
-    few = o.add_rmsnorm_int8(stream[fine][:40].contiguous(), None, weight, eps)  # a row's bytes do not depend on how many there are
-    assert torch.equal(few.values, got.values[fine][:40])
+    for rows in (1, 40, 400):  # a row does not depend on how many there are
+        few = o.add_rmsnorm_int8(stream[fine][:rows].contiguous(), None, weight, eps)
+        assert torch.equal(few.values, got.values[fine][:rows]) and torch.equal(few.scales, got.scales[fine][:rows])
     o.check_errors(torch.device(DEV))
 
 
