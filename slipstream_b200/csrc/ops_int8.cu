@@ -255,8 +255,10 @@ __device__ __forceinline__ void warp_sums(const float (&part)[NG], float* sums, 
     if (lane % STEP == 0 && lane / STEP < NG) sums[lane / STEP * stride] = a[0];
 }
 __device__ __forceinline__ float sum_of_sums(const float* sums, int width) {
-    float total = 0.f;
-    for (int c = threadIdx.x & 31; c < (width + 127) / 128; c += 32) total += sums[c];
+    const int sets = (width + 127) / 128;
+    int c = threadIdx.x & 31;
+    float total = c < sets ? sums[c] : 0.f;
+    for (c += 32; c < sets; c += 32) total += sums[c];
     return warp_sum(total);
 }
 __device__ __forceinline__ float norm_scale(uint32_t top, float squares, int width, float eps) {

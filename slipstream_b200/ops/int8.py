@@ -21,7 +21,7 @@ from struct import Struct
 
 import torch
 
-from .functions import KernelError, _check, _code, _need, _ptr, _stream, error_word, gemm_library, ops_library, sm_count
+from .functions import KernelError, _check, _code, _get_device, _need, _stream, error_word, gemm_library, ops_library, sm_count
 
 RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
 MAX_K = 133143  # 127^2 K stays below 2^31
@@ -56,15 +56,46 @@ class Int8Rows:
         return dequantize_rows_int8(self, dtype)
 
 
+class _Device:
+    """What the calls ask of a device: its multiprocessors, where its error word is, and how many clusters of 1 to 8 blocks of the
+    product of few tokens it holds at the same time, with its ring sized for one block an SM and for two."""
+
+    def __init__(self, device: torch.device) -> None:
+        self.sms = sm_count(device)
+        self.error_ptr = error_word(device).data_ptr()  # (the word lives as long as the process)
+        ops, gemm = ops_library(), gemm_library()
+        self.quantize, self.dequantize, self.norm = ops.ss_quantize_rows_int8, ops.ss_dequantize_rows_int8, ops.ss_add_rmsnorm_int8
+        self.product = gemm.ss_gemm_int8
+        self.resident = tuple(tuple(gemm.ss_gemm_int8_resident(n, per) or self.sms * per // n for n in range(1, 9)) for per in (1, 2))
+
+
+_devices: dict[torch.device, _Device] = {}
+
+
+def _device(device: torch.device) -> _Device:
+    with torch.cuda.device(device):
+        found = _devices[device] = _Device(device)
+    return found
+
+
+# torch's short way to an allocation on the current device (0.85 us where torch.empty_strided takes 1.5), where it has one
+_empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def _empty(shape: tuple[int, ...], stride: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if _empty_here is not None and _get_device is not None and device.index == _get_device():
+        return _empty_here(shape, stride, dtype)
+    return torch.empty_strided(shape, stride, dtype=dtype, device=device)
+
+
 def int8_rows_like(rows: int, width: int, device: torch.device) -> Int8Rows:
     """Int8 rows with nothing in them yet."""
-    values = torch.empty_strided((rows, width), ((width + 15) & -16, 1), dtype=_I8, device=device)
-    return Int8Rows(values, torch.empty_strided((rows,), (1,), dtype=_F32, device=device))
+    return Int8Rows(_empty((rows, width), ((width + 15) & -16, 1), _I8, device), _empty((rows,), (1,), _F32, device))
 
 
-def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int]:
-    """(rows, width, stride) of int8 rows that the kernels take."""
-    if not isinstance(r, Int8Rows):
+def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int, int]:
+    """(rows, width, stride, address) of int8 rows that the kernels take."""
+    if type(r) is not Int8Rows:
         raise KernelError(f"{what} must be Int8Rows, not {type(r).__name__}")
     v, s = r.values, r.scales
     if v.dim() != 2 or v.dtype is not _I8 or not v.is_cuda:
@@ -75,14 +106,15 @@ def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int]:
     stride, step = v.stride()
     if n < 2:
         stride = (k + 15) & -16
-    if n and k and (step != 1 and k > 1 or stride & 15 or stride < k or v.data_ptr() & 15):
+    at = v.data_ptr()
+    if n and k and (step != 1 and k > 1 or stride & 15 or stride < k or at & 15):
         raise KernelError(f"{what}: rows must be contiguous and start on 16 bytes (a stride that is a multiple of 16), got strides {v.stride()}")
-    return n, k, stride
+    return n, k, stride, at
 
 
 def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Rows:
     """The rows of ``x`` (float32 or bfloat16 [N, K], any row stride) as int8 rows: ``a = max |x_n|``, ``scale = a / 127``,
-    ``q = rint(x * (127 / a))``, ties to even.  Tokens of activations, or output features of a weight.
+    ``q = rint(x * (127 / a))`` in float32, ties to even.  Tokens of activations, or output features of a weight.
 
     ``activations``: the rows are a product's activations, not its weights, and the kernel behind may start early."""
     if not x.is_cuda or x.dim() != 2:
@@ -93,25 +125,24 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     stride, step = x.stride()
     if k > 1 and step != 1:
         raise KernelError(f"the rows of x must be contiguous, got strides {x.stride()}")
-    code = _code(x.dtype)
-    out = int8_rows_like(n, k, x.device)
+    code, device, q_stride = _code(x.dtype), x.device, (k + 15) & -16
+    values, scales = _empty((n, k), (q_stride, 1), _I8, device), _empty((n,), (1,), _F32, device)
     if n:
-        _check(ops_library().ss_quantize_rows_int8(_ROWS_CALL(
-            x.data_ptr(), stride, out.values.data_ptr(), (k + 15) & -16, out.scales.data_ptr(), n, k, code, activations, 0, 0, 0, 0, 0.0,
-            error_word(x.device).data_ptr(), _stream())), "quantize_rows_int8")
-    return out
+        d = _devices.get(device) or _device(device)
+        _check(d.quantize(_ROWS_CALL(x.data_ptr(), stride, values.data_ptr(), q_stride, scales.data_ptr(), n, k, code, activations, 0, 0, 0, 0,
+                                     0.0, d.error_ptr, _stream())), "quantize_rows_int8")
+    return Int8Rows(values, scales)
 
 
 def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
     """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once."""
-    n, k, stride = _need_rows(rows, "rows")
-    code = _code(dtype)
-    values = rows.values
-    out = torch.empty_strided((n, k), (k, 1), dtype=dtype, device=values.device)
+    n, k, stride, at = _need_rows(rows, "rows")
+    code, device = _code(dtype), rows.values.device
+    out = _empty((n, k), (k, 1), dtype, device)
     if n and k:
-        _check(ops_library().ss_dequantize_rows_int8(_ROWS_CALL(
-            0, 0, values.data_ptr(), stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, 0, _stream())),
-            "dequantize_rows_int8")
+        d = _devices.get(device) or _device(device)
+        _check(d.dequantize(_ROWS_CALL(0, 0, at, stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, 0, _stream())),
+               "dequantize_rows_int8")
     return out
 
 
@@ -121,61 +152,38 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
     ``x / sqrt(mean(x^2) + eps) * weight`` of the new stream, formed in float32, as int8 rows.
 
     ``residual_out`` (float32 [N, H]) gets the new stream instead, and ``residual`` stays as it is.  ``weight`` is bfloat16 or
-    float32."""
+    float32.  A row's result does not depend on the other rows, nor on how many there are."""
     _need(residual, _F32, "residual")
-    if residual.dim() != 2:
-        raise KernelError(f"residual must be [tokens, features], got {tuple(residual.shape)}")
-    n, h = residual.shape
-    if h < 1:
-        raise KernelError("rows without elements have no norm")
-    code = 1
+    shape = residual.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise KernelError(f"residual must be [tokens, features], got {tuple(shape)}")
+    n, h = shape
+    from_ptr = residual.data_ptr()
+    code, delta_ptr, to = 1, 0, 0
     if delta is not None:
         _need(delta, None, "delta")
-        code = _code(delta.dtype)
-        if delta.shape != residual.shape:
-            raise KernelError(f"delta {tuple(delta.shape)} does not match residual {tuple(residual.shape)}")
+        code, delta_ptr, to = _code(delta.dtype), delta.data_ptr(), from_ptr
+        if delta.shape != shape:
+            raise KernelError(f"delta {tuple(delta.shape)} does not match residual {tuple(shape)}")
     _need(weight, None, "norm weight")
-    if weight.numel() != h or weight.dtype not in (_BF16, _F32):
+    w_dtype = weight.dtype
+    if weight.numel() != h or (w_dtype is not _BF16 and w_dtype is not _F32):
         raise KernelError("norm weight has the wrong size or dtype")
     if residual_out is not None:
         _need(residual_out, _F32, "residual_out")
-        if residual_out.shape != residual.shape:
-            raise KernelError(f"residual_out {tuple(residual_out.shape)} does not match residual {tuple(residual.shape)}")
+        if residual_out.shape != shape:
+            raise KernelError(f"residual_out {tuple(residual_out.shape)} does not match residual {tuple(shape)}")
         to = residual_out.data_ptr()
-    else:
-        to = residual.data_ptr() if delta is not None else 0
-    out = int8_rows_like(n, h, residual.device)
+    device, q_stride = residual.device, (h + 15) & -16
+    values, scales = _empty((n, h), (q_stride, 1), _I8, device), _empty((n,), (1,), _F32, device)
     if n:
-        _check(ops_library().ss_add_rmsnorm_int8(_ROWS_CALL(
-            residual.data_ptr(), h, out.values.data_ptr(), (h + 15) & -16, out.scales.data_ptr(), n, h, code, 0, to, _ptr(delta) or 0,
-            weight.data_ptr(), weight.dtype is _F32, float(eps),
-            error_word(residual.device).data_ptr(), _stream())), "add_rmsnorm_int8")
-    return out
+        d = _devices.get(device) or _device(device)
+        _check(d.norm(_ROWS_CALL(from_ptr, h, values.data_ptr(), q_stride, scales.data_ptr(), n, h, code, 0, to, delta_ptr, weight.data_ptr(),
+                                 w_dtype is _F32, eps, d.error_ptr, _stream())), "add_rmsnorm_int8")
+    return Int8Rows(values, scales)
 
 
 # --------------------------------------------------------------------------- products
-
-class _Device:
-    """What the products ask of a device: its multiprocessors, where its error word is, and how many clusters of 1 to 8 blocks of
-    the kernel for few tokens it holds at the same time, with its ring sized for one block an SM and for two."""
-
-    def __init__(self, device: torch.device) -> None:
-        self.sms = sm_count(device)
-        self.error_ptr = error_word(device).data_ptr()  # (the word lives as long as the process)
-        lib = gemm_library()
-        self.resident = tuple(tuple(lib.ss_gemm_int8_resident(n, per) or self.sms * per // n for n in range(1, 9)) for per in (1, 2))
-
-
-_devices: dict[torch.device, _Device] = {}
-
-
-def _device(device: torch.device) -> _Device:
-    found = _devices.get(device)
-    if found is None:
-        with torch.cuda.device(device):
-            found = _devices[device] = _Device(device)
-    return found
-
 
 def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
               resident: tuple[tuple[int, ...], tuple[int, ...]] | None = None) -> tuple[int, int, int, int]:
@@ -242,8 +250,8 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
 
 def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype: torch.dtype, gated: bool, columns: int | None,
              plan: tuple[int, int, int, int] | None, what: str) -> torch.Tensor:
-    tokens, k, ldx = _need_rows(x, "x")
-    features, k_w, ldw = _need_rows(weight, "weight")
+    tokens, k, ldx, x_ptr = _need_rows(x, "x")
+    features, k_w, ldw, w_ptr = _need_rows(weight, "weight")
     if k_w != k:
         raise KernelError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
     if not 1 <= k <= MAX_K:
@@ -264,16 +272,16 @@ def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype
             raise KernelError("bias has the wrong size or dtype")
         bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is _F32
     device = x.values.device
-    if weight.values.device != device:
+    if weight.values.get_device() != device.index:
         raise KernelError(f"x is on {device}, weight on {weight.values.device}")
-    out = torch.empty_strided((tokens, columns), (columns, 1), dtype=out_dtype, device=device)
+    out = _empty((tokens, columns), (columns, 1), out_dtype, device)
     if tokens == 0 or columns == 0:
         return out
-    d = _device(device)
+    d = _devices.get(device) or _device(device)
     many, tile, slices, per_sm = plan or int8_plan(tokens, features, k, d.sms, gated, d.resident)
-    _check(gemm_library().ss_gemm_int8(_PRODUCT_CALL(
-        x.values.data_ptr(), ldx, x.scales.data_ptr(), weight.values.data_ptr(), ldw, weight.scales.data_ptr(), bias_ptr, bias_f32,
-        out.data_ptr(), columns, out_f32, tokens, features, k, gated, columns, many, tile, slices, per_sm, d.error_ptr, _stream())), what)
+    _check(d.product(_PRODUCT_CALL(x_ptr, ldx, x.scales.data_ptr(), w_ptr, ldw, weight.scales.data_ptr(), bias_ptr, bias_f32, out.data_ptr(),
+                                   columns, out_f32, tokens, features, k, gated, columns, many, tile, slices, per_sm, d.error_ptr,
+                                   _stream())), what)
     return out
 
 
