@@ -1,7 +1,7 @@
 // Matrix product of 8-bit integers on the 5th-generation tensor cores of sm_100a:
 //   Y[m, n] = (sum_k X[m, k] * W[n, k]) * x_scale[m] * w_scale[n] (+ bias[n])
 // X: activations, one row and one scale a token; W: weights, one row and one scale an output feature; both int8 and K-major.
-// The sum is exact: products and additions are 32-bit integers (tcgen05.mma kind::i8; 127^2 K < 2^31 up to K = 133,143), so a
+// The sum is exact: products and additions are 32-bit integers (tcgen05.mma kind::i8; 2^14 K < 2^31 up to K = 131,071, whatever the bytes), so a
 // result does not depend on how K is cut, on the kernel or on what else is in the batch.  What follows is float32: the sum is
 // converted (one rounding from 2^24 on), multiplied by the token's scale, then by the feature's, then the bias is added, and
 // the result is rounded once to the output type.  The gated form pairs the features of a feed-forward's gate and up matrices
@@ -14,7 +14,7 @@
 //
 // Tensor memory is taken BEHIND griddepcontrol.wait, and the kernel behind is let go only when it has been taken: a kernel
 // that takes it before the kernel in front is through, or lets a kernel start that may take it first, can wait for a block
-// that waits for it.
+// that waits for it.  Before that wait a block reads only the weights, their scales and the bias, which it takes for constant.
 
 #include <cuda.h>
 
@@ -37,7 +37,7 @@ struct Int8Args {
     int out_f32, bias_f32, gated;
     int bn;                // few tokens: the tokens of a tile; many tokens: the features of a tile
     int stages, slices;
-    int wide_copies;        // many tokens: the two steps of a stage come in one copy (K is a multiple of 128)
+    int wide_copies;       // many tokens: the two steps of a stage come in one copy (K is a multiple of 128)
 };
 
 __device__ __forceinline__ void i8_load(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
@@ -239,7 +239,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
         if (n_sl > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         pdl_wait();  // the output may still be in use by the kernels in front, which also wrote the tokens' scales
-        for (int i = threadIdx.x - 64; i < live; i += 128) xs_s[i] = __ldg(g.x_scale + t0 + i);
+        for (int i = threadIdx.x - 64; i < live; i += 128) xs_s[i] = g.x_scale[t0 + i];
         asm volatile("bar.sync 2, 160;" ::: "memory");  // the scales are there, and the tensor memory's address
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(quarter * 32) << 16);
@@ -369,7 +369,7 @@ __device__ __forceinline__ void i8_values32(uint32_t (&r)[32], float xs, const f
     }
 }
 // A warp's 32 tokens x 32 outputs, a token a thread, through 2 KB of shared memory of the warp's own, so that it writes whole
-// 64-byte runs of a row instead of 16 bytes of 32 rows at a time (2,048 x 3,584 x 9,472: <TIME>).  Rows of 64 bytes lie in `stage`
+// 64-byte runs of a row instead of 16 bytes of 32 rows at a time (2,048 x 3,584 x 9,472: 49.8 to 46.3 us).  Rows of 64 bytes lie in `stage`
 // with their four 16-byte pieces turned by (row / 2) % 4, which keeps both directions free of bank conflicts.
 __device__ __forceinline__ void i8_write_run(const Int8Args& g, unsigned char* stage, const uint32_t (&w)[16], int m0, int f, int width) {
     const int lane = threadIdx.x & 31, size = g.out_f32 ? 4 : 2;
@@ -538,7 +538,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             const bool in = col < bn && n0 + col < g.features;
             ws[col] = in ? __ldg(g.w_scale + n0 + col) : 0.f;
             bs[col] = in && g.bias ? i8_bias(g, n0 + col) : 0.f;
-            const float xs = m < g.tokens ? __ldg(g.x_scale + m) : 0.f;
+            const float xs = m < g.tokens ? g.x_scale[m] : 0.f;
             // (a buffer is written again two tiles later, behind the barrier that every warp reaches when it is through with it)
             asm volatile("bar.sync 1, 256;" ::: "memory");
             // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
@@ -655,14 +655,14 @@ static int launch_many(const Int8Call& c, Int8Args& g) {
     return SS_LAUNCH_CHECK();
 }
 
-// Row strides are multiples of 16 bytes and bases stand on 16 bytes; K <= 133,143.
+// Row strides are multiples of 16 bytes and bases stand on 16 bytes; K <= 131,071.
 // gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
 // many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for.
 // many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
 extern "C" int ss_gemm_int8(const Int8Call* call) {
     const Int8Call& c = *call;
     if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
-    if (c.tokens > INT32_MAX - 256 || c.features > INT32_MAX - 256 || c.K <= 0 || c.K > 133143 || c.ldx % 16 || c.ldw % 16 || c.ldx < c.K || c.ldw < c.K) return -2003;
+    if (c.tokens > INT32_MAX - 256 || c.features > INT32_MAX - 256 || c.K <= 0 || c.K > 131071 || c.ldx % 16 || c.ldw % 16 || c.ldx < c.K || c.ldw < c.K) return -2003;
     if (((uintptr_t)c.x & 15) || ((uintptr_t)c.w & 15) || ((uintptr_t)c.out & 15)) return -2004;
     if (c.gated ? (c.features % 128 || c.out_features > c.features / 2) : c.out_features != c.features) return -2005;
     const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;

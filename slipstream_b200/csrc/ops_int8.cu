@@ -7,7 +7,9 @@
 //
 // Rows of q start on 16 bytes (their stride is a multiple of 16); what lies between a row's end and the next row is not written.
 //
-// All three kernels are bound by memory: a row is read once, into registers, and its results are written from there.
+// All kernels are bound by memory: a row is read once, and its results are written from registers.  What a kernel reads may be written
+// while it has already been launched (it waits, griddepcontrol.wait), so those pointers are not __restrict__: the loads must not go
+// through the read-only path.
 
 #include "tc5.cuh"
 
@@ -177,7 +179,7 @@ struct RawVec {
 
 template <typename T, bool ALIGNED, int NG>
 __global__ void __launch_bounds__(most_threads<NG>())
-quantize_rows_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales,
+quantize_rows_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales,
                      int width, int early) {
     using Vec = RawVec<T>;
     constexpr int G = Vec::G;
@@ -269,7 +271,7 @@ __device__ __forceinline__ float norm_scale(uint32_t top, float squares, int wid
 // A block per row; NG groups of four elements a thread stay in registers; NG = 0: rows of any width, read twice.
 template <typename T, bool ALIGNED, int NG>
 __global__ void __launch_bounds__(most_threads<NG>())
-add_rmsnorm_int8_kernel(const float* residual, const T* __restrict__ delta, float* residual_out, const void* __restrict__ weight,
+add_rmsnorm_int8_kernel(const float* residual, const T* delta, float* residual_out, const void* __restrict__ weight,
                         int w_f32, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int width, float eps) {
     // few rows: the weights do not depend on the kernels in front and are on the way before those are through
     constexpr bool EARLY_W = NG == 1 || NG == 2;
@@ -420,7 +422,7 @@ __device__ __forceinline__ void drain_ring(const RowRing& r, int issued, int* er
 
 template <typename T, int NG>
 __global__ void __launch_bounds__(RING_THREADS, ring_blocks(NG))
-quantize_ring_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int rows,
+quantize_ring_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int rows,
                      int width, int stages, int early, int* err) {
     using Vec = RawVec<T>;
     constexpr int G = Vec::G;
@@ -469,7 +471,7 @@ quantize_ring_kernel(const T* __restrict__ x, int64_t stride, int8_t* __restrict
 
 template <typename T, int NG>
 __global__ void __launch_bounds__(RING_THREADS, ring_blocks(NG))
-add_rmsnorm_int8_ring_kernel(const float* residual, const T* __restrict__ delta, float* residual_out, const void* __restrict__ weight,
+add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* residual_out, const void* __restrict__ weight,
                              int w_f32, int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int rows, int width, float eps,
                              int stages, int* err) {
     extern __shared__ __align__(128) unsigned char ring_smem[];
@@ -551,7 +553,7 @@ constexpr int DEQ_THREADS = 256, DEQ_GROUPS = 4;
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(DEQ_THREADS)
-dequantize_rows_kernel(const int8_t* __restrict__ q, int64_t q_stride, const float* __restrict__ scales, T* __restrict__ y, int width,
+dequantize_rows_kernel(const int8_t* q, int64_t q_stride, const float* scales, T* y, int width,
                        int spans) {
     constexpr int G = ALIGNED ? 16 / (int)sizeof(T) : 1;
     pdl_launch_dependents();

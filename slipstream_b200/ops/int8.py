@@ -9,8 +9,8 @@ from it is NaN.
 Rows of values start on 16 bytes: their stride is a multiple of 16, whatever their width.  ``int8_rows_like`` makes such rows,
 and every function here that returns int8 rows uses it.
 
-Weights are taken for constant, as in the other products of this package: `linear_int8` may read them before the kernels in
-front of it are through.  `quantize_rows_int8` therefore keeps the kernels behind it waiting unless it is told
+Weights, their scales, biases and the weights of a norm are taken for constant, as elsewhere in this package: a kernel may read them
+before the kernels in front of it are through.  `quantize_rows_int8` therefore keeps the kernels behind it waiting unless it is told
 (``activations=True``) that its rows will not be a product's weights.
 """
 
@@ -24,7 +24,7 @@ import torch
 from .functions import KernelError, _check, _code, _get_device, _need, _stream, error_word, gemm_library, ops_library, sm_count
 
 RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
-MAX_K = 133143  # 127^2 K stays below 2^31
+MAX_K = 131071  # 2^14 K, the largest sum of products of two bytes, stays below 2^31
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 _ROWS_CALL = Struct("=13qd2q").pack  # csrc/ops_int8.cu: Int8RowsCall
 _PRODUCT_CALL = Struct("=22q").pack  # csrc/gemm_int8.cu: Int8Call

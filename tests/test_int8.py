@@ -41,7 +41,7 @@ RESIDENT = ((148, 74, 45, 33, 26, 22, 15, 15), (296, 148, 93, 71, 56, 45, 37, 33
 def test_plans_are_forms_that_the_kernels_have(sms, resident):
     for gated in (False, True):
         for tokens in (1, 2, 15, 16, 17, 100, 255, 256, 257, 640, 641, 5000, 100000):
-            for features, k in ((128, 1), (128, 17), (256, 128), (1152, 896), (4608, 3584), (3584, 18944), (37888, 3584), (128, 133143)):
+            for features, k in ((128, 1), (128, 17), (256, 128), (1152, 896), (4608, 3584), (3584, 18944), (37888, 3584), (128, 131071)):
                 many, tile, slices, per = int8_plan(tokens, features, k, sms, gated, resident)
                 if many:
                     assert tile % 32 == 0 and 32 <= tile <= 256 and tokens > 64 and (not gated or tile % 128 == 0)
