@@ -18,6 +18,7 @@
 
 #include <cuda.h>
 
+#include "int8_calls.h"
 #include "tc5.cuh"
 
 #define I8_BM 128
@@ -620,23 +621,6 @@ extern "C" int ss_gemm_int8_resident(int n, int per_sm) {
     if (n < 1 || n > 8 || per_sm < 1 || ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return 0;
     return ss_resident_clusters(gemm_int8_few_kernel, I8_THREADS, per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX, n);
 }
-
-// The arguments of a product as one record: a call through ctypes takes 2.0 us for 22 arguments and 0.6 us for the address of a
-// packed record.
-struct Int8Call {
-    const void* x;  // [tokens, K] int8, row stride ldx
-    int64_t ldx;
-    const float* x_scale;
-    const void* w;  // [features, K] int8, row stride ldw
-    int64_t ldw;
-    const float* w_scale;
-    const void* bias;
-    int64_t bias_f32;
-    void* out;  // [tokens, ldc]
-    int64_t ldc, out_f32, tokens, features, K, gated, out_features, many, bn, slices, per_sm;
-    int* err;
-    cudaStream_t stream;
-};
 
 template <int STEPS>
 static int launch_many(const Int8Call& c, Int8Args& g) {

@@ -11,25 +11,8 @@
 // while it has already been launched (it waits, griddepcontrol.wait), so those pointers are not __restrict__: the loads must not go
 // through the read-only path.
 
+#include "int8_calls.h"
 #include "tc5.cuh"
-
-// The arguments of a call as one record (a call through ctypes takes 0.1 us an argument).
-struct Int8RowsCall {
-    const void* x;  // quantize: [rows, width], row stride `stride` elements; dequantize: unused; norm: the stream, [rows, width]
-    int64_t stride;
-    int8_t* q;  // [rows, width], row stride q_stride
-    int64_t q_stride;
-    float* scales;
-    int64_t rows, width, dtype;  // of x; of the values; of delta
-    int64_t early;               // quantize, see below
-    void* y;                     // dequantize: [rows, width]; norm: residual_out or null (may be x)
-    const void* delta;           // norm: [rows, width] or null
-    const void* weight;
-    int64_t w_f32;
-    double eps;
-    int* err;
-    cudaStream_t stream;
-};
 
 namespace {
 

@@ -15,7 +15,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import functools
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_float, c_int, c_int64, c_void_p
 
 import numpy as np
 import torch
@@ -49,7 +49,6 @@ _OPS_SIGNATURES = {
     "ss_swiglu": [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p],
     "ss_gemm_simt": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int64,
                      c_int64, c_int, c_int, c_void_p],
-    "ss_quantize_rows_int8": [c_char_p], "ss_dequantize_rows_int8": [c_char_p], "ss_add_rmsnorm_int8": [c_char_p],
     "ss_argmax": [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p],
     "ss_sample": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                   c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p],
@@ -186,7 +185,7 @@ _GEMM_SIGNATURES = {
                             c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "ss_gemm_tc5_scaled": [c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                            c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-    "ss_gemm_int8": [c_char_p], "ss_gemm_int8_resident": [c_int, c_int],
+    "ss_gemm_int8_resident": [c_int, c_int],
 }
 
 _state: dict[str, object] = {}

@@ -16,18 +16,16 @@ before the kernels in front of it are through.  `quantize_rows_int8` therefore k
 
 from __future__ import annotations
 
+import ctypes
 import functools
-from struct import Struct
 
 import torch
 
-from .functions import KernelError, _check, _code, _get_device, _need, _stream, error_word, gemm_library, ops_library, sm_count
+from .functions import KernelError, _launches, error_word, gemm_library, ops_library, sm_count
+from .library import load_calls
 
-RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many
-MAX_K = 131071  # 2^14 K, the largest sum of products of two bytes, stays below 2^31
-_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
-_ROWS_CALL = Struct("=13qd2q").pack  # csrc/ops_int8.cu: Int8RowsCall
-_PRODUCT_CALL = Struct("=22q").pack  # csrc/gemm_int8.cu: Int8Call
+RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many (csrc/int8_calls.cpp)
+_BF16 = torch.bfloat16
 
 
 class Int8Rows:
@@ -56,60 +54,47 @@ class Int8Rows:
         return dequantize_rows_int8(self, dtype)
 
 
-class _Device:
-    """What the calls ask of a device: its multiprocessors, where its error word is, and how many clusters of 1 to 8 blocks of the
-    product of few tokens it holds at the same time, with its ring sized for one block an SM and for two."""
-
-    def __init__(self, device: torch.device) -> None:
-        self.sms = sm_count(device)
-        self.error_ptr = error_word(device).data_ptr()  # (the word lives as long as the process)
-        ops, gemm = ops_library(), gemm_library()
-        self.quantize, self.dequantize, self.norm = ops.ss_quantize_rows_int8, ops.ss_dequantize_rows_int8, ops.ss_add_rmsnorm_int8
-        self.product = gemm.ss_gemm_int8
-        self.resident = tuple(tuple(gemm.ss_gemm_int8_resident(n, per) or self.sms * per // n for n in range(1, 9)) for per in (1, 2))
+_native = None
 
 
-_devices: dict[torch.device, _Device] = {}
+def _calls():
+    """The calls' host side (csrc/int8_calls.cpp), loaded and told its entry points at the first call."""
+    global _native
+    if _native is None:
+        ops, gemm, module = ops_library(), gemm_library(), load_calls()
+        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (ops.ss_quantize_rows_int8, ops.ss_dequantize_rows_int8,
+                                                                   ops.ss_add_rmsnorm_int8, gemm.ss_gemm_int8)]
+        module.use(KernelError, *entries, _error_address, _plan_on)
+        _native = module
+    return _native
 
 
-def _device(device: torch.device) -> _Device:
-    with torch.cuda.device(device):
-        found = _devices[device] = _Device(device)
-    return found
+def _error_address(index: int) -> int:
+    return error_word(torch.device("cuda", index)).data_ptr()  # (the word lives as long as the process)
 
 
-# torch's short way to an allocation on the current device (0.85 us where torch.empty_strided takes 1.5), where it has one
-_empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+@functools.lru_cache(maxsize=None)
+def _resident(index: int) -> tuple[tuple[int, ...], tuple[int, ...]]:
+    """How many clusters of 1 to 8 blocks of the product of few tokens the device holds at the same time, with its ring sized for
+    one block an SM and for two."""
+    lib, sms = gemm_library(), sm_count(index)
+    with torch.cuda.device(index):
+        return tuple(tuple(lib.ss_gemm_int8_resident(n, per) or sms * per // n for n in range(1, 9)) for per in (1, 2))
 
 
-def _empty(shape: tuple[int, ...], stride: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    if _empty_here is not None and _get_device is not None and device.index == _get_device():
-        return _empty_here(shape, stride, dtype)
-    return torch.empty_strided(shape, stride, dtype=dtype, device=device)
+def _plan_on(tokens: int, features: int, k: int, gated: int, index: int) -> tuple[int, int, int, int]:
+    return int8_plan(tokens, features, k, sm_count(index), bool(gated), _resident(index))
 
 
 def int8_rows_like(rows: int, width: int, device: torch.device) -> Int8Rows:
     """Int8 rows with nothing in them yet."""
-    return Int8Rows(_empty((rows, width), ((width + 15) & -16, 1), _I8, device), _empty((rows,), (1,), _F32, device))
+    values = torch.empty_strided((rows, width), ((width + 15) & -16, 1), dtype=torch.int8, device=device)
+    return Int8Rows(values, torch.empty(rows, dtype=torch.float32, device=device))
 
 
-def _need_rows(r: Int8Rows, what: str) -> tuple[int, int, int, int]:
-    """(rows, width, stride, address) of int8 rows that the kernels take."""
-    if type(r) is not Int8Rows:
+def _need_rows(r: Int8Rows, what: str) -> None:
+    if not isinstance(r, Int8Rows):
         raise KernelError(f"{what} must be Int8Rows, not {type(r).__name__}")
-    v, s = r.values, r.scales
-    if v.dim() != 2 or v.dtype is not _I8 or not v.is_cuda:
-        raise KernelError(f"{what}: the values must be a two-dimensional int8 CUDA tensor, got {v.dtype} {tuple(v.shape)} on {v.device}")
-    n, k = v.shape
-    if s.dtype is not _F32 or s.numel() != n or not s.is_contiguous() or s.get_device() != v.get_device():
-        raise KernelError(f"{what}: the scales must be {n} contiguous float32 numbers beside the values")
-    stride, step = v.stride()
-    if n < 2:
-        stride = (k + 15) & -16
-    at = v.data_ptr()
-    if n and k and (step != 1 and k > 1 or stride & 15 or stride < k or at & 15):
-        raise KernelError(f"{what}: rows must be contiguous and start on 16 bytes (a stride that is a multiple of 16), got strides {v.stride()}")
-    return n, k, stride, at
 
 
 def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Rows:
@@ -117,33 +102,15 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     ``q = rint(x * (127 / a))`` in float32, ties to even.  Tokens of activations, or output features of a weight.
 
     ``activations``: the rows are a product's activations, not its weights, and the kernel behind may start early."""
-    if not x.is_cuda or x.dim() != 2:
-        raise KernelError(f"x must be a two-dimensional CUDA tensor, got {tuple(x.shape)} on {x.device}")
-    n, k = x.shape
-    if k < 1:
-        raise KernelError("rows without elements have no scale")
-    stride, step = x.stride()
-    if k > 1 and step != 1:
-        raise KernelError(f"the rows of x must be contiguous, got strides {x.stride()}")
-    code, device, q_stride = _code(x.dtype), x.device, (k + 15) & -16
-    values, scales = _empty((n, k), (q_stride, 1), _I8, device), _empty((n,), (1,), _F32, device)
-    if n:
-        d = _devices.get(device) or _device(device)
-        _check(d.quantize(_ROWS_CALL(x.data_ptr(), stride, values.data_ptr(), q_stride, scales.data_ptr(), n, k, code, activations, 0, 0, 0, 0,
-                                     0.0, d.error_ptr, _stream())), "quantize_rows_int8")
-    return Int8Rows(values, scales)
+    _launches[0] += 1
+    return Int8Rows(*(_native or _calls()).quantize(x, activations))
 
 
 def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
     """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once."""
-    n, k, stride, at = _need_rows(rows, "rows")
-    code, device = _code(dtype), rows.values.device
-    out = _empty((n, k), (k, 1), dtype, device)
-    if n and k:
-        d = _devices.get(device) or _device(device)
-        _check(d.dequantize(_ROWS_CALL(0, 0, at, stride, rows.scales.data_ptr(), n, k, code, 0, out.data_ptr(), 0, 0, 0, 0.0, 0, _stream())),
-               "dequantize_rows_int8")
-    return out
+    _need_rows(rows, "rows")
+    _launches[0] += 1
+    return (_native or _calls()).dequantize(rows.values, rows.scales, dtype)
 
 
 def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
@@ -153,34 +120,8 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
 
     ``residual_out`` (float32 [N, H]) gets the new stream instead, and ``residual`` stays as it is.  ``weight`` is bfloat16 or
     float32.  A row's result does not depend on the other rows, nor on how many there are."""
-    _need(residual, _F32, "residual")
-    shape = residual.shape
-    if len(shape) != 2 or shape[1] < 1:
-        raise KernelError(f"residual must be [tokens, features], got {tuple(shape)}")
-    n, h = shape
-    from_ptr = residual.data_ptr()
-    code, delta_ptr, to = 1, 0, 0
-    if delta is not None:
-        _need(delta, None, "delta")
-        code, delta_ptr, to = _code(delta.dtype), delta.data_ptr(), from_ptr
-        if delta.shape != shape:
-            raise KernelError(f"delta {tuple(delta.shape)} does not match residual {tuple(shape)}")
-    _need(weight, None, "norm weight")
-    w_dtype = weight.dtype
-    if weight.numel() != h or (w_dtype is not _BF16 and w_dtype is not _F32):
-        raise KernelError("norm weight has the wrong size or dtype")
-    if residual_out is not None:
-        _need(residual_out, _F32, "residual_out")
-        if residual_out.shape != shape:
-            raise KernelError(f"residual_out {tuple(residual_out.shape)} does not match residual {tuple(shape)}")
-        to = residual_out.data_ptr()
-    device, q_stride = residual.device, (h + 15) & -16
-    values, scales = _empty((n, h), (q_stride, 1), _I8, device), _empty((n,), (1,), _F32, device)
-    if n:
-        d = _devices.get(device) or _device(device)
-        _check(d.norm(_ROWS_CALL(from_ptr, h, values.data_ptr(), q_stride, scales.data_ptr(), n, h, code, 0, to, delta_ptr, weight.data_ptr(),
-                                 w_dtype is _F32, eps, d.error_ptr, _stream())), "add_rmsnorm_int8")
-    return Int8Rows(values, scales)
+    _launches[0] += 1
+    return Int8Rows(*(_native or _calls()).norm(residual, delta, weight, eps, residual_out))
 
 
 # --------------------------------------------------------------------------- products
@@ -248,49 +189,16 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
     return best[1]
 
 
-def _product(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None, out_dtype: torch.dtype, gated: bool, columns: int | None,
-             plan: tuple[int, int, int, int] | None, what: str) -> torch.Tensor:
-    tokens, k, ldx, x_ptr = _need_rows(x, "x")
-    features, k_w, ldw, w_ptr = _need_rows(weight, "weight")
-    if k_w != k:
-        raise KernelError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
-    if not 1 <= k <= MAX_K:
-        raise KernelError(f"an int8 product takes 1 to {MAX_K} elements of K, not {k}")
-    if gated:
-        if features % (2 * RUN):
-            raise KernelError(f"gate and up rows alternate in runs of {RUN}: {features} rows are no multiple of {2 * RUN}")
-        columns = features // 2 if columns is None else columns
-        if not 0 <= columns <= features // 2:
-            raise KernelError(f"{columns} features asked of {features // 2}")
-    else:
-        columns = features
-    out_f32 = 1 - _code(out_dtype)
-    bias_ptr = bias_f32 = 0
-    if bias is not None:
-        _need(bias, None, "bias")
-        if bias.numel() != features or bias.dtype not in (_BF16, _F32):
-            raise KernelError("bias has the wrong size or dtype")
-        bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is _F32
-    device = x.values.device
-    if weight.values.get_device() != device.index:
-        raise KernelError(f"x is on {device}, weight on {weight.values.device}")
-    out = _empty((tokens, columns), (columns, 1), out_dtype, device)
-    if tokens == 0 or columns == 0:
-        return out
-    d = _devices.get(device) or _device(device)
-    many, tile, slices, per_sm = plan or int8_plan(tokens, features, k, d.sms, gated, d.resident)
-    _check(d.product(_PRODUCT_CALL(x_ptr, ldx, x.scales.data_ptr(), w_ptr, ldw, weight.scales.data_ptr(), bias_ptr, bias_f32, out.data_ptr(),
-                                   columns, out_f32, tokens, features, k, gated, columns, many, tile, slices, per_sm, d.error_ptr,
-                                   _stream())), what)
-    return out
-
-
 def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
                 plan: tuple[int, int, int, int] | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` for int8 rows: ``x`` [tokens, K] with a scale a token, ``weight`` [features, K] with a scale a
-    feature.  The sum over K is exact (32-bit integers); it is multiplied by both scales and the bias (bfloat16 or float32
-    [features]) is added in float32, and the result is rounded once to ``out_dtype`` (bfloat16 or float32)."""
-    return _product(x, weight, bias, out_dtype, False, None, plan, "linear_int8")
+    feature.  The sum over K (up to 131,071 elements) is exact, in 32-bit integers; it is multiplied by both scales and the bias
+    (bfloat16 or float32 [features]) is added in float32, and the result is rounded once to ``out_dtype`` (bfloat16 or float32).
+    ``plan``: see `int8_plan`; every plan gives the same bits."""
+    _need_rows(x, "x")
+    _need_rows(weight, "weight")
+    _launches[0] += 1
+    return (_native or _calls()).product(x.values, x.scales, weight.values, weight.scales, bias, out_dtype, False, None, plan)
 
 
 def gate_up_swiglu_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
@@ -298,7 +206,10 @@ def gate_up_swiglu_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None
     """``silu(gate(x)) * up(x)`` for int8 rows, the products as in `linear_int8`, the unit formed in float32 in the product's
     epilogue and rounded once.  The rows of ``weight`` (and of ``bias``) alternate ``RUN`` gate and ``RUN`` up features
     (`stack_gate_up`); ``features``: how many of the weight's pairs are real (those behind them pad the last run)."""
-    return _product(x, weight, bias, out_dtype, True, features, plan, "gate_up_swiglu_int8")
+    _need_rows(x, "x")
+    _need_rows(weight, "weight")
+    _launches[0] += 1
+    return (_native or _calls()).product(x.values, x.scales, weight.values, weight.scales, bias, out_dtype, True, features, plan)
 
 
 def stack_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

@@ -30,6 +30,8 @@ OPS_SOURCES = ["ops.cu", "ops_streams.cu", "ops_mixers.cu", "ops_cells.cu", "ops
                "ops_int8.cu", "sampling.cu"]
 # the tensor-core matrix products
 GEMM_SOURCES = ["gemm_tc5.cu", "gemm_f32.cu", "gemm_int8.cu"]
+# calls whose host side is native: an extension module of this Python and torch
+CALLS_SOURCES = ["int8_calls.cpp"]
 CSRC = Path(__file__).resolve().parent.parent / "csrc"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--shared", "-Xcompiler", "-fPIC",
@@ -81,12 +83,26 @@ def _digest(sources: list[Path], flags: list[str]) -> str:
 
 
 _lock = threading.Lock()
-_loaded: dict[str, ctypes.CDLL] = {}
+_loaded: dict[str, object] = {}
 
 
-def library_path(name: str, sources: list[str], defines: dict[str, object] | None = None) -> tuple[Path, list[str]]:
+def torch_flags() -> list[str]:
+    """What an extension module of this Python and torch is compiled and linked with."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    flags = ["-I", sysconfig.get_paths()["include"], "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
+             "-L", str(root / "lib"), "-Xlinker", "-rpath", "-Xlinker", str(root / "lib"),
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-DBUILT_WITH_TORCH={torch.__version__.replace('+', '_')}"]
+    return flags + [f"-l{lib}" for lib in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")]
+
+
+def library_path(name: str, sources: list[str], defines: dict[str, object] | None = None,
+                 extra: list[str] | None = None) -> tuple[Path, list[str]]:
     srcs = [CSRC / s for s in sources]
-    flags = BASE_FLAGS + ARCH_FLAGS + [f"-D{k}={v}" for k, v in sorted((defines or {}).items())]
+    flags = BASE_FLAGS + ARCH_FLAGS + [f"-D{k}={v}" for k, v in sorted((defines or {}).items())] + (extra or [])
     tag = _digest(srcs, flags)
     suffix = "".join(f"_{k.lower()}{v}" for k, v in sorted((defines or {}).items()))
     # look in every candidate folder for an up-to-date build before compiling
@@ -98,14 +114,14 @@ def library_path(name: str, sources: list[str], defines: dict[str, object] | Non
 
 
 def compile_library(name: str, sources: list[str], defines: dict[str, object] | None = None,
-                    verbose: bool = False) -> Path:
+                    verbose: bool = False, extra: list[str] | None = None) -> Path:
     """Compile (if no up-to-date build exists) and return the .so path."""
-    out, flags = library_path(name, sources, defines)
+    out, flags = library_path(name, sources, defines, extra)
     if out.is_file():
         return out
     nvcc = _find_nvcc()
     tmp = out.with_suffix(f".tmp{os.getpid()}_{threading.get_ident()}.so")
-    cmd = [nvcc, *flags, "-I", str(CSRC), "-o", str(tmp), *[str(CSRC / s) for s in sources]]
+    cmd = [nvcc, "-I", str(CSRC), "-o", str(tmp), *[str(CSRC / s) for s in sources], *flags]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     label = out.name
@@ -154,6 +170,29 @@ def load_library(name: str, sources: list[str], defines: dict[str, object] | Non
                 raise KernelBuildError(f"cannot load {path}: {exc}") from exc
             _loaded[key] = lib
         return lib
+
+
+def compile_calls() -> Path:
+    return compile_library("slipstream_int8_calls", CALLS_SOURCES, extra=torch_flags())
+
+
+def load_calls():
+    """The extension module of ``CALLS_SOURCES``."""
+    import importlib.machinery
+    import importlib.util
+
+    with _lock:
+        module = _loaded.get("calls")
+        if module is None:
+            path = compile_calls()
+            try:
+                loader = importlib.machinery.ExtensionFileLoader("slipstream_int8_calls", str(path))
+                module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("slipstream_int8_calls", str(path), loader=loader))
+                loader.exec_module(module)
+            except ImportError as exc:
+                raise KernelBuildError(f"cannot load {path}: {exc}") from exc
+            _loaded["calls"] = module
+        return module
 
 
 def require_cuda() -> None:
