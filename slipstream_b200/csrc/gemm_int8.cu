@@ -614,12 +614,16 @@ static int i8_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
 #define I8_SMEM_SM 233472   // 228 KB of an SM, 1 KB of it each block's own
 #define I8_SMEM_REST 2560   // alignment, barriers, scales
 
+// Only asked about, never launched: blocks of the shape of the kernel for few tokens.  About a kernel that takes tensor memory the
+// runtime answers one block an SM, whatever it takes of it; two are resident (11.1 of their 12 warps active on average).
+__global__ void __launch_bounds__(I8_THREADS) i8_few_shape() {}
+
 // How many clusters of `n` blocks of the kernel for few tokens run at the same time where the ring is sized for `per_sm` blocks an
 // SM (n = 1: blocks).
 extern "C" int ss_gemm_int8_resident(int n, int per_sm) {
     static SsPerDevice opted;
-    if (n < 1 || n > 8 || per_sm < 1 || ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return 0;
-    return ss_resident_clusters(gemm_int8_few_kernel, I8_THREADS, per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX, n);
+    if (n < 1 || n > 8 || per_sm < 1 || ss_opt_in_smem(i8_few_shape, I8_SMEM_MAX, opted)) return 0;
+    return ss_resident_clusters(i8_few_shape, I8_THREADS, per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX, n);
 }
 
 template <int STEPS>

@@ -399,6 +399,15 @@ def test_layer_on_another_stream_and_in_a_graph():
     o.check_errors(torch.device(DEV))
 
 
+def test_two_blocks_share_an_sm_where_the_plan_says_so():
+    from slipstream_b200.ops import int8
+
+    one, two = int8._resident(0)
+    sms = ops().sm_count(0)
+    assert one[0] == sms and two[0] == 2 * sms and all(b > a for a, b in zip(one, two))
+    assert int8._plan_on(8, 37888, 3584, 1, 0) == (0, 16, 1, 2)
+
+
 def test_refusals():
     o = ops()
     err = o.KernelError
