@@ -52,6 +52,31 @@ __device__ __forceinline__ void i8_load_once(void* dst, const CUtensorMap* map, 
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
         ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(k), "r"(row), "l"(policy) : "memory");
 }
+// Two steps of K in one copy: the map's third coordinate counts steps.
+__device__ __forceinline__ void i8_load_steps(void* dst, const CUtensorMap* map, int step, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(0), "r"(row), "r"(step) : "memory");
+}
+__device__ __forceinline__ void i8_load_steps_once(void* dst, const CUtensorMap* map, int step, int row, uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+        ::"r"(s_addr(dst)), "l"(map), "r"(s_addr(bar)), "r"(0), "r"(row), "r"(step), "l"(policy) : "memory");
+}
+// `rows` rows of the steps of K of stage k, as [step][row][128 bytes]
+template <int STEPS, bool ONCE>
+__device__ __forceinline__ void i8_load_stage(unsigned char* dst, const CUtensorMap* map, bool wide, int k, int row, int rows, uint64_t* bar, uint64_t policy) {
+    if (STEPS == 2 && wide) {
+        if (ONCE) i8_load_steps_once(dst, map, 2 * k, row, bar, policy);
+        else i8_load_steps(dst, map, 2 * k, row, bar);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        if (ONCE) i8_load_once(dst + i * rows * I8_BK, map, (STEPS * k + i) * I8_BK, row, bar, policy);
+        else i8_load(dst + i * rows * I8_BK, map, (STEPS * k + i) * I8_BK, row, bar);
+    }
+}
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -122,11 +147,13 @@ __device__ __forceinline__ uint32_t i8_remote(const void* p, uint32_t rank) {
 // block's shared memory from its registers (red.async; whole numbers, so in any order), which counts the bytes on a barrier of its
 // own.  No block waits for another but for these sums.  Warp 0 (one lane) fetches, warp 1 issues the products, warps 2 to 5
 // write the result out.
+template <int STEPS>
 __global__ void __launch_bounds__(I8_THREADS)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Int8Args g) {
     extern __shared__ unsigned char smem_raw[];
     const int bn = g.bn, stages = g.stages, n_sl = g.slices;
-    const int w_bytes = I8_BM * I8_BK, stage_bytes = w_bytes + bn * I8_BK;
+    constexpr int w_bytes = STEPS * I8_BM * I8_BK;
+    const int stage_bytes = w_bytes + STEPS * bn * I8_BK;
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);
     uint64_t* empty = full + stages;
@@ -143,7 +170,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     const int live = min(bn, g.tokens - t0);                   // columns that hold tokens
     const int rank = n_sl > 1 ? (int)cluster_rank() : 0;
     const int mine = live > rank ? (live - 1 - rank) / n_sl + 1 : 0;  // columns rank, rank + slices, ...
-    const int k_total = (g.K + I8_BK - 1) / I8_BK;
+    const int k_steps = (g.K + I8_BK - 1) / I8_BK, k_total = (k_steps + STEPS - 1) / STEPS;  // stages of K, of all slices
     const int per = (k_total + n_sl - 1) / n_sl;
     const int k_begin = blockIdx.z * per, k_iters = max(0, min(k_total, k_begin + per) - k_begin);
     const int senders = (k_total + per - 1) / per;  // blocks that have any K
@@ -162,7 +189,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const uint64_t once = l2_evict_first_policy();
         for (int it = 0; it < ahead; ++it) {
             mbar_expect_tx(&full[it], stage_bytes);
-            i8_load_once(tiles + it * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[it], once);
+            i8_load_stage<STEPS, true>(tiles + it * stage_bytes, &map_w, g.wide_copies, k_begin + it, f0, I8_BM, &full[it], once);
         }
     } else if (warp >= 2 && n_sl > 1) {
         for (int i = threadIdx.x - 64; i < mine * (I8_BM / 4); i += 128) reinterpret_cast<int4*>(sums)[i] = make_int4(0, 0, 0, 0);
@@ -179,7 +206,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             const uint64_t once = l2_evict_first_policy();
             pdl_wait();
             for (int it = 0; it < ahead; ++it)
-                i8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[it]);
+                i8_load_stage<STEPS, false>(tiles + it * stage_bytes + w_bytes, &map_x, g.wide_copies, k_begin + it, t0, bn, &full[it], once);
             // (a stage's number and its parity are counted, not divided out: the loops of this thread and of the issuer are what a
             // step takes where its products are small)
             int it = ahead, s = 0;
@@ -187,8 +214,8 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (; it < k_iters; ++it) {
                 if (!mbar_wait(&empty[s], parity, gave_up)) break;
                 mbar_expect_tx(&full[s], stage_bytes);
-                i8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * I8_BK, f0, &full[s], once);
-                i8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * I8_BK, t0, &full[s]);
+                i8_load_stage<STEPS, true>(tiles + s * stage_bytes, &map_w, g.wide_copies, k_begin + it, f0, I8_BM, &full[s], once);
+                i8_load_stage<STEPS, false>(tiles + s * stage_bytes + w_bytes, &map_x, g.wide_copies, k_begin + it, t0, bn, &full[s], once);
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
             if (*gave_up)
@@ -205,7 +232,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
         const uint32_t idesc = i8_idesc(I8_BM, bn);
         const uint64_t w_first = smem_desc(tiles), x_first = smem_desc(tiles + w_bytes);
-        const uint32_t stage_step = (uint32_t)stage_bytes >> 4;  // of a descriptor's address
+        const uint32_t stage_step = (uint32_t)stage_bytes >> 4, x_step = (uint32_t)(bn * I8_BK) >> 4;  // of a descriptor's address
         int s = 0;
         uint32_t parity = 0;
         for (int it = 0; it < k_iters; ++it) {
@@ -216,6 +243,11 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 #pragma unroll
                 for (int kk = 0; kk < I8_BK / 32; ++kk)  // 32 bytes further along the swizzled row
                     umma_i8(tmem_acc, w_desc + (uint64_t)(kk * 2), x_desc + (uint64_t)(kk * 2), idesc, (it | kk) != 0);
+                if (STEPS == 2 && 2 * (k_begin + it) + 1 < k_steps) {
+#pragma unroll
+                    for (int kk = 0; kk < I8_BK / 32; ++kk)
+                        umma_i8(tmem_acc, w_desc + (uint64_t)(I8_BM * I8_BK / 16 + kk * 2), x_desc + (uint64_t)(x_step + kk * 2), idesc, 1);
+                }
                 umma_commit(&empty[s]);
             }
             __syncwarp();
@@ -324,7 +356,7 @@ __device__ __forceinline__ void i8_load_pair_steps(void* dst, const CUtensorMap*
 }
 // `rows` rows of the steps of K of stage k, as [step][row][128 bytes]
 template <int STEPS>
-__device__ __forceinline__ void i8_load_stage(unsigned char* dst, const CUtensorMap* map, bool wide, int k, int row, int rows, uint64_t* bar) {
+__device__ __forceinline__ void i8_load_pair_stage(unsigned char* dst, const CUtensorMap* map, bool wide, int k, int row, int rows, uint64_t* bar) {
     if (STEPS == 2 && wide) {
         i8_load_pair_steps(dst, map, 2 * k, row, bar);
         return;
@@ -455,7 +487,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
         for (int k = 0; k < first; ++k) {
             if (rank == 0) mbar_expect_tx(&full[k], bytes);
-            i8_load_stage<STEPS>(tiles + k * stage_bytes + x_bytes, &map_w, g.wide_copies, k, (pair / n_m) * bn + rank * w_rows, w_rows, &full[k]);
+            i8_load_pair_stage<STEPS>(tiles + k * stage_bytes + x_bytes, &map_w, g.wide_copies, k, (pair / n_m) * bn + rank * w_rows, w_rows, &full[k]);
         }
     }
     pdl_wait();
@@ -465,7 +497,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
     } else if (threadIdx.x == 0) {
         for (int k = 0; k < first; ++k)
-            i8_load_stage<STEPS>(tiles + k * stage_bytes, &map_x, g.wide_copies, k, (pair % n_m) * 2 * I8_BM + rank * I8_BM, I8_BM, &full[k]);
+            i8_load_pair_stage<STEPS>(tiles + k * stage_bytes, &map_x, g.wide_copies, k, (pair % n_m) * 2 * I8_BM + rank * I8_BM, I8_BM, &full[k]);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // the tensor memory of both blocks has been taken
@@ -483,8 +515,8 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     if (!mbar_wait(&empty[s], parity, gave_up)) { ok = false; break; }
                     if (rank == 0) mbar_expect_tx(&full[s], bytes);
                     unsigned char* x_tile = tiles + s * stage_bytes;
-                    i8_load_stage<STEPS>(x_tile, &map_x, g.wide_copies, k, m0, I8_BM, &full[s]);
-                    i8_load_stage<STEPS>(x_tile + x_bytes, &map_w, g.wide_copies, k, n0, w_rows, &full[s]);
+                    i8_load_pair_stage<STEPS>(x_tile, &map_x, g.wide_copies, k, m0, I8_BM, &full[s]);
+                    i8_load_pair_stage<STEPS>(x_tile + x_bytes, &map_w, g.wide_copies, k, n0, w_rows, &full[s]);
                 }
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
@@ -643,30 +675,16 @@ static int launch_many(const Int8Call& c, Int8Args& g) {
     return SS_LAUNCH_CHECK();
 }
 
-// Row strides are multiples of 16 bytes and bases stand on 16 bytes; K <= 131,071.
-// gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
-// many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for.
-// many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
-extern "C" int ss_gemm_int8(const Int8Call* call) {
-    const Int8Call& c = *call;
-    if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
-    if (c.tokens > INT32_MAX - 256 || c.features > INT32_MAX - 256 || c.K <= 0 || c.K > 131071 || c.ldx % 16 || c.ldw % 16 || c.ldx < c.K || c.ldw < c.K) return -2003;
-    if (((uintptr_t)c.x & 15) || ((uintptr_t)c.w & 15) || ((uintptr_t)c.out & 15)) return -2004;
-    if (c.gated ? (c.features % 128 || c.out_features > c.features / 2) : c.out_features != c.features) return -2005;
-    const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;
-    if (bn < 16 || bn > I8_MAX_BN || bn % (c.many ? 32 : 16) || (c.many && c.gated && bn % 128)
-        || (!c.many && (slices < 1 || slices > 8 || per_sm < 1 || per_sm > 4 || (c.features + I8_BM - 1) / I8_BM > 65535))) return -2006;
-    Int8Args g = {};
-    g.x_scale = c.x_scale; g.w_scale = c.w_scale; g.bias = c.bias; g.out = c.out; g.err = c.err; g.ldc = c.ldc;
-    g.tokens = (int)c.tokens; g.features = (int)c.features; g.K = (int)c.K; g.out_features = (int)c.out_features;
-    g.out_f32 = (int)c.out_f32; g.bias_f32 = (int)c.bias_f32; g.gated = (int)c.gated; g.bn = bn; g.slices = slices;
-    if (c.many) return bn <= 192 ? launch_many<2>(c, g) : launch_many<1>(c, g);
+template <int STEPS>
+static int launch_few(const Int8Call& c, Int8Args& g, int per_sm) {
     CUtensorMap map_x, map_w;
-    if (int rc = i8_map(&map_x, c.x, g.tokens, g.K, c.ldx, bn)) return rc;
-    if (int rc = i8_map(&map_w, c.w, g.features, g.K, c.ldw, I8_BM)) return rc;
+    const int bn = g.bn, slices = g.slices;
+    g.wide_copies = STEPS == 2 && g.K % I8_BK == 0;
+    if (int rc = i8_map(&map_x, c.x, g.tokens, g.K, c.ldx, bn, g.wide_copies)) return rc;
+    if (int rc = i8_map(&map_w, c.w, g.features, g.K, c.ldw, I8_BM, g.wide_copies)) return rc;
     static SsPerDevice opted;
-    if (int rc = ss_opt_in_smem(gemm_int8_few_kernel, I8_SMEM_MAX, opted)) return rc;
-    const int stage = I8_BM * I8_BK + bn * I8_BK;
+    if (int rc = ss_opt_in_smem(gemm_int8_few_kernel<STEPS>, I8_SMEM_MAX, opted)) return rc;
+    const int stage = STEPS * (I8_BM + bn) * I8_BK;
     const int rest = I8_SMEM_REST + (slices > 1 ? (bn + slices - 1) / slices * I8_BM * 4 : 0);  // a cluster's blocks: the columns they own
     const int room = per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX;
     int stages = (room - rest) / stage;
@@ -676,7 +694,29 @@ extern "C" int ss_gemm_int8(const Int8Call* call) {
     const int smem = stages * stage + rest;
     if (smem > I8_SMEM_MAX) return -2007;
     const dim3 grid((g.tokens + bn - 1) / bn, (g.features + I8_BM - 1) / I8_BM, slices);
-    if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, c.stream, slices, map_w, map_x, g);
-    else ss_launch(gemm_int8_few_kernel, grid, dim3(I8_THREADS), smem, c.stream, map_w, map_x, g);
+    if (slices > 1) ss_launch_cluster(gemm_int8_few_kernel<STEPS>, grid, dim3(I8_THREADS), smem, c.stream, slices, map_w, map_x, g);
+    else ss_launch(gemm_int8_few_kernel<STEPS>, grid, dim3(I8_THREADS), smem, c.stream, map_w, map_x, g);
     return SS_LAUNCH_CHECK();
+}
+
+// Row strides are multiples of 16 bytes and bases stand on 16 bytes; K <= 131,071.
+// gated: w's rows alternate 64 gate and 64 up features; out_features <= features / 2 columns of silu(gate) * up are written.
+// many = 0: bn tokens a tile (a multiple of 16 up to 256), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for.
+// many = 1: bn features a tile (a multiple of 32 up to 256; gated: 128 or 256).
+// steps: 1 or 2 steps of K in a stage.
+extern "C" int ss_gemm_int8(const Int8Call* call) {
+    const Int8Call& c = *call;
+    if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
+    if (c.tokens > INT32_MAX - 256 || c.features > INT32_MAX - 256 || c.K <= 0 || c.K > 131071 || c.ldx % 16 || c.ldw % 16 || c.ldx < c.K || c.ldw < c.K) return -2003;
+    if (((uintptr_t)c.x & 15) || ((uintptr_t)c.w & 15) || ((uintptr_t)c.out & 15)) return -2004;
+    if (c.gated ? (c.features % 128 || c.out_features > c.features / 2) : c.out_features != c.features) return -2005;
+    const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;
+    if (bn < 16 || bn > I8_MAX_BN || c.steps < 1 || c.steps > 2 || bn % (c.many ? 32 : 16) || (c.many && c.gated && bn % 128)
+        || (!c.many && (slices < 1 || slices > 8 || per_sm < 1 || per_sm > 4 || (c.features + I8_BM - 1) / I8_BM > 65535))) return -2006;
+    Int8Args g = {};
+    g.x_scale = c.x_scale; g.w_scale = c.w_scale; g.bias = c.bias; g.out = c.out; g.err = c.err; g.ldc = c.ldc;
+    g.tokens = (int)c.tokens; g.features = (int)c.features; g.K = (int)c.K; g.out_features = (int)c.out_features;
+    g.out_f32 = (int)c.out_f32; g.bias_f32 = (int)c.bias_f32; g.gated = (int)c.gated; g.bn = bn; g.slices = slices;
+    if (c.many) return c.steps == 2 ? launch_many<2>(c, g) : launch_many<1>(c, g);
+    return c.steps == 2 ? launch_few<2>(c, g, per_sm) : launch_few<1>(c, g, per_sm);
 }

@@ -38,7 +38,7 @@ int (*dequantize_entry)(const Int8RowsCall*);
 int (*norm_entry)(const Int8RowsCall*);
 int (*product_entry)(const Int8Call*);
 
-using Plan = std::array<int64_t, 4>;
+using Plan = std::array<int64_t, 5>;
 std::map<int64_t, int*> error_words;                                                      // by device
 std::map<std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t>, Plan> plans;           // by (device, features, K, gated, tokens)
 
@@ -103,9 +103,10 @@ Plan plan_of(PyObject* given, int64_t tokens, int64_t features, int64_t k, int64
         made = given = PyObject_CallFunction(plan_function, "LLLLL", (long long)tokens, (long long)features, (long long)k, (long long)gated, (long long)device);
         if (!given) throw python_error();
     }
-    long long p[4];
-    const int ok = PyArg_ParseTuple(given, "LLLL", &p[0], &p[1], &p[2], &p[3]);
-    Plan plan{p[0], p[1], p[2], p[3]};
+    long long p[5];
+    const int ok = PyArg_ParseTuple(given, "LLLLL", &p[0], &p[1], &p[2], &p[3], &p[4]);
+    Plan plan{};
+    if (ok) plan = Plan{p[0], p[1], p[2], p[3], p[4]};
     if (made) {
         Py_DECREF(made);
         if (ok) plans[key] = plan;
@@ -281,7 +282,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t) {
         c.x = x.values->data_ptr(); c.ldx = x.stride; c.x_scale = (const float*)x.scales->data_ptr();
         c.w = w.values->data_ptr(); c.ldw = w.stride; c.w_scale = (const float*)w.scales->data_ptr();
         c.out = out.data_ptr(); c.ldc = columns; c.tokens = tokens; c.features = features; c.K = k; c.gated = gated; c.out_features = columns;
-        c.many = plan[0]; c.bn = plan[1]; c.slices = plan[2]; c.per_sm = plan[3];
+        c.many = plan[0]; c.bn = plan[1]; c.slices = plan[2]; c.per_sm = plan[3]; c.steps = plan[4];
         c.err = error_word(device); c.stream = c10::cuda::getCurrentCUDAStream().stream();
         check(product_entry(&c), what);
     }

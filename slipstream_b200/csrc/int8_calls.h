@@ -31,7 +31,7 @@ struct Int8Call {
     const void* bias;
     int64_t bias_f32;
     void* out;  // [tokens, ldc]
-    int64_t ldc, out_f32, tokens, features, K, gated, out_features, many, bn, slices, per_sm;
+    int64_t ldc, out_f32, tokens, features, K, gated, out_features, many, bn, slices, per_sm, steps;
     int* err;
     cudaStream_t stream;
 };

@@ -82,7 +82,7 @@ def _resident(index: int) -> tuple[tuple[int, ...], tuple[int, ...]]:
         return tuple(tuple(lib.ss_gemm_int8_resident(n, per) or sms * per // n for n in range(1, 9)) for per in (1, 2))
 
 
-def _plan_on(tokens: int, features: int, k: int, gated: int, index: int) -> tuple[int, int, int, int]:
+def _plan_on(tokens: int, features: int, k: int, gated: int, index: int) -> tuple[int, int, int, int, int]:
     return int8_plan(tokens, features, k, sm_count(index), bool(gated), _resident(index))
 
 
@@ -127,22 +127,23 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
 # --------------------------------------------------------------------------- products
 
 def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
-              resident: tuple[tuple[int, ...], tuple[int, ...]] | None = None) -> tuple[int, int, int, int]:
-    """(many, tile, K slices, blocks an SM) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
-    (tokens of the first, features of the second), and for the first the slices of K and how many blocks an SM the ring is sized
-    for.  ``resident``: clusters of 1 to 8 blocks that run at the same time, with the ring sized for one block an SM and for two.
+              resident: tuple[tuple[int, ...], tuple[int, ...]] | None = None) -> tuple[int, int, int, int, int]:
+    """(many, tile, K slices, blocks an SM, steps) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its
+    tile (tokens of the first, features of the second), for the first the slices of K and how many blocks an SM the ring is sized
+    for, and for both how many steps of K a stage holds.  ``resident``: clusters of 1 to 8 blocks that run at the same time, with the
+    ring sized for one block an SM and for two.
 
-    The choice is the cheapest by an estimate of cycles whose constants are fitted to 4,220 measured products (1 to 4,096 tokens, the
-    projections of the 0.5B, 1.5B and 7B layer sizes, tiles and slices of all sizes).  What it takes is on average 2 % slower than the
-    fastest of them at the same sizes, and at worst 17 %; one tile for all tokens up to 256 and K in one slice, else tiles of 256 x 256,
-    would be 43 % slower."""
+    The choice is the cheapest by an estimate of cycles whose constants are fitted to 9,592 measured products (1 to 4,096 tokens, the
+    projections of the 0.5B, 1.5B and 7B layer sizes, tiles, slices and stages of all sizes).  What it takes is on average 2 % slower
+    than the fastest of them at the same sizes, and at worst 29 % (gated products of 416 to 640 tokens at the 0.5B sizes); one tile for all tokens up to 256 with K in one slice, else tiles of
+    256 x 256, would be 44 % slower."""
     # what follows depends on the tokens in steps of 16 (their tiles) up to 640 and of 256 beyond: few plans for many counts
     step = 16 if tokens <= 640 else 256
     return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
 
 
 @functools.lru_cache(maxsize=None)
-def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -> tuple[int, int, int, int]:
+def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -> tuple[int, int, int, int, int]:
     if resident is None:
         resident = tuple(tuple(sms * per // n for n in range(1, 9)) for per in (1, 2))
     k_steps = (k + 127) // 128
@@ -158,39 +159,44 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
                 break
             if slices == 7:  # (clusters that fit worst into the GPU's processor clusters)
                 continue
-            for per in (1, 2) if tile <= 128 else (1,):
+            for per, steps in ((1, 1), (1, 2), (2, 1), (2, 2)) if tile <= 128 else ((1, 1), (1, 2)):
                 rest = 2560 + ((tile + slices - 1) // slices * 512 if slices > 1 else 0)
-                stages = max(2, min(12, ((232448 if per == 1 else 115712) - rest) // ((128 + tile) * 128)))
+                stages = min(12, ((232448 if per == 1 else 115712) - rest) // (steps * (128 + tile) * 128))
+                if stages < 2:
+                    continue
                 held = max(1, resident[per - 1][slices - 1]) * slices  # blocks that run at the same time
                 waves = (blocks + held - 1) // held
                 shared = max(1.0, min(float(per), blocks / sms))
                 # a step of K: the loops of the fetching and issuing threads; what an SM takes in; the ring's latency; the memory
-                cycles = max(330.0, shared * (128 + tile) * 128 / 56, 2470 / stages, min(blocks, held) * 16384 * 148 / (3070 * sms))
-                cost = 3870 + waves * ((k_steps + slices - 1) // slices * cycles + 465 + 17.4 * tile)
+                cycles = max(543.0 if steps == 1 else 216.0, shared * (128 + tile) * 128 / 60, 2940 / (stages * steps),
+                             min(blocks, held) * 16384 * 148 / (5120 * sms))
+                mine = (k_steps + slices * steps - 1) // (slices * steps) * steps
+                cost = 2880 + waves * (mine * cycles + 165 + 42.9 * tile)
                 if slices > 1:
-                    cost += waves * (148 + 61 * tile * (slices - 1) / slices)
+                    cost += waves * 105 * tile * (slices - 1) / slices
                 if waves > 1:
-                    cost += 4440
+                    cost += 950
                 elif per == 2 and blocks <= (0.5 if slices == 1 else 0.45) * held:  # the kernel behind has room for its first stages
-                    cost -= 900
+                    cost -= 2950
                 if best is None or cost < best[0]:
-                    best = (cost, (0, tile, slices, per))
+                    best = (cost, (0, tile, slices, per, steps))
     if tokens > 64:
         rows = (tokens + 255) // 256
         for tile in ((128, 256) if gated else (32, 64, 96, 128, 160, 192, 224, 256)):
             tiles = rows * ((features + tile - 1) // tile)
             pairs = max(1, sms // 2)
             rounds = (tiles + pairs - 1) // pairs
-            cycles = max(322.0 if tile <= 192 else 493.0, 2.43 * tile, (min(128, tokens) + tile / 2) * 128 / 60,
-                         min(tiles, pairs) * tile * 128 * 148 / (3070 * sms * min(rows, tiles, pairs)))
-            cost = 3840 + rounds * k_steps * cycles + 2120 + 18.6 * tile + (rounds - 1) * 1270 + (10.8 * tile if gated else 0)
-            if best is None or cost < best[0]:
-                best = (cost, (1, tile, 1, 1))
+            for steps in (1, 2):
+                cycles = max(412.0 if steps == 1 else 249.0, (2.3 if steps == 1 else 2.83) * tile,
+                             min(tiles, pairs) * tile * 128 * 148 / (5120 * sms * min(rows, pairs)))
+                cost = 7060 + rounds * k_steps * cycles + 26.6 * tile + (rounds - 1) * 2400
+                if best is None or cost < best[0]:
+                    best = (cost, (1, tile, 1, 1, steps))
     return best[1]
 
 
 def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
-                plan: tuple[int, int, int, int] | None = None) -> torch.Tensor:
+                plan: tuple[int, int, int, int, int] | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` for int8 rows: ``x`` [tokens, K] with a scale a token, ``weight`` [features, K] with a scale a
     feature.  The sum over K (up to 131,071 elements) is exact, in 32-bit integers; it is multiplied by both scales and the bias
     (bfloat16 or float32 [features]) is added in float32, and the result is rounded once to ``out_dtype`` (bfloat16 or float32).
@@ -202,7 +208,7 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
 
 
 def gate_up_swiglu_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
-                        features: int | None = None, plan: tuple[int, int, int, int] | None = None) -> torch.Tensor:
+                        features: int | None = None, plan: tuple[int, int, int, int, int] | None = None) -> torch.Tensor:
     """``silu(gate(x)) * up(x)`` for int8 rows, the products as in `linear_int8`, the unit formed in float32 in the product's
     epilogue and rounded once.  The rows of ``weight`` (and of ``bias``) alternate ``RUN`` gate and ``RUN`` up features
     (`stack_gate_up`); ``features``: how many of the weight's pairs are real (those behind them pad the last run)."""

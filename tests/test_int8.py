@@ -42,14 +42,15 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
     for gated in (False, True):
         for tokens in (1, 2, 15, 16, 17, 100, 255, 256, 257, 640, 641, 5000, 100000):
             for features, k in ((128, 1), (128, 17), (256, 128), (1152, 896), (4608, 3584), (3584, 18944), (37888, 3584), (128, 131071)):
-                many, tile, slices, per = int8_plan(tokens, features, k, sms, gated, resident)
+                many, tile, slices, per, steps = int8_plan(tokens, features, k, sms, gated, resident)
+                assert steps in (1, 2)
                 if many:
                     assert tile % 32 == 0 and 32 <= tile <= 256 and tokens > 64 and (not gated or tile % 128 == 0)
                 else:
                     assert tile % 16 == 0 and 16 <= tile <= 256 and 1 <= slices <= min(8, -(-k // 128)) and per in (1, 2) and tokens <= 640
                     # what the kernel keeps in shared memory: two stages of the ring, and its share of the sums
                     rest = 2560 + (-(-tile // slices) * 512 if slices > 1 else 0)
-                    assert 2 * (128 + tile) * 128 + rest <= 232448
+                    assert 2 * steps * (128 + tile) * 128 + rest <= 232448
 
 
 def test_plans_do_not_change_within_a_step_of_tokens():
@@ -60,10 +61,11 @@ def test_plans_do_not_change_within_a_step_of_tokens():
 
 
 def test_decode_plans_cut_k_where_tiles_are_few():
-    """The o and q/k/v projections of the 7B layer sizes: K in slices, blocks that leave room for the kernel behind."""
-    assert int8_plan(8, 3584, 3584, 148, False, RESIDENT) == (0, 16, 4, 2)
-    assert int8_plan(8, 4608, 3584, 148, False, RESIDENT) == (0, 16, 3, 2)
-    assert int8_plan(8, 37888, 3584, 148, True, RESIDENT) == (0, 16, 1, 2)
+    """The o, q/k/v and gate/up projections of the 7B layer sizes: K in slices where there are fewer tiles than multiprocessors."""
+    for tokens in (1, 8, 16):
+        for features, gated in ((3584, False), (4608, False), (37888, True)):
+            many, tile, slices, per, steps = int8_plan(tokens, features, 3584, 148, gated, RESIDENT)
+            assert (many, tile) == (0, 16) and (slices > 1) == (features < 37888) and features // 128 * slices <= 2 * 148
 
 
 def test_stacked_gate_and_up_rows():

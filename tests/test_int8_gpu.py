@@ -236,11 +236,12 @@ def test_linear(tokens, k, features):
 
 def plans(tokens, k, gated):
     few = max(16, min(256, (tokens + 15) // 16 * 16))
-    out = [(0, tile, slices, per_sm) for tile in {16, 32, 48, few, 128, 256} for slices in (1, 2, 5, 8) for per_sm in (1, 2, 4) if tile <= 2 * few]
-    return out + [(1, tile, 1, 1) for tile in ((128, 256) if gated else (32, 96, 128, 224, 256))]
+    out = [(0, tile, slices, per_sm, steps) for tile in {16, 32, 48, few, 128, 208} for slices in (1, 2, 5, 8) for per_sm, steps in ((1, 1), (2, 1), (4, 1), (1, 2), (2, 2))
+           if tile <= 2 * few and steps * tile <= 256]
+    return out + [(1, tile, 1, 1, steps) for tile in ((128, 256) if gated else (32, 96, 128, 224, 256)) for steps in (1, 2)]
 
 
-@pytest.mark.parametrize("tokens, k, features", [(1, 200, 130), (19, 1500, 515), (150, 3584, 700), (515, 900, 1024)])
+@pytest.mark.parametrize("tokens, k, features", [(1, 200, 130), (19, 1500, 515), (150, 3584, 700), (515, 900, 1024), (33, 1152, 300)])
 def test_linear_in_every_form(tokens, k, features):
     """The same bits from both kernels, whatever their tiles and however K is cut (more slices than there is K, too)."""
     o, g = ops(), gen(tokens)
@@ -405,7 +406,7 @@ def test_two_blocks_share_an_sm_where_the_plan_says_so():
     one, two = int8._resident(0)
     sms = ops().sm_count(0)
     assert one[0] == sms and two[0] == 2 * sms and all(b > a for a, b in zip(one, two))
-    assert int8._plan_on(8, 37888, 3584, 1, 0) == (0, 16, 1, 2)
+    assert int8._plan_on(8, 37888, 3584, 1, 0)[:4] == (0, 16, 1, 2)
 
 
 def test_refusals():
@@ -453,8 +454,8 @@ def test_refusals():
                  lambda: o.linear_int8(good, w, torch.zeros(127, device=DEV)), lambda: o.linear_int8(good, w, torch.zeros(128, device=DEV).half()),
                  lambda: o.linear_int8(good, w, None, torch.float16), lambda: o.gate_up_swiglu_int8(good, good),
                  lambda: o.gate_up_swiglu_int8(good, w, features=65), lambda: o.stack_gate_up(x, x[:2]),
-                 lambda: o.linear_int8(good, w, plan=(0, 24, 1, 1)), lambda: o.linear_int8(good, w, plan=(0, 16, 9, 1)),
-                 lambda: o.linear_int8(good, w, plan=(1, 48, 1, 1)), lambda: o.gate_up_swiglu_int8(good, w, plan=(1, 96, 1, 1))):
+                 lambda: o.linear_int8(good, w, plan=(0, 24, 1, 1, 1)), lambda: o.linear_int8(good, w, plan=(0, 16, 9, 1, 1)), lambda: o.linear_int8(good, w, plan=(0, 16, 1, 1, 3)),
+                 lambda: o.linear_int8(good, w, plan=(1, 48, 1, 1, 1)), lambda: o.gate_up_swiglu_int8(good, w, plan=(1, 96, 1, 1, 1))):
         with pytest.raises(err):
             call()
     assert o.linear_int8(o.quantize_rows_int8(torch.empty(0, 64, device=DEV)), w).shape == (0, 128)
