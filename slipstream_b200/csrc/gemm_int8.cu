@@ -88,10 +88,14 @@ __device__ __forceinline__ uint32_t i8_idesc(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// One wait for a copy of this block that is still in flight after a wait gave up (its own limit, blind to the flag).
-__device__ __forceinline__ void i8_drain(uint64_t* bar, uint32_t parity) {
-    volatile int none = 0;
-    (void)mbar_wait(bar, parity, &none);
+// Behind a wait that gave up: the error word, and a wait for the last of the `copies` stages that were sent for, which may still be
+// in flight (each with its own limit, blind to the flag).
+__device__ __noinline__ void i8_gave_up(const Int8Args& g, uint64_t* full, int stages, int copies) {
+    atomicOr(g.err, SS_ERR_WAIT_LIMIT);
+    for (int i = max(0, copies - stages); i < copies; ++i) {
+        volatile int none = 0;
+        (void)mbar_wait(&full[i % stages], (i / stages) & 1, &none);
+    }
 }
 
 __device__ __forceinline__ float i8_bias(const Int8Args& g, int f) {
@@ -176,6 +180,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     const int senders = (k_total + per - 1) / per;  // blocks that have any K
     const int ahead = min(stages, k_iters);
     const uint32_t tmem_cols = bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256;
+    int copies = 0;  // stages that thread 0 has sent for
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -218,8 +223,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 i8_load_stage<STEPS, false>(tiles + s * stage_bytes + w_bytes, &map_x, g.wide_copies, k_begin + it, t0, bn, &full[s], once);
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
-            if (*gave_up)
-                for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
+            copies = it;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -321,9 +325,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
         asm volatile("barrier.cluster.wait;" ::: "memory");
     }
-    if (*gave_up && threadIdx.x == 0) atomicOr(g.err, SS_ERR_WAIT_LIMIT);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (*gave_up && threadIdx.x == 0) i8_gave_up(g, full, stages, copies);
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
@@ -503,6 +507,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     cluster_sync_all();  // the tensor memory of both blocks has been taken
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    int copies = 0;  // stages that thread 0 has sent for
 
     if (warp == 0 && lane == 0) {
         int it = 0, s = 0;
@@ -521,8 +526,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
         }
-        if (*gave_up && rank == 0)
-            for (int back = max(0, it - stages); back < it; ++back) i8_drain(&full[back % stages], (back / stages) & 1);
+        copies = it;
     } else if (warp == 1 && rank == 0) {
         const uint32_t idesc = i8_idesc(2 * I8_BM, bn);
         const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + x_bytes);
@@ -606,8 +610,9 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             if (lane == 0) i8_arrive_leader(&acc_empty[buf]);
         }
     }
-    if (*gave_up && threadIdx.x == 0) atomicOr(g.err, SS_ERR_WAIT_LIMIT);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*gave_up && threadIdx.x == 0) i8_gave_up(g, full, stages, rank == 0 ? copies : 0);  // (both blocks' bytes count on the leader's barriers)
     cluster_sync_all();  // neither block leaves (or frees tensor memory) while the other may still signal it
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
