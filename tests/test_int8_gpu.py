@@ -252,6 +252,24 @@ def test_linear_in_every_form(tokens, k, features):
     o.check_errors(torch.device(DEV))
 
 
+@pytest.mark.parametrize("tokens", [3, 33, 257])
+@pytest.mark.parametrize("features", [1, 2, 31, 33, 63, 94, 257, 258, 260, 264, 287, 513])
+def test_many_tokens_with_output_rows_that_start_anywhere(tokens, features):
+    """Rows of the output that start on 2, 4, 8 or 16 bytes, and tiles that end within their first or last run of 64 bytes."""
+    o, g = ops(), gen(tokens * 1000 + features)
+    x, w, bias = int8_rows(g, tokens, 200), int8_rows(g, features, 200), normal(g, features, dtype=BF16)
+    gated = int8_rows(g, (features + 63) // 64 * 128, 200)
+    x.scales.mul_(20.0 / 200 ** 0.5)
+    for dtype in (F32, BF16):
+        for tile in (32, 96, 256):
+            assert torch.equal(o.linear_int8(x, w, bias, dtype, plan=(1, tile, 1, 1, 2)), linear_of(x, w, bias).to(dtype)), (dtype, tile)
+        for tile in (128, 256):
+            got = o.gate_up_swiglu_int8(x, gated, None, dtype, features=features, plan=(1, tile, 1, 1, 1))
+            assert torch.equal(got, o.gate_up_swiglu_int8(x, gated, None, dtype, features=features, plan=(0, 32, 1, 1, 1))), (dtype, tile)
+            assert gated_close(got, gated_of(x, gated, None, features))
+    o.check_errors(torch.device(DEV))
+
+
 def test_linear_largest_sums():
     """The longest K, every product 128 * 128: the sum stays below 2^31."""
     o = ops()
