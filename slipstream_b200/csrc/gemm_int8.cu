@@ -340,10 +340,16 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 // A persistent kernel on pairs of SMs (tcgen05.mma.cta_group::2).  A pair walks over tiles of 256 tokens x bn features, token
 // tiles fastest.  Block r of the pair fetches tokens r * 128 .. of the tile and half of its features' weights; the leader
 // (block 0) issues the products, which leave the tokens of block r in block r's tensor memory.  The accumulator is
-// double-buffered (2 x 256 columns): the eight epilogue warps of each block write a tile out while the next one is formed.
+// double-buffered (2 x 256 columns): the sixteen epilogue warps of each block write a tile out while the next one is formed.
 //   full[s]      in the leader: the bytes of both blocks' copies;     empty[s]     in each block: the products have read the stage
-//   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all sixteen epilogue warps are
-#define I8_MANY_THREADS 320  // producer, issuer, eight epilogue warps
+//   acc_full[b]  in each block: the tile's products are through;      acc_empty[b] in the leader: all 32 epilogue warps are
+//
+// The epilogue has as many warps as registers allow, four of a scheduler's: with eight, which took about 14,000 cycles of latencies for a
+// gated tile of 256 x 256, products of short K waited for them.  For the same reason the kernel is compiled for each output type, with
+// and without the gate, what a tile's epilogue reads is fetched a tile ahead, and an accumulator is handed back as soon as it
+// has been read, not when the outputs have been written.  Gated 4,096 x 896 x 9,728: 70.7 to 39.6 us, 2,048 x 1,536 x 17,920: 66.1 to 44,
+// 4,099 x 3,584 x 37,888: 353 to 345 (in a burst).
+#define I8_MANY_THREADS 576  // producer, issuer, sixteen epilogue warps
 
 __device__ __forceinline__ uint32_t i8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
 
@@ -378,26 +384,32 @@ __device__ __forceinline__ void i8_commit_pair(uint64_t* bar) {  // arrives at `
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(s_addr(bar)), "h"((unsigned short)3) : "memory");
 }
-__device__ __forceinline__ void i8_arrive_leader(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(i8_leader(bar)) : "memory");
+// A warp is through with what it read of an accumulator (its tcgen05.wait::ld is behind it).  Nothing that it wrote is handed on
+// with the arrival, so that need not wait for its stores to global memory, as one with release semantics does.
+__device__ __forceinline__ void i8_release_acc(uint64_t* bar) {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(i8_leader(bar)) : "memory");
 }
 
-__device__ __forceinline__ void i8_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// 16 columns of the accumulator, or (both) 16 and the 16 that stand 64 behind them
+__device__ __forceinline__ void i8_tmem_ld16(uint32_t taddr, bool both, uint32_t (&r)[16], uint32_t (&u)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr) : "memory");
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    if (both) {
+        tmem_ld16(taddr + 64, u);  // (waits for both)
+        return;
+    }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// 32 sums of a token as values, in place; ws and bs: the features' scales and biases, in shared memory.
-__device__ __forceinline__ void i8_values32(uint32_t (&r)[32], float xs, const float* ws, const float* bs) {
+// 16 sums of a token as values, in place; ws and bs: the features' scales and biases, in shared memory.
+__device__ __forceinline__ void i8_values16(uint32_t (&r)[16], float xs, const float* ws, const float* bs) {
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
+    for (int e = 0; e < 16; e += 4) {
         const float4 w = *reinterpret_cast<const float4*>(ws + e), b = *reinterpret_cast<const float4*>(bs + e);
         r[e] = __float_as_uint(i8_value((int)r[e], xs, w.x, b.x));
         r[e + 1] = __float_as_uint(i8_value((int)r[e + 1], xs, w.y, b.y));
@@ -405,14 +417,14 @@ __device__ __forceinline__ void i8_values32(uint32_t (&r)[32], float xs, const f
         r[e + 3] = __float_as_uint(i8_value((int)r[e + 3], xs, w.w, b.w));
     }
 }
-// A warp's 32 rows of 64 bytes from `stage` to rows of the output that start on P bytes, P bytes a thread; `limit`: the bytes
+// 16 rows of 64 bytes from `stage` to rows of the output that start on P bytes, P bytes a thread; `limit`: the bytes
 // of a run that are there.
 template <typename P>
 __device__ __forceinline__ void i8_copy_run(const unsigned char* stage, unsigned char* out, int64_t pitch, int rows, int limit) {
     constexpr int per_row = 64 / (int)sizeof(P);
     const int lane = threadIdx.x & 31, at = lane % per_row * (int)sizeof(P);
-#pragma unroll 4
-    for (int i = 0; i < per_row; ++i) {
+#pragma unroll
+    for (int i = 0; i < per_row / 2; ++i) {
         const int r = i * (32 / per_row) + lane / per_row;
         const P v = *reinterpret_cast<const P*>(stage + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15));
         if (r < rows && at < limit) *reinterpret_cast<P*>(out + r * pitch + at) = v;
@@ -420,11 +432,11 @@ __device__ __forceinline__ void i8_copy_run(const unsigned char* stage, unsigned
 }
 // The same for rows of any number of bfloat16 elements, in words: what lies in `stage` of a row that starts between two words begins
 // with its second element and has two elements less, which are written elsewhere.  (2,047 x 3,584 x 4,613 to bfloat16: 37.8 us element by
-// element, 32.6 so; to float32, where it is the loop above that copies words, 36.8 to 32.6.)
+// element, 31.4 so; to float32, where it is the loop above that copies words, 36.8 to 31.6.)
 __device__ __forceinline__ void i8_copy_run_odd(const unsigned char* stage, unsigned char* out, int64_t pitch, int rows, int limit) {
     const int lane = threadIdx.x & 31, at = (lane & 15) * 4;
 #pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const int r = 2 * i + (lane >> 4);
         const uint32_t v = *reinterpret_cast<const uint32_t*>(stage + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15));
         unsigned char* to = out + r * pitch;
@@ -435,54 +447,73 @@ __device__ __forceinline__ void i8_copy_run_odd(const unsigned char* stage, unsi
         else if (left == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)v;
     }
 }
-// A warp's 32 tokens x 32 outputs, a token a thread, through 2 KB of shared memory of the warp's own, so that it writes whole
+// A warp's 32 rows of 64 bytes, a row a thread, through 1 KB of shared memory of the warp's own, so that it writes whole
 // 64-byte runs of a row instead of 16 bytes of 32 rows at a time (2,048 x 3,584 x 9,472: 49.8 to 46.3 us).  Rows of 64 bytes lie in `stage`
 // with their four 16-byte pieces turned by (row / 2) % 4, which keeps both directions free of bank conflicts.
-template <int PIECE>
+template <typename T, int PIECE>
 __device__ __forceinline__ void i8_write_run(const Int8Args& g, unsigned char* stage, const uint32_t (&w)[16], int m0, int f) {
-    const int lane = threadIdx.x & 31, size = g.out_f32 ? 4 : 2;
-    __syncwarp();
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-    __syncwarp();
+    const int lane = threadIdx.x & 31, size = (int)sizeof(T), row = lane & 15;
     const int64_t pitch = g.ldc * size;
     unsigned char* out = (unsigned char*)g.out + m0 * pitch + (int64_t)f * size;
     const int rows = g.tokens - m0, limit = min(64, (g.out_features - f) * size);
-    if constexpr (PIECE == 16) i8_copy_run<uint4>(stage, out, pitch, rows, limit);
-    else if constexpr (PIECE == 4) i8_copy_run<uint32_t>(stage, out, pitch, rows, limit);
-    else i8_copy_run_odd(stage, out, pitch, rows, limit);
-}
-template <int PIECE>
-__device__ __forceinline__ void i8_write32(const Int8Args& g, unsigned char* stage, const uint32_t (&r)[32], int m0, int f) {
-    uint32_t w[16];
-    if (g.out_f32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h) {
+        __syncwarp();
+        if (lane >> 4 == h) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = r[16 * h + e];
-            i8_write_run<PIECE>(g, stage, w, m0, f + 16 * h);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(stage + row * 64 + ((q ^ ((row >> 1) & 3)) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
         }
-    } else {
-        const int64_t at = (int64_t)(m0 + (threadIdx.x & 31)) * g.ldc + f;
-        const bool odd = PIECE == 2 && (at & 1);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const uint32_t lo = odd ? r[2 * e + 1] : r[2 * e], hi = odd ? r[(2 * e + 2) & 31] : r[2 * e + 1];
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
-            w[e] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (odd && m0 + (threadIdx.x & 31) < g.tokens) {
-            bf16* out = (bf16*)g.out + at;
-            if (f < g.out_features) out[0] = __float2bfloat16_rn(__uint_as_float(r[0]));
-            if (f + 31 < g.out_features) out[31] = __float2bfloat16_rn(__uint_as_float(r[31]));
-        }
-        i8_write_run<PIECE>(g, stage, w, m0, f);
+        __syncwarp();
+        if constexpr (PIECE == 16) i8_copy_run<uint4>(stage, out + 16 * h * pitch, pitch, rows - 16 * h, limit);
+        else if constexpr (PIECE == 4) i8_copy_run<uint32_t>(stage, out + 16 * h * pitch, pitch, rows - 16 * h, limit);
+        else i8_copy_run_odd(stage, out + 16 * h * pitch, pitch, rows - 16 * h, limit);
     }
+}
+// A run of 64 bytes (16 or 32 outputs) of each of a warp's 32 tokens, from f on, from the accumulator's columns at `acc` on, whose
+// scales and biases are at ws and bs.  `through`: the barrier to arrive at when the accumulator has been read, or null.
+template <typename T, int PIECE, bool GATED>
+__device__ __forceinline__ void i8_write_outputs(const Int8Args& g, unsigned char* stage, uint32_t acc, float xs, const float* ws, const float* bs, int m0, int f, uint64_t* through) {
+    constexpr int PARTS = (int)sizeof(T) == 4 ? 1 : 2;
+    uint32_t w[16];
+#pragma unroll
+    for (int h = 0; h < PARTS; ++h) {
+        uint32_t r[16], u[16];
+        i8_tmem_ld16(acc + 16 * h, GATED, r, u);
+        if (h == PARTS - 1 && through) i8_release_acc(through);
+        i8_values16(r, xs, ws + 16 * h, bs + 16 * h);
+        if constexpr (GATED) {
+            i8_values16(u, xs, ws + 64 + 16 * h, bs + 64 + 16 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(silu_mul<PARTS == 2>(__uint_as_float(r[e]), __uint_as_float(u[e])));
+        }
+#pragma unroll
+        for (int e = 0; e < 16 / PARTS; ++e) {
+            if constexpr (PARTS == 1) {
+                w[e] = r[e];
+            } else {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+                w[8 * h + e] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
+    }
+    if constexpr (PIECE == 2) {
+        const int m = m0 + (threadIdx.x & 31);
+        const int64_t at = (int64_t)m * g.ldc + f;
+        if (at & 1) {
+            if (m < g.tokens) {
+                if (f < g.out_features) ((uint16_t*)g.out)[at] = (uint16_t)w[0];
+                if (f + 31 < g.out_features) ((uint16_t*)g.out)[at + 31] = (uint16_t)(w[15] >> 16);
+            }
+#pragma unroll
+            for (int e = 0; e < 15; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], 16);
+        }
+    }
+    i8_write_run<T, PIECE>(g, stage, w, m0, f);
 }
 
 // PIECE: 16, 4 or 2 bytes that the rows of the output start on and are a multiple of.
-template <int STEPS, int PIECE>
+template <int STEPS, typename T, int PIECE, bool GATED>
 __global__ void __launch_bounds__(I8_MANY_THREADS)
 gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Int8Args g) {
     constexpr int x_bytes = STEPS * I8_BM * I8_BK;
@@ -497,7 +528,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* ws_s = reinterpret_cast<float*>(full) + 64;  // [2][256] scales and [2][256] biases of a tile's features
     float* bs_s = ws_s + 2 * I8_MAX_BN;
-    unsigned char* runs = reinterpret_cast<unsigned char*>(bs_s + 2 * I8_MAX_BN);  // 2 KB for each epilogue warp
+    unsigned char* runs = reinterpret_cast<unsigned char*>(bs_s + 2 * I8_MAX_BN);  // 1 KB for each epilogue warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();  // 0: the leader
@@ -508,7 +539,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 16); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 32); }
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -518,6 +549,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const int bytes = 2 * stage_bytes;  // of both blocks
     if (threadIdx.x == 0) {
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
+#pragma unroll 1
         for (int k = 0; k < first; ++k) {
             if (rank == 0) mbar_expect_tx(&full[k], bytes);
             i8_load_pair_stage<STEPS>(tiles + k * stage_bytes + x_bytes, &map_w, g.wide_copies, k, (pair / n_m) * bn + rank * w_rows, w_rows, &full[k]);
@@ -529,6 +561,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
         pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
     } else if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int k = 0; k < first; ++k)
             i8_load_pair_stage<STEPS>(tiles + k * stage_bytes, &map_x, g.wide_copies, k, (pair % n_m) * 2 * I8_BM + rank * I8_BM, I8_BM, &full[k]);
     }
@@ -542,8 +575,10 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         int it = 0, s = 0;
         uint32_t parity = 1;  // of the round before the first: the stages are free
         bool ok = true;
+#pragma unroll 1
         for (int t = pair; t < n_tiles && ok; t += n_pairs) {
             const int m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM, n0 = (t / n_m) * bn + rank * w_rows;
+#pragma unroll 1
             for (int k = 0; k < k_iters; ++k, ++it) {
                 if (it >= first) {
                     if (!mbar_wait(&empty[s], parity, gave_up)) { ok = false; break; }
@@ -564,11 +599,13 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         int j = 0, s = 0;
         uint32_t parity = 0;
         bool ok = true;
+#pragma unroll 1
         for (int t = pair; t < n_tiles && ok; t += n_pairs, ++j) {
             const int buf = j & 1;
             if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1, gave_up))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem + buf * I8_MAX_BN;
+#pragma unroll 1
             for (int k = 0; k < k_iters; ++k) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&full[s], parity, gave_up))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -591,52 +628,48 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             __syncwarp();
         }
     } else if (warp >= 2) {
-        // warps 2 to 5 write out the first half of a tile's columns, warps 6 to 9 the second, each its quarter of the rows
-        const int quarter = warp & 3, half = (warp - 2) >> 2, col = threadIdx.x - 64;
-        const int cols = (bn / 2 + 31) / 32 * 32;
-        unsigned char* stage = runs + (warp - 2) * 2048;
-        int j = 0;
-        for (int t = pair; t < n_tiles; t += n_pairs, ++j) {
-            const int buf = j & 1, n0 = (t / n_m) * bn;
+        // each warp its quarter of the rows, and every fourth run of 64 bytes of them
+        const int quarter = warp & 3, part = (warp - 2) >> 2, col = (threadIdx.x - 64) & 255;
+        unsigned char* stage = runs + (warp - 2) * 1024;
+        constexpr int run = 64 / (int)sizeof(T);
+        const int columns = GATED ? bn / 2 : bn;
+        // a feature's scale (parts 0 and 1) or bias, and a token's scale: fetched a tile ahead
+        const auto feature_value = [&](int t) {
+            const int f = (t / n_m) * bn + col;
+            if (col >= bn || t >= n_tiles || f >= g.features) return 0.f;
+            return part < 2 ? __ldg(g.w_scale + f) : g.bias ? i8_bias(g, f) : 0.f;
+        };
+        const auto token_scale = [&](int t) {
             const int m = (t % n_m) * 2 * I8_BM + rank * I8_BM + quarter * 32 + lane;
+            return t < n_tiles && m < g.tokens ? g.x_scale[m] : 0.f;
+        };
+        float next_value = feature_value(pair), next_scale = token_scale(pair);
+        int j = 0;
+#pragma unroll 1
+        for (int t = pair; t < n_tiles; t += n_pairs, ++j) {
+            const int buf = j & 1, n0 = (t / n_m) * bn, m0 = (t % n_m) * 2 * I8_BM + rank * I8_BM + quarter * 32;
             float* ws = ws_s + buf * I8_MAX_BN;
             float* bs = bs_s + buf * I8_MAX_BN;
-            const bool in = col < bn && n0 + col < g.features;
-            ws[col] = in ? __ldg(g.w_scale + n0 + col) : 0.f;
-            bs[col] = in && g.bias ? i8_bias(g, n0 + col) : 0.f;
-            const float xs = m < g.tokens ? g.x_scale[m] : 0.f;
+            (part < 2 ? ws : bs)[col] = next_value;
+            const float xs = next_scale;
             // (a buffer is written again two tiles later, behind the barrier that every warp reaches when it is through with it)
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            next_value = feature_value(t + n_pairs);
+            next_scale = token_scale(t + n_pairs);
             // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
             const bool formed = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * I8_MAX_BN;
-            if (!formed) {
-            } else if (!g.gated) {
-#pragma unroll 1
-                for (int c = half * cols; c < min(bn, (half + 1) * cols); c += 32) {
-                    uint32_t r[32];
-                    i8_tmem_ld32(acc + c, r);
-                    i8_values32(r, xs, ws + c, bs + c);
-                    i8_write32<PIECE>(g, stage, r, m - lane, n0 + c);
-                }
-            } else {
-#pragma unroll 1
-                for (int c = half * 32; c < bn / 2; c += 64) {  // outputs
-                    const int gc = (c / 64) * 128 + (c % 64);
-                    uint32_t r[32], u[32];
-                    i8_tmem_ld32(acc + gc, r);
-                    i8_tmem_ld32(acc + gc + 64, u);
-                    i8_values32(r, xs, ws + gc, bs + gc);
-                    i8_values32(u, xs, ws + gc + 64, bs + gc + 64);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(i8_gate(g, __uint_as_float(r[e]), __uint_as_float(u[e])));
-                    i8_write32<PIECE>(g, stage, r, m - lane, n0 / 2 + c);
-                }
+            if (!formed || part * run >= columns) {
+                i8_release_acc(&acc_empty[buf]);
+                continue;
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) i8_arrive_leader(&acc_empty[buf]);
+#pragma unroll 1
+            for (int f = part * run; f < columns; f += 4 * run) {
+                const int c = GATED ? f / 64 * 128 + f % 64 : f;  // the gate's column; the up's stands 64 behind it
+                i8_write_outputs<T, PIECE, GATED>(g, stage, acc + c, xs, ws + c, bs + c, m0, (GATED ? n0 / 2 : n0) + f,
+                                                  f + 4 * run < columns ? nullptr : &acc_empty[buf]);
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -692,21 +725,28 @@ extern "C" int ss_gemm_int8_resident(int n, int per_sm) {
     return ss_resident_clusters(i8_few_shape, I8_THREADS, per_sm > 1 ? I8_SMEM_SM / per_sm - 1024 : I8_SMEM_MAX, n);
 }
 
-template <int STEPS, int PIECE>
+template <int STEPS, bool GATED, typename T, int PIECE>
 static int launch_many(const Int8Call& c, Int8Args& g) {
     CUtensorMap map_x, map_w;
     g.wide_copies = STEPS == 2 && g.K % I8_BK == 0;
     if (int rc = i8_map(&map_x, c.x, g.tokens, g.K, c.ldx, I8_BM, g.wide_copies)) return rc;
     if (int rc = i8_map(&map_w, c.w, g.features, g.K, c.ldw, g.bn / 2, g.wide_copies)) return rc;
     static SsPerDevice opted;
-    if (int rc = ss_opt_in_smem(gemm_int8_many_kernel<STEPS, PIECE>, I8_SMEM_MAX, opted)) return rc;
-    constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 8 * 2048;
+    if (int rc = ss_opt_in_smem(gemm_int8_many_kernel<STEPS, T, PIECE, GATED>, I8_SMEM_MAX, opted)) return rc;
+    constexpr int rest = I8_SMEM_REST + 4 * I8_MAX_BN * 4 + 16 * 1024;
     const int stage = STEPS * (I8_BM + g.bn / 2) * I8_BK;
     g.stages = (I8_SMEM_MAX - rest) / stage;
     const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + g.bn - 1) / g.bn);
     const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-    ss_launch_cluster_x(gemm_int8_many_kernel<STEPS, PIECE>, dim3(2 * pairs), dim3(I8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
+    ss_launch_cluster_x(gemm_int8_many_kernel<STEPS, T, PIECE, GATED>, dim3(2 * pairs), dim3(I8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
     return SS_LAUNCH_CHECK();
+}
+
+// `row`: a number of bytes whose powers of two the rows of the output start on
+template <int STEPS, bool GATED>
+static int launch_many_as(const Int8Call& c, Int8Args& g, int64_t row) {
+    if (g.out_f32) return row % 16 ? launch_many<STEPS, GATED, float, 4>(c, g) : launch_many<STEPS, GATED, float, 16>(c, g);
+    return row % 4 ? launch_many<STEPS, GATED, bf16, 2>(c, g) : row % 16 ? launch_many<STEPS, GATED, bf16, 4>(c, g) : launch_many<STEPS, GATED, bf16, 16>(c, g);
 }
 
 template <int STEPS>
@@ -752,10 +792,9 @@ extern "C" int ss_gemm_int8(const Int8Call* call) {
     g.tokens = (int)c.tokens; g.features = (int)c.features; g.K = (int)c.K; g.out_features = (int)c.out_features;
     g.out_f32 = (int)c.out_f32; g.bias_f32 = (int)c.bias_f32; g.gated = (int)c.gated; g.bn = bn; g.slices = slices;
     if (c.many) {
-        const int64_t rows = (g.ldc | g.out_features) * (g.out_f32 ? 4 : 2);
-        if (rows % 16 == 0) return c.steps == 2 ? launch_many<2, 16>(c, g) : launch_many<1, 16>(c, g);
-        if (rows % 4 == 0) return c.steps == 2 ? launch_many<2, 4>(c, g) : launch_many<1, 4>(c, g);
-        return c.steps == 2 ? launch_many<2, 2>(c, g) : launch_many<1, 2>(c, g);
+        const int64_t row = (g.ldc | g.out_features) * (g.out_f32 ? 4 : 2);
+        if (c.steps == 2) return g.gated ? launch_many_as<2, true>(c, g, row) : launch_many_as<2, false>(c, g, row);
+        return g.gated ? launch_many_as<1, true>(c, g, row) : launch_many_as<1, false>(c, g, row);
     }
     return c.steps == 2 ? launch_few<2>(c, g, per_sm) : launch_few<1>(c, g, per_sm);
 }
