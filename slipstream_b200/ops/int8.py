@@ -135,8 +135,8 @@ def int8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
 
     The choice is the cheapest by an estimate of cycles whose constants are fitted to 9,592 measured products (1 to 4,096 tokens, the
     projections of the 0.5B, 1.5B and 7B layer sizes, tiles, slices and stages of all sizes).  What it takes is on average 2 % slower
-    than the fastest of them at the same sizes, and at worst 29 % (gated products of 416 to 640 tokens at the 0.5B sizes); one tile for all tokens up to 256 with K in one slice, else tiles of
-    256 x 256, would be 44 % slower."""
+    than the fastest of them at the same sizes, and at worst 17 %; one tile for all tokens up to 256 with K in one slice, else tiles of
+    256 x 256, would be 42 % slower."""
     # what follows depends on the tokens in steps of 16 (their tiles) up to 640 and of 256 beyond: few plans for many counts
     step = 16 if tokens <= 640 else 256
     return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
@@ -168,16 +168,16 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
                 waves = (blocks + held - 1) // held
                 shared = max(1.0, min(float(per), blocks / sms))
                 # a step of K: the loops of the fetching and issuing threads; what an SM takes in; the ring's latency; the memory
-                cycles = max(543.0 if steps == 1 else 216.0, shared * (128 + tile) * 128 / 60, 2940 / (stages * steps),
-                             min(blocks, held) * 16384 * 148 / (5120 * sms))
+                cycles = max(537.0 if steps == 1 else 235.0, shared * (128 + tile) * 128 / 60, 2905 / (stages * steps),
+                             min(blocks, held) * 16384 * 148 / (5155 * sms))
                 mine = (k_steps + slices * steps - 1) // (slices * steps) * steps
-                cost = 2880 + waves * (mine * cycles + 165 + 42.9 * tile)
+                cost = 3190 + waves * (mine * cycles + 12 + 41.5 * tile)
                 if slices > 1:
-                    cost += waves * 105 * tile * (slices - 1) / slices
+                    cost += waves * 107.6 * tile * (slices - 1) / slices
                 if waves > 1:
-                    cost += 950
+                    cost += 540
                 elif per == 2 and blocks <= (0.5 if slices == 1 else 0.45) * held:  # the kernel behind has room for its first stages
-                    cost -= 2950
+                    cost -= 2970
                 if best is None or cost < best[0]:
                     best = (cost, (0, tile, slices, per, steps))
     if tokens > 64:
@@ -187,9 +187,9 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
             pairs = max(1, sms // 2)
             rounds = (tiles + pairs - 1) // pairs
             for steps in (1, 2):
-                cycles = max(412.0 if steps == 1 else 249.0, (2.3 if steps == 1 else 2.83) * tile,
-                             min(tiles, pairs) * tile * 128 * 148 / (5120 * sms * min(rows, pairs)))
-                cost = 7060 + rounds * k_steps * cycles + 26.6 * tile + (rounds - 1) * 2400
+                cycles = max(411.0 if steps == 1 else 230.0, (2.06 if steps == 1 else 2.78) * tile,
+                             min(tiles, pairs) * tile * 128 * 148 / (5155 * sms * min(rows, pairs)))
+                cost = 10450 + rounds * k_steps * cycles + 6.8 * tile + (rounds - 1) * 750
                 if best is None or cost < best[0]:
                     best = (cost, (1, tile, 1, 1, steps))
     return best[1]
