@@ -190,7 +190,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     CALL_END
 }
 
-// (values, scales, dtype) -> tensor
+// (values, scales, dtype, early) -> tensor
 PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     CALL_BEGIN
     const Rows r = rows_of(args[0], args[1], "rows");
@@ -201,7 +201,7 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     if (r.rows && r.width) {
         Int8RowsCall c = {};
         c.q = (int8_t*)r.values->data_ptr(); c.q_stride = r.stride; c.scales = (float*)r.scales->data_ptr();
-        c.rows = r.rows; c.width = r.width; c.dtype = code; c.y = out.data_ptr();
+        c.rows = r.rows; c.width = r.width; c.dtype = code; c.y = out.data_ptr(); c.early = args[3] == Py_True;
         c.stream = c10::cuda::getCurrentCUDAStream().stream();
         check(dequantize_entry(&c), "dequantize_rows_int8");
     }

@@ -11,7 +11,7 @@ struct Int8RowsCall {
     int64_t q_stride;
     float* scales;
     int64_t rows, width, dtype;  // SS_F32 or SS_BF16: of x; of the values; of delta
-    int64_t early;               // quantize: the kernel behind may start at once
+    int64_t early;               // quantize and dequantize: the kernel behind may start at once
     void* y;                     // dequantize: [rows, width]; norm: residual_out or null (may be x)
     const void* delta;           // norm: [rows, width] or null
     const void* weight;

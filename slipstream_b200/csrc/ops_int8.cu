@@ -537,9 +537,9 @@ constexpr int DEQ_THREADS = 256, DEQ_GROUPS = 4;
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(DEQ_THREADS)
 dequantize_rows_kernel(const int8_t* q, int64_t q_stride, const float* scales, T* y, int width,
-                       int spans) {
+                       int spans, int early) {
     constexpr int G = ALIGNED ? 16 / (int)sizeof(T) : 1;
-    pdl_launch_dependents();
+    if (early) pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.x / spans, first = (blockIdx.x - row * spans) * (int)(blockDim.x * DEQ_GROUPS) + threadIdx.x;
     const float s = scales[row];
@@ -662,8 +662,8 @@ static int int8_rows_refused(const Int8RowsCall& c) {
     return c.width <= 0 || c.width > INT32_MAX - 8 || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
 }
 
-// early: the kernel behind may start at once; it may then have read what it takes for constant before q is written, so only
-// for q that it does not take for that (weights are).
+// early, here and in the way back: the kernel behind may start at once; it may then have read what it takes for constant before the
+// results are written, so only for results that it does not take for that (weights are).
 extern "C" int ss_quantize_rows_int8(const Int8RowsCall* call) {
     const Int8RowsCall& c = *call;
     if (c.rows <= 0) return 0;
@@ -710,7 +710,7 @@ extern "C" int ss_dequantize_rows_int8(const Int8RowsCall* call) {
     threads = threads > DEQ_THREADS ? DEQ_THREADS : threads;
     const int span = threads * DEQ_GROUPS, spans = (groups + span - 1) / span;
     if (c.rows * spans > INT32_MAX) return -2003;
-#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows * spans), dim3(threads), 0, c.stream, c.q, c.q_stride, c.scales, (T*)c.y, width, spans)
+#define DEQ(T, A) ss_launch(dequantize_rows_kernel<T, A>, dim3(rows * spans), dim3(threads), 0, c.stream, c.q, c.q_stride, c.scales, (T*)c.y, width, spans, (int)c.early)
     if (c.dtype == SS_BF16) { if (aligned) DEQ(bf16, true); else DEQ(bf16, false); }
     else { if (aligned) DEQ(float, true); else DEQ(float, false); }
 #undef DEQ

@@ -10,8 +10,9 @@ Rows of values start on 16 bytes: their stride is a multiple of 16, whatever the
 and every function here that returns int8 rows uses it.
 
 Weights, their scales, biases and the weights of a norm are taken for constant, as elsewhere in this package: a kernel may read them
-before the kernels in front of it are through.  `quantize_rows_int8` therefore keeps the kernels behind it waiting unless it is told
-(``activations=True``) that its rows will not be a product's weights.
+before the kernels in front of it are through.  `quantize_rows_int8` and `dequantize_rows_int8` therefore keep the kernels behind them
+waiting unless they are told (``activations=True``) that what they write will not be a product's weights.  The results of the norm and
+of products are activations.
 """
 
 from __future__ import annotations
@@ -50,8 +51,8 @@ class Int8Rows:
         """Bytes a pass over the rows reads (without what pads them)."""
         return self.values.numel() + 4 * self.scales.numel()
 
-    def dequantize(self, dtype: torch.dtype) -> torch.Tensor:
-        return dequantize_rows_int8(self, dtype)
+    def dequantize(self, dtype: torch.dtype, *, activations: bool = False) -> torch.Tensor:
+        return dequantize_rows_int8(self, dtype, activations=activations)
 
 
 _native = None
@@ -106,11 +107,13 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     return Int8Rows(*(_native or _calls()).quantize(x, activations))
 
 
-def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
-    """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once."""
+def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype, *, activations: bool = False) -> torch.Tensor:
+    """``values * scales`` as a tensor [N, K] of ``dtype`` (float32 or bfloat16), rounded once.
+
+    ``activations``: the tensor is a product's activations, not its weights, and the kernel behind may start early."""
     _need_rows(rows, "rows")
     _launches[0] += 1
-    return (_native or _calls()).dequantize(rows.values, rows.scales, dtype)
+    return (_native or _calls()).dequantize(rows.values, rows.scales, dtype, activations)
 
 
 def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, *,

@@ -385,6 +385,25 @@ def test_weights_rounded_right_in_front_of_their_product():
         assert torch.equal(got, linear_of(x, w, None))
 
 
+@pytest.mark.parametrize("tokens", [3, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weights_turned_back_right_in_front_of_their_product(dtype, tokens):
+    """The same for the product of the values: against the same product a second time, when everything in front of it is through.
+    The weights' memory holds NaN before."""
+    o, g = ops(), gen(10)
+    x = normal(g, tokens, 4096, dtype=dtype)
+    for seed in range(20):
+        rows = int8_rows(gen(seed), 6144, 4096)
+        torch.cuda.synchronize()
+        weight = rows.dequantize(dtype)
+        got = o.linear(x, weight)
+        torch.cuda.synchronize()
+        assert torch.equal(weight, (rows.values.float() * rows.scales[:, None]).to(dtype))
+        assert torch.equal(got, o.linear(x, weight)), seed
+        weight.fill_(float("nan"))
+        del weight  # (the next one takes its memory)
+
+
 def test_layer_on_another_stream_and_in_a_graph():
     """Norm, product, rounding, gated product, product: on a stream of its own, and captured and replayed with other inputs."""
     o, g = ops(), gen(21)
