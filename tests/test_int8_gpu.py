@@ -404,6 +404,34 @@ def test_weights_turned_back_right_in_front_of_their_product(dtype, tokens):
         del weight  # (the next one takes its memory)
 
 
+@pytest.mark.parametrize("tokens", [3, 300])
+@pytest.mark.parametrize("back", [False, True])
+def test_weights_written_two_kernels_in_front_of_their_product(back, tokens):
+    """Between the weights and the product stands a kernel that lets the one behind it go at once, as in a program: the norm whose
+    rows the product takes, or the rounding of its activations.  Weights of both kernels that round: a block per row, and the ring."""
+    o = ops()
+    for seed in range(10):
+        g, k = gen(seed), 8192 if seed % 2 else 4096
+        matrix, stream, norm_w = normal(g, 2600 if seed % 2 else 512, k, dtype=BF16), normal(g, tokens, k), torch.ones(k, device=DEV)
+        torch.cuda.synchronize()
+        if back:
+            rows = o.quantize_rows_int8(matrix)
+            weight = rows.dequantize(BF16)
+            x = o.quantize_rows_int8(stream, activations=True).dequantize(BF16, activations=True)
+            got = o.linear(x, weight)
+            torch.cuda.synchronize()
+            assert torch.equal(weight, (rows.values.float() * rows.scales[:, None]).to(BF16))
+            assert torch.equal(got, o.linear(x, weight))
+        else:
+            weight = o.quantize_rows_int8(matrix)
+            x = o.add_rmsnorm_int8(stream, None, norm_w, 1e-6)
+            got = o.linear_int8(x, weight, None, F32)
+            assert torch.equal(got, linear_of(x, weight, None))
+            weight.values.zero_()
+            weight.scales.fill_(float("nan"))
+        del weight  # (the next one may take its memory)
+
+
 def test_layer_on_another_stream_and_in_a_graph():
     """Norm, product, rounding, gated product, product: on a stream of its own, and captured and replayed with other inputs."""
     o, g = ops(), gen(21)
