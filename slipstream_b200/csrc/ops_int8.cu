@@ -381,10 +381,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  ::"r"(s_addr(dst)), "l"(src), "r"(bytes), "r"(s_addr(bar)) : "memory");
 }
 struct RowRing {
-    unsigned char* rows;  // [stages][row_bytes]
+    unsigned char* rows;  // [stages][bytes of a row]
     uint64_t* full;
     int* gave_up;
-    int stages, row_bytes;
+    int stages;
 };
 // smem: the rows (16-byte aligned), then the barriers, then the flag
 __device__ __forceinline__ RowRing row_ring(unsigned char* smem, int stages, int row_bytes) {
@@ -393,7 +393,6 @@ __device__ __forceinline__ RowRing row_ring(unsigned char* smem, int stages, int
     r.full = reinterpret_cast<uint64_t*>(smem + stages * row_bytes);
     r.gave_up = reinterpret_cast<int*>(r.full + stages);
     r.stages = stages;
-    r.row_bytes = row_bytes;
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) mbar_init(&r.full[s], 1);
         *r.gave_up = 0;
@@ -404,14 +403,11 @@ __device__ __forceinline__ RowRing row_ring(unsigned char* smem, int stages, int
     return r;
 }
 
-// Behind a wait that gave up: the block does not end under its copies in flight, the last of the `issued` ones (each wait has its
-// own limit).
+// Behind a wait that gave up (the block has left its loop at that row): the error word, and a wait for the block's copies in flight,
+// the last of the `issued` ones that thread 0 has sent for.
 __device__ __forceinline__ void drain_ring(const RowRing& r, int issued, int* err) {
     if (!*(volatile int*)r.gave_up || threadIdx.x) return;
-    for (int i = max(0, issued - r.stages); i < issued; ++i) {
-        volatile int none = 0;
-        (void)mbar_wait(&r.full[i % r.stages], (i / r.stages) & 1, &none);
-    }
+    for (int i = max(0, issued - r.stages); i < issued; ++i) mbar_drain(&r.full[i % r.stages], (i / r.stages) & 1);
     atomicOr(err, SS_ERR_WAIT_LIMIT);
 }
 
@@ -427,7 +423,9 @@ quantize_ring_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t
     const RowRing ring = row_ring(ring_smem, stages, bytes);
     if (early) pdl_launch_dependents();
     pdl_wait();
+    int issued = 0;  // copies that thread 0 has sent for
     auto fetch = [&](int64_t row, int s) {
+        ++issued;
         mbar_expect_tx(&ring.full[s], bytes);
         bulk_load(ring.rows + s * bytes, x + row * stride, bytes, &ring.full[s]);
     };
@@ -436,7 +434,7 @@ quantize_ring_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t
     int s = 0, n = 0;
     uint32_t parity = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
-        mbar_wait(&ring.full[s], parity, ring.gave_up);
+        const bool landed = mbar_wait(&ring.full[s], parity, ring.gave_up);
         const T* from = reinterpret_cast<const T*>(ring.rows + s * bytes);
         Vec v[NG];
         uint32_t top = 0;
@@ -448,7 +446,7 @@ quantize_ring_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t
         }
         top = __reduce_max_sync(0xffffffffu, Vec::top_bits(top));
         if (lane == 0) tops[n & 1][warp] = top;  // (two sets: the next row's are written while slow warps still read these)
-        __syncthreads();
+        if (!__syncthreads_and(landed)) break;  // nothing of the row is written, nothing more is sent for
         if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
         top = __reduce_max_sync(0xffffffffu, lane < RING_THREADS / 32 ? tops[n & 1][lane] : 0u);
         const RowScale r = row_scale(top);
@@ -461,7 +459,7 @@ quantize_ring_kernel(const T* x, int64_t stride, int8_t* __restrict__ q, int64_t
         }
         if (++s == stages) { s = 0; parity ^= 1; }
     }
-    drain_ring(ring, n, err);  // (the block's rows are its copies, in order)
+    drain_ring(ring, issued, err);
     if (!early) publish_results();
 }
 
@@ -485,7 +483,9 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* resid
         else load4<true>((const bf16*)weight + j, width - j, w[i]);
     }
     pdl_wait();
+    int issued = 0;  // copies that thread 0 has sent for
     auto fetch = [&](int64_t row, int s) {
+        ++issued;
         mbar_expect_tx(&ring.full[s], bytes);
         bulk_load(ring.rows + s * bytes, residual + row * width, x_bytes, &ring.full[s]);
         if (d_bytes) bulk_load(ring.rows + s * bytes + x_bytes, delta + row * width, d_bytes, &ring.full[s]);
@@ -495,7 +495,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* resid
     int s = 0, n = 0;
     uint32_t parity = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
-        mbar_wait(&ring.full[s], parity, ring.gave_up);
+        const bool landed = mbar_wait(&ring.full[s], parity, ring.gave_up);
         const float* from = reinterpret_cast<const float*>(ring.rows + s * bytes);
         const T* from_d = reinterpret_cast<const T*>(ring.rows + s * bytes + x_bytes);
         float v[NG][4], part[NG];
@@ -511,7 +511,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* resid
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[i][e] = __fadd_rn(v[i][e], d[e]);
                 }
-                if (residual_out) *reinterpret_cast<float4*>(residual_out + row * width + j) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                if (residual_out && landed) *reinterpret_cast<float4*>(residual_out + row * width + j) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
@@ -524,7 +524,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* resid
         top = __reduce_max_sync(0xffffffffu, top);
         warp_sums(part, sums[n & 1] + warp, RING_THREADS / 32);
         if (lane == 0) tops[n & 1][warp] = top;
-        __syncthreads();
+        if (!__syncthreads_and(landed)) break;  // (of the stream threads have written what they saw land)
         if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
         top = __reduce_max_sync(0xffffffffu, lane < RING_THREADS / 32 ? tops[n & 1][lane] : 0u);
         const float ss = sum_of_sums(sums[n & 1], width);
@@ -538,7 +538,7 @@ add_rmsnorm_int8_ring_kernel(const float* residual, const T* delta, float* resid
         }
         if (++s == stages) { s = 0; parity ^= 1; }
     }
-    drain_ring(ring, n, err);  // (the block's rows are its copies, in order)
+    drain_ring(ring, issued, err);
 }
 
 // ---------------------------------------------------------------- int8 rows to values

@@ -4,6 +4,10 @@
 #include "common.cuh"
 
 #define WAIT_LIMIT (1u << 20)
+// Polls after which a wait gives up.  A build may set 0: every wait gives up at once, which shows what a kernel does then.
+#ifndef WAIT_POLLS
+#define WAIT_POLLS WAIT_LIMIT
+#endif
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -13,20 +17,27 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(bar)), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done) : "r"(s_addr(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 // Bounded wait: false when the limit ran out (or another role already gave up).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-    for (uint32_t spins = 0; spins < WAIT_LIMIT; ++spins) {
-        uint32_t done;
-        asm volatile(
-            "{\n.reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done) : "r"(s_addr(bar)), "r"(parity) : "memory");
-        if (done) return true;
+    for (uint32_t spins = 0; spins < WAIT_POLLS; ++spins) {
+        if (mbar_try_wait(bar, parity)) return true;
         if ((spins & 1023u) == 1023u && *gave_up) return false;
     }
     *gave_up = 1;
     return false;
+}
+// A block that gave up waits here, before it ends, for what is in flight to it: with a limit of its own, whatever the other waits'.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+    for (uint32_t spins = 0; spins < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++spins) {}
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
