@@ -89,14 +89,15 @@ __device__ __forceinline__ uint32_t i8_idesc(int m, int n) {
 }
 
 // Behind a wait that gave up: the error word, and a wait for the last of the `copies` stages that were sent for, which may still be
-// in flight (each with its own limit, blind to the flag).
+// in flight.
 __device__ __noinline__ void i8_gave_up(const Int8Args& g, uint64_t* full, int stages, int copies) {
     atomicOr(g.err, SS_ERR_WAIT_LIMIT);
-    for (int i = max(0, copies - stages); i < copies; ++i) {
-        volatile int none = 0;
-        (void)mbar_wait(&full[i % stages], (i / stages) & 1, &none);
-    }
+    for (int i = max(0, copies - stages); i < copies; ++i) mbar_drain(&full[i % stages], (i / stages) & 1);
 }
+
+// A barrier that is used once a launch, behind a wait that gave up.  (Out of line, as i8_gave_up: in the epilogue's way it cost 0.1 us of
+// 13 at 16 x 18,944 x 3,584.)
+__device__ __noinline__ void i8_drain(uint64_t* bar) { mbar_drain(bar, 0); }
 
 __device__ __forceinline__ float i8_bias(const Int8Args& g, int f) {
     return g.bias_f32 ? ((const float*)g.bias)[f] : to_float(((const bf16*)g.bias)[f]);
@@ -107,6 +108,17 @@ __device__ __forceinline__ float i8_value(int sum, float xs, float ws, float bia
 }
 __device__ __forceinline__ float i8_gate(const Int8Args& g, float gate, float up) {
     return g.out_f32 ? silu_mul<false>(gate, up) : silu_mul<true>(gate, up);
+}
+
+// Whether `v` holds in all 128 threads of the few tokens' epilogue; a barrier of theirs.
+__device__ __forceinline__ bool i8_epilogue_all(bool v) {
+    uint32_t all;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\n"
+        "bar.red.and.pred p, 1, 128, q;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(all) : "r"((uint32_t)v) : "memory");
+    return all != 0;
 }
 
 // Four outputs of a token, `apart` features from one another.
@@ -280,22 +292,27 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         asm volatile("bar.sync 2, 160;" ::: "memory");  // the scales are there, and the tensor memory's address
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(quarter * 32) << 16);
-        bool ok = mbar_wait(acc_ready, 0, gave_up);
+        // (the flag, not the wait's result: an issuer that gave up still commits, so that the accumulator can be waited for, and copies may
+        // then be landing where the sums would go; a vote over the results cost 0.3 us)
+        (void)mbar_wait(acc_ready, 0, gave_up);
+        bool ok = !__shfl_sync(0xffffffffu, *gave_up, 0);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (n_sl == 1) {
-            for (int c = 0; c < live; c += 16) {
+            for (int c = 0; ok && c < live; c += 16) {
                 uint32_t r[16];
                 tmem_ld16(acc + c, r);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) sums[(c + j) * I8_BM + quarter * 32 + lane] = (int)r[j];
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            ok = i8_epilogue_all(ok);
         } else {
             if (k_iters > 0) {
                 int owner = 0, at = 0;  // of column c: block c % slices, its column c / slices
                 for (int c = 0; c < live; c += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(acc + c, r);
+                    // a warp that gave up sends zeros: the bytes that the owners count always arrive, so that none of them leaves with
+                    // sums on their way to it (what they write is wrong then; the error word says so)
+                    uint32_t r[16] = {};
+                    if (ok) tmem_ld16(acc + c, r);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         if (c + j < live)
@@ -304,10 +321,11 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     }
                 }
             }
-            ok = mbar_wait(sums_ready, 0, gave_up) && ok;
+            if (!mbar_wait(sums_ready, 0, gave_up)) i8_drain(sums_ready);
+            ok = !*gave_up;
         }
         // a warp takes a token column (gated: each of its halves one) at a time, a lane four features of it
-        for (int i = g.gated ? 2 * quarter + half : quarter; i < mine; i += g.gated ? 8 : 4) {
+        for (int i = g.gated ? 2 * quarter + half : quarter; ok && i < mine; i += g.gated ? 8 : 4) {
             const int c = rank + i * n_sl;
             const int* from = sums + i * I8_BM + fl;
             const float xs = xs_s[c];
@@ -320,7 +338,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             i8_store4(g, t0 + c, (g.gated ? f0 / 2 : f0) + fl, apart, v);
         }
     }
-    if (n_sl > 1) {  // nobody leaves while sums may still be on their way to it, whatever gave up
+    if (n_sl > 1) {  // nobody leaves while others may still send to it: each has seen the sums that it owns arrive
         __syncwarp();
         asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
         asm volatile("barrier.cluster.wait;" ::: "memory");
@@ -329,6 +347,8 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     __syncthreads();
     if (*gave_up && threadIdx.x == 0) i8_gave_up(g, full, stages, copies);
     if (warp == 1) {
+        if (*gave_up) i8_drain(acc_ready);  // products in flight
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t tmem_acc = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(tmem_cols));

@@ -21,6 +21,13 @@ class RowsCall(ctypes.Structure):  # csrc/int8_calls.h, Int8RowsCall
                 ("w_f32", c_int64), ("eps", c_double), ("err", c_void_p), ("stream", c_void_p)]
 
 
+class ProductCall(ctypes.Structure):  # Int8Call
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("x_scale", c_void_p), ("w", c_void_p), ("ldw", c_int64), ("w_scale", c_void_p),
+                ("bias", c_void_p), ("bias_f32", c_int64), ("out", c_void_p)]
+    _fields_ += [(name, c_int64) for name in ("ldc", "out_f32", "tokens", "features", "K", "gated", "out_features", "many", "bn", "slices", "per_sm", "steps")]
+    _fields_ += [("err", c_void_p), ("stream", c_void_p)]
+
+
 def without_waits(name, source):
     from slipstream_b200.ops.library import compile_library
 
@@ -30,6 +37,11 @@ def without_waits(name, source):
 @pytest.fixture(scope="module")
 def rows_library():
     return without_waits("slipstream_int8_rows", "ops_int8.cu")
+
+
+@pytest.fixture(scope="module")
+def products_library():
+    return without_waits("slipstream_int8_products", "gemm_int8.cu")
 
 
 def ran(entry, call):
@@ -80,3 +92,34 @@ def test_norm_of_many_rows(rows_library, delta, width, in_place):
     ops.add_rmsnorm_int8(stream, d, weight, 1e-6)
     assert torch.equal(stream, residual if d is None else residual + d.float())
     ops.check_errors(torch.device(DEV))
+
+
+def gives_up(library, tokens, k, features, plan, gated, dtype):
+    """A product with the build that gives up, then with the ordinary one."""
+    from slipstream_b200 import ops
+
+    def int8_rows(n):
+        store = torch.randint(-127, 128, (n, (k + 15) & -16), device=DEV, dtype=torch.int8)
+        return ops.Int8Rows(store[:, :k], torch.rand(n, device=DEV))
+
+    x, w = int8_rows(tokens), int8_rows(features)
+    columns = features // 2 if gated else features
+    out = torch.full((tokens, columns), 7.0, device=DEV, dtype=dtype)
+    many, bn, slices, per_sm, steps = plan
+    call = ProductCall(x=x.values.data_ptr(), ldx=x.values.stride(0), x_scale=x.scales.data_ptr(), w=w.values.data_ptr(), ldw=w.values.stride(0),
+                       w_scale=w.scales.data_ptr(), out=out.data_ptr(), ldc=columns, out_f32=int(dtype == F32), tokens=tokens, features=features,
+                       K=k, gated=int(gated), out_features=columns, many=many, bn=bn, slices=slices, per_sm=per_sm, steps=steps)
+    assert ran(library.ss_gemm_int8, call) == WAIT_LIMIT
+    assert (out == 7).all()
+    if not gated:
+        sums = x.values.to(torch.float64) @ w.values.to(torch.float64).t()
+        assert torch.equal(ops.linear_int8(x, w, None, F32, plan=plan), sums.to(F32) * x.scales[:, None] * w.scales)
+    ops.check_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens, k, plan", [(1, 100, (0, 16, 1, 1, 1)), (9, 3584, (0, 16, 1, 2, 2)), (200, 18944, (0, 208, 1, 1, 1)), (100, 2000, (0, 48, 1, 1, 2)),
+                                             (16, 3584, (0, 16, 4, 2, 2)), (33, 896, (0, 48, 2, 1, 1)), (250, 18944, (0, 256, 5, 1, 1)), (60, 300, (0, 32, 8, 1, 1))])
+def test_products_of_few_tokens(products_library, tokens, k, plan, gated, dtype):
+    gives_up(products_library, tokens, k, 1152, plan, gated, dtype)
