@@ -532,6 +532,44 @@ __device__ __forceinline__ void i8_write_outputs(const Int8Args& g, unsigned cha
     i8_write_run<T, PIECE>(g, stage, w, m0, f);
 }
 
+// What a block of a pair has sent for and formed, for the other one to read where a wait gave up.
+struct I8PairCounts {
+    int copies;  // stages that it has sent for
+    int tiles;   // leader: accumulators that it has committed
+};
+// The other block's flag: its waits may go well, for an accumulator that is committed but not formed.
+__device__ __noinline__ void i8_tell_pair(volatile int* gave_up) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(i8_remote((const void*)gave_up, cluster_rank() ^ 1)), "r"(1) : "memory");
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+// Where a wait of either block gave up, both come here: the error word, and a wait for what is in flight to them.  Both blocks' bytes count
+// on the leader's barriers (`bytes` a stage, half of them each's), and one may have sent for stages that the other has not: the leader
+// arrives for those that it has not sent for itself, and counts the half that nobody sent as landed.
+__device__ __noinline__ void i8_pair_gave_up(const Int8Args& g, uint64_t* full, uint64_t* acc_full, int stages, int bytes, const I8PairCounts* counts) {
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        atomicOr(g.err, SS_ERR_WAIT_LIMIT);
+        const auto of = [&](uint32_t block, const int* p) {
+            int v;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(i8_remote(p, block)) : "memory");
+            return v;
+        };
+        const int tiles = of(0, &counts->tiles);
+        if (rank == 0) {
+            const int mine = counts->copies, other = of(1, &counts->copies), all = max(mine, other);
+            for (int i = max(0, all - stages); i < all; ++i) {
+                uint64_t* bar = &full[i % stages];
+                if (i >= mine) mbar_expect_tx(bar, bytes);
+                if (i >= min(mine, other))
+                    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(s_addr(bar)), "r"(bytes / 2) : "memory");
+                mbar_drain(bar, (i / stages) & 1);
+            }
+        }
+        for (int j = max(0, tiles - 2); j < tiles; ++j) mbar_drain(&acc_full[j & 1], (j >> 1) & 1);
+    }
+    cluster_sync_all();
+}
+
 // PIECE: 16, 4 or 2 bytes that the rows of the output start on and are a multiple of.
 template <int STEPS, typename T, int PIECE, bool GATED>
 __global__ void __launch_bounds__(I8_MANY_THREADS)
@@ -546,6 +584,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    I8PairCounts* counts = reinterpret_cast<I8PairCounts*>(tmem_slot + 2);
     float* ws_s = reinterpret_cast<float*>(full) + 64;  // [2][256] scales and [2][256] biases of a tile's features
     float* bs_s = ws_s + 2 * I8_MAX_BN;
     unsigned char* runs = reinterpret_cast<unsigned char*>(bs_s + 2 * I8_MAX_BN);  // 1 KB for each epilogue warp
@@ -561,6 +600,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 32); }
         *gave_up = 0;
+        counts->copies = counts->tiles = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -589,7 +629,6 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     cluster_sync_all();  // the tensor memory of both blocks has been taken
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    int copies = 0;  // stages that thread 0 has sent for
 
     if (warp == 0 && lane == 0) {
         int it = 0, s = 0;
@@ -610,7 +649,7 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
         }
-        copies = it;
+        counts->copies = it;
     } else if (warp == 1 && rank == 0) {
         const uint32_t idesc = i8_idesc(2 * I8_BM, bn);
         const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + x_bytes);
@@ -622,11 +661,11 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 #pragma unroll 1
         for (int t = pair; t < n_tiles && ok; t += n_pairs, ++j) {
             const int buf = j & 1;
-            if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1, gave_up))) break;
+            ok = j < 2 || __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1, gave_up));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem + buf * I8_MAX_BN;
 #pragma unroll 1
-            for (int k = 0; k < k_iters; ++k) {
+            for (int k = 0; ok && k < k_iters; ++k) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&full[s], parity, gave_up))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t x_desc = x_first + s * stage_step, w_desc = w_first + s * stage_step;
@@ -644,9 +683,12 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 __syncwarp();
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
+            if (!ok) i8_tell_pair(gave_up);
+            __syncwarp();
             if (elect_one()) i8_commit_pair(&acc_full[buf]);
             __syncwarp();
         }
+        if (lane == 0) counts->tiles = j;
     } else if (warp >= 2) {
         // each warp its quarter of the rows, and every fourth run of 64 bytes of them
         const int quarter = warp & 3, part = (warp - 2) >> 2, col = (threadIdx.x - 64) & 255;
@@ -677,7 +719,9 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             next_value = feature_value(t + n_pairs);
             next_scale = token_scale(t + n_pairs);
             // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
-            const bool formed = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up));
+            // (the flag, not the wait's result: an issuer that gave up still commits, so that the accumulator can be waited for)
+            (void)mbar_wait(&acc_full[buf], (j >> 1) & 1, gave_up);
+            const bool formed = !__shfl_sync(0xffffffffu, *gave_up, 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * I8_MAX_BN;
             if (!formed || part * run >= columns) {
@@ -694,8 +738,9 @@ gemm_int8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (*gave_up && threadIdx.x == 0) i8_gave_up(g, full, stages, rank == 0 ? copies : 0);  // (both blocks' bytes count on the leader's barriers)
+    if (*gave_up && threadIdx.x == 0) i8_tell_pair(gave_up);  // the other block comes along
     cluster_sync_all();  // neither block leaves (or frees tensor memory) while the other may still signal it
+    if (*gave_up) i8_pair_gave_up(g, full, acc_full, stages, bytes, counts);
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));

@@ -123,3 +123,11 @@ def gives_up(library, tokens, k, features, plan, gated, dtype):
                                              (16, 3584, (0, 16, 4, 2, 2)), (33, 896, (0, 48, 2, 1, 1)), (250, 18944, (0, 256, 5, 1, 1)), (60, 300, (0, 32, 8, 1, 1))])
 def test_products_of_few_tokens(products_library, tokens, k, plan, gated, dtype):
     gives_up(products_library, tokens, k, 1152, plan, gated, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens, k, features, plan", [(1, 100, 128, (1, 128, 1, 1, 1)), (300, 896, 1152, (1, 256, 1, 1, 2)), (2047, 3584, 4608, (1, 256, 1, 1, 1)),
+                                                       (4099, 300, 9728, (1, 128, 1, 1, 2)), (515, 18944, 3584, (1, 256, 1, 1, 1))])
+def test_products_of_many_tokens(products_library, tokens, k, features, plan, gated, dtype):
+    gives_up(products_library, tokens, k, features, plan, gated, dtype)
