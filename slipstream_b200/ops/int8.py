@@ -151,7 +151,8 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
         resident = tuple(tuple(sms * per // n for n in range(1, 9)) for per in (1, 2))
     k_steps = (k + 127) // 128
     best = None
-    for parts in range(1, 9) if tokens <= 640 else ():
+    few = tokens <= 640 and (features + 127) // 128 <= 65535  # (its tiles of features are blocks along grid.y)
+    for parts in range(1, 9) if few else ():
         tile = ((tokens + parts - 1) // parts + 15) // 16 * 16
         if tile > 256 or (parts > 1 and tile <= 16):
             continue
@@ -183,7 +184,7 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
                     cost -= 2970
                 if best is None or cost < best[0]:
                     best = (cost, (0, tile, slices, per, steps))
-    if tokens > 64:
+    if tokens > 64 or not few:
         rows = (tokens + 255) // 256
         for tile in ((128, 256) if gated else (32, 64, 96, 128, 160, 192, 224, 256)):
             tiles = rows * ((features + tile - 1) // tile)

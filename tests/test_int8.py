@@ -53,6 +53,15 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
                     assert 2 * steps * (128 + tile) * 128 + rest <= 232448
 
 
+def test_plans_of_more_features_than_a_grid_has_rows_for_their_tiles():
+    """The kernel for few tokens has its tiles of 128 features along grid.y: up to 65,535 of them."""
+    for tokens in (1, 64, 65, 640, 700):
+        for gated in (False, True):
+            assert tokens > 64 or int8_plan(tokens, 65535 * 128, 16, 148, gated, RESIDENT)[0] == 0
+            many, tile, slices, per, steps = int8_plan(tokens, 65535 * 128 + (128 if gated else 1), 16, 148, gated, RESIDENT)
+            assert many == 1 and tile % (128 if gated else 32) == 0 and steps in (1, 2)
+
+
 def test_plans_do_not_change_within_a_step_of_tokens():
     for tokens in (1, 17, 300, 1000):
         step = 16 if tokens <= 640 else 256

@@ -285,6 +285,18 @@ def test_linear_largest_sums():
         assert torch.equal(got, linear_of(x, w, None)) and got.max() == float(128 * 128 * k) and got.min() == -float(127 * 128 * k)
 
 
+def test_more_features_than_a_grid_has_rows_for_their_tiles():
+    o, g = ops(), gen(12)
+    features = 65536 * 128
+    x, w = int8_rows(g, 3, 16), int8_rows(g, features, 16)
+    for n in (features - 127, features):
+        part = o.Int8Rows(w.values[:n], w.scales[:n])
+        assert torch.equal(o.linear_int8(x, part, None, F32), linear_of(x, part, None))
+    x.scales.mul_(5.0)
+    assert gated_close(o.gate_up_swiglu_int8(x, w, None, F32), gated_of(x, w, None, features // 2))
+    o.check_errors(torch.device(DEV))
+
+
 def test_linear_scales_that_are_not_numbers():
     o, g = ops(), gen(11)
     for tokens in (4, 300):
