@@ -128,6 +128,11 @@ void check(int code, const char* what) {
     if (code) refuse(std::string(what) + ": CUDA error " + std::to_string(code) + " at launch");
 }
 
+void check_size(int64_t rows, int64_t width) {
+    if (width > INT8_MAX_WIDTH || rows > INT32_MAX)
+        refuse("int8 rows are formed " + std::to_string(INT32_MAX) + " at most, of " + std::to_string(INT8_MAX_WIDTH) + " elements at most, not " + std::to_string(rows) + " of " + std::to_string(width));
+}
+
 struct Rows {
     int64_t rows, width, stride;
     const at::Tensor *values, *scales;
@@ -176,6 +181,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     if (x.dim() != 2) refuse("x must be two-dimensional, got " + say(x.sizes()));
     const int64_t n = x.size(0), k = x.size(1), q_stride = (k + 15) & -16, code = code_of(x.scalar_type());
     if (k < 1) refuse("rows without elements have no scale");
+    check_size(n, k);
     if (k > 1 && x.stride(1) != 1) refuse("the rows of x must be contiguous, got strides " + say(x.strides()));
     OnDevice here(x);
     auto [values, scales] = empty_rows(n, k, q_stride, x);
@@ -196,6 +202,7 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     const Rows r = rows_of(args[0], args[1], "rows");
     const at::ScalarType type = dtype_of(args[2]);
     const int64_t code = code_of(type);
+    check_size(r.rows, r.width);
     OnDevice here(*r.values);
     at::Tensor out = empty(r.rows, r.width, type, *r.values);
     if (r.rows && r.width) {
@@ -216,6 +223,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t) {
     if (residual.scalar_type() != at::kFloat) refuse(std::string("residual must be float32, got ") + c10::toString(residual.scalar_type()));
     if (residual.dim() != 2 || residual.size(1) < 1) refuse("residual must be [tokens, features], got " + say(residual.sizes()));
     const int64_t n = residual.size(0), h = residual.size(1), q_stride = (h + 15) & -16;
+    check_size(n, h);
     Int8RowsCall c = {};
     c.x = residual.data_ptr(); c.stride = h; c.rows = n; c.width = h; c.dtype = 1;
     if (args[1] != Py_None) {

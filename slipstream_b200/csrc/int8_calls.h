@@ -4,6 +4,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+// The widest row: its kernels count elements in 32 bits, and a loop of theirs steps over up to 4,096 at a time.
+constexpr int64_t INT8_MAX_WIDTH = INT32_MAX - 8192;
+
 struct Int8RowsCall {
     const void* x;  // quantize: [rows, width], row stride `stride` elements; dequantize: unused; norm: the stream, [rows, width]
     int64_t stride;

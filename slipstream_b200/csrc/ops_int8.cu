@@ -673,7 +673,7 @@ inline bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 }  // namespace
 
 static int int8_rows_refused(const Int8RowsCall& c) {
-    return c.width <= 0 || c.width > INT32_MAX - 8 || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
+    return c.width <= 0 || c.width > INT8_MAX_WIDTH || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
 }
 
 // early, here and in the way back: the kernel behind may start at once; it may then have read what it takes for constant before the

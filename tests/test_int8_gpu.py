@@ -125,6 +125,38 @@ def test_quantize_rows_without_a_scale(dtype, width):
     assert (got.values[7] == -127).all() and torch.isfinite(got.scales[7])
 
 
+def test_widest_rows():
+    """One row of as many elements as the kernels count, and one of one more.  Three elements are not zero, the first and the last
+    among them."""
+    o, widest = ops(), 2 ** 31 - 1 - 8192
+    at = torch.tensor([0, 2 ** 30 + 1, widest - 1], device=DEV)
+    values = torch.tensor([3.0, 1.0, -4.0], device=DEV)
+    x = torch.zeros(1, widest, device=DEV, dtype=BF16)
+    x[0, at] = values.to(BF16)
+    rows = o.quantize_rows_int8(x)
+    assert rows.scales.tolist() == [(torch.tensor(4.0) / 127).item()]
+    assert rows.values[0, at].tolist() == [95, 32, -127] and rows.values.count_nonzero() == 3
+    x.fill_(7.0)
+    back = rows.dequantize(BF16)
+    assert torch.equal(back[0, at], (rows.values[0, at].float() * rows.scales).to(BF16)) and back.count_nonzero() == 3
+    del x, back, rows
+    stream, weight = torch.zeros(1, widest, device=DEV), torch.ones(1, device=DEV, dtype=BF16).expand(widest).contiguous()
+    stream[0, at] = values
+    rows = o.add_rmsnorm_int8(stream, None, weight, 0.0)
+    assert rows.values[0, at].tolist() == [95, 32, -127] and rows.values.count_nonzero() == 3
+    assert abs(rows.scales.item() / (4 / (26 / widest) ** 0.5 / 127) - 1) < 2.0 ** -17
+    del stream, weight, rows
+    for wide in (torch.empty(1, widest + 1, device=DEV, dtype=BF16), torch.empty(1, 2 ** 31 - 8, device=DEV, dtype=BF16)):
+        with pytest.raises(o.KernelError, match="elements at most"):
+            o.quantize_rows_int8(wide)
+    wide = torch.empty(1, widest + 1, device=DEV)
+    with pytest.raises(o.KernelError, match="elements at most"):
+        o.add_rmsnorm_int8(wide, None, wide[0], 1e-6)
+    with pytest.raises(o.KernelError, match="elements at most"):
+        o.dequantize_rows_int8(o.Int8Rows(wide.view(torch.int8)[:, :widest + 1], torch.ones(1, device=DEV)), BF16)
+    torch.cuda.empty_cache()
+
+
 def test_quantize_does_not_write_between_rows():
     o = ops()
     rows = o.int8_rows_like(6, 37, torch.device(DEV))
