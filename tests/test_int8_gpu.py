@@ -170,6 +170,42 @@ def test_quantize_does_not_write_between_rows():
     assert torch.equal(got.values, again.values) and torch.equal(whole[:, 37:], before)
 
 
+def marked(rows, width):
+    """The address of memory as large as int8 rows are together with their scales, every byte of it 90, which the next ones get."""
+    t = torch.full((rows * ((width + 15) // 16 * 16 + 4),), 90, dtype=torch.int8, device=DEV)
+    return t.data_ptr()
+
+
+def check_padding(rows, address):
+    n, width = rows.values.shape
+    stride = (width + 15) // 16 * 16
+    assert rows.values.data_ptr() == address and rows.values.stride() == (stride, 1)
+    assert (torch.as_strided(rows.values, (n, stride), (stride, 1))[:, width:] == 90).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, width", [*((7, 33 + i) for i in range(16)), (700, 897), (700, 1001), (5, 24001), (5, 50005), (2400, 4100), (2400, 8200), (2400, 8204), (2400, 9736)])
+def test_what_lies_between_rows_is_not_written(dtype, rows, width):
+    """Every kernel that forms rows, at every number of bytes between two: what stood there stays, and behind the last row the scales."""
+    o, eps = ops(), 1e-6
+    store = normal(gen(width), rows, width + 3, dtype=dtype)
+    weight, top = torch.ones(width, device=DEV), lambda t: t.float().abs().amax(dim=1)
+    for x in (store[:, 3:], store[:, 3:].contiguous()):
+        address = marked(rows, width)
+        got = o.quantize_rows_int8(x)
+        check_padding(got, address)
+        assert torch.equal(got.scales, top(x) / torch.full_like(top(x), 127.0))
+        del got
+    stream = normal(gen(width), rows, width)
+    expected = o.add_rmsnorm_int8(stream, x, weight, eps, residual_out=torch.empty_like(stream))
+    want, scales = expected.values.clone(), expected.scales.clone()
+    del expected
+    address = marked(rows, width)
+    got = o.add_rmsnorm_int8(stream, x, weight, eps)
+    check_padding(got, address)
+    assert torch.equal(got.values, want) and torch.equal(got.scales, scales)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("width", WIDTHS)
 def test_dequantize_rows(dtype, width):
