@@ -124,8 +124,10 @@ Plan plan_of(PyObject* given, int64_t tokens, int64_t features, int64_t k, int64
     return plan;
 }
 
+int64_t launches;  // kernels launched here so far
 void check(int code, const char* what) {
     if (code) refuse(std::string(what) + ": CUDA error " + std::to_string(code) + " at launch");
+    ++launches;
 }
 
 void check_size(int64_t rows, int64_t width) {
@@ -320,8 +322,11 @@ PyObject* use(PyObject*, PyObject* const* args, Py_ssize_t) {
     Py_RETURN_NONE;
 }
 
+// () -> how many kernels these calls have launched
+PyObject* launched(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(launches); }
+
 #define METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(use), METHOD(quantize), METHOD(dequantize), METHOD(norm), METHOD(product), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(use), METHOD(quantize), METHOD(dequantize), METHOD(norm), METHOD(product), METHOD(launched), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "slipstream_int8_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -292,12 +292,13 @@ def _stream() -> int:
 
 
 _launches = [0]
+_native_launches: list = []  # where calls from native code are counted: functions that return how many kernels they have launched
 
 
 def launch_count() -> int:
     """Kernels of this package launched so far (each entry point below launches exactly one;
     a replayed CUDA graph adds the kernels it holds, see ``count_launches``)."""
-    return _launches[0]
+    return _launches[0] + sum(launched() for launched in _native_launches)
 
 
 def count_launches(n: int) -> None:

@@ -22,7 +22,7 @@ import functools
 
 import torch
 
-from .functions import KernelError, _launches, error_word, gemm_library, ops_library, sm_count
+from .functions import KernelError, _native_launches, error_word, gemm_library, ops_library, sm_count
 from .library import load_calls
 
 RUN = 64  # gate and up rows of a stacked weight alternate in runs of this many (csrc/int8_calls.cpp)
@@ -66,6 +66,7 @@ def _calls():
         entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (ops.ss_quantize_rows_int8, ops.ss_dequantize_rows_int8,
                                                                    ops.ss_add_rmsnorm_int8, gemm.ss_gemm_int8)]
         module.use(KernelError, *entries, _error_address, _plan_on)
+        _native_launches.append(module.launched)
         _native = module
     return _native
 
@@ -103,7 +104,6 @@ def quantize_rows_int8(x: torch.Tensor, *, activations: bool = False) -> Int8Row
     ``q = rint(x * (127 / a))`` in float32, ties to even.  Tokens of activations, or output features of a weight.
 
     ``activations``: the rows are a product's activations, not its weights, and the kernel behind may start early."""
-    _launches[0] += 1
     return Int8Rows(*(_native or _calls()).quantize(x, activations))
 
 
@@ -112,7 +112,6 @@ def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype, *, activations: boo
 
     ``activations``: the tensor is a product's activations, not its weights, and the kernel behind may start early."""
     _need_rows(rows, "rows")
-    _launches[0] += 1
     return (_native or _calls()).dequantize(rows.values, rows.scales, dtype, activations)
 
 
@@ -123,7 +122,6 @@ def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight:
 
     ``residual_out`` (float32 [N, H]) gets the new stream instead, and ``residual`` stays as it is.  ``weight`` is bfloat16 or
     float32.  A row's result does not depend on the other rows, nor on how many there are."""
-    _launches[0] += 1
     return Int8Rows(*(_native or _calls()).norm(residual, delta, weight, eps, residual_out))
 
 
@@ -207,7 +205,6 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
     ``plan``: see `int8_plan`; every plan gives the same bits."""
     _need_rows(x, "x")
     _need_rows(weight, "weight")
-    _launches[0] += 1
     return (_native or _calls()).product(x.values, x.scales, weight.values, weight.scales, bias, out_dtype, False, None, plan)
 
 
@@ -218,7 +215,6 @@ def gate_up_swiglu_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None
     (`stack_gate_up`); ``features``: how many of the weight's pairs are real (those behind them pad the last run)."""
     _need_rows(x, "x")
     _need_rows(weight, "weight")
-    _launches[0] += 1
     return (_native or _calls()).product(x.values, x.scales, weight.values, weight.scales, bias, out_dtype, True, features, plan)
 
 

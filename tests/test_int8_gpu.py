@@ -554,6 +554,31 @@ def test_two_blocks_share_an_sm_where_the_plan_says_so():
     assert int8._plan_on(8, 37888, 3584, 1, 0)[:4] == (0, 16, 1, 2)
 
 
+def test_launches_are_counted_where_there_are_any():
+    o = ops()
+    x, weight = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV)
+    rows, w = o.quantize_rows_int8(x), o.quantize_rows_int8(torch.ones(128, 64, device=DEV))
+    none = o.quantize_rows_int8(x[:0])
+
+    def counted(call):
+        before = o.launch_count()
+        try:
+            call()
+        except o.KernelError:
+            pass
+        return o.launch_count() - before
+
+    for call in (lambda: o.quantize_rows_int8(x), lambda: rows.dequantize(F32), lambda: o.add_rmsnorm_int8(x, None, weight, 1e-6),
+                 lambda: o.linear_int8(rows, w), lambda: o.gate_up_swiglu_int8(rows, w)):
+        assert counted(call) == 1
+    for call in (lambda: o.quantize_rows_int8(x[:0]), lambda: none.dequantize(F32), lambda: o.add_rmsnorm_int8(x[:0], None, weight, 1e-6),
+                 lambda: o.linear_int8(none, w), lambda: o.gate_up_swiglu_int8(none, w), lambda: o.gate_up_swiglu_int8(rows, w, features=0)):
+        assert counted(call) == 0
+    for call in (lambda: o.quantize_rows_int8(x.half()), lambda: rows.dequantize(torch.float16), lambda: o.add_rmsnorm_int8(x, None, weight[:5], 1e-6),
+                 lambda: o.linear_int8(rows, w, weight), lambda: o.linear_int8(rows, w, plan=(0, 24, 1, 1, 1)), lambda: o.gate_up_swiglu_int8(rows, rows)):
+        assert counted(call) == 0
+
+
 def test_refusals():
     o = ops()
     err = o.KernelError
