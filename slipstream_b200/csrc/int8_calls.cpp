@@ -112,15 +112,17 @@ Plan plan_of(PyObject* given, int64_t tokens, int64_t features, int64_t k, int64
         made = given = PyObject_CallFunction(plan_function, "LLLLL", (long long)tokens, (long long)features, (long long)k, (long long)gated, (long long)device);
         if (!given) throw python_error();
     }
-    long long p[5];
-    const int ok = PyArg_ParseTuple(given, "LLLLL", &p[0], &p[1], &p[2], &p[3], &p[4]);
     Plan plan{};
-    if (ok) plan = Plan{p[0], p[1], p[2], p[3], p[4]};
-    if (made) {
-        Py_DECREF(made);
-        if (ok) plans[key] = plan;
+    bool ok = PyTuple_Check(given) && PyTuple_GET_SIZE(given) == (Py_ssize_t)plan.size();
+    for (size_t i = 0; ok && i < plan.size(); ++i) {
+        PyObject* v = PyTuple_GET_ITEM(given, i);
+        int past = 0;
+        if ((ok = PyLong_Check(v))) plan[i] = PyLong_AsLongLongAndOverflow(v, &past);
+        ok = ok && !past && plan[i] >= 0 && plan[i] <= INT32_MAX;
     }
-    if (!ok) throw python_error();
+    Py_XDECREF(made);
+    if (!ok) refuse("a plan is a tuple of five whole numbers (ops.int8_plan)");
+    if (made) plans[key] = plan;
     return plan;
 }
 

@@ -554,6 +554,17 @@ def test_two_blocks_share_an_sm_where_the_plan_says_so():
     assert int8._plan_on(8, 37888, 3584, 1, 0)[:4] == (0, 16, 1, 2)
 
 
+@pytest.mark.parametrize("plan", [[0, 16, 1, 1, 1], (0, 16, 1, 1), (0, 16, 1, 1, 1, 1), (0, 16.0, 1, 1, 1), (0, 2 ** 32 + 16, 1, 1, 1), (0, 16, 2 ** 70, 1, 1),
+                                  (0, -16, 1, 1, 1), (-1, 32, 1, 1, 1), 16, "01111"])
+def test_plans_that_are_none(plan):
+    o = ops()
+    rows, w = o.quantize_rows_int8(torch.ones(4, 64, device=DEV)), o.quantize_rows_int8(torch.ones(128, 64, device=DEV))
+    with pytest.raises(o.KernelError):
+        o.linear_int8(rows, w, plan=plan)
+    with pytest.raises(o.KernelError):
+        o.gate_up_swiglu_int8(rows, w, plan=plan)
+
+
 def test_launches_are_counted_where_there_are_any():
     o = ops()
     x, weight = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV)
