@@ -10,7 +10,8 @@
 // A row's stage in shared memory is 128 bytes, 128 elements of K, under the 128-byte swizzle; an instruction takes 32 of them.
 //
 // Every wait on an mbarrier is bounded: after WAIT_LIMIT polls the kernel sets SS_ERR_WAIT_LIMIT in the error word, stops
-// waiting everywhere, waits for its copies in flight, frees its tensor memory and returns.
+// waiting everywhere, writes out nothing that it has not formed, waits (with the same limit) for its copies and products in flight,
+// frees its tensor memory and returns.
 //
 // Tensor memory is taken BEHIND griddepcontrol.wait, and the kernel behind is let go only when it has been taken: a kernel
 // that takes it before the kernel in front is through, or lets a kernel start that may take it first, can wait for a block
@@ -38,7 +39,7 @@ struct Int8Args {
     int out_f32, bias_f32, gated;
     int bn;                // few tokens: the tokens of a tile; many tokens: the features of a tile
     int stages, slices;
-    int wide_copies;       // many tokens: the two steps of a stage come in one copy (K is a multiple of 128)
+    int wide_copies;       // the two steps of a stage come in one copy (K is a multiple of 128)
 };
 
 __device__ __forceinline__ void i8_load(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {

@@ -6,8 +6,9 @@ scales are applied to the sum.  ``quantize_rows_int8`` is symmetric and has no z
 127 (or -127), a row of zeros has the scale 0, and a row that holds an infinity or NaN has the scale NaN, so that what is formed
 from it is NaN.
 
-Rows of values start on 16 bytes: their stride is a multiple of 16, whatever their width.  ``int8_rows_like`` makes such rows,
-and every function here that returns int8 rows uses it.
+Rows of values start on 16 bytes: their stride is a multiple of 16, whatever their width.  The functions here that return int8 rows make
+them so (csrc/int8_calls.cpp), in one allocation, the scales behind the values: what keeps or saves either keeps or saves both.
+`int8_rows_like` makes rows in two allocations, for a program that fills them itself.
 
 Weights, their scales, biases and the weights of a norm are taken for constant, as elsewhere in this package: a kernel may read them
 before the kernels in front of it are through.  `quantize_rows_int8` and `dequantize_rows_int8` therefore keep the kernels behind them
@@ -89,7 +90,7 @@ def _plan_on(tokens: int, features: int, k: int, gated: int, index: int) -> tupl
 
 
 def int8_rows_like(rows: int, width: int, device: torch.device) -> Int8Rows:
-    """Int8 rows with nothing in them yet."""
+    """Int8 rows with nothing in them yet, for a program that fills them itself."""
     values = torch.empty_strided((rows, width), ((width + 15) & -16, 1), dtype=torch.int8, device=device)
     return Int8Rows(values, torch.empty(rows, dtype=torch.float32, device=device))
 
@@ -118,7 +119,7 @@ def dequantize_rows_int8(rows: Int8Rows, dtype: torch.dtype, *, activations: boo
 def add_rmsnorm_int8(residual: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
                      residual_out: torch.Tensor | None = None) -> Int8Rows:
     """``add_rmsnorm`` that ends in int8 rows: ``residual`` (float32 [N, H]) += ``delta`` (float32 or bfloat16, or None), and
-    ``x / sqrt(mean(x^2) + eps) * weight`` of the new stream, formed in float32, as int8 rows.
+    ``x / sqrt(mean(x^2) + eps) * weight`` of the new stream, formed in float32 (from ``x * weight``, which has to be finite), as int8 rows.
 
     ``residual_out`` (float32 [N, H]) gets the new stream instead, and ``residual`` stays as it is.  ``weight`` is bfloat16 or
     float32.  A row's result does not depend on the other rows, nor on how many there are."""
