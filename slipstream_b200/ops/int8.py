@@ -67,7 +67,8 @@ def _calls():
         entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (ops.ss_quantize_rows_int8, ops.ss_dequantize_rows_int8,
                                                                    ops.ss_add_rmsnorm_int8, gemm.ss_gemm_int8)]
         module.use(KernelError, *entries, _error_address, _plan_on)
-        _native_launches.append(module.launched)
+        if module.launched not in _native_launches:  # (two threads may make the first call)
+            _native_launches.append(module.launched)
         _native = module
     return _native
 
