@@ -52,7 +52,8 @@ __device__ __forceinline__ uint32_t top_of(uint32_t top, const float (&v)[4]) {
 // Behind a block's last store where the kernel behind was not let go early, so that it starts when every block has ended: it may
 // take the results for constant and read them (with plain loads or by TMA) in front of its griddepcontrol.wait, which is what would make
 // them visible otherwise.  One thread's fence, behind a barrier, covers the block's stores; the end of a block then waits for them
-// (rounding 2,048 x 18,944 and back 39.6 to 41.3 us; 1,531 x 2,051, element by element, 9.9 to 11.8; a fence of every thread 42.0 and 14.3).
+// (back to values 2,048 x 18,944 18.5 to 19.8 us, 1,531 x 2,051, element by element, 6.1 to 6.9; rounding 21.6 to 21.7 and 4.0 to 4.8; with a
+// fence of every thread the pair takes 42.0 instead of 41.5, and 14.3 instead of 11.8).
 __device__ __forceinline__ void publish_results() {
     __syncthreads();
     if (threadIdx.x) return;
@@ -369,8 +370,8 @@ add_rmsnorm_int8_kernel(const float* residual, const T* delta, float* residual_o
 // of `stages` rows in shared memory that one thread fills by bulk copies, so that the rows behind are on their way through the two
 // passes over this one (with registers alone DRAM was 40 % busy: too few warps fit beside what they hold).  A block's stage is free
 // when all its threads have read their part, behind the one barrier a row.  NG vectors a thread; rows of a multiple of 16 bytes that
-// start on 16 bytes.  Norm of 4,096 x 3,584 (bfloat16 branch): 29.4 us, 84 % of the measured copy rate, a block per row 35.0;
-// 2,048 x 8,192 33.3 and 44.7; rounding 2,048 x 18,944 (bfloat16) 20.8 and 22.0.  Rows below 16 KB stay with a block per row: a row's
+// start on 16 bytes.  Norm of 4,096 x 3,584 (bfloat16 branch): 29.7 us, 83 % of the measured copy rate, a block per row 36.3;
+// 2,048 x 8,192 33.5 and 52.0; rounding 2,048 x 18,944 (bfloat16) 21.7 and 26.1 (four inputs in turn, back to back).  Rows below 16 KB stay with a block per row: a row's
 // chain of two passes and a barrier is about 1,500 cycles however narrow it is, and many small blocks hide more of them (norm of
 // 4,096 x 896: 10.5 us through a ring, 8.7 so; rounding 4,096 x 3,584: 10.5 and 9.8).
 constexpr int RING_THREADS = 256;
