@@ -5,78 +5,25 @@
 // product, 4.0 to 4.4 and 3.5 to 4.5 us so, of which the launch itself is 1.6 to 2.5.  Results are as if allocated by torch.empty on the inputs'
 // device; an error is the package's KernelError.
 
-#include <Python.h>
-
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <map>
-#include <string>
 #include <tuple>
 
+#include "calls.h"
 #include "int8_calls.h"
 
 namespace {
 
 constexpr int64_t RUN = 64, MAX_K = 131071;  // as ops/int8.py says them
 
-struct Refused {
-    std::string text;
-};
-[[noreturn]] void refuse(const std::string& text) { throw Refused{text}; }
-
-// What ops/int8.py hands over: the error's class, the entry points, and two functions, (device index) -> address of the device's
-// error word, (tokens, features, K, gated, device index) -> plan.
-PyObject *error_class, *device_function, *plan_function;
+// What ops/int8.py hands over beside that: the entry points, and a function (tokens, features, K, gated, device index) -> plan.
+PyObject* plan_function;
 int (*quantize_entry)(const Int8RowsCall*);
 int (*dequantize_entry)(const Int8RowsCall*);
 int (*norm_entry)(const Int8RowsCall*);
 int (*product_entry)(const Int8Call*);
 
 using Plan = std::array<int64_t, 5>;
-std::map<int64_t, int*> error_words;                                                      // by device
 std::map<std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t>, Plan> plans;           // by (device, features, K, gated, tokens)
 
-std::string say(at::IntArrayRef v) {
-    std::string s = "(";
-    for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
-    return s + ")";
-}
-
-const at::Tensor& tensor_of(PyObject* o, const char* what) {
-    if (!THPVariable_Check(o)) refuse(std::string(what) + " must be a tensor, not " + Py_TYPE(o)->tp_name);
-    const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda()) refuse(std::string(what) + " must be a CUDA tensor");
-    if (t.layout() != at::kStrided) refuse(std::string(what) + " must be a strided tensor");
-    return t;
-}
-const at::Tensor& contiguous_of(PyObject* o, const char* what) {
-    const at::Tensor& t = tensor_of(o, what);
-    if (!t.is_contiguous()) refuse(std::string(what) + " must be contiguous");
-    return t;
-}
-void same_device(const at::Tensor& a, const at::Tensor& b, const char* what) {
-    if (a.get_device() != b.get_device()) refuse(std::string(what) + " is on " + b.device().str() + ", not on " + a.device().str());
-}
-// 0 float32, 1 bfloat16: the kernels' codes
-int64_t code_of(at::ScalarType t) {
-    if (t == at::kBFloat16) return 1;
-    if (t != at::kFloat) refuse(std::string("kernels take float32 or bfloat16 tensors, not ") + c10::toString(t));
-    return 0;
-}
-at::ScalarType dtype_of(PyObject* o) {
-    if (!THPDtype_Check(o)) refuse("dtype must be torch.float32 or torch.bfloat16");
-    return reinterpret_cast<THPDtype*>(o)->scalar_type;
-}
-
-at::Tensor empty(int64_t rows, int64_t width, at::ScalarType type, const at::Tensor& beside) {
-    return at::Tensor(at::detail::empty_strided_cuda({rows, width}, {width, 1}, type, beside.device()));
-}
 struct NewRows {
     at::Tensor values, scales;
 };
@@ -88,17 +35,6 @@ NewRows empty_rows(int64_t rows, int64_t width, int64_t stride, const at::Tensor
     scales.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef({rows}), c10::IntArrayRef({1}));
     values.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef({rows, width}), c10::IntArrayRef({stride, 1}));
     return {std::move(values), std::move(scales)};
-}
-
-int* error_word(int64_t device) {
-    auto found = error_words.find(device);
-    if (found != error_words.end()) return found->second;
-    PyObject* address = PyObject_CallFunction(device_function, "L", (long long)device);
-    if (!address) throw python_error();
-    int* word = (int*)PyLong_AsVoidPtr(address);
-    Py_DECREF(address);
-    if (PyErr_Occurred()) throw python_error();
-    return error_words[device] = word;
 }
 
 Plan plan_of(PyObject* given, int64_t tokens, int64_t features, int64_t k, int64_t gated, int64_t device) {
@@ -126,12 +62,6 @@ Plan plan_of(PyObject* given, int64_t tokens, int64_t features, int64_t k, int64
     return plan;
 }
 
-int64_t launches;  // kernels launched here so far
-void check(int code, const char* what) {
-    if (code) refuse(std::string(what) + ": CUDA error " + std::to_string(code) + " at launch");
-    ++launches;
-}
-
 void check_size(int64_t rows, int64_t width) {
     if (width > INT8_MAX_WIDTH || rows > INT32_MAX)
         refuse("int8 rows are formed " + std::to_string(INT32_MAX) + " at most, of " + std::to_string(INT8_MAX_WIDTH) + " elements at most, not " + std::to_string(rows) + " of " + std::to_string(width));
@@ -153,30 +83,6 @@ Rows rows_of(PyObject* values, PyObject* scales, const char* what) {
         refuse(std::string(what) + ": rows must be contiguous and start on 16 bytes (a stride that is a multiple of 16), got strides " + say(v.strides()));
     return {n, k, stride, &v, &s};
 }
-
-// The device of a call's tensors is made the current one for the launch where it is not.
-struct OnDevice {
-    c10::cuda::OptionalCUDAGuard guard;
-    explicit OnDevice(const at::Tensor& t) {
-        if (t.get_device() != c10::cuda::current_device()) guard.set_device(t.device());
-    }
-};
-
-PyObject* pair(at::Tensor a, at::Tensor b) {
-    PyObject* out = PyTuple_New(2);
-    if (!out) throw python_error();
-    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(a)));
-    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(b)));
-    return out;
-}
-
-#define CALL_BEGIN HANDLE_TH_ERRORS try {
-#define CALL_END                                                  \
-    } catch (const Refused& r) {                                  \
-        PyErr_SetString(error_class, r.text.c_str());             \
-        return nullptr;                                           \
-    }                                                             \
-    END_HANDLE_TH_ERRORS
 
 // (x, early) -> values, scales
 PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t) {
@@ -327,7 +233,6 @@ PyObject* use(PyObject*, PyObject* const* args, Py_ssize_t) {
 // () -> how many kernels these calls have launched
 PyObject* launched(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(launches); }
 
-#define METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(use), METHOD(quantize), METHOD(dequantize), METHOD(norm), METHOD(product), METHOD(launched), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "slipstream_int8_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

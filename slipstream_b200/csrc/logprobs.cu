@@ -1,0 +1,401 @@
+// Log probabilities of given tokens, their ranks, the entropy and the largest log probabilities of rows of logits:
+//   m = max z, S = sum exp(z - m), T = sum exp(z - m) (z - m);   log p(t) = z_t - m - log S;   entropy = log S - T / S
+//   rank = 1 + #{z_j > z_t} + #{j < t : z_j = z_t};   the k largest by (z, lower index first)
+//
+// One pass over a row: every thread keeps the largest value of its vectors, and S, T relative to it (rescaled when it rises), and counts
+// what stands in front of the token.  Masked tokens (z = -inf) add nothing.  The sums of the threads are joined in 64 bits.
+//
+// The k largest come out of the same pass: a thread knows its largest element.  The k-th largest of the largest elements of 128 groups
+// of four threads is a bound that at least k elements of the row reach, and hardly more do (k of them in k groups; 24 for k = 20).  Only
+// the threads whose largest element reaches it can hold such elements, and only their vectors are looked at again.  Elements are compared
+// as (value, index), so no two are equal and ties need no rule of their own; where the values stand so that too many reach the bound,
+// the k largest are taken one after the other among the same threads' vectors.
+//
+// Bound by memory: a row is read once (and about 5 % of it again for k = 20).  A row has a block of 512 threads, or, where rows are few, a
+// thread-block cluster of up to 8, which put their results together through shared memory.
+
+#include "common.cuh"
+#include "logprob_calls.h"
+
+namespace {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4, UNROLL = 4, CANDIDATES = 512;
+typedef unsigned long long Key;  // value in the upper half, in an order of unsigned integers; the complement of the index below; 0: none
+
+__device__ __forceinline__ Key key_of(float z, int index) {  // z is no NaN
+    const uint32_t bits = __float_as_uint(z + 0.f);  // (both zeros are one)
+    const uint32_t order = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    return (Key)order << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t order = (uint32_t)(k >> 32);
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ int index_of(Key k) { return (int)~(uint32_t)k; }
+
+// The next float32 above z, for z >= up: z > z0; of infinity and NaN NaN, which nothing reaches.
+__device__ __forceinline__ float next_above(float z) {
+    if (!(z < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);
+    const uint32_t bits = __float_as_uint(z + 0.f);
+    return __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
+}
+
+template <typename T>
+struct Vec {
+    static constexpr int G = 16 / (int)sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float at(int e) const {
+        const uint32_t w = G == 4 ? (e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w)
+                                  : (e < 2 ? raw.x : e < 4 ? raw.y : e < 6 ? raw.z : raw.w);
+        return G == 4 ? __uint_as_float(w) : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
+};
+
+// A row as the block sees it: elements in front of the first whole 16 bytes and behind the last (one a thread, of the first and of the
+// last block), and vectors between them, first .. end - 1 of them the block's.
+template <typename T>
+struct Row {
+    const T* z;
+    int head, tail_from, vocabulary;  // elements 0 .. head - 1; tail_from .. vocabulary - 1
+    int first, end;
+    bool has_head, has_tail;
+    __device__ __forceinline__ const Vec<T>* vectors() const { return reinterpret_cast<const Vec<T>*>(z + head); }
+    __device__ __forceinline__ int index(int v, int e) const { return head + v * Vec<T>::G + e; }
+    // f(index, value) of all elements of thread t, dealt out over the lanes of a warp
+    template <typename F>
+    __device__ __forceinline__ void each_of_thread(int t, int lane, F f) const {
+        if (lane == 0) {
+            if (has_head && t < head) f(t, to_float(z[t]));
+            if (has_tail && tail_from + t < vocabulary) f(tail_from + t, to_float(z[tail_from + t]));
+        }
+        for (int v = first + t + lane * THREADS; v < end; v += 32 * THREADS) {
+            const Vec<T> x = vectors()[v];
+#pragma unroll
+            for (int e = 0; e < Vec<T>::G; ++e) f(index(v, e), x.at(e));
+        }
+    }
+};
+
+// What a thread has seen: the largest value, where it stands, sums relative to it, and how many elements stand in front of the token.
+struct Seen {
+    float m, s, t;
+    int at;  // vector, or -1 - element: of the head or tail; INT_MIN: nothing yet
+    int ahead;
+};
+constexpr int NOTHING = INT32_MIN;
+
+__device__ __forceinline__ void raise_to(Seen& a, float m, int at) {
+    if (m > a.m || (a.at == NOTHING && m == m)) {
+        if (a.s > 0.f) {
+            const float d = a.m - m, f = __expf(d);
+            a.t = f * fmaf(a.s, d, a.t);
+            a.s *= f;
+        }
+        a.m = m;
+        a.at = at;
+    }
+}
+__device__ __forceinline__ void add(Seen& a, float z, float m) {
+    const float d = z - m, p = __expf(d);
+    a.s += p;
+    a.t = fmaf(p, fmaxf(d, -200.f), a.t);  // (p is 0 below that; a NaN is in s)
+}
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+
+struct Part {  // of a block
+    double s, t;
+    float m;
+    int ahead;
+};
+
+template <bool TOP>
+struct alignas(16) Shared {  // (every array starts on 16 bytes)
+    Key groups[TOP ? GROUPS : 2];
+    Key found[TOP ? CANDIDATES : 2];
+    Key best[TOP ? LOGPROBS_MAX_TOP : 2];  // the block's largest, in order
+    Key warp_best[WARPS];
+    double sums[2][WARPS];
+    Part part;
+    Key bound;
+    float tops[WARPS];
+    int counts[WARPS], chosen[TOP ? THREADS : 4];
+    int n_found, n_chosen;
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS)
+token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int wide, float* __restrict__ out, int vocabulary, int top, int blocks, int* err) {
+    constexpr int G = Vec<T>::G;
+    __shared__ Shared<TOP> sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t r = blockIdx.x / blocks;
+    const int rank = (int)(blockIdx.x - r * blocks);
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int64_t given = wide ? ((const int64_t*)tokens)[r] : (int64_t)((const int*)tokens)[r];
+    const bool there = given >= 0 && given < vocabulary;
+    if (given >= vocabulary && rank == 0 && tid == 0) atomicOr(err, SS_ERR_TOKEN_RANGE);
+    const int token = there ? (int)given : -1;
+
+    Row<T> row;
+    row.z = logits + r * stride;
+    row.vocabulary = vocabulary;
+    row.head = min(vocabulary, (int)((16 - ((uintptr_t)row.z & 15)) & 15) / (int)sizeof(T));
+    const int n_vec = (vocabulary - row.head) / G, per = (n_vec + blocks - 1) / blocks;
+    row.tail_from = row.head + n_vec * G;
+    row.first = min(n_vec, rank * per);
+    row.end = min(n_vec, row.first + per);
+    row.has_head = rank == 0;
+    row.has_tail = rank == blocks - 1;
+
+    const float z_token = there ? to_float(row.z[token]) : __uint_as_float(0x7fffffffu);
+    const float above = next_above(z_token);
+    Seen a = {-INFINITY, 0.f, 0.f, NOTHING, 0};
+    if (row.has_head && tid < row.head) {
+        const float z = to_float(row.z[tid]);
+        raise_to(a, z, -1 - tid);
+        add(a, z, reference(a.m));
+        a.ahead += z >= (tid < token ? z_token : above);
+    }
+    // vectors: in front of the token equal values count, from its own vector on (whose elements in front of it are looked at below) they do not
+    auto take = [&](const Vec<T>& x, int v, float m) {
+        const float limit = row.index(v, G - 1) < token ? z_token : above;
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+            const float z = x.at(e);
+            add(a, z, m);
+            a.ahead += z >= limit;
+        }
+    };
+    int v = row.first + tid;
+    for (; v + (UNROLL - 1) * THREADS < row.end; v += UNROLL * THREADS) {
+        Vec<T> x[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) x[u] = row.vectors()[v + u * THREADS];
+        float m = x[0].at(0);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int e = 0; e < G; ++e) m = fmaxf(m, x[u].at(e));
+        raise_to(a, m, v);
+        const float ref = reference(a.m);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) take(x[u], v + u * THREADS, ref);
+    }
+    for (; v < row.end; v += THREADS) {
+        const Vec<T> x = row.vectors()[v];
+        float m = x.at(0);
+#pragma unroll
+        for (int e = 1; e < G; ++e) m = fmaxf(m, x.at(e));
+        raise_to(a, m, v);
+        take(x, v, reference(a.m));
+    }
+    if (row.has_tail && row.tail_from + tid < vocabulary) {
+        const int i = row.tail_from + tid;
+        const float z = to_float(row.z[i]);
+        raise_to(a, z, -1 - i);
+        add(a, z, reference(a.m));
+        a.ahead += z >= (i < token ? z_token : above);
+    }
+    if (token >= row.head && token < row.tail_from && tid < (token - row.head) % G && row.first <= (token - row.head) / G && (token - row.head) / G < row.end)
+        a.ahead += to_float(row.z[token - 1 - tid]) == z_token;
+
+    // the block's sums
+    const float warp_m = warp_max(a.m);
+    if (lane == 0) sh.tops[warp] = warp_m;
+    if (tid == 0) sh.n_found = sh.n_chosen = 0;
+    __syncthreads();
+    const float block_m = warp_max(lane < WARPS ? sh.tops[lane] : -INFINITY);
+    {
+        const float d = a.m - block_m, f = a.m == -INFINITY ? 0.f : __expf(d);
+        double s = (double)(a.s * f), t = a.m == -INFINITY ? s : (double)(f * fmaf(a.s, d, a.t));
+        int n = a.ahead;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+        if (lane == 0) { sh.sums[0][warp] = s; sh.sums[1][warp] = t; sh.counts[warp] = n; }
+    }
+
+    if constexpr (TOP) {
+        Key mine = 0;
+        if (a.at != NOTHING) {
+            if (a.at < 0) {
+                mine = key_of(a.m, -1 - a.at);
+            } else {  // the first of its (at most four) vectors' elements that has the value
+                for (int w = a.at; w < row.end && !mine; w += THREADS) {
+                    const Vec<T> x = row.vectors()[w];
+#pragma unroll
+                    for (int e = G - 1; e >= 0; --e)
+                        if (x.at(e) == a.m) mine = key_of(a.m, row.index(w, e));
+                }
+            }
+        }
+        Key group = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        group = max(group, __shfl_xor_sync(0xffffffffu, group, 2));
+        if ((lane & 3) == 0) sh.groups[tid >> 2] = group;
+        if (tid == 0) sh.bound = 0;  // fewer than `top` groups have elements: all of them count
+        __syncthreads();
+        // the place of each group's largest element among them, two at a time of what all threads of a warp look at together
+        if (tid < GROUPS) {
+            const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(sh.groups);
+            const Key own = sh.groups[tid];
+            int place = 0;
+#pragma unroll 8
+            for (int j = 0; j < GROUPS / 2; ++j) {
+                const ulonglong2 k = pairs[j];
+                place += (k.x > own) + (k.y > own);
+            }
+            if (own && place == top - 1) sh.bound = own;
+        }
+        __syncthreads();
+        const Key limit = sh.bound;
+        if (mine && mine >= limit) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = tid;
+        __syncthreads();
+        const int threads = sh.n_chosen;
+        for (int i = warp; i < threads; i += WARPS)
+            row.each_of_thread(sh.chosen[i], lane, [&](int index, float z) {
+                if (z == z) {
+                    const Key k = key_of(z, index);
+                    if (k >= limit) {
+                        const int at = atomicAdd(&sh.n_found, 1);
+                        if (at < CANDIDATES) sh.found[at] = k;
+                    }
+                }
+            });
+        __syncthreads();
+        const int n = sh.n_found;
+        if (tid < top) sh.best[tid] = 0;
+        if (n <= CANDIDATES) {
+            __syncthreads();
+            if (tid < n) {
+                const Key own = sh.found[tid];
+                int place = 0;
+                for (int j = 0; j < n; ++j) place += sh.found[j] > own;
+                if (place < top) sh.best[place] = own;
+            }
+        } else {
+            Key below = ~(Key)0;
+            for (int j = 0; j < top; ++j) {
+                Key k = 0;
+                for (int i = warp; i < threads; i += WARPS)
+                    row.each_of_thread(sh.chosen[i], lane, [&](int index, float z) {
+                        if (z == z) {
+                            const Key c = key_of(z, index);
+                            if (c < below && c > k) k = c;
+                        }
+                    });
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+                __syncthreads();
+                if (lane == 0) sh.warp_best[warp] = k;
+                __syncthreads();
+                k = sh.warp_best[0];
+                for (int w = 1; w < WARPS; ++w) k = max(k, sh.warp_best[w]);
+                if (tid == 0) sh.best[j] = k;
+                below = k;
+                if (!k) break;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        double s = 0, t = 0;
+        int n = 0;
+        for (int w = 0; w < WARPS; ++w) { s += sh.sums[0][w]; t += sh.sums[1][w]; n += sh.counts[w]; }
+        sh.part = {s, t, block_m, n};
+    }
+    if (blocks > 1) cluster_sync_all();
+    else __syncthreads();
+    if (rank == 0) {
+        const float m_own = sh.part.m;
+        float m = m_own;
+        auto remote = [&](const void* p, int b) { return ld_cluster_u64((const unsigned long long*)p, (uint32_t)b); };
+        double s = sh.part.s, t = sh.part.t;
+        int n = sh.part.ahead;
+        for (int b = 1; b < blocks; ++b) {
+            const unsigned long long word = remote(&sh.part.m, b);
+            const float mb = __uint_as_float((uint32_t)word);
+            double sb = __longlong_as_double((long long)remote(&sh.part.s, b)), tb = __longlong_as_double((long long)remote(&sh.part.t, b));
+            n += (int)(word >> 32);
+            const float high = fmaxf(m, mb);
+            auto rescale = [&](float from, double& s, double& t) {
+                if (from == high) return;
+                const double d = (double)from - (double)high, f = from == -INFINITY ? 0. : exp(d);
+                t = from == -INFINITY ? s * 0. : f * (t + s * d);
+                s *= f;
+            };
+            rescale(m, s, t);
+            rescale(mb, sb, tb);
+            s += sb;
+            t += tb;
+            m = high;
+        }
+        const double log_s = log(s), ref = (double)reference(m);  // (z - m first: beside a far m log S would be lost)
+        float* to = out + r * (3 + 2 * top);
+        if (tid == 0) {
+            to[0] = (float)((double)z_token - ref - log_s);
+            to[1] = (float)(log_s - t / s);
+            reinterpret_cast<int*>(to)[2] = z_token == z_token ? n + 1 : 0;
+        }
+        if constexpr (TOP) {
+            const float nan = __uint_as_float(0x7fffffffu);
+            const auto write = [&](int place, Key k) {
+                to[3 + place] = k ? (float)((double)value_of(k) - ref - log_s) : nan;
+                reinterpret_cast<int*>(to)[3 + top + place] = k ? index_of(k) : -1;
+            };
+            if (blocks == 1) {
+                if (tid < top) write(tid, sh.best[tid]);
+            } else {
+                // (up to 8 * 64 = 512 keys, in `found`)
+                const int all = blocks * top;
+                __syncthreads();
+                Key own = 0;
+                if (tid < all) {
+                    const int b = tid / top;
+                    own = b ? (Key)remote(&sh.best[tid - b * top], b) : sh.best[tid];
+                    sh.found[tid] = own;
+                }
+                __syncthreads();
+                if (tid < all) {
+                    int place = 0;
+                    for (int j = 0; j < all; ++j) place += sh.found[j] > own || (!own && !sh.found[j] && j < tid);
+                    if (place < top) write(place, own);
+                }
+            }
+        }
+    }
+    if (blocks > 1) cluster_sync_before_exit();
+}
+
+template <typename T>
+int launch(const LogprobCall& c, int blocks) {
+    const dim3 grid((unsigned)(c.rows * blocks));
+#define LOGPROBS(TOP) \
+    if (blocks > 1) ss_launch_cluster_x(token_logprobs_kernel<T, TOP>, grid, dim3(THREADS), 0, c.stream, blocks, (const T*)c.logits, c.stride, c.tokens, (int)c.wide, c.out, (int)c.vocabulary, (int)c.top, blocks, c.err); \
+    else ss_launch(token_logprobs_kernel<T, TOP>, grid, dim3(THREADS), 0, c.stream, (const T*)c.logits, c.stride, c.tokens, (int)c.wide, c.out, (int)c.vocabulary, (int)c.top, blocks, c.err)
+    if (c.top) { LOGPROBS(true); } else { LOGPROBS(false); }
+#undef LOGPROBS
+    return SS_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+// stride in elements, of any alignment that the type has.
+extern "C" int ss_token_logprobs(const LogprobCall* call) {
+    const LogprobCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (c.vocabulary < 1 || c.vocabulary > INT32_MAX - 65536 || c.top < 0 || c.top > LOGPROBS_MAX_TOP || c.rows > INT32_MAX / 8) return -2003;
+    const uintptr_t size = c.dtype == SS_BF16 ? 2 : 4;
+    if ((uintptr_t)c.logits % size || (uintptr_t)c.tokens % (c.wide ? 8 : 4) || (uintptr_t)c.out % 4) return -2004;
+    // blocks a row: as many as have an SM's half each, while each has four vectors a thread or more
+    int blocks = 1;
+    const int64_t vectors = c.vocabulary * (c.dtype == SS_BF16 ? 2 : 4) / 16;
+    while (blocks < 8 && c.rows * blocks * 2 <= 2 * ss_sm_count() && vectors >= blocks * 2 * 4 * THREADS) blocks *= 2;
+    return c.dtype == SS_BF16 ? launch<bf16>(c, blocks) : launch<float>(c, blocks);
+}
+
+extern "C" void ss_set_pdl(int on) { ss_pdl_flag() = on; }

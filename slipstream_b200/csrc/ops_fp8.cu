@@ -1,0 +1,402 @@
+// Rows and weights in 8-bit floats with a scale for each block of 128 (fp8.cuh): how they are formed, and the way back.
+//
+// Rows of q start on 16 bytes (their stride is a multiple of 16); what lies between a row's end and the next row is not written.
+//
+// All kernels are bound by memory: a value is read once, and the results are written from registers.  What a kernel reads may be
+// written while it has already been launched (it waits, griddepcontrol.wait), so those pointers are not __restrict__: the loads must
+// not go through the read-only path.
+
+#include "fp8.cuh"
+#include "fp8_calls.h"
+#include "tc5.cuh"
+
+namespace {
+
+// Elements of a row from memory into registers, V (four or eight) of them: 16 bytes in one load where rows are aligned for it (float32:
+// 4, bfloat16: 8 or, for 4, 8 bytes), else one by one, the `left` that there are.
+template <int V, bool ALIGNED>
+__device__ __forceinline__ void load(const float* p, int left, float (&v)[V]) {
+    static_assert(V == 4, "");
+    if (ALIGNED && left >= 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? p[e] : 0.f;
+}
+template <int V, bool ALIGNED>
+__device__ __forceinline__ void load(const bf16* p, int left, float (&v)[V]) {
+    if (ALIGNED && left >= V) {
+        uint32_t w[V / 2];
+        if constexpr (V == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < left ? to_float(p[e]) : 0.f;
+}
+template <int V>
+__device__ __forceinline__ uint32_t top_of(uint32_t top, const float (&v)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    return top;
+}
+template <int V>
+__device__ __forceinline__ void store(uint8_t* q, int left, const float (&v)[V], const Fp8Scale& r) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        const float four[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        w[i] = fp8_quantize4(four, r);
+    }
+    if (V == 8 && left >= 8) {
+        *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[V / 4 - 1]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) fp8_store4(q + 4 * i, left - 4 * i, w[i]);
+}
+
+// Behind a block's last store where the kernel behind was not let go early, so that it starts when every block has ended: it may
+// take the results for constant and read them (with plain loads or by TMA) in front of its griddepcontrol.wait, which is what would make
+// them visible otherwise.  One thread's fence, behind a barrier, covers the block's stores.
+__device__ __forceinline__ void publish_results() {
+    __syncthreads();
+    if (threadIdx.x) return;
+    __threadfence();
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+// Where a warp's groups of 128 or 256 columns stand: `groups` of them a row, dealt out to the block's warps.
+constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32, ROW_GROUPS = 4;  // groups a warp
+struct Place {
+    int64_t row;
+    int group;
+};
+__device__ __forceinline__ Place place_of(int i, int groups) {  // the i-th group of the warp
+    const int64_t first = (int64_t)blockIdx.x * (ROW_WARPS * ROW_GROUPS);
+    const int64_t row = groups == 1 ? first : first / groups;
+    const uint32_t at = (uint32_t)(first - row * groups) + i * ROW_WARPS + (threadIdx.x >> 5);
+    Place p;
+    p.row = row + at / (uint32_t)groups;
+    p.group = (int)(at % (uint32_t)groups);
+    return p;
+}
+
+// ---------------------------------------------------------------- rows to fp8
+//
+// A lane takes 16 bytes of a row: a block of 128 is 32 lanes of float32 or 16 of bfloat16, whose largest magnitude is found by
+// shuffles.  No block depends on another, so a warp takes four groups of 32 lanes from anywhere, all loaded before the first is written.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(ROW_THREADS)
+quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
+                     int64_t scale_block, int64_t rows, int width, int groups, int early) {
+    constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V;
+    const int lane = threadIdx.x & 31;
+    if (early) pdl_launch_dependents();
+    pdl_wait();
+    float v[ROW_GROUPS][V];
+#pragma unroll
+    for (int i = 0; i < ROW_GROUPS; ++i) {
+        const Place p = place_of(i, groups);
+        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
+        const bool in = p.row < rows && j < width;
+        load<V, ALIGNED>(x + (in ? p.row * stride + j : 0), in ? (int)(width - j) : 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < ROW_GROUPS; ++i) {
+        const Place p = place_of(i, groups);
+        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
+        uint32_t top = top_of(0u, v[i]);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (p.row >= rows || j >= width) continue;
+        const Fp8Scale r = fp8_scale(top);
+        if (lane % LANES == 0) scales[p.row * scale_row + j / FP8_BLOCK * scale_block] = r.scale;
+        store(q + p.row * q_stride + j, (int)(width - j), v[i], r);
+    }
+    if (!early) publish_results();
+}
+
+// ---------------------------------------------------------------- weights to fp8
+//
+// A block of threads per 128 x 128 elements, which stay in registers.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(ROW_THREADS)
+quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
+                       int64_t scale_block, int64_t rows, int width) {
+    constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V, AT_ONCE = ROW_THREADS / LANES, N = FP8_BLOCK / AT_ONCE;
+    __shared__ uint32_t tops[ROW_WARPS];
+    pdl_wait();
+    const int64_t r0 = (int64_t)blockIdx.x * FP8_BLOCK + threadIdx.x / LANES;
+    const int64_t j = (int64_t)blockIdx.y * FP8_BLOCK + threadIdx.x % LANES * V;
+    const int left = (int)min((int64_t)V, max((int64_t)0, width - j));
+    float v[N][V];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int64_t r = r0 + i * AT_ONCE;
+        const bool in = r < rows && left > 0;
+        load<V, ALIGNED>(x + (in ? r * stride + j : 0), in ? left : 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = top_of(top, v[i]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, tops[threadIdx.x % ROW_WARPS]);
+    const Fp8Scale s = fp8_scale(top);
+    if (threadIdx.x == 0) scales[blockIdx.x * scale_row + blockIdx.y * scale_block] = s.scale;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int64_t r = r0 + i * AT_ONCE;
+        if (r < rows && left > 0) store(q + r * q_stride + j, left, v[i], s);
+    }
+    publish_results();
+}
+
+// ---------------------------------------------------------------- add + RMS norm to fp8
+//
+// x = residual + delta, written to residual_out (if there is one); v = x / sqrt(mean(x^2) + eps) * w, as rows of blocks.  The norm's
+// factor is the same for the whole row, so q is that of x * w, and the factor enters the scales alone: a warp, which holds a block of
+// 128 (four elements a lane), writes its q at once, and only the scales wait for the row's sum of squares.
+// The squares' sum does not depend on how many rows there are, whatever shape the launch takes for them: a block's sum (a warp's) is
+// formed first, then lane l adds the sums of blocks l, l + 32, ... of the row, then the lanes.
+__device__ __forceinline__ float squares_of(const float (&v)[4]) {
+    return fmaf(v[3], v[3], fmaf(v[2], v[2], fmaf(v[1], v[1], v[0] * v[0])));
+}
+
+// A block of threads per row; NG groups of four elements a thread, or (NG = 0) rows of any width.  sums: [blocks of the row], then tops.
+template <typename T, bool ALIGNED, int NG>
+__global__ void __launch_bounds__(1024)
+add_rmsnorm_fp8_kernel(const float* residual, const T* delta, float* residual_out, const void* __restrict__ weight, int w_f32,
+                       uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row, int64_t scale_block, int width, float eps) {
+    extern __shared__ float sums[];
+    const int blocks = (width + FP8_BLOCK - 1) / FP8_BLOCK;
+    uint32_t* tops = reinterpret_cast<uint32_t*>(sums + blocks);
+    const int lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    auto load_w = [&](int j, float (&to)[4]) {
+        if (w_f32) load<4, ALIGNED>((const float*)weight + j, width - j, to);
+        else load<4, ALIGNED>((const bf16*)weight + j, width - j, to);
+    };
+    float w[NG ? NG : 1][4];  // the weights do not depend on the kernels in front and are on the way before those are through
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) load_w((threadIdx.x + i * blockDim.x) * 4, w[i]);
+    }
+    pdl_wait();
+    const int64_t at = (int64_t)blockIdx.x * width;
+    uint8_t* out = q + (int64_t)blockIdx.x * q_stride;
+    auto load_x = [&](int j, float (&x)[4], float (&d)[4]) {
+        load<4, ALIGNED>(residual + at + j, width - j, x);
+        if (delta) load<4, ALIGNED>(delta + at + j, width - j, d);
+    };
+    auto finish = [&](int j, float (&x)[4], const float (&d)[4], const float (&wi)[4]) {
+        if (delta) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __fadd_rn(x[e], d[e]);
+        }
+        if (residual_out && j < width) {
+            float* to = residual_out + at + j;
+            if (ALIGNED && j + 4 <= width) {
+                *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < width) to[e] = x[e];
+            }
+        }
+        const float squares = warp_sum(squares_of(x));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= wi[e];
+        const uint32_t top = __reduce_max_sync(0xffffffffu, fp8_top(0u, x));
+        if (lane == 0 && j < width) {
+            sums[j / FP8_BLOCK] = squares;
+            tops[j / FP8_BLOCK] = top;
+        }
+        if (j < width) fp8_store4(out + j, width - j, fp8_quantize4(x, fp8_scale(top)));
+    };
+    float x[NG ? NG : 1][4], d[NG ? NG : 1][4];
+    if constexpr (NG > 0) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) load_x((threadIdx.x + i * blockDim.x) * 4, x[i], d[i]);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) finish((threadIdx.x + i * blockDim.x) * 4, x[i], d[i], w[i]);
+    } else {
+        for (int j0 = 0; j0 < width; j0 += blockDim.x * 4) {  // (whole warps come along)
+            const int j = j0 + threadIdx.x * 4;
+            load_w(j, w[0]);
+            load_x(j, x[0], d[0]);
+            finish(j, x[0], d[0], w[0]);
+        }
+    }
+    __syncthreads();
+    float total = 0.f;
+    for (int b = lane; b < blocks; b += 32) total += sums[b];
+    total = warp_sum(total);
+    const float rstd = 1.0f / sqrtf(total / (float)width + eps);
+    for (int b = threadIdx.x; b < blocks; b += blockDim.x) {
+        const uint32_t top = tops[b];
+        scales[blockIdx.x * scale_row + b * scale_block] = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top) * rstd, FP8_TOP) : __uint_as_float(0x7fffffffu);
+    }
+}
+
+// ---------------------------------------------------------------- fp8 to values
+//
+// y = q * s, rounded once.  A lane takes eight (bfloat16) or four (float32) elements; groups are dealt out as in the way there.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(ROW_THREADS)
+dequantize_kernel(const uint8_t* q, int64_t q_stride, const float* scales, int64_t scale_row, int64_t scale_block, T* __restrict__ y, int64_t rows,
+                  int width, int groups, int shift, int early) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    if (early) pdl_launch_dependents();
+    pdl_wait();
+    uint32_t w[ROW_GROUPS][V / 4];
+    float s[ROW_GROUPS];
+#pragma unroll
+    for (int i = 0; i < ROW_GROUPS; ++i) {
+        const Place p = place_of(i, groups);
+        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
+        if (p.row >= rows || j >= width) continue;
+        const uint8_t* from = q + p.row * q_stride + j;
+        s[i] = scales[(p.row >> shift) * scale_row + j / FP8_BLOCK * scale_block];
+        if (j + V <= width) {
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(from);
+            else w[i][0] = *reinterpret_cast<const uint32_t*>(from);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (e % 4 == 0) w[i][e / 4] = 0;
+                if (j + e < width) w[i][e / 4] |= (uint32_t)from[e] << (8 * (e % 4));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ROW_GROUPS; ++i) {
+        const Place p = place_of(i, groups);
+        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
+        if (p.row >= rows || j >= width) continue;
+        T v[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            float f[4];
+            fp8_values4(w[i][e / 4], f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[e + k] = from_float<T>(f[k] * s[i]);
+        }
+        T* to = y + p.row * width + j;
+        if (ALIGNED && j + V <= width) {
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (j + e < width) to[e] = v[e];
+        }
+    }
+    if (!early) publish_results();
+}
+
+// ---------------------------------------------------------------- launches
+
+inline bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int refused(const Fp8RowsCall& c) {
+    return c.width <= 0 || c.width > FP8_MAX_WIDTH || c.rows > INT32_MAX || c.q_stride % 16 || !on16(c.q) ? -2003 : 0;
+}
+
+// Blocks of threads for `rows` rows of `groups` groups, or 0 where they are too many.
+unsigned row_blocks(int64_t rows, int groups) {
+    const int64_t n = (rows * groups + ROW_WARPS * ROW_GROUPS - 1) / (ROW_WARPS * ROW_GROUPS);
+    return n > INT32_MAX ? 0u : (unsigned)n;
+}
+
+template <typename T, bool ALIGNED>
+int launch_quantize(const Fp8RowsCall& c) {
+    const int width = (int)c.width, groups = (int)((c.width + 512 / sizeof(T) - 1) / (512 / sizeof(T)));
+    if (c.blocks) {
+        const int64_t across = (c.width + FP8_BLOCK - 1) / FP8_BLOCK;
+        if (across > 65535) return -2003;
+        ss_launch(quantize_blocks_kernel<T, ALIGNED>, dim3((unsigned)((c.rows + FP8_BLOCK - 1) / FP8_BLOCK), (unsigned)across), dim3(ROW_THREADS), 0, c.stream,
+                  (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, c.scale_row, c.scale_block, c.rows, width);
+    } else {
+        const unsigned n = row_blocks(c.rows, groups);
+        if (!n) return -2003;
+        ss_launch(quantize_rows_kernel<T, ALIGNED>, dim3(n), dim3(ROW_THREADS), 0, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, c.scale_row,
+                  c.scale_block, c.rows, width, groups, (int)c.early);
+    }
+    return SS_LAUNCH_CHECK();
+}
+
+// Groups of four of a row: NG a thread and the threads of a block (NG = 0: a loop).
+struct RowShape { int ng, threads; };
+inline RowShape norm_shape(int width, int64_t rows) {
+    const int groups = (width + 3) / 4;
+    const bool few = rows <= 2 * (int64_t)ss_sm_count();
+    for (int ng : {1, 2, 4}) {
+        const int threads = ((groups + ng - 1) / ng + 31) / 32 * 32;
+        if (threads <= (few ? 1024 : 512)) return {ng, threads};
+    }
+    return {0, 512};
+}
+
+template <typename T, bool ALIGNED>
+int launch_norm(const Fp8RowsCall& c) {
+    const int width = (int)c.width;
+    const RowShape shape = norm_shape(width, c.rows);
+    const int64_t smem = (c.width + FP8_BLOCK - 1) / FP8_BLOCK * 8;
+    if (smem > 48 * 1024) return -2003;
+#define NORM(NG) case NG: ss_launch(add_rmsnorm_fp8_kernel<T, ALIGNED, NG>, dim3((unsigned)c.rows), dim3(shape.threads), (size_t)smem, c.stream, (const float*)c.x, (const T*)c.delta, (float*)c.y, c.weight, (int)c.w_f32, c.q, c.q_stride, c.scales, c.scale_row, c.scale_block, width, (float)c.eps); break
+    switch (shape.ng) { NORM(0); NORM(1); NORM(2); NORM(4); }
+#undef NORM
+    return SS_LAUNCH_CHECK();
+}
+
+template <typename T, bool ALIGNED>
+int launch_dequantize(const Fp8RowsCall& c) {
+    const int groups = (int)((c.width + 512 / sizeof(T) - 1) / (512 / sizeof(T)));
+    const unsigned n = row_blocks(c.rows, groups);
+    if (!n) return -2003;
+    ss_launch(dequantize_kernel<T, ALIGNED>, dim3(n), dim3(ROW_THREADS), 0, c.stream, c.q, c.q_stride, c.scales, c.scale_row, c.scale_block, (T*)c.y, c.rows,
+              (int)c.width, groups, c.blocks ? 7 : 0, (int)c.early);
+    return SS_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+extern "C" int ss_quantize_fp8(const Fp8RowsCall* call) {
+    const Fp8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = refused(c)) return rc;
+    const bool aligned = on16(c.x) && c.stride * (c.dtype == SS_BF16 ? 2 : 4) % 16 == 0;
+    if (c.dtype == SS_BF16) return aligned ? launch_quantize<bf16, true>(c) : launch_quantize<bf16, false>(c);
+    return aligned ? launch_quantize<float, true>(c) : launch_quantize<float, false>(c);
+}
+
+extern "C" int ss_add_rmsnorm_fp8(const Fp8RowsCall* call) {
+    const Fp8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = refused(c)) return rc;
+    const bool aligned = c.width % 4 == 0 && on16(c.x) && on16(c.delta) && on16(c.y) && on16(c.weight);
+    if (c.dtype == SS_BF16) return aligned ? launch_norm<bf16, true>(c) : launch_norm<bf16, false>(c);
+    return aligned ? launch_norm<float, true>(c) : launch_norm<float, false>(c);
+}
+
+// early, here and in rows of the way there: the kernel behind may start at once; it may then have read what it takes for constant before the results are written, so only for
+// results that it does not take for that (weights are).
+extern "C" int ss_dequantize_fp8(const Fp8RowsCall* call) {
+    const Fp8RowsCall& c = *call;
+    if (c.rows <= 0) return 0;
+    if (int rc = refused(c)) return rc;
+    const bool aligned = on16(c.y) && c.width * (c.dtype == SS_BF16 ? 2 : 4) % 16 == 0;
+    if (c.dtype == SS_BF16) return aligned ? launch_dequantize<bf16, true>(c) : launch_dequantize<bf16, false>(c);
+    return aligned ? launch_dequantize<float, true>(c) : launch_dequantize<float, false>(c);
+}
+extern "C" void ss_set_pdl(int on) { ss_pdl_flag() = on; }

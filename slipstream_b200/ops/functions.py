@@ -20,7 +20,7 @@ from ctypes import c_float, c_int, c_int64, c_void_p
 import numpy as np
 import torch
 
-from .library import GEMM_SOURCES, OPS_SOURCES, KernelBuildError, load_library, require_cuda
+from .library import FP8_SOURCES, GEMM_SOURCES, LOGPROBS_SOURCES, OPS_SOURCES, KernelBuildError, load_library, require_cuda
 
 SS_F32, SS_BF16 = 0, 1
 
@@ -188,6 +188,8 @@ _GEMM_SIGNATURES = {
     "ss_gemm_int8_resident": [c_int, c_int],
 }
 
+_FP8_SIGNATURES = {"ss_gemm_fp8_resident": [c_int, c_int]}
+
 _state: dict[str, object] = {}
 
 
@@ -220,6 +222,33 @@ def gemm_library() -> ctypes.CDLL:
     return lib  # type: ignore[return-value]
 
 
+def _set_pdl(lib: ctypes.CDLL, enabled: bool) -> None:
+    lib.ss_set_pdl.argtypes = [c_int]
+    lib.ss_set_pdl.restype = None
+    lib.ss_set_pdl(int(enabled))
+
+
+def fp8_library() -> ctypes.CDLL:
+    lib = _state.get("fp8")
+    if lib is None:
+        require_cuda()
+        lib = load_library("slipstream_fp8", FP8_SOURCES)
+        _declare(lib, _FP8_SIGNATURES)
+        _set_pdl(lib, bool(_state.get("pdl", True)))
+        _state["fp8"] = lib
+    return lib  # type: ignore[return-value]
+
+
+def logprobs_library() -> ctypes.CDLL:
+    lib = _state.get("logprobs")
+    if lib is None:
+        require_cuda()
+        lib = load_library("slipstream_logprobs", LOGPROBS_SOURCES)
+        _set_pdl(lib, bool(_state.get("pdl", True)))
+        _state["logprobs"] = lib
+    return lib  # type: ignore[return-value]
+
+
 def attention_library(head_dim: int) -> ctypes.CDLL:
     key = f"attn{head_dim}"
     lib = _state.get(key)
@@ -248,6 +277,11 @@ def error_word(device: torch.device) -> torch.Tensor:
 
 _ERR_NAMES = {1: "a token id outside the vocabulary", 2: "a cache slot outside the pool",
               4: "a block-table entry outside the pool", 8: "a bounded wait gave up"}
+
+
+def error_address(index: int) -> int:
+    """Where the error word of the CUDA device ``index`` stands (for as long as the process lives)."""
+    return error_word(torch.device("cuda", index)).data_ptr()
 
 
 def raise_for_status(value: int, device: torch.device) -> None:
@@ -2946,11 +2980,10 @@ def normed_pair(a: torch.Tensor, a_weight: torch.Tensor, b: torch.Tensor, b_weig
 
 def set_programmatic_launch(enabled: bool) -> None:
     """Turn programmatic dependent launch of this package's kernels on or off (on by default)."""
-    libs = [ops_library(), gemm_library()] + [lib for key, lib in _state.items() if isinstance(key, str) and key.startswith("attn")]
+    libs = [ops_library(), gemm_library()] + [lib for key, lib in _state.items()
+                                               if isinstance(key, str) and (key.startswith("attn") or key in ("fp8", "logprobs"))]
     for lib in libs:
-        lib.ss_set_pdl.argtypes = [c_int]
-        lib.ss_set_pdl.restype = None
-        lib.ss_set_pdl(int(enabled))
+        _set_pdl(lib, enabled)
     _state["pdl"] = bool(enabled)
 
 

@@ -30,8 +30,12 @@ OPS_SOURCES = ["ops.cu", "ops_streams.cu", "ops_mixers.cu", "ops_cells.cu", "ops
                "ops_int8.cu", "sampling.cu"]
 # the tensor-core matrix products
 GEMM_SOURCES = ["gemm_tc5.cu", "gemm_f32.cu", "gemm_int8.cu"]
-# calls whose host side is native: an extension module of this Python and torch
-CALLS_SOURCES = ["int8_calls.cpp"]
+# rows, weights and products in 8-bit floats with a scale for each block
+FP8_SOURCES = ["ops_fp8.cu", "gemm_fp8.cu"]
+# log probabilities of given tokens
+LOGPROBS_SOURCES = ["logprobs.cu"]
+# calls whose host side is native: extension modules of this Python and torch, slipstream_<name>
+CALLS = ("int8_calls", "fp8_calls", "logprob_calls")
 CSRC = Path(__file__).resolve().parent.parent / "csrc"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--shared", "-Xcompiler", "-fPIC",
@@ -172,26 +176,26 @@ def load_library(name: str, sources: list[str], defines: dict[str, object] | Non
         return lib
 
 
-def compile_calls() -> Path:
-    return compile_library("slipstream_int8_calls", CALLS_SOURCES, extra=torch_flags())
+def compile_calls(name: str = "int8_calls") -> Path:
+    return compile_library(f"slipstream_{name}", [f"{name}.cpp"], extra=torch_flags())
 
 
-def load_calls():
-    """The extension module of ``CALLS_SOURCES``."""
+def load_calls(name: str = "int8_calls"):
+    """The extension module ``slipstream_<name>``, one of ``CALLS``."""
     import importlib.machinery
     import importlib.util
 
     with _lock:
-        module = _loaded.get("calls")
+        module = _loaded.get(name)
         if module is None:
-            path = compile_calls()
+            path = compile_calls(name)
             try:
-                loader = importlib.machinery.ExtensionFileLoader("slipstream_int8_calls", str(path))
-                module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("slipstream_int8_calls", str(path), loader=loader))
+                loader = importlib.machinery.ExtensionFileLoader(f"slipstream_{name}", str(path))
+                module = importlib.util.module_from_spec(importlib.util.spec_from_file_location(f"slipstream_{name}", str(path), loader=loader))
                 loader.exec_module(module)
             except ImportError as exc:
                 raise KernelBuildError(f"cannot load {path}: {exc}") from exc
-            _loaded["calls"] = module
+            _loaded[name] = module
         return module
 
 
