@@ -26,7 +26,7 @@
 
 #define F8_BM 128
 #define F8_BK FP8_BLOCK  // K elements, and bytes of a row, in a stage
-#define F8_THREADS 320   // producer, issuer, eight epilogue warps
+#define F8_THREADS 320   // few tokens: producer, issuer, eight epilogue warps
 #define F8_MAX_BN 256
 #define F8_OUT_FP8 2
 
@@ -69,6 +69,38 @@ __device__ __forceinline__ uint32_t f8_idesc(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// mbar_wait of a whole warp, the same result in all lanes.  What a warp issues for itself (products, copies) it issues in one elected lane
+// behind such waits: where the compiler sees that all lanes go the same way, operands stand in uniform registers; a loop of one lane took
+// 0.5 us a block of K, this one 0.26.
+__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    for (uint32_t spins = 0; spins < WAIT_POLLS; ++spins) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((spins & 1023u) == 1023u && __any_sync(0xffffffffu, *gave_up)) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+// For two barriers: a look at one takes 150 to 290 cycles beside products that read shared memory, at both together hardly more.
+__device__ __forceinline__ bool f8_wait(uint64_t* a, uint32_t a_parity, uint64_t* b, uint32_t b_parity, volatile int* gave_up) {
+    for (uint32_t spins = 0; spins < WAIT_POLLS; ++spins) {
+        const bool first = mbar_try_wait(a, a_parity), second = mbar_try_wait(b, b_parity);
+        if (__all_sync(0xffffffffu, first && second)) return true;
+        if ((spins & 1023u) == 1023u && __any_sync(0xffffffffu, *gave_up)) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+// A look at a barrier that does not wait.  (Where every wait gives up at once, it sees nothing.)
+__device__ __forceinline__ uint32_t f8_look(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done) : "r"(s_addr(bar)), "r"(parity) : "memory");
+    return WAIT_POLLS ? done : 0;
+}
+
 // Behind a wait that gave up: the error word, and a wait for the last of the `copies` stages that were sent for, which may still be
 // in flight.
 __device__ __noinline__ void f8_gave_up(const Fp8Args& g, uint64_t* full, int stages, int copies) {
@@ -76,7 +108,7 @@ __device__ __noinline__ void f8_gave_up(const Fp8Args& g, uint64_t* full, int st
     for (int i = max(0, copies - stages); i < copies; ++i) mbar_drain(&full[i % stages], (i / stages) & 1);
 }
 // ... and for the last of `count` uses of a ring of `n` barriers (sums that were committed).
-__device__ __noinline__ void f8_drain_ring(uint64_t* bars, int n, int count) {
+__device__ __forceinline__ void f8_drain_ring(uint64_t* bars, int n, int count) {
     for (int i = max(0, count - n); i < count; ++i) mbar_drain(&bars[i % n], (i / n) & 1);
 }
 
@@ -84,7 +116,7 @@ __device__ __forceinline__ float f8_bias(const Fp8Args& g, int f) {
     return g.bias_f32 ? ((const float*)g.bias)[f] : to_float(((const bf16*)g.bias)[f]);
 }
 __device__ __forceinline__ float f8_gate(const Fp8Args& g, float gate, float up) {
-    return g.out_type == SS_BF16 ? silu_mul<true>(gate, up) : silu_mul<false>(gate, up);
+    return g.out_type == SS_F32 ? silu_mul<false>(gate, up) : silu_mul<true>(gate, up);
 }
 
 // Whether `v` holds in all threads of the few tokens' epilogue; a barrier of theirs.
@@ -130,28 +162,59 @@ __device__ __forceinline__ uint32_t f8_remote(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(p)), "r"(rank));
     return remote;
 }
-// W columns of tensor memory (8, 16 or 32).
+// Scales on their way to a thread: four bytes from memory to shared memory, without registers, `FLIGHT` blocks of K ahead of their use (one
+// block ahead, in registers, the loop of the epilogue took as long as a load from L2: 0.6 us a block of K at any tile).  A group a
+// block; what a thread sent for is there for itself when all but the last FLIGHT - 1 groups are through, for its warp behind __syncwarp.
+__device__ __forceinline__ void f8_send_for(float* to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s_addr(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void f8_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void f8_arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
+
+// W columns of tensor memory (8, 16 or 32); the registers hold them behind the wait, through which they pass, so that nothing that reads
+// them moves in front of it.
 template <int W>
-__device__ __forceinline__ void f8_tmem_ld(uint32_t taddr, float (&r)[W]) {
+__device__ __forceinline__ void f8_tmem_load(uint32_t taddr, float (&r)[W]) {
     static_assert(W == 8 || W == 16 || W == 32, "");
     if constexpr (W == 8) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
-                     "tcgen05.wait::ld.sync.aligned;"
-                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "r"(taddr) : "memory");
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "r"(taddr));
     } else if constexpr (W == 16) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-                     "tcgen05.wait::ld.sync.aligned;"
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
-                       "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]) : "r"(taddr) : "memory");
+                       "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]) : "r"(taddr));
     } else {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                     "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-                     "tcgen05.wait::ld.sync.aligned;"
+                     "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
                        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
                        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
-                       "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]) : "r"(taddr) : "memory");
+                       "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]) : "r"(taddr));
     }
+}
+template <int W>
+__device__ __forceinline__ void f8_tmem_wait(float (&r)[W]) {
+    if constexpr (W == 8) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7])::"memory");
+    } else if constexpr (W == 16) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                       "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])::"memory");
+    } else {
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                       "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                       "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                       "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])::"memory");
+    }
+}
+
+// acc = r * f + acc for two elements in one instruction, each rounded as fmaf does.
+__device__ __forceinline__ void f8_add2(float (&acc)[2], float r0, float r1, float f) {
+    asm("{\n.reg .b64 a, r, f;\nmov.b64 a, {%0, %1};\nmov.b64 r, {%2, %3};\nmov.b64 f, {%4, %4};\nfma.rn.f32x2 a, r, f, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(acc[0]), "+f"(acc[1]) : "f"(r0), "f"(r1), "f"(f));
 }
 
 // ---------------------------------------------------------------- few tokens: the weights' bytes are the work
@@ -167,6 +230,10 @@ __device__ __forceinline__ void f8_tmem_ld(uint32_t taddr, float (&r)[W]) {
 // Registers: an SM's scheduler has 16,384 for its warps.  Three warps of one block (ten in all) may have 168 each; two blocks on an SM
 // 96, which the sums of up to 64 token columns (gated 32) fit into.
 constexpr bool f8_few_shares(int mt, int c) { return mt * c <= 32; }
+// Blocks of K that a warp's scales are fetched ahead, and the floats that it needs for them: those, then two sets of factors.
+constexpr int f8_few_flight(int mt, int c) { return mt * c <= 32 ? 8 : 4; }
+constexpr int f8_few_raw(int mt, int c) { return (c + mt + 3) / 4 * 4; }
+constexpr int f8_few_floats(int mt, int c) { return f8_few_flight(mt, c) * f8_few_raw(mt, c) + 2 * mt * c; }
 
 template <int MT, int C>
 __global__ void __launch_bounds__(F8_THREADS, f8_few_shares(MT, C) ? 2 : 1)
@@ -183,9 +250,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint64_t* sums_ready = part_empty + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_ready + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* factors = reinterpret_cast<float*>(full) + 128;  // [8 warps][2][MT][C], behind the barriers
+    float* factors = reinterpret_cast<float*>(full) + 128;  // of the eight warps, behind the barriers
     // [senders][own columns][FL]: of a cluster's block behind the factors; alone ([columns][FL]) over the ring, when all its stages have been used
-    float* sums = n_sl > 1 ? factors + 16 * MT * C : reinterpret_cast<float*>(tiles);
+    float* sums = n_sl > 1 ? factors + 8 * f8_few_floats(MT, C) : reinterpret_cast<float*>(tiles);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t0 = blockIdx.x * bn, f0 = blockIdx.y * FL;      // first token, first feature (row of the weight)
@@ -222,22 +289,24 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
 
     if (warp == 0) {
-        if (lane == 0) {
-            const uint64_t once = l2_evict_first_policy();
-            pdl_wait();
+        const uint64_t once = l2_evict_first_policy();
+        pdl_wait();
+        if (elect_one())
             for (int it = 0; it < ahead; ++it) f8_load(tiles + it * stage_bytes + w_bytes, &map_x, (k_begin + it) * F8_BK, t0, &full[it]);
-            int it = ahead, s = 0;
-            uint32_t parity = 0;
-            for (; it < k_iters; ++it) {
-                if (!mbar_wait(&empty[s], parity, gave_up)) break;
+        __syncwarp();
+        int it = ahead, s = 0;
+        uint32_t parity = 0;
+        for (; it < k_iters; ++it) {
+            if (!f8_wait(&empty[s], parity, gave_up)) break;
+            if (elect_one()) {
                 mbar_expect_tx(&full[s], stage_bytes);
                 f8_load_once(tiles + s * stage_bytes, &map_w, (k_begin + it) * F8_BK, f0, &full[s], once);
                 f8_load(tiles + s * stage_bytes + w_bytes, &map_x, (k_begin + it) * F8_BK, t0, &full[s]);
-                if (++s == stages) { s = 0; parity ^= 1; }
             }
-            copies = it;
+            __syncwarp();
+            if (++s == stages) { s = 0; parity ^= 1; }
         }
-        __syncwarp();
+        copies = it;
     } else if (warp == 1) {
         pdl_wait();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(tmem_slot)), "r"(tmem_cols));
@@ -252,7 +321,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         int s = 0, slot = 0, it = 0;
         uint32_t parity = 0, free_parity = 1;  // (of the round before the first: the slots are free)
         for (; it < k_iters; ++it) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&part_empty[slot], free_parity, gave_up) && mbar_wait(&full[s], parity, gave_up))) break;
+            if (!f8_wait(&full[s], parity, &part_empty[slot], free_parity, gave_up)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t w_desc = w_first + s * stage_step, x_desc = x_first + s * stage_step;
             const uint32_t acc = tmem + slot * MT * g.slot_columns;
@@ -262,19 +331,21 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 #pragma unroll
                     for (int kk = 0; kk < F8_BK / 32; ++kk)  // 32 bytes further along the swizzled row
                         umma_f8(acc + m * g.slot_columns, w_desc + (uint64_t)(m * F8_BM * F8_BK / 16 + kk * 2), x_desc + (uint64_t)(kk * 2), idesc, kk != 0);
-                umma_commit(&empty[s]);
                 umma_commit(&part_full[slot]);
+                umma_commit(&empty[s]);
             }
             __syncwarp();
             if (++s == stages) { s = 0; parity ^= 1; }
             if (++slot == slots) { slot = 0; free_parity ^= 1; }
         }
-        // (a warp that gave up: products in flight end before the block does)
+        // (where it gave up: products in flight end before the block does)
         if (it < k_iters) f8_drain_ring(part_full, slots, it);
         __syncwarp();
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2, hc = bn / 2, c0 = half * hc;  // its columns: c0 .. c0 + hc - 1
-        float* fac = factors + (warp - 2) * 2 * MT * C;
+        constexpr int FLIGHT = f8_few_flight(MT, C), RAW = f8_few_raw(MT, C);
+        float* raw = factors + (warp - 2) * f8_few_floats(MT, C);  // [FLIGHT][C of the tokens, MT of the weights]
+        float* fac = raw + FLIGHT * RAW;                             // [2][MT][C]
         // nor do the bias of the four features (gated: four pairs) depend on the kernels in front that a lane writes out: neighbours, or,
         // where the output's rows do not start on four elements, one of each quarter of the tile
         const int of0 = f0 / MT;  // first output feature
@@ -291,17 +362,26 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         if (n_sl > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         pdl_wait();  // the output may still be in use by the kernels in front, which also wrote the tokens' scales
         constexpr int XS = (C + 31) / 32, W = C < 16 ? C : MT * C <= 64 ? (C < 32 ? 16 : 32) : 16;
-        float next_x[XS], next_w[MT];
-        auto fetch_scales = [&](int it) {
+        int sent = 0, sent_at = 0;  // blocks of K whose scales are sent for, and the place of the next
+        const auto send_for_scales = [&]() {
+            if (sent < k_iters) {
+                float* to = raw + sent_at * RAW;
 #pragma unroll
-            for (int i = 0; i < XS; ++i) {
-                const int c = i * 32 + lane, t = c0 + c;
-                next_x[i] = it < k_iters && c < hc && t < live ? g.x_scale[(int64_t)(t0 + t) * g.x_row + (int64_t)(k_begin + it) * g.x_block] : 0.f;
+                for (int i = 0; i < XS; ++i) {
+                    const int c = i * 32 + lane, t = c0 + c;
+                    if (c < hc && t < live) f8_send_for(to + c, g.x_scale + (int64_t)(t0 + t) * g.x_row + (int64_t)(k_begin + sent) * g.x_block);
+                }
+                if (lane < MT) f8_send_for(to + C + lane, ws + lane * g.w_row + (int64_t)sent * g.w_block);
+                if (++sent_at == FLIGHT) sent_at = 0;
             }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) next_w[m] = it < k_iters ? __ldg(ws + m * g.w_row + (int64_t)it * g.w_block) : 0.f;
+            f8_group();
+            ++sent;
         };
-        fetch_scales(0);
+        // (columns without a token keep the zeros that stand there first)
+        for (int i = lane; i < FLIGHT * RAW; i += 32) raw[i] = 0.f;
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < FLIGHT - 1; ++i) send_for_scales();
         asm volatile("bar.sync 2, 288;" ::: "memory");  // the tensor memory's address is there
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(quarter * 32) << 16) + c0;
@@ -310,20 +390,23 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int c = 0; c < C; ++c) acc[m][c] = 0.f;
-        int slot = 0;
+        int slot = 0, raw_at = 0;
         uint32_t parity = 0;
         bool ok = true;
         for (int it = 0; it < k_iters; ++it) {
             float* f = fac + (it & 1) * MT * C;
+            f8_arrived<FLIGHT - 2>();
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < XS; ++i)
                 if (i * 32 + lane < C) {
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) f[m * C + i * 32 + lane] = __fmul_rn(next_x[i], next_w[m]);
+                    for (int m = 0; m < MT; ++m) f[m * C + i * 32 + lane] = __fmul_rn(raw[raw_at * RAW + i * 32 + lane], raw[raw_at * RAW + C + m]);
                 }
-            fetch_scales(it + 1);
+            if (++raw_at == FLIGHT) raw_at = 0;
             __syncwarp();
-            if (!__all_sync(0xffffffffu, mbar_wait(&part_full[slot], parity, gave_up))) { ok = false; break; }
+            send_for_scales();  // (into the place that was read a block of K ago)
+            if (!f8_wait(&part_full[slot], parity, gave_up)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at = tmem + slot * MT * g.slot_columns;
 #pragma unroll
@@ -333,7 +416,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                     if (c < hc) {
                         // (columns from hc on, up to the slot's end, are taken out too and belong to nobody)
                         float r[W];
-                        f8_tmem_ld<W>(at + m * g.slot_columns + c, r);
+                        f8_tmem_load<W>(at + m * g.slot_columns + c, r);
+                        f8_tmem_wait<W>(r);
 #pragma unroll
                         for (int e = 0; e < W; e += 4) {
                             const float4 s4 = *reinterpret_cast<const float4*>(f + m * C + c + e);
@@ -348,6 +432,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             if (lane == 0) mbar_arrive(&part_empty[slot]);
             if (++slot == slots) { slot = 0; parity ^= 1; }
         }
+        f8_arrived<0>();
         // (where a wait gave up, copies may be landing where the sums would go: only the flag says that all is formed)
         ok = ok && !__shfl_sync(0xffffffffu, *gave_up, 0);
         if (n_sl == 1) {
@@ -434,6 +519,12 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 //   full[s]       in the leader: the bytes of both blocks' copies;      empty[s]      in each block: the products have read the stage
 //   part_full[b]  in each block: the sums of a block of K are formed;   part_empty[b] in the leader: all 16 epilogue warps have them
 
+//
+// Registers: three warps a scheduler are launched with 168 each; the first four warps (producer, issuer, two that do nothing) hand back
+// all but 40 of theirs, and the epilogue's have 232: 128 sums and 64 columns on their way.
+#define F8_MANY_THREADS 384
+#define F8_FLIGHT 4
+
 __device__ __forceinline__ uint32_t f8_leader(const void* p) { return s_addr(p) & 0xFEFFFFFFu; }  // same offset in block 0 of the pair
 
 __device__ __forceinline__ void f8_load_pair(void* dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
@@ -471,8 +562,8 @@ __device__ __forceinline__ int f8_column(int part, int i) {
 
 // What a block of a pair has sent for and formed, for the other one to read where a wait gave up.
 struct F8PairCounts {
-    int copies;  // stages that it has sent for
-    int parts;   // leader: sums that it has committed
+    int x_copies, w_copies;  // stages that it has sent for
+    int parts;               // leader: sums that it has committed
 };
 // The other block's flag: its waits may go well, for a sum that is committed but not formed.
 __device__ __noinline__ void f8_tell_pair(volatile int* gave_up) {
@@ -480,9 +571,10 @@ __device__ __noinline__ void f8_tell_pair(volatile int* gave_up) {
     asm volatile("fence.acq_rel.cluster;" ::: "memory");
 }
 // Where a wait of either block gave up, both come here: the error word, and a wait for what is in flight to them.  Both blocks' bytes count
-// on the leader's barriers (`bytes` a stage, half of them each's), and one may have sent for stages that the other has not: the leader
-// arrives for those that it has not sent for itself, and counts the half that nobody sent as landed.
-__device__ __noinline__ void f8_pair_gave_up(const Fp8Args& g, uint64_t* full, uint64_t* part_full, int stages, int bytes, const F8PairCounts* counts) {
+// on the leader's barriers (a stage is x_bytes and w_bytes of each), and some may have been sent for that belong to stages of which others
+// have not: the leader arrives for those that it has not arrived for, and counts what nobody sent as landed.
+template <int x_bytes, int w_bytes>
+__device__ __noinline__ void f8_pair_gave_up(const Fp8Args& g, uint64_t* full, uint64_t* part_full, int stages, const F8PairCounts* counts) {
     const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
         atomicOr(g.err, SS_ERR_WAIT_LIMIT);
@@ -493,12 +585,13 @@ __device__ __noinline__ void f8_pair_gave_up(const Fp8Args& g, uint64_t* full, u
         };
         const int parts = of(0, &counts->parts);
         if (rank == 0) {
-            const int mine = counts->copies, other = of(1, &counts->copies), all = max(mine, other);
+            const int x0 = counts->x_copies, w0 = counts->w_copies, x1 = of(1, &counts->x_copies), w1 = of(1, &counts->w_copies);
+            const int all = max(max(x0, w0), max(x1, w1));
             for (int i = max(0, all - stages); i < all; ++i) {
                 uint64_t* bar = &full[i % stages];
-                if (i >= mine) mbar_expect_tx(bar, bytes);
-                if (i >= min(mine, other))
-                    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(s_addr(bar)), "r"(bytes / 2) : "memory");
+                if (i >= x0) mbar_expect_tx(bar, 2 * (x_bytes + w_bytes));
+                const int missing = ((i >= x0) + (i >= x1)) * x_bytes + ((i >= w0) + (i >= w1)) * w_bytes;
+                if (missing) asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(s_addr(bar)), "r"(missing) : "memory");
                 mbar_drain(bar, (i / stages) & 1);
             }
         }
@@ -545,7 +638,7 @@ __device__ __forceinline__ void f8_write_run(const Fp8Args& g, unsigned char* st
 
 // T: float, bf16, or (gated) uint8_t, e4m3.
 template <int NC, bool GATED, typename T, typename P>
-__global__ void __launch_bounds__(F8_THREADS, 1)
+__global__ void __launch_bounds__(F8_MANY_THREADS, 1)
 gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Args g) {
     constexpr int bn = 64 * NC, w_rows = bn / 2, x_bytes = F8_BM * F8_BK, stage_bytes = x_bytes + w_rows * F8_BK;  // this block's halves
     static_assert(GATED ? NC == 4 : sizeof(T) > 1, "");
@@ -572,7 +665,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < slots; ++s) { mbar_init(&part_full[s], 1); mbar_init(&part_empty[s], 16); }
         *gave_up = 0;
-        counts->copies = counts->parts = 0;
+        counts->x_copies = counts->w_copies = counts->parts = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -601,59 +694,13 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        int it = 0, s = 0;
-        uint32_t parity = 1;  // of the round before the first: the stages are free
-        bool ok = true;
-#pragma unroll 1
-        for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-            const int m0 = (t % n_m) * 2 * F8_BM + rank * F8_BM, n0 = (t / n_m) * bn + rank * w_rows;
-#pragma unroll 1
-            for (int k = 0; k < k_iters; ++k, ++it) {
-                if (it >= first) {
-                    if (!mbar_wait(&empty[s], parity, gave_up)) { ok = false; break; }
-                    if (rank == 0) mbar_expect_tx(&full[s], bytes);
-                    unsigned char* x_tile = tiles + s * stage_bytes;
-                    f8_load_pair(x_tile, &map_x, k * F8_BK, m0, &full[s]);
-                    f8_load_pair(x_tile + x_bytes, &map_w, k * F8_BK, n0, &full[s]);
-                }
-                if (++s == stages) { s = 0; parity ^= 1; }
-            }
-        }
-        counts->copies = it;
-    } else if (warp == 1 && rank == 0) {
-        const uint32_t idesc = f8_idesc(2 * F8_BM, bn);
-        const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + x_bytes);
-        int it = 0, s = 0, slot = 0;
-        uint32_t parity = 0, free_parity = 1;  // (of the round before the first: the slots are free)
-        bool ok = true;
-#pragma unroll 1
-        for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-#pragma unroll 1
-            for (int k = 0; k < k_iters; ++k, ++it) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&part_empty[slot], free_parity, gave_up) && mbar_wait(&full[s], parity, gave_up))) { ok = false; break; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t x_desc = x_first + s * (stage_bytes >> 4), w_desc = w_first + s * (stage_bytes >> 4);
-                const uint32_t acc = tmem + slot * g.slot_columns;
-                if (elect_one()) {
-#pragma unroll
-                    for (int kk = 0; kk < F8_BK / 32; ++kk) umma_f8_pair(acc, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, kk != 0);
-                    f8_commit_pair(&empty[s]);
-                    f8_commit_pair(&part_full[slot]);
-                }
-                __syncwarp();
-                if (++s == stages) { s = 0; parity ^= 1; }
-                if (++slot == slots) { slot = 0; free_parity ^= 1; }
-            }
-        }
-        if (!ok) f8_tell_pair(gave_up);
-        if (lane == 0) counts->parts = it;
-    } else if (warp >= 2) {
-        const int quarter = warp & 3, part = (warp - 2) >> 2;
-        unsigned char* stage = runs + (warp - 2) * 1024;
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
+        unsigned char* stage = runs + (warp - 4) * 1024;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         int slot = 0, turn = 0;
-        uint32_t parity = 0;
+        uint32_t parity = 0, there = 0;
         bool ok = true;
 #pragma unroll 1
         for (int t = pair; t < n_tiles; t += n_pairs) {
@@ -663,39 +710,60 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             for (int i = 0; i < NC; ++i)
 #pragma unroll
                 for (int e = 0; e < 32; ++e) acc[i][e] = 0.f;
-            // the scales of a block of K, fetched a block ahead: the token's, and those of the chunks' features (no chunk lies in two blocks;
-            // a part's chunks lie in one where the tile has 128 or 256 features, gated in two)
-            constexpr int NW = GATED ? 2 : NC == 3 ? 3 : 1, PER = NC / NW;
-            const float* xs = g.x_scale + (int64_t)m * g.x_row;
-            float next_x = 0.f, next_w[NW];
+            // the scales of a block of K: the token's, and those of the chunks' features (no chunk lies in two blocks;
+            // a part's chunks lie in one, gated in two)
+            constexpr int NW = GATED ? 2 : 1, PER = NC / NW;
+            // Fetched F8_FLIGHT blocks ahead, into registers: one block ahead, the loop took as long as a load from L2.
+            const float* xs = g.x_scale + (int64_t)min(m, g.tokens - 1) * g.x_row;  // (rows behind the last token are not written)
             const float* ws[NW];
 #pragma unroll
             for (int i = 0; i < NW; ++i)
                 ws[i] = g.w_scale + (int64_t)min((n0 + f8_column<NC, GATED>(part, i * PER)) / FP8_BLOCK, (g.features - 1) / FP8_BLOCK) * g.w_row;
-            const auto fetch_scales = [&](int k) {
-                if (m < g.tokens) next_x = xs[(int64_t)k * g.x_block];
+            float next_x[F8_FLIGHT], next_w[F8_FLIGHT][NW];
+            int fetched = 0;
+            const auto fetch_scales = [&](int u) {
+                if (fetched >= k_iters) return;
+                ++fetched;
+                next_x[u] = *xs;
+                xs += g.x_block;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) next_w[i] = __ldg(ws[i] + (int64_t)k * g.w_block);
+                for (int i = 0; i < NW; ++i) {
+                    next_w[u][i] = __ldg(ws[i]);
+                    ws[i] += g.w_block;
+                }
             };
-            fetch_scales(0);
-#pragma unroll 1
-            for (int k = 0; ok && k < k_iters; ++k) {
-                float f[NW];
 #pragma unroll
-                for (int i = 0; i < NW; ++i) f[i] = __fmul_rn(next_x, next_w[i]);
-                if (k + 1 < k_iters) fetch_scales(k + 1);
-                if (!__all_sync(0xffffffffu, mbar_wait(&part_full[slot], parity, gave_up))) { ok = false; break; }
+            for (int u = 0; u < F8_FLIGHT; ++u) fetch_scales(u);
+            const auto take_sums = [&](int u) {
+                if (!__all_sync(0xffffffffu, there) && !f8_wait(&part_full[slot], parity, gave_up)) { ok = false; return; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = lanes + slot * g.slot_columns;
+                // 32 columns are on their way while the 32 before them are added
+                float r[2][32], f[NW];
+                f8_tmem_load<32>(at + f8_column<NC, GATED>(part, 0), r[0]);
 #pragma unroll
-                for (int i = 0; i < 2 * NC; ++i) {
-                    float r[16];
-                    f8_tmem_ld<16>(at + f8_column<NC, GATED>(part, i >> 1) + 16 * (i & 1), r);
-                    if (i == 2 * NC - 1) f8_release_slot(&part_empty[slot]);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i >> 1][16 * (i & 1) + e] = fmaf(r[e], f[(i >> 1) / PER], acc[i >> 1][16 * (i & 1) + e]);
-                }
+                for (int i = 0; i < NW; ++i) f[i] = __fmul_rn(next_x[u], next_w[u][i]);
+                fetch_scales(u);
+                uint64_t* through = &part_empty[slot];
                 if (++slot == slots) { slot = 0; parity ^= 1; }
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    f8_tmem_wait<32>(r[i & 1]);
+                    if (i + 1 < NC) {
+                        f8_tmem_load<32>(at + f8_column<NC, GATED>(part, i + 1), r[(i + 1) & 1]);
+                    } else {
+                        f8_release_slot(through);
+                        there = f8_look(&part_full[slot], parity);  // (the answer is here when the last columns are added)
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) f8_add2(reinterpret_cast<float(&)[2]>(acc[i][e]), r[i & 1][e], r[i & 1][e + 1], f[i / PER]);
+                }
+            };
+#pragma unroll 1
+            for (int k = 0; ok && k < k_iters; k += F8_FLIGHT) {
+#pragma unroll
+                for (int u = 0; u < F8_FLIGHT; ++u)
+                    if (ok && k + u < k_iters) take_sums(u);
             }
             // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
             // (the flag, not the waits' results: an issuer that gave up has committed what is not formed)
@@ -715,7 +783,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) acc[i][e] = silu_mul<sizeof(T) == 2>(acc[i][e], acc[NC - 2 + i][e]);
+                    for (int e = 0; e < 32; ++e) acc[i][e] = silu_mul<sizeof(T) < 4>(acc[i][e], acc[NC - 2 + i][e]);
             }
             if constexpr (sizeof(T) == 1) {
                 const int f = of0 + 64 * part, left = g.out_features - f;
@@ -776,12 +844,67 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 }
             }
         }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 || warp == 2) {  // the tokens' rows, and the weights'
+            const bool x = warp == 0;
+            const CUtensorMap* map = x ? &map_x : &map_w;
+            unsigned char* to = tiles + (x ? 0 : x_bytes);
+            int it = 0, s = 0;
+            uint32_t parity = 1;  // of the round before the first: the stages are free
+            bool ok = true;
+#pragma unroll 1
+            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+                const int row = x ? (t % n_m) * 2 * F8_BM + rank * F8_BM : (t / n_m) * bn + rank * w_rows;
+#pragma unroll 1
+                for (int k = 0; k < k_iters; ++k, ++it) {
+                    if (it >= first) {
+                        if (!f8_wait(&empty[s], parity, gave_up)) { ok = false; break; }
+                        if (elect_one()) {
+                            if (x && rank == 0) mbar_expect_tx(&full[s], bytes);
+                            f8_load_pair(to + s * stage_bytes, map, k * F8_BK, row, &full[s]);
+                        }
+                        __syncwarp();
+                    }
+                    if (++s == stages) { s = 0; parity ^= 1; }
+                }
+            }
+            if (lane == 0) (x ? counts->x_copies : counts->w_copies) = it;
+        } else if (warp == 1 && rank == 0) {
+            const uint32_t idesc = f8_idesc(2 * F8_BM, bn);
+            const uint64_t x_first = smem_desc(tiles), w_first = smem_desc(tiles + x_bytes);
+            int it = 0, s = 0, slot = 0;
+            uint32_t parity = 0, free_parity = 1;  // (of the round before the first: the slots are free)
+            bool ok = true;
+#pragma unroll 1
+            for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+#pragma unroll 1
+                for (int k = 0; k < k_iters; ++k, ++it) {
+                    if (!f8_wait(&full[s], parity, &part_empty[slot], free_parity, gave_up)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t x_desc = x_first + s * (stage_bytes >> 4), w_desc = w_first + s * (stage_bytes >> 4);
+                    const uint32_t acc = tmem + slot * g.slot_columns;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < F8_BK / 32; ++kk) umma_f8_pair(acc, x_desc + (uint64_t)(kk * 2), w_desc + (uint64_t)(kk * 2), idesc, kk != 0);
+                        f8_commit_pair(&part_full[slot]);
+                        f8_commit_pair(&empty[s]);
+                    }
+                    __syncwarp();
+                    if (++s == stages) { s = 0; parity ^= 1; }
+                    if (++slot == slots) { slot = 0; free_parity ^= 1; }
+                }
+            }
+            if (!ok) f8_tell_pair(gave_up);
+            if (lane == 0) counts->parts = it;
+        }
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (*gave_up && threadIdx.x == 0) f8_tell_pair(gave_up);  // the other block comes along
     cluster_sync_all();  // neither block leaves (or frees tensor memory) while the other may still signal it
-    if (*gave_up) f8_pair_gave_up(g, full, part_full, stages, bytes, counts);
+    if (*gave_up) f8_pair_gave_up<x_bytes, w_rows * F8_BK>(g, full, part_full, stages, counts);
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
@@ -838,6 +961,12 @@ static int launch_many(const Fp8Call& c, Fp8Args& g) {
     if (int rc = f8_map(&map_w, c.w, g.features, g.K, c.ldw, bn / 2)) return rc;
     static SsPerDevice opted;
     if (int rc = ss_opt_in_smem(gemm_fp8_many_kernel<NC, GATED, T, P>, F8_SMEM_MAX, opted)) return rc;
+    // what the warps take of the registers is what the block is launched with: a build with fewer would wait for the rest
+    static const int registers = [] {
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, gemm_fp8_many_kernel<NC, GATED, T, P>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (registers * F8_MANY_THREADS < 128 * 40 + 256 * 232) return -2008;
     constexpr int rest = F8_SMEM_REST + 2 * 2 * F8_BM * 4 + 8 * 1024, stage = (F8_BM + bn / 2) * F8_BK;
     g.stages = (F8_SMEM_MAX - rest) / stage;
     if (g.stages > 12) g.stages = 12;
@@ -846,7 +975,7 @@ static int launch_many(const Fp8Call& c, Fp8Args& g) {
     const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + bn - 1) / bn);
     if (n_tiles > INT32_MAX / 2) return -2003;
     const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-    ss_launch_cluster_x(gemm_fp8_many_kernel<NC, GATED, T, P>, dim3(2 * pairs), dim3(F8_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
+    ss_launch_cluster_x(gemm_fp8_many_kernel<NC, GATED, T, P>, dim3(2 * pairs), dim3(F8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
     return SS_LAUNCH_CHECK();
 }
 
@@ -869,7 +998,7 @@ static int launch_few(const Fp8Call& c, Fp8Args& g, int per_sm) {
     static SsPerDevice opted;
     if (int rc = ss_opt_in_smem(gemm_fp8_few_kernel<MT, C>, F8_SMEM_MAX, opted)) return rc;
     const int stage = (FL + bn) * F8_BK;
-    const int rest = F8_SMEM_REST + 16 * MT * C * 4 + (slices > 1 ? slices * ((bn + slices - 1) / slices) * FL * 4 : 0);  // a cluster's blocks: the sums they own
+    const int rest = F8_SMEM_REST + 32 * f8_few_floats(MT, C) + (slices > 1 ? slices * ((bn + slices - 1) / slices) * FL * 4 : 0);  // a cluster's blocks: the sums they own
     g.slot_columns = 2 * C < 32 ? 32 : 2 * C;
     const int tmem = per_sm > 1 ? 256 : 512;
     g.slots = tmem / (MT * g.slot_columns);
@@ -892,7 +1021,7 @@ static int launch_few(const Fp8Call& c, Fp8Args& g, int per_sm) {
 // gated: w's rows alternate 128 gate and 128 up features; out_features <= features / 2 columns of silu(gate) * up are written.
 // many = 0: bn tokens a tile (a multiple of 16 up to 256, gated 128), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for
 // (2: bn up to 64, gated 32).
-// many = 1: bn features a tile (64, 128, 192 or 256; gated: 256).
+// many = 1: bn features a tile (64, 128 or 256; gated: 256).
 extern "C" int ss_gemm_fp8(const Fp8Call* call) {
     const Fp8Call& c = *call;
     if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
@@ -901,7 +1030,7 @@ extern "C" int ss_gemm_fp8(const Fp8Call* call) {
     if (c.gated ? (c.features % 256 || c.out_features > c.features / 2) : (c.out_features != c.features || c.out_type == F8_OUT_FP8)) return -2005;
     if (c.out_type == F8_OUT_FP8 && c.ldc % 16) return -2005;
     const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;
-    if (bn < 16 || bn > F8_MAX_BN || bn % (c.many ? 64 : 16) || (c.many && c.gated && bn != 256)
+    if (bn < 16 || bn > F8_MAX_BN || (c.many ? bn != 64 && bn != 128 && bn != 256 : bn % 16) || (c.many && c.gated && bn != 256)
         || (!c.many && (bn > (c.gated ? 128 : 256) / (per_sm > 1 ? 4 : 1) || slices < 1 || slices > 8 || per_sm < 1 || per_sm > 2
                         || (c.features + F8_BM - 1) / F8_BM > 65535))) return -2006;
     Fp8Args g = {};
@@ -911,7 +1040,7 @@ extern "C" int ss_gemm_fp8(const Fp8Call* call) {
     g.out_type = (int)c.out_type; g.bias_f32 = (int)c.bias_f32; g.bn = bn; g.slices = slices;
     if (c.many) {
         if (c.gated) return launch_many_as<4, true>(c, g);
-        return bn == 64 ? launch_many_as<1, false>(c, g) : bn == 128 ? launch_many_as<2, false>(c, g) : bn == 192 ? launch_many_as<3, false>(c, g) : launch_many_as<4, false>(c, g);
+        return bn == 64 ? launch_many_as<1, false>(c, g) : bn == 128 ? launch_many_as<2, false>(c, g) : launch_many_as<4, false>(c, g);
     }
     if (c.gated)
         return bn <= 16 ? launch_few<2, 8>(c, g, per_sm) : bn <= 32 ? launch_few<2, 16>(c, g, per_sm) : bn <= 64 ? launch_few<2, 32>(c, g, per_sm) : launch_few<2, 64>(c, g, per_sm);

@@ -143,6 +143,14 @@ def fp8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
     return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
 
 
+def _few_rest(tile: int, slices: int, gated: bool) -> int:
+    """Bytes of shared memory that a block of the kernel for few tokens has beside its ring (csrc/gemm_fp8.cu, launch_few)."""
+    parts = 2 if gated else 1
+    half = next(c for c in (8, 16, 32, 64, 128) if 2 * c >= tile)
+    floats = (8 if parts * half <= 32 else 4) * ((half + parts + 3) // 4 * 4) + 2 * parts * half
+    return 1536 + 32 * floats + (slices * ((tile + slices - 1) // slices) * 512 * parts if slices > 1 else 0)
+
+
 @functools.lru_cache(maxsize=None)
 def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -> tuple[int, int, int, int]:
     if resident is None:
@@ -157,7 +165,6 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
         if tile > 256 // parts or (across > 1 and tile <= 16):
             continue
         tiles = down * ((tokens + tile - 1) // tile)
-        half = next(c for c in (8, 16, 32, 64, 128) if 2 * c >= tile)
         for slices in range(1, min(8, blocks) + 1):
             count = tiles * slices
             if slices > 1 and count > 3 * sms:
@@ -165,7 +172,7 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
             if slices == 7:  # (clusters that fit worst into the GPU's processor clusters)
                 continue
             for per in (1, 2) if tile <= 64 // parts else (1,):
-                rest = 1536 + 64 * parts * half + (slices * ((tile + slices - 1) // slices) * 512 * parts if slices > 1 else 0)
+                rest = _few_rest(tile, slices, gated)
                 stage = (128 * parts + tile) * 128
                 stages = min(12, ((232448 if per == 1 else 115712) - rest) // stage)
                 if stages < (2 if slices > 1 else -(-tile * 512 * parts // stage)):
@@ -185,7 +192,7 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
                     best = (cost, (0, tile, slices, per))
     if tokens > 64 or not few:
         rows = (tokens + 255) // 256
-        for tile in ((256,) if gated else (64, 128, 192, 256)):
+        for tile in ((256,) if gated else (64, 128, 256)):
             tiles = rows * ((features + tile - 1) // tile)
             pairs = max(1, sms // 2)
             rounds = (tiles + pairs - 1) // pairs
@@ -212,7 +219,8 @@ def linear_fp8(x: Fp8Rows, weight: Fp8Blocks, bias: torch.Tensor | None = None, 
 def gate_up_swiglu_fp8(x: Fp8Rows, weight: Fp8Blocks, bias: torch.Tensor | None = None, out_dtype: torch.dtype = _BF16, *,
                        features: int | None = None, plan: tuple[int, int, int, int] | None = None) -> torch.Tensor | Fp8Rows:
     """``silu(gate(x)) * up(x)`` for fp8 operands, the products as in `linear_fp8`, the unit formed in float32 in the product's epilogue
-    and rounded once: to bfloat16 or float32, or (``out_dtype`` float8_e4m3fn) to fp8 rows, as `quantize_rows_fp8` of the float32 unit.
+    and rounded once: to bfloat16 or float32, or (``out_dtype`` float8_e4m3fn) to fp8 rows, as `quantize_rows_fp8` does.  (But for float32
+    outputs the exponential and the division are the approximate ones, off by about 2^-21.)
     The rows of ``weight`` (and of ``bias``) alternate ``FP8_BLOCK`` gate and ``FP8_BLOCK`` up features (`stack_gate_up_fp8`);
     ``features``: how many of the weight's pairs are real (those behind them pad the last run)."""
     _need(x, Fp8Rows, "x")

@@ -18,13 +18,14 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
             for features, k in ((256, 1), (256, 17), (256, 128), (1280, 896), (4608, 3584), (3584, 18944), (37888, 3584), (256, 1000000)):
                 many, tile, slices, per = fp8_plan(tokens, features, k, sms, gated, resident)
                 if many:
-                    assert tile in (64, 128, 192, 256) and tokens > 64 and (not gated or tile == 256)
+                    assert tile in (64, 128, 256) and tokens > 64 and (not gated or tile == 256)
                 else:
                     assert tile % 16 == 0 and 16 <= tile <= 256 // parts and 1 <= slices <= min(8, -(-k // 128)) and tokens <= 640
                     assert per == 1 or (per == 2 and tile <= 64 // parts)
                     # what the kernel keeps in shared memory: two stages of the ring, the factors, and where K is cut the sums that it owns
                     half = next(c for c in (8, 16, 32, 64, 128) if 2 * c >= tile)
-                    rest = 1536 + 64 * parts * half + (slices * -(-tile // slices) * 512 * parts if slices > 1 else 0)
+                    floats = (8 if parts * half <= 32 else 4) * -(-(half + parts) // 4) * 4 + 2 * parts * half
+                    rest = 1536 + 32 * floats + (slices * -(-tile // slices) * 512 * parts if slices > 1 else 0)
                     assert 2 * (128 * parts + tile) * 128 + rest <= 232448
 
 

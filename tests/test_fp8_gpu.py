@@ -229,14 +229,14 @@ def plans(tokens, k, gated):
     """Forms that take such a call: both kernels, every tile, slices of K, blocks an SM.  (The sums of the widest tiles leave no room for
     two stages where K is cut.)"""
     out = []
-    for tile in (16, 32, 48, 64, 96, 112, 128, 160, 208, 240, 256):
+    for tile in (16, 32, 48, 64, 96, 128, 160, 208, 256):
         if tile > (128 if gated else 256):
             continue
-        for slices in (1, 2, 3, 8) if tile < (128 if gated else 256) else (1,):
+        for slices in (1, 2, 3, 8) if tile <= (96 if gated else 208) else (1,):
             for per in (1, 2) if tile <= (32 if gated else 64) else (1,):
                 if slices <= blocks_of(k):
                     out.append((0, tile, slices, per))
-    return out + [(1, tile, 1, 1) for tile in ((256,) if gated else (64, 128, 192, 256))]
+    return out + [(1, tile, 1, 1) for tile in ((256,) if gated else (64, 128, 256))]
 
 
 def products_of(x, w, bias):
@@ -395,16 +395,18 @@ def test_gate_up_swiglu_in_every_form(tokens):
             unit_close(o.gate_up_swiglu_fp8(x, w, bias, dtype, features=500, plan=plan), ref)
 
 
-def test_gated_unit_rounded_is_the_float32_unit_rounded():
-    """fp8 outputs are what rounding the float32 outputs of the same plan gives, bit for bit; fewer features than the weight has, too."""
+def test_gated_unit_in_fp8_beside_the_float32_unit():
+    """fp8 outputs are the float32 outputs of the same plan, rounded, but for the approximate exponential and division (2^-19 of a value
+    at most); fewer features than the weight has, too."""
     o = ops()
     for tokens in (1, 9, 300):
         g, x, w = gated_inputs(tokens, 700, 640, tokens)
         for features in (640, 600, 129, 128, 3):
-            for plan in ((0, 16, 1, 1), (0, 16, 3, 2), (0, 112, 2, 1), (0, 128, 1, 1), (1, 256, 1, 1)):
-                rounded = o.quantize_rows_fp8(o.gate_up_swiglu_fp8(x, w, None, F32, features=features, plan=plan))
+            for plan in ((0, 16, 1, 1), (0, 16, 3, 2), (0, 96, 2, 1), (0, 128, 1, 1), (1, 256, 1, 1)):
+                unit = o.gate_up_swiglu_fp8(x, w, None, F32, features=features, plan=plan).to(F64)
                 got = o.gate_up_swiglu_fp8(x, w, None, E4M3, features=features, plan=plan)
-                assert torch.equal(got.scales, rounded.scales) and torch.equal(got.values.view(torch.uint8), rounded.values.view(torch.uint8))
+                assert got.shape == (tokens, features) and got.scales.shape == (tokens, blocks_of(features))
+                check_near(got, unit, unit.abs() * 2.0 ** -19)
 
 
 def test_gate_far_out():
@@ -529,7 +531,7 @@ def test_two_blocks_share_an_sm_where_the_plan_says_so():
 
 
 @pytest.mark.parametrize("plan", [[0, 16, 1, 1], (0, 16, 1), (0, 16, 1, 1, 1), (0, 16.0, 1, 1), (0, 2 ** 32 + 16, 1, 1), (0, 16, 2 ** 70, 1), (0, -16, 1, 1),
-                                  (-1, 64, 1, 1), 16, "0111", (0, 24, 1, 1), (0, 16, 9, 1), (0, 16, 0, 1), (0, 16, 1, 3), (0, 272, 1, 1), (0, 80, 1, 2), (1, 32, 1, 1), (1, 320, 1, 1)])
+                                  (-1, 64, 1, 1), 16, "0111", (0, 24, 1, 1), (0, 16, 9, 1), (0, 16, 0, 1), (0, 16, 1, 3), (0, 272, 1, 1), (0, 80, 1, 2), (1, 32, 1, 1), (1, 192, 1, 1), (1, 320, 1, 1)])
 def test_plans_that_are_none(plan):
     o = ops()
     rows, w = o.quantize_rows_fp8(torch.ones(4, 64, device=DEV)), o.quantize_blocks_fp8(torch.ones(256, 64, device=DEV))
