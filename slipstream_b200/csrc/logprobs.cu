@@ -5,8 +5,8 @@
 // One pass over a row: every thread keeps the largest value of its vectors, and S, T relative to it (rescaled when it rises), and counts
 // what stands in front of the token.  Masked tokens (z = -inf) add nothing.  The sums of the threads are joined in 64 bits.
 //
-// The k largest come out of the same pass: a thread knows its largest element.  The k-th largest of the largest elements of 128 groups
-// of four threads is a bound that at least k elements of the row reach, and hardly more do (k of them in k groups; 24 for k = 20).  Only
+// The k largest come out of the same pass: a thread knows its largest element.  The k-th largest of the largest elements of 64 or 128
+// groups of threads is a bound that at least k elements of the row reach, and hardly more do (24 for k = 20).  Only
 // the threads whose largest element reaches it can hold such elements, and only their vectors are looked at again.  Elements are compared
 // as (value, index), so no two are equal and ties need no rule of their own; where the values stand so that too many reach the bound,
 // the k largest are taken one after the other among the same threads' vectors.
@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4, UNROLL = 4, CANDIDATES = 512;
+constexpr int THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4, FEW_GROUPS = THREADS / 8, UNROLL = 4, CANDIDATES = 512;
 typedef unsigned long long Key;  // value in the upper half, in an order of unsigned integers; the complement of the index below; 0: none
 
 __device__ __forceinline__ Key key_of(float z, int index) {  // z is no NaN
@@ -43,6 +43,7 @@ __device__ __forceinline__ float next_above(float z) {
 template <typename T>
 struct Vec {
     static constexpr int G = 16 / (int)sizeof(T);
+    static constexpr uint32_t NONE = G == 4 ? 0xff800000u : 0xff80ff80u;  // -inf
     uint4 raw;
     __device__ __forceinline__ float at(int e) const {
         const uint32_t w = G == 4 ? (e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w)
@@ -158,21 +159,15 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         add(a, z, reference(a.m));
         a.ahead += z >= (tid < token ? z_token : above);
     }
-    // vectors: in front of the token equal values count, from its own vector on (whose elements in front of it are looked at below) they do not
-    auto take = [&](const Vec<T>& x, int v, float m) {
-        const float limit = row.index(v, G - 1) < token ? z_token : above;
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-            const float z = x.at(e);
-            add(a, z, m);
-            a.ahead += z >= limit;
-        }
-    };
-    int v = row.first + tid;
-    for (; v + (UNROLL - 1) * THREADS < row.end; v += UNROLL * THREADS) {
+    // vectors: in front of the token equal values count, from its own vector on (whose elements in front of it are looked at below) they do
+    // not; a vector behind the block's last is all -inf and counts nothing
+    for (int v = row.first + tid; v < row.end; v += UNROLL * THREADS) {
         Vec<T> x[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) x[u] = row.vectors()[v + u * THREADS];
+        for (int u = 0; u < UNROLL; ++u) {
+            x[u].raw = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+            if (v + u * THREADS < row.end) x[u] = row.vectors()[v + u * THREADS];
+        }
         float m = x[0].at(0);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -181,15 +176,15 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         raise_to(a, m, v);
         const float ref = reference(a.m);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) take(x[u], v + u * THREADS, ref);
-    }
-    for (; v < row.end; v += THREADS) {
-        const Vec<T> x = row.vectors()[v];
-        float m = x.at(0);
+        for (int u = 0; u < UNROLL; ++u) {
+            const float limit = v + u * THREADS >= row.end ? __uint_as_float(0x7fffffffu) : row.index(v + u * THREADS, G - 1) < token ? z_token : above;
 #pragma unroll
-        for (int e = 1; e < G; ++e) m = fmaxf(m, x.at(e));
-        raise_to(a, m, v);
-        take(x, v, reference(a.m));
+            for (int e = 0; e < G; ++e) {
+                const float z = x[u].at(e);
+                add(a, z, ref);
+                a.ahead += z >= limit;
+            }
+        }
     }
     if (row.has_tail && row.tail_from + tid < vocabulary) {
         const int i = row.tail_from + tid;
@@ -234,18 +229,20 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
                 }
             }
         }
+        const int groups = top <= FEW_GROUPS * 3 / 8 ? FEW_GROUPS : GROUPS, per_group = THREADS / groups;
         Key group = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
         group = max(group, __shfl_xor_sync(0xffffffffu, group, 2));
-        if ((lane & 3) == 0) sh.groups[tid >> 2] = group;
+        if (per_group == 8) group = max(group, __shfl_xor_sync(0xffffffffu, group, 4));
+        if (lane % per_group == 0) sh.groups[tid / per_group] = group;
         if (tid == 0) sh.bound = 0;  // fewer than `top` groups have elements: all of them count
         __syncthreads();
         // the place of each group's largest element among them, two at a time of what all threads of a warp look at together
-        if (tid < GROUPS) {
+        if (tid < groups) {
             const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(sh.groups);
             const Key own = sh.groups[tid];
             int place = 0;
 #pragma unroll 8
-            for (int j = 0; j < GROUPS / 2; ++j) {
+            for (int j = 0; j < groups / 2; ++j) {
                 const ulonglong2 k = pairs[j];
                 place += (k.x > own) + (k.y > own);
             }
@@ -256,16 +253,40 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         if (mine && mine >= limit) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = tid;
         __syncthreads();
         const int threads = sh.n_chosen;
-        for (int i = warp; i < threads; i += WARPS)
-            row.each_of_thread(sh.chosen[i], lane, [&](int index, float z) {
-                if (z == z) {
-                    const Key k = key_of(z, index);
-                    if (k >= limit) {
-                        const int at = atomicAdd(&sh.n_found, 1);
-                        if (at < CANDIDATES) sh.found[at] = k;
-                    }
+        const auto consider = [&](int index, float z) {
+            if (z == z) {
+                const Key k = key_of(z, index);
+                if (k >= limit) {
+                    const int at = atomicAdd(&sh.n_found, 1);
+                    if (at < CANDIDATES) sh.found[at] = k;
                 }
-            });
+            }
+        };
+        // the chosen threads' vectors, dealt out to all threads, several on their way at a time
+        {
+            const int each = (row.end - row.first + THREADS - 1) / THREADS, all = threads * each;
+            for (int i = tid; i < all; i += UNROLL * THREADS) {
+                Vec<T> x[UNROLL];
+                int at[UNROLL];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) {
+                    const int f = i + u * THREADS, owner = f / each;
+                    at[u] = f < all ? row.first + sh.chosen[owner] + (f - owner * each) * THREADS : row.end;
+                    if (at[u] < row.end) x[u] = row.vectors()[at[u]];
+                }
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u)
+                    if (at[u] < row.end) {
+#pragma unroll
+                        for (int e = 0; e < G; ++e) consider(row.index(at[u], e), x[u].at(e));
+                    }
+            }
+            for (int i = tid; i < threads; i += THREADS) {
+                const int t = sh.chosen[i];
+                if (row.has_head && t < row.head) consider(t, to_float(row.z[t]));
+                if (row.has_tail && row.tail_from + t < vocabulary) consider(row.tail_from + t, to_float(row.z[row.tail_from + t]));
+            }
+        }
         __syncthreads();
         const int n = sh.n_found;
         if (tid < top) sh.best[tid] = 0;
@@ -311,38 +332,46 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
     if (blocks > 1) cluster_sync_all();
     else __syncthreads();
     if (rank == 0) {
-        const float m_own = sh.part.m;
-        float m = m_own;
         auto remote = [&](const void* p, int b) { return ld_cluster_u64((const unsigned long long*)p, (uint32_t)b); };
-        double s = sh.part.s, t = sh.part.t;
-        int n = sh.part.ahead;
-        for (int b = 1; b < blocks; ++b) {
-            const unsigned long long word = remote(&sh.part.m, b);
-            const float mb = __uint_as_float((uint32_t)word);
-            double sb = __longlong_as_double((long long)remote(&sh.part.s, b)), tb = __longlong_as_double((long long)remote(&sh.part.t, b));
-            n += (int)(word >> 32);
-            const float high = fmaxf(m, mb);
-            auto rescale = [&](float from, double& s, double& t) {
-                if (from == high) return;
-                const double d = (double)from - (double)high, f = from == -INFINITY ? 0. : exp(d);
-                t = from == -INFINITY ? s * 0. : f * (t + s * d);
-                s *= f;
-            };
-            rescale(m, s, t);
-            rescale(mb, sb, tb);
-            s += sb;
-            t += tb;
-            m = high;
-        }
-        const double log_s = log(s), ref = (double)reference(m);  // (z - m first: beside a far m log S would be lost)
         float* to = out + r * (3 + 2 * top);
-        if (tid == 0) {
-            to[0] = (float)((double)z_token - ref - log_s);
-            to[1] = (float)(log_s - t / s);
-            reinterpret_cast<int*>(to)[2] = z_token == z_token ? n + 1 : 0;
+        if (warp == 0) {  // a block a lane
+            float m = -INFINITY;
+            double s = 0, t = 0;
+            int n = 0;
+            if (blocks == 1 && lane == 0) {
+                m = sh.part.m; s = sh.part.s; t = sh.part.t; n = sh.part.ahead;
+            } else if (blocks > 1 && lane < blocks) {
+                const unsigned long long word = remote(&sh.part.m, lane);
+                m = __uint_as_float((uint32_t)word);
+                n = (int)(word >> 32);
+                s = __longlong_as_double((long long)remote(&sh.part.s, lane));
+                t = __longlong_as_double((long long)remote(&sh.part.t, lane));
+            }
+            const float high = warp_max(m), d = m - high;
+            if (d != 0.f) {  // (a NaN too: of two infinities)
+                const double f = m == -INFINITY ? 0. : (double)__expf(d);
+                t = m == -INFINITY ? s * 0. : f * (t + s * (double)d);
+                s *= f;
+            }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) {  // (up to eight blocks; the same bits in all of the first eight lanes)
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+                t += __shfl_xor_sync(0xffffffffu, t, o);
+                n += __shfl_xor_sync(0xffffffffu, n, o);
+            }
+            if (lane == 0) {
+                const double log_s = log(s), ref = (double)reference(high);  // (z - m first: beside a far m log S would be lost)
+                to[0] = (float)((double)z_token - ref - log_s);
+                to[1] = (float)(log_s - t / s);
+                reinterpret_cast<int*>(to)[2] = z_token == z_token ? n + 1 : 0;
+                sh.sums[0][0] = ref;
+                sh.sums[0][1] = log_s;
+            }
         }
         if constexpr (TOP) {
+            __syncthreads();
             const float nan = __uint_as_float(0x7fffffffu);
+            const double ref = sh.sums[0][0], log_s = sh.sums[0][1];
             const auto write = [&](int place, Key k) {
                 to[3 + place] = k ? (float)((double)value_of(k) - ref - log_s) : nan;
                 reinterpret_cast<int*>(to)[3 + top + place] = k ? index_of(k) : -1;
@@ -352,7 +381,6 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
             } else {
                 // (up to 8 * 64 = 512 keys, in `found`)
                 const int all = blocks * top;
-                __syncthreads();
                 Key own = 0;
                 if (tid < all) {
                     const int b = tid / top;

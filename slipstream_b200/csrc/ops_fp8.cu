@@ -73,20 +73,17 @@ __device__ __forceinline__ void publish_results() {
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// Where a warp's groups of 128 or 256 columns stand: `groups` of them a row, dealt out to the block's warps.
+// Rows are dealt out to warps in groups of 32 vectors (128 or 256 columns), `groups` of them a row, all rows in one sequence, of which a
+// block of threads takes ROW_WARPS * ROW_GROUPS.  (Fewer than 2^32 of them: launch.)
 constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32, ROW_GROUPS = 4;  // groups a warp
 struct Place {
-    int64_t row;
-    int group;
+    uint32_t row;
+    int column;  // the group's first
 };
+template <int V>
 __device__ __forceinline__ Place place_of(int i, int groups) {  // the i-th group of the warp
-    const int64_t first = (int64_t)blockIdx.x * (ROW_WARPS * ROW_GROUPS);
-    const int64_t row = groups == 1 ? first : first / groups;
-    const uint32_t at = (uint32_t)(first - row * groups) + i * ROW_WARPS + (threadIdx.x >> 5);
-    Place p;
-    p.row = row + at / (uint32_t)groups;
-    p.group = (int)(at % (uint32_t)groups);
-    return p;
+    const uint32_t at = blockIdx.x * (uint32_t)(ROW_WARPS * ROW_GROUPS) + i * ROW_WARPS + (threadIdx.x >> 5), row = at / (uint32_t)groups;
+    return {row, (int)(at - row * groups) * 32 * V};
 }
 
 // ---------------------------------------------------------------- rows to fp8
@@ -102,40 +99,41 @@ quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_
     if (early) pdl_launch_dependents();
     pdl_wait();
     float v[ROW_GROUPS][V];
+    Place p[ROW_GROUPS];
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        const Place p = place_of(i, groups);
-        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
-        const bool in = p.row < rows && j < width;
-        load<V, ALIGNED>(x + (in ? p.row * stride + j : 0), in ? (int)(width - j) : 0, v[i]);
+        p[i] = place_of<V>(i, groups);
+        p[i].column += lane * V;
+        const bool in = p[i].row < rows && p[i].column < width;
+        load<V, ALIGNED>(x + (in ? p[i].row * stride + p[i].column : 0), in ? width - p[i].column : 0, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        const Place p = place_of(i, groups);
-        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
         uint32_t top = top_of(0u, v[i]);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (p.row >= rows || j >= width) continue;
+        if (p[i].row >= rows || p[i].column >= width) continue;
         const Fp8Scale r = fp8_scale(top);
-        if (lane % LANES == 0) scales[p.row * scale_row + j / FP8_BLOCK * scale_block] = r.scale;
-        store(q + p.row * q_stride + j, (int)(width - j), v[i], r);
+        if (lane % LANES == 0) scales[p[i].row * scale_row + p[i].column / FP8_BLOCK * scale_block] = r.scale;
+        store(q + p[i].row * q_stride + p[i].column, width - p[i].column, v[i], r);
     }
     if (!early) publish_results();
 }
 
 // ---------------------------------------------------------------- weights to fp8
 //
-// A block of threads per 128 x 128 elements, which stay in registers.
+// A block of threads per 128 x 128 elements, which stay in registers.  Neighbouring blocks take neighbours of the same rows, so that the
+// pieces of a row in memory are read at the same time.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS)
 quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
-                       int64_t scale_block, int64_t rows, int width) {
+                       int64_t scale_block, int64_t rows, int width, unsigned across) {
     constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V, AT_ONCE = ROW_THREADS / LANES, N = FP8_BLOCK / AT_ONCE;
     __shared__ uint32_t tops[ROW_WARPS];
     pdl_wait();
-    const int64_t r0 = (int64_t)blockIdx.x * FP8_BLOCK + threadIdx.x / LANES;
-    const int64_t j = (int64_t)blockIdx.y * FP8_BLOCK + threadIdx.x % LANES * V;
+    const unsigned down = blockIdx.x / across, right = blockIdx.x - down * across;
+    const int64_t r0 = (int64_t)down * FP8_BLOCK + threadIdx.x / LANES;
+    const int64_t j = (int64_t)right * FP8_BLOCK + threadIdx.x % LANES * V;
     const int left = (int)min((int64_t)V, max((int64_t)0, width - j));
     float v[N][V];
     uint32_t top = 0;
@@ -152,7 +150,7 @@ quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int6
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, tops[threadIdx.x % ROW_WARPS]);
     const Fp8Scale s = fp8_scale(top);
-    if (threadIdx.x == 0) scales[blockIdx.x * scale_row + blockIdx.y * scale_block] = s.scale;
+    if (threadIdx.x == 0) scales[down * scale_row + right * scale_block] = s.scale;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int64_t r = r0 + i * AT_ONCE;
@@ -170,6 +168,33 @@ quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int6
 // formed first, then lane l adds the sums of blocks l, l + 32, ... of the row, then the lanes.
 __device__ __forceinline__ float squares_of(const float (&v)[4]) {
     return fmaf(v[3], v[3], fmaf(v[2], v[2], fmaf(v[1], v[1], v[0] * v[0])));
+}
+
+// The warp's sums of NG values a thread, sum i to sums[i * stride].  At every level half of the sums that are left go to the other
+// half of the lanes (P values in P + log2(32 / P) shuffles, not 5 P); a sum adds the same pairs as warp_sum does.
+template <int NG>
+__device__ __forceinline__ void warp_sums(const float (&part)[NG], float* sums, int stride) {
+    constexpr int P = NG == 1 ? 1 : NG == 2 ? 2 : NG <= 4 ? 4 : NG <= 8 ? 8 : 16, STEP = 32 / P;
+    const int lane = threadIdx.x & 31;
+    float a[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) a[i] = i < NG ? part[i] : 0.f;
+    int w = 16;
+#pragma unroll
+    for (int n = P / 2; n >= 1; n /= 2, w /= 2) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float send = lane & w ? a[i] : a[i + n], keep = lane & w ? a[i + n] : a[i];
+            a[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+        }
+    }
+#pragma unroll
+    for (; w >= 1; w /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], w);
+    if (lane % STEP == 0 && lane / STEP < NG) sums[lane / STEP * stride] = a[0];
+}
+// The scale of a block whose largest |x * w| has the bits `top`.
+__device__ __forceinline__ float norm_scale(uint32_t top, float rstd) {
+    return top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top) * rstd, FP8_TOP) : __uint_as_float(0x7fffffffu);
 }
 
 // A block of threads per row; NG groups of four elements a thread, or (NG = 0) rows of any width.  sums: [blocks of the row], then tops.
@@ -242,15 +267,117 @@ add_rmsnorm_fp8_kernel(const float* residual, const T* delta, float* residual_ou
     for (int b = lane; b < blocks; b += 32) total += sums[b];
     total = warp_sum(total);
     const float rstd = 1.0f / sqrtf(total / (float)width + eps);
-    for (int b = threadIdx.x; b < blocks; b += blockDim.x) {
-        const uint32_t top = tops[b];
-        scales[blockIdx.x * scale_row + b * scale_block] = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top) * rstd, FP8_TOP) : __uint_as_float(0x7fffffffu);
+    for (int b = threadIdx.x; b < blocks; b += blockDim.x) scales[blockIdx.x * scale_row + b * scale_block] = norm_scale(tops[b], rstd);
+}
+
+// Many wide rows: two or three blocks an SM, each taking rows blockIdx.x, + gridDim.x, ... through a ring of `stages` rows in shared
+// memory that one thread fills by bulk copies, so that the rows behind are on their way through both passes over this one.  A stage is
+// free when all threads have read their part of it, behind the one barrier a row.  NG groups of four a thread; rows of a multiple of 16
+// bytes that start on 16 bytes.
+constexpr int RING_THREADS = 256;
+constexpr int ring_blocks(int ng) { return ng <= 4 ? 3 : 2; }  // blocks an SM at most
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(s_addr(dst)), "l"(src), "r"(bytes), "r"(s_addr(bar)) : "memory");
+}
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(RING_THREADS, ring_blocks(NG))
+add_rmsnorm_fp8_ring_kernel(const float* residual, const T* delta, float* residual_out, const void* __restrict__ weight, int w_f32,
+                            uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row, int64_t scale_block, int rows, int width,
+                            float eps, int stages, int* err) {
+    extern __shared__ __align__(128) unsigned char ring_smem[];
+    constexpr int SETS = NG * RING_THREADS / 32;  // blocks of 128 of the widest row
+    __shared__ uint32_t tops[2][SETS];            // (two sets: the next row's are written while slow warps still read these)
+    __shared__ float sums[2][SETS];
+    __shared__ int gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (width + FP8_BLOCK - 1) / FP8_BLOCK;
+    const int x_bytes = width * 4, d_bytes = delta ? width * (int)sizeof(T) : 0, bytes = x_bytes + d_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring_smem + stages * bytes);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    float w[NG][4];  // for all rows of the block
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int j = (threadIdx.x + i * RING_THREADS) * 4;
+        if (w_f32) load<4, true>((const float*)weight + j, width - j, w[i]);
+        else load<4, true>((const bf16*)weight + j, width - j, w[i]);
+    }
+    pdl_wait();
+    int issued = 0;  // copies that thread 0 has sent for
+    auto fetch = [&](int64_t row, int s) {
+        ++issued;
+        mbar_expect_tx(&full[s], bytes);
+        bulk_load(ring_smem + s * bytes, residual + row * width, x_bytes, &full[s]);
+        if (d_bytes) bulk_load(ring_smem + s * bytes + x_bytes, delta + row * width, d_bytes, &full[s]);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages && blockIdx.x + (int64_t)s * gridDim.x < rows; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+    int s = 0, n = 0;
+    uint32_t parity = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, n ^= 1) {
+        const bool landed = mbar_wait(&full[s], parity, &gave_up);
+        const float* from = reinterpret_cast<const float*>(ring_smem + s * bytes);
+        const T* from_d = reinterpret_cast<const T*>(ring_smem + s * bytes + x_bytes);
+        float v[NG][4], part[NG];
+        uint32_t top[NG];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * 4;
+            if (j < width) {
+                load<4, true>(from + j, 4, v[i]);
+                if (d_bytes) {
+                    float d[4];
+                    load<4, true>(from_d + j, 4, d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][e] = __fadd_rn(v[i][e], d[e]);
+                }
+                if (residual_out && landed) *reinterpret_cast<float4*>(residual_out + row * width + j) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
+            }
+            part[i] = squares_of(v[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] *= w[i][e];
+            top[i] = __reduce_max_sync(0xffffffffu, fp8_top(0u, v[i]));
+            if (lane == 0) tops[n][i * (RING_THREADS / 32) + warp] = top[i];
+        }
+        warp_sums(part, &sums[n][warp], RING_THREADS / 32);
+        if (!__syncthreads_and(landed)) break;  // nothing more of the row is written, nothing more is sent for
+        if (threadIdx.x == 0 && row + (int64_t)stages * gridDim.x < rows) fetch(row + (int64_t)stages * gridDim.x, s);
+        float total = 0.f;
+        for (int b = lane; b < blocks; b += 32) total += sums[n][b];
+        total = warp_sum(total);
+        const float rstd = 1.0f / sqrtf(total / (float)width + eps);
+        for (int b = threadIdx.x; b < blocks; b += RING_THREADS) scales[row * scale_row + b * scale_block] = norm_scale(tops[n][b], rstd);
+        uint8_t* out = q + row * q_stride;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int j = (threadIdx.x + i * RING_THREADS) * 4;
+            if (j < width) *reinterpret_cast<uint32_t*>(out + j) = fp8_quantize4(v[i], fp8_scale(top[i]));
+        }
+        if (++s == stages) { s = 0; parity ^= 1; }
+    }
+    // behind a wait that gave up: the error word, and a wait for the block's copies in flight, the last of those that thread 0 has sent for
+    if (*(volatile int*)&gave_up && threadIdx.x == 0) {
+        for (int i = max(0, issued - stages); i < issued; ++i) mbar_drain(&full[i % stages], (i / stages) & 1);
+        atomicOr(err, SS_ERR_WAIT_LIMIT);
     }
 }
 
 // ---------------------------------------------------------------- fp8 to values
 //
-// y = q * s, rounded once.  A lane takes eight (bfloat16) or four (float32) elements; groups are dealt out as in the way there.
+// y = q * s, rounded once.  A lane takes eight (bfloat16) or four (float32) elements, side by side where the output's rows start on 16
+// bytes, else 32 apart, so that a warp writes whole pieces of a row either way (1,531 x 2,051 to bfloat16, side by side and one by one:
+// 22.4 us).  Groups are dealt out as in the way there.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS)
 dequantize_kernel(const uint8_t* q, int64_t q_stride, const float* scales, int64_t scale_row, int64_t scale_block, T* __restrict__ y, int64_t rows,
@@ -259,46 +386,54 @@ dequantize_kernel(const uint8_t* q, int64_t q_stride, const float* scales, int64
     const int lane = threadIdx.x & 31;
     if (early) pdl_launch_dependents();
     pdl_wait();
+    Place p[ROW_GROUPS];
     uint32_t w[ROW_GROUPS][V / 4];
-    float s[ROW_GROUPS];
+    float s[ROW_GROUPS][ALIGNED ? 1 : (32 * V + FP8_BLOCK - 1) / FP8_BLOCK];
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        const Place p = place_of(i, groups);
-        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
-        if (p.row >= rows || j >= width) continue;
-        const uint8_t* from = q + p.row * q_stride + j;
-        s[i] = scales[(p.row >> shift) * scale_row + j / FP8_BLOCK * scale_block];
-        if (j + V <= width) {
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(from);
-            else w[i][0] = *reinterpret_cast<const uint32_t*>(from);
+        p[i] = place_of<V>(i, groups);
+        if (p[i].row >= rows) continue;
+        const uint8_t* from = q + p[i].row * q_stride;
+        const float* scale = scales + (p[i].row >> shift) * scale_row;
+        if constexpr (ALIGNED) {
+            p[i].column += lane * V;
+            if (p[i].column >= width) continue;
+            s[i][0] = scale[p[i].column / FP8_BLOCK * scale_block];
+            // (the width is a multiple of V)
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(from + p[i].column);
+            else w[i][0] = *reinterpret_cast<const uint32_t*>(from + p[i].column);
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (e % 4 == 0) w[i][e / 4] = 0;
-                if (j + e < width) w[i][e / 4] |= (uint32_t)from[e] << (8 * (e % 4));
+                const int j = p[i].column + e * 32 + lane;
+                if (e % 4 == 0) {
+                    w[i][e / 4] = 0;
+                    s[i][e / 4] = j - lane < width ? scale[(j - lane) / FP8_BLOCK * scale_block] : 0.f;  // (four times 32 columns: a block)
+                }
+                if (j < width) w[i][e / 4] |= (uint32_t)from[j] << (8 * (e % 4));
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        const Place p = place_of(i, groups);
-        const int64_t j = (int64_t)(p.group * 32 + lane) * V;
-        if (p.row >= rows || j >= width) continue;
+        if (p[i].row >= rows || (ALIGNED && p[i].column >= width)) continue;
+        T* to = y + (int64_t)p[i].row * width;
         T v[V];
 #pragma unroll
         for (int e = 0; e < V; e += 4) {
             float f[4];
             fp8_values4(w[i][e / 4], f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[e + k] = from_float<T>(f[k] * s[i]);
+            for (int k = 0; k < 4; ++k) v[e + k] = from_float<T>(f[k] * s[i][ALIGNED ? 0 : e / 4]);
         }
-        T* to = y + p.row * width + j;
-        if (ALIGNED && j + V <= width) {
-            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
+        if constexpr (ALIGNED) {
+            *reinterpret_cast<uint4*>(to + p[i].column) = *reinterpret_cast<const uint4*>(v);
         } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (j + e < width) to[e] = v[e];
+            for (int e = 0; e < V; ++e) {
+                const int j = p[i].column + e * 32 + lane;
+                if (j < width) to[j] = v[e];
+            }
         }
     }
     if (!early) publish_results();
@@ -315,7 +450,7 @@ int refused(const Fp8RowsCall& c) {
 // Blocks of threads for `rows` rows of `groups` groups, or 0 where they are too many.
 unsigned row_blocks(int64_t rows, int groups) {
     const int64_t n = (rows * groups + ROW_WARPS * ROW_GROUPS - 1) / (ROW_WARPS * ROW_GROUPS);
-    return n > INT32_MAX ? 0u : (unsigned)n;
+    return n * ROW_WARPS * ROW_GROUPS > UINT32_MAX ? 0u : (unsigned)n;
 }
 
 template <typename T, bool ALIGNED>
@@ -323,9 +458,10 @@ int launch_quantize(const Fp8RowsCall& c) {
     const int width = (int)c.width, groups = (int)((c.width + 512 / sizeof(T) - 1) / (512 / sizeof(T)));
     if (c.blocks) {
         const int64_t across = (c.width + FP8_BLOCK - 1) / FP8_BLOCK;
-        if (across > 65535) return -2003;
-        ss_launch(quantize_blocks_kernel<T, ALIGNED>, dim3((unsigned)((c.rows + FP8_BLOCK - 1) / FP8_BLOCK), (unsigned)across), dim3(ROW_THREADS), 0, c.stream,
-                  (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, c.scale_row, c.scale_block, c.rows, width);
+        const int64_t n = across * ((c.rows + FP8_BLOCK - 1) / FP8_BLOCK);
+        if (n > INT32_MAX) return -2003;
+        ss_launch(quantize_blocks_kernel<T, ALIGNED>, dim3((unsigned)n), dim3(ROW_THREADS), 0, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales,
+                  c.scale_row, c.scale_block, c.rows, width, (unsigned)across);
     } else {
         const unsigned n = row_blocks(c.rows, groups);
         if (!n) return -2003;
@@ -347,8 +483,43 @@ inline RowShape norm_shape(int width, int64_t rows) {
     return {0, 512};
 }
 
+// The ring: blocks an SM, and stages of a block's ring (0: the rows are too few, too narrow or too wide).  Three rows in flight a
+// block where three blocks share an SM, else two at least; four rows a block at least.
+struct RingShape { int blocks, stages; };
+constexpr int RING_SMEM = 112 * 1024;  // of a block, two of which share an SM
+inline int ring_groups(int width) {
+    const int ng = (width / 4 + RING_THREADS - 1) / RING_THREADS;
+    return ng <= 4 ? ng : ng <= 6 ? 6 : ng <= 8 ? 8 : ng <= 10 ? 10 : 12;
+}
+inline RingShape ring_shape(const Fp8RowsCall& c) {
+    const int64_t bytes = c.width * (4 + (!c.delta ? 0 : c.dtype == SS_BF16 ? 2 : 4));
+    if (bytes < 16384 || c.width > 12 * 4 * RING_THREADS || bytes % 16 || (c.delta && c.width * 2 % 16)) return {0, 0};
+    for (int blocks = ring_blocks(ring_groups((int)c.width)); blocks >= 2; --blocks) {
+        const int64_t stages = (220 * 1024 / blocks - 3072) / (bytes + 8);
+        if (stages >= blocks && c.rows >= 4 * (int64_t)blocks * ss_sm_count()) return {blocks, (int)stages};
+    }
+    return {0, 0};
+}
+template <typename T>
+int launch_norm_ring(const Fp8RowsCall& c, RingShape shape) {
+    const int smem = (int)(shape.stages * (c.width * (4 + (c.delta ? sizeof(T) : 0)) + 8)) + 64;
+    int rc = 0;
+#define NORM(NG) case NG: { \
+        static SsPerDevice opted; \
+        if ((rc = ss_opt_in_smem(add_rmsnorm_fp8_ring_kernel<T, NG>, RING_SMEM, opted))) return rc; \
+        ss_launch(add_rmsnorm_fp8_ring_kernel<T, NG>, dim3(shape.blocks * ss_sm_count()), dim3(RING_THREADS), smem, c.stream, (const float*)c.x, (const T*)c.delta, (float*)c.y, c.weight, (int)c.w_f32, c.q, c.q_stride, c.scales, c.scale_row, c.scale_block, (int)c.rows, (int)c.width, (float)c.eps, shape.stages, c.err); \
+    } break
+    switch (ring_groups((int)c.width)) { NORM(2); NORM(3); NORM(4); NORM(6); NORM(8); NORM(10); NORM(12); }
+#undef NORM
+    return SS_LAUNCH_CHECK();
+}
+
 template <typename T, bool ALIGNED>
 int launch_norm(const Fp8RowsCall& c) {
+    if constexpr (ALIGNED) {
+        const RingShape ring = ring_shape(c);
+        if (ring.blocks) return launch_norm_ring<T>(c, ring);
+    }
     const int width = (int)c.width;
     const RowShape shape = norm_shape(width, c.rows);
     const int64_t smem = (c.width + FP8_BLOCK - 1) / FP8_BLOCK * 8;

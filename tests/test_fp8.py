@@ -18,7 +18,7 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
             for features, k in ((256, 1), (256, 17), (256, 128), (1280, 896), (4608, 3584), (3584, 18944), (37888, 3584), (256, 1000000)):
                 many, tile, slices, per = fp8_plan(tokens, features, k, sms, gated, resident)
                 if many:
-                    assert tile in (64, 128, 256) and tokens > 64 and (not gated or tile == 256)
+                    assert tile in (64, 128, 256) and tokens > 32 and (not gated or tile == 256)
                 else:
                     assert tile % 16 == 0 and 16 <= tile <= 256 // parts and 1 <= slices <= min(8, -(-k // 128)) and tokens <= 640
                     assert per == 1 or (per == 2 and tile <= 64 // parts)
@@ -31,8 +31,8 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
 
 def test_plans_of_more_features_than_a_grid_has_rows_for_their_tiles():
     """The kernel for few tokens has its tiles of features along grid.y: up to 65,535 of them."""
-    for tokens in (1, 64, 65, 640, 700):
-        assert tokens > 64 or fp8_plan(tokens, 65535 * 128, 16, 148, False, RESIDENT)[0] == 0
+    for tokens in (1, 32, 65, 640, 700):
+        assert tokens > 32 or fp8_plan(tokens, 65535 * 128, 16, 148, False, RESIDENT)[0] == 0
         assert fp8_plan(tokens, 65535 * 128 + 128, 16, 148, False, RESIDENT)[0] == 1
 
 
