@@ -27,6 +27,20 @@ __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t top) {
     r.keep = fine ? 0xffffffffu : 0u;
     return r;
 }
+// One of a block's two quotients, where a warp's lanes share the work of them: what values are multiplied by (0: they are written as
+// zeros), or the scale.  The same bits as fp8_scale gives.
+struct Fp8Factor {
+    float value, before;
+};
+__device__ __forceinline__ Fp8Factor fp8_factor(uint32_t top, bool inverse) {
+    const float a = __uint_as_float(top);
+    const bool finite = top < 0x7f800000u;
+    Fp8Factor f;
+    f.before = a < 0x1p-100f ? 0x1p64f : 1.f;
+    const float r = __fdiv_rn(inverse ? FP8_TOP : a, inverse ? a * f.before : FP8_TOP);
+    f.value = inverse ? (finite && top > 0 ? r : 0.f) : finite ? r : __uint_as_float(0x7fffffffu);
+    return f;
+}
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
     uint16_t lo, hi;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));

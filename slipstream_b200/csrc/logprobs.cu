@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4, FEW_GROUPS = THREADS / 8, UNROLL = 4, CANDIDATES = 512;
+constexpr int THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4, FEW_GROUPS = THREADS / 8, CANDIDATES = 512;
 typedef unsigned long long Key;  // value in the upper half, in an order of unsigned integers; the complement of the index below; 0: none
 
 __device__ __forceinline__ Key key_of(float z, int index) {  // z is no NaN
@@ -40,6 +40,14 @@ __device__ __forceinline__ float next_above(float z) {
     return __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
 }
 
+constexpr float LOG2_E = 1.4426950408889634f;
+// exp(d) for d <= 0, as 2^(d log2 e); results below 2^-126 are 0 (without that, __expf takes four instructions more).
+__device__ __forceinline__ float exp_of(float d) {
+    float p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(d * LOG2_E));
+    return p;
+}
+
 template <typename T>
 struct Vec {
     static constexpr int G = 16 / (int)sizeof(T);
@@ -49,6 +57,29 @@ struct Vec {
         const uint32_t w = G == 4 ? (e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w)
                                   : (e < 2 ? raw.x : e < 4 ? raw.y : e < 6 ? raw.z : raw.w);
         return G == 4 ? __uint_as_float(w) : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
+    // the largest element that is a number (NaN: none is); of bfloat16 pairs at a time
+    __device__ __forceinline__ float largest() const {
+        if constexpr (G == 4) {
+            return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
+        } else {
+            const auto pair = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+            const __nv_bfloat162 m = __hmax2(__hmax2(pair(raw.x), pair(raw.y)), __hmax2(pair(raw.z), pair(raw.w)));
+            return fmaxf(__low2float(m), __high2float(m));
+        }
+    }
+    // how many elements reach z (which is a T), or exceed it; above: next_above(z)
+    __device__ __forceinline__ int reaching(float z, float above, bool exceed) const {
+        if constexpr (G == 4) {
+            const float limit = exceed ? above : z;
+            return (at(0) >= limit) + (at(1) >= limit) + (at(2) >= limit) + (at(3) >= limit);
+        } else {
+            const auto pair = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+            const __nv_bfloat162 limit = __float2bfloat162_rn(z);
+            const auto count = [&](const uint32_t& w) { return exceed ? __hgt2(pair(w), limit) : __hge2(pair(w), limit); };
+            const __nv_bfloat162 n = __hadd2(__hadd2(count(raw.x), count(raw.y)), __hadd2(count(raw.z), count(raw.w)));  // (exact: up to 4)
+            return (int)(__low2float(n) + __high2float(n));
+        }
     }
 };
 
@@ -80,10 +111,10 @@ struct Row {
 // What a thread has seen: the largest value, where it stands, sums relative to it, and how many elements stand in front of the token.
 struct Seen {
     float m, s, t;
-    int at;  // vector, or -1 - element: of the head or tail; INT_MIN: nothing yet
+    int at;  // the first element of the vectors (or the element of the head or tail) among which it is; -1: nothing yet
     int ahead;
 };
-constexpr int NOTHING = INT32_MIN;
+constexpr int NOTHING = -1;
 
 __device__ __forceinline__ void raise_to(Seen& a, float m, int at) {
     if (m > a.m || (a.at == NOTHING && m == m)) {
@@ -97,9 +128,36 @@ __device__ __forceinline__ void raise_to(Seen& a, float m, int at) {
     }
 }
 __device__ __forceinline__ void add(Seen& a, float z, float m) {
-    const float d = z - m, p = __expf(d);
+    const float d = z - m, p = exp_of(d);
     a.s += p;
     a.t = fmaf(p, fmaxf(d, -200.f), a.t);  // (p is 0 below that; a NaN is in s)
+}
+// The same for pairs: two sums each, an instruction for two elements but for the exponentials.
+struct Sums {
+    unsigned long long s, t;
+};
+__device__ __forceinline__ unsigned long long two(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float sum_of(unsigned long long v) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return a + b;
+}
+__device__ __forceinline__ void add2(Sums& a, float z0, float z1, unsigned long long minus_m) {
+    unsigned long long d, u, p;
+    float d0, d1, u0, u1, p0, p1;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(two(z0, z1)), "l"(minus_m));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(u) : "l"(d), "l"(two(LOG2_E, LOG2_E)));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(u0), "=f"(u1) : "l"(u));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(u0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(u1));
+    p = two(p0, p1);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.s) : "l"(p));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a.t) : "l"(p), "l"(two(fmaxf(d0, -200.f), fmaxf(d1, -200.f))));
 }
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -124,9 +182,9 @@ struct alignas(16) Shared {  // (every array starts on 16 bytes)
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 3)
 token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int wide, float* __restrict__ out, int vocabulary, int top, int blocks, int* err) {
-    constexpr int G = Vec<T>::G;
+    constexpr int G = Vec<T>::G, UNROLL = 16 / G;  // vectors on their way: 16 elements
     __shared__ Shared<TOP> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t r = blockIdx.x / blocks;
@@ -150,49 +208,60 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
     row.has_head = rank == 0;
     row.has_tail = rank == blocks - 1;
 
-    const float z_token = there ? to_float(row.z[token]) : __uint_as_float(0x7fffffffu);
-    const float above = next_above(z_token);
-    Seen a = {-INFINITY, 0.f, 0.f, NOTHING, 0};
-    if (row.has_head && tid < row.head) {
-        const float z = to_float(row.z[tid]);
-        raise_to(a, z, -1 - tid);
-        add(a, z, reference(a.m));
-        a.ahead += z >= (tid < token ? z_token : above);
-    }
-    // vectors: in front of the token equal values count, from its own vector on (whose elements in front of it are looked at below) they do
-    // not; a vector behind the block's last is all -inf and counts nothing
-    for (int v = row.first + tid; v < row.end; v += UNROLL * THREADS) {
-        Vec<T> x[UNROLL];
+    // all that does not wait for the token is on its way first: a thread's element of the head and of the tail, and its first vectors
+    Vec<T> x[UNROLL];
+    const auto fetch = [&](int v) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             x[u].raw = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
             if (v + u * THREADS < row.end) x[u] = row.vectors()[v + u * THREADS];
         }
-        float m = x[0].at(0);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-            for (int e = 0; e < G; ++e) m = fmaxf(m, x[u].at(e));
-        raise_to(a, m, v);
-        const float ref = reference(a.m);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const float limit = v + u * THREADS >= row.end ? __uint_as_float(0x7fffffffu) : row.index(v + u * THREADS, G - 1) < token ? z_token : above;
-#pragma unroll
-            for (int e = 0; e < G; ++e) {
-                const float z = x[u].at(e);
-                add(a, z, ref);
-                a.ahead += z >= limit;
-            }
-        }
-    }
-    if (row.has_tail && row.tail_from + tid < vocabulary) {
-        const int i = row.tail_from + tid;
-        const float z = to_float(row.z[i]);
-        raise_to(a, z, -1 - i);
+    };
+    int v = row.first + tid;
+    fetch(v);
+    const bool in_head = row.has_head && tid < row.head, in_tail = row.has_tail && row.tail_from + tid < vocabulary;
+    const float head = in_head ? to_float(row.z[tid]) : 0.f, tail = in_tail ? to_float(row.z[row.tail_from + tid]) : 0.f;
+    const float z_token = there ? to_float(row.z[token]) : __uint_as_float(0x7fffffffu);
+    const float above = next_above(z_token);
+    Seen a = {-INFINITY, 0.f, 0.f, NOTHING, 0};
+    const auto one = [&](float z, int i) {
+        raise_to(a, z, i);
         add(a, z, reference(a.m));
         a.ahead += z >= (i < token ? z_token : above);
+    };
+    if (in_head) one(head, tid);
+    // vectors: in front of the token equal values count, from its own vector on (whose elements in front of it are looked at below) they do
+    // not; a vector behind the block's last is all -inf and counts nothing
+    while (v < row.end) {
+        float m = x[0].largest();
+#pragma unroll
+        for (int u = 1; u < UNROLL; ++u) m = fmaxf(m, x[u].largest());
+        raise_to(a, m, row.index(v, 0));
+        const float ref = reference(a.m);
+        if constexpr (G == 8) {  // (the instructions are the work: 1,024 x 151,936 88.4 to 82.7 us)
+            const unsigned long long minus = two(-ref, -ref);
+            Sums sums = {0, 0};
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int e = 0; e < G; e += 2) add2(sums, x[u].at(e), x[u].at(e + 1), minus);
+            a.s += sum_of(sums.s);
+            a.t += sum_of(sums.t);
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int e = 0; e < G; ++e) add(a, x[u].at(e), ref);
+        }
+        if (m >= z_token) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+                if (v + u * THREADS < row.end) a.ahead += x[u].reaching(z_token, above, row.index(v + u * THREADS, G - 1) >= token);
+        }
+        v += UNROLL * THREADS;
+        fetch(v);
     }
+    if (in_tail) one(tail, row.tail_from + tid);
     if (token >= row.head && token < row.tail_from && tid < (token - row.head) % G && row.first <= (token - row.head) / G && (token - row.head) / G < row.end)
         a.ahead += to_float(row.z[token - 1 - tid]) == z_token;
 
@@ -216,21 +285,16 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
     }
 
     if constexpr (TOP) {
-        Key mine = 0;
+        // where its largest element stands a thread knows but for its last vectors: what it brings to the bound stands at their last
+        // element, so that its own is not behind, and it is chosen as if its own stood at their first
+        Key mine = 0, least = 0;
         if (a.at != NOTHING) {
-            if (a.at < 0) {
-                mine = key_of(a.m, -1 - a.at);
-            } else {  // the first of its (at most four) vectors' elements that has the value
-                for (int w = a.at; w < row.end && !mine; w += THREADS) {
-                    const Vec<T> x = row.vectors()[w];
-#pragma unroll
-                    for (int e = G - 1; e >= 0; --e)
-                        if (x.at(e) == a.m) mine = key_of(a.m, row.index(w, e));
-                }
-            }
+            const bool single = a.at < row.head || a.at >= row.tail_from;
+            mine = key_of(a.m, a.at);
+            least = key_of(a.m, single ? a.at : a.at + (UNROLL - 1) * THREADS * G + G - 1);  // (which may be none of the row's: it is only a bound)
         }
         const int groups = top <= FEW_GROUPS * 3 / 8 ? FEW_GROUPS : GROUPS, per_group = THREADS / groups;
-        Key group = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        Key group = max(least, __shfl_xor_sync(0xffffffffu, least, 1));
         group = max(group, __shfl_xor_sync(0xffffffffu, group, 2));
         if (per_group == 8) group = max(group, __shfl_xor_sync(0xffffffffu, group, 4));
         if (lane % per_group == 0) sh.groups[tid / per_group] = group;
@@ -419,10 +483,9 @@ extern "C" int ss_token_logprobs(const LogprobCall* call) {
     if (c.vocabulary < 1 || c.vocabulary > INT32_MAX - 65536 || c.top < 0 || c.top > LOGPROBS_MAX_TOP || c.rows > INT32_MAX / 8) return -2003;
     const uintptr_t size = c.dtype == SS_BF16 ? 2 : 4;
     if ((uintptr_t)c.logits % size || (uintptr_t)c.tokens % (c.wide ? 8 : 4) || (uintptr_t)c.out % 4) return -2004;
-    // blocks a row: as many as have an SM's half each, while each has four vectors a thread or more
+    // blocks a row: as many as run at the same time (three an SM), while each has 16 elements a thread or more
     int blocks = 1;
-    const int64_t vectors = c.vocabulary * (c.dtype == SS_BF16 ? 2 : 4) / 16;
-    while (blocks < 8 && c.rows * blocks * 2 <= 2 * ss_sm_count() && vectors >= blocks * 2 * 4 * THREADS) blocks *= 2;
+    while (blocks < 8 && c.rows * blocks * 2 <= 3 * (int64_t)ss_sm_count() && c.vocabulary >= blocks * 2 * 16 * THREADS) blocks *= 2;
     return c.dtype == SS_BF16 ? launch<bf16>(c, blocks) : launch<float>(c, blocks);
 }
 

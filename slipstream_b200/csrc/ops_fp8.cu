@@ -41,28 +41,56 @@ __device__ __forceinline__ void load(const bf16* p, int left, float (&v)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = e < left ? to_float(p[e]) : 0.f;
 }
-template <int V>
-__device__ __forceinline__ uint32_t top_of(uint32_t top, const float (&v)[V]) {
+// 16 bytes of a row as they came.
+template <typename T>
+struct RawVec {
+    static constexpr int V = 16 / (int)sizeof(T);
+    uint4 raw;
+    template <bool ALIGNED>
+    __device__ __forceinline__ void load(const T* p, int left) {
+        if (ALIGNED && left >= V) {
+            raw = *reinterpret_cast<const uint4*>(p);
+            return;
+        }
+        uint32_t w[4] = {};
 #pragma unroll
-    for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-    return top;
-}
-template <int V>
-__device__ __forceinline__ void store(uint8_t* q, int left, const float (&v)[V], const Fp8Scale& r) {
-    uint32_t w[V / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-        const float four[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-        w[i] = fp8_quantize4(four, r);
+        for (int e = 0; e < V; ++e)
+            if (e < left) {
+                if constexpr (V == 4) w[e] = __float_as_uint(p[e]);
+                else w[e / 2] |= (uint32_t)__bfloat16_as_ushort(p[e]) << (16 * (e % 2));
+            }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (V == 8 && left >= 8) {
-        *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[V / 4 - 1]);
-        return;
+    // bits of the largest magnitude: of bfloat16 values pairs at a time
+    __device__ __forceinline__ uint32_t top() const {
+        if constexpr (V == 4) return max(max(raw.x & 0x7fffffffu, raw.y & 0x7fffffffu), max(raw.z & 0x7fffffffu, raw.w & 0x7fffffffu));
+        const uint32_t t = __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu), __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+        return max(t << 16, t & 0xffff0000u);
     }
+    __device__ __forceinline__ void store(uint8_t* q, int left, const Fp8Scale& r) const {
+        float v[V];
+        values(v);
+        if (r.before != 1.f) {  // (very small values)
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) fp8_store4(q + 4 * i, left - 4 * i, w[i]);
-}
-
+            for (int e = 0; e < V; ++e) v[e] *= r.before;
+        }
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            w[i] = fp8_pack4(__fmul_rn(v[4 * i], r.inverse), __fmul_rn(v[4 * i + 1], r.inverse), __fmul_rn(v[4 * i + 2], r.inverse), __fmul_rn(v[4 * i + 3], r.inverse)) & r.keep;
+        if (V == 8 && left >= 8) {
+            *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[V / 4 - 1]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) fp8_store4(q + 4 * i, left - 4 * i, w[i]);
+    }
+    __device__ __forceinline__ void values(float (&v)[V]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = V == 4 ? __uint_as_float(w[e]) : __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+};
 // Behind a block's last store where the kernel behind was not let go early, so that it starts when every block has ended: it may
 // take the results for constant and read them (with plain loads or by TMA) in front of its griddepcontrol.wait, which is what would make
 // them visible otherwise.  One thread's fence, behind a barrier, covers the block's stores.
@@ -89,33 +117,53 @@ __device__ __forceinline__ Place place_of(int i, int groups) {  // the i-th grou
 // ---------------------------------------------------------------- rows to fp8
 //
 // A lane takes 16 bytes of a row: a block of 128 is 32 lanes of float32 or 16 of bfloat16, whose largest magnitude is found by
-// shuffles.  No block depends on another, so a warp takes four groups of 32 lanes from anywhere, all loaded before the first is written.
+// shuffles.  A block of threads takes 32 vectors (128 or 256 columns) of each of 32 rows, a warp four rows, all loaded before the first is
+// written; neighbouring blocks take neighbours of the same rows.  The scales of 32 rows stand side by side in memory and are written so
+// (each by the warp that formed it, one at a time: 4,096 x 3,584 18.6 us).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS)
 quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
-                     int64_t scale_block, int64_t rows, int width, int groups, int early) {
-    constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V;
-    const int lane = threadIdx.x & 31;
+                     int64_t scale_block, int64_t rows, int width, unsigned groups, int early) {
+    constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V, PER = 32 / LANES, BLOCKS = ROW_GROUPS * PER;
+    __shared__ float formed[PER][ROW_WARPS * ROW_GROUPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned down = blockIdx.x / groups;
+    const int first = (int)(blockIdx.x - down * groups) * 32 * V, column = first + lane * V, left = width - column;
+    const int64_t row0 = (int64_t)down * (ROW_WARPS * ROW_GROUPS) + warp * ROW_GROUPS;
     if (early) pdl_launch_dependents();
     pdl_wait();
-    float v[ROW_GROUPS][V];
-    Place p[ROW_GROUPS];
+    RawVec<T> v[ROW_GROUPS];
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        p[i] = place_of<V>(i, groups);
-        p[i].column += lane * V;
-        const bool in = p[i].row < rows && p[i].column < width;
-        load<V, ALIGNED>(x + (in ? p[i].row * stride + p[i].column : 0), in ? width - p[i].column : 0, v[i]);
+        const bool in = row0 + i < rows && left > 0;
+        v[i].template load<ALIGNED>(x + (in ? (row0 + i) * stride + column : 0), in ? left : 0);
     }
+    // The warp holds ROW_GROUPS * PER blocks.  A division takes as long as all that is done with eight elements beside it, so each lane
+    // does one: lane b what the values of block b are multiplied by, lane 16 + b its scale.
+    const int mine = lane % 16, half = lane / LANES;
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < ROW_GROUPS; ++i) {
-        uint32_t top = top_of(0u, v[i]);
+        uint32_t t = v[i].top();
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (p[i].row >= rows || p[i].column >= width) continue;
-        const Fp8Scale r = fp8_scale(top);
-        if (lane % LANES == 0) scales[p[i].row * scale_row + p[i].column / FP8_BLOCK * scale_block] = r.scale;
-        store(q + p[i].row * q_stride + p[i].column, width - p[i].column, v[i], r);
+        for (int o = LANES / 2; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+        t = __shfl_sync(0xffffffffu, t, mine % PER * LANES);
+        if (mine / PER == i) top = t;
+    }
+    const Fp8Factor f = fp8_factor(top, lane < 16);
+    if (lane >= 16 && mine < BLOCKS) formed[mine % PER][warp * ROW_GROUPS + mine / PER] = f.value;
+#pragma unroll
+    for (int i = 0; i < ROW_GROUPS; ++i) {
+        Fp8Scale r;
+        r.inverse = __shfl_sync(0xffffffffu, f.value, i * PER + half);
+        r.before = __shfl_sync(0xffffffffu, f.before, i * PER + half);
+        r.keep = r.inverse == 0.f ? 0u : 0xffffffffu;
+        if (row0 + i < rows && left > 0) v[i].store(q + (row0 + i) * q_stride + column, left, r);
+    }
+    __syncthreads();
+    if (warp < PER && first + warp * FP8_BLOCK < width) {
+        const int64_t row = (int64_t)down * (ROW_WARPS * ROW_GROUPS) + lane;
+        if (row < rows) scales[row * scale_row + (first / FP8_BLOCK + warp) * scale_block] = formed[warp][lane];
     }
     if (!early) publish_results();
 }
@@ -125,7 +173,7 @@ quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_
 // A block of threads per 128 x 128 elements, which stay in registers.  Neighbouring blocks take neighbours of the same rows, so that the
 // pieces of a row in memory are read at the same time.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 4 : 3)
 quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
                        int64_t scale_block, int64_t rows, int width, unsigned across) {
     constexpr int V = 16 / (int)sizeof(T), LANES = FP8_BLOCK / V, AT_ONCE = ROW_THREADS / LANES, N = FP8_BLOCK / AT_ONCE;
@@ -135,16 +183,15 @@ quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int6
     const int64_t r0 = (int64_t)down * FP8_BLOCK + threadIdx.x / LANES;
     const int64_t j = (int64_t)right * FP8_BLOCK + threadIdx.x % LANES * V;
     const int left = (int)min((int64_t)V, max((int64_t)0, width - j));
-    float v[N][V];
+    RawVec<T> v[N];  // as they came: bfloat16 values take half the registers of float32 ones
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int64_t r = r0 + i * AT_ONCE;
-        const bool in = r < rows && left > 0;
-        load<V, ALIGNED>(x + (in ? r * stride + j : 0), in ? left : 0, v[i]);
+        v[i].template load<ALIGNED>(x + (r < rows && left > 0 ? r * stride + j : 0), r < rows ? left : 0);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = top_of(top, v[i]);
+    for (int i = 0; i < N; ++i) top = max(top, v[i].top());
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -154,7 +201,7 @@ quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int6
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int64_t r = r0 + i * AT_ONCE;
-        if (r < rows && left > 0) store(q + r * q_stride + j, left, v[i], s);
+        if (r < rows && left > 0) v[i].store(q + r * q_stride + j, left, s);
     }
     publish_results();
 }
@@ -358,11 +405,21 @@ add_rmsnorm_fp8_ring_kernel(const float* residual, const T* delta, float* residu
         total = warp_sum(total);
         const float rstd = 1.0f / sqrtf(total / (float)width + eps);
         for (int b = threadIdx.x; b < blocks; b += RING_THREADS) scales[row * scale_row + b * scale_block] = norm_scale(tops[n][b], rstd);
+        // (a lane a division: lane i what the values of the warp's block i are multiplied by)
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+            if (lane == i) mine = top[i];
+        const Fp8Factor f = fp8_factor(mine, true);
         uint8_t* out = q + row * q_stride;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             const int j = (threadIdx.x + i * RING_THREADS) * 4;
-            if (j < width) *reinterpret_cast<uint32_t*>(out + j) = fp8_quantize4(v[i], fp8_scale(top[i]));
+            Fp8Scale r;
+            r.inverse = __shfl_sync(0xffffffffu, f.value, i);
+            r.before = __shfl_sync(0xffffffffu, f.before, i);
+            r.keep = r.inverse == 0.f ? 0u : 0xffffffffu;
+            if (j < width) *reinterpret_cast<uint32_t*>(out + j) = fp8_quantize4(v[i], r);
         }
         if (++s == stages) { s = 0; parity ^= 1; }
     }
@@ -463,10 +520,10 @@ int launch_quantize(const Fp8RowsCall& c) {
         ss_launch(quantize_blocks_kernel<T, ALIGNED>, dim3((unsigned)n), dim3(ROW_THREADS), 0, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales,
                   c.scale_row, c.scale_block, c.rows, width, (unsigned)across);
     } else {
-        const unsigned n = row_blocks(c.rows, groups);
-        if (!n) return -2003;
-        ss_launch(quantize_rows_kernel<T, ALIGNED>, dim3(n), dim3(ROW_THREADS), 0, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, c.scale_row,
-                  c.scale_block, c.rows, width, groups, (int)c.early);
+        const int64_t n = (c.rows + ROW_WARPS * ROW_GROUPS - 1) / (ROW_WARPS * ROW_GROUPS) * groups;
+        if (n > INT32_MAX) return -2003;
+        ss_launch(quantize_rows_kernel<T, ALIGNED>, dim3((unsigned)n), dim3(ROW_THREADS), 0, c.stream, (const T*)c.x, c.stride, c.q, c.q_stride, c.scales, c.scale_row,
+                  c.scale_block, c.rows, width, (unsigned)groups, (int)c.early);
     }
     return SS_LAUNCH_CHECK();
 }
