@@ -14,7 +14,7 @@ from .config.engine_config import CacheConfig, EngineConfig, ModelConfig, ModelO
 from .config.sampling_params import SamplingParams
 
 __all__ = ["CacheConfig", "EngineConfig", "ModelConfig", "ModelOptions", "ParallelConfig", "SchedulerConfig", "SamplingParams",
-           "LLM", "LLMEngine", "Request"]
+           "LLM", "LLMEngine", "Request", "TokenLogprob"]
 
 
 def __getattr__(name: str):
@@ -22,4 +22,8 @@ def __getattr__(name: str):
         from .engine import llm_engine
 
         return getattr(llm_engine, name)
+    if name == "TokenLogprob":
+        from .engine.logprobs import TokenLogprob
+
+        return TokenLogprob
     raise AttributeError(name)

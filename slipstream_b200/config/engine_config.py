@@ -25,7 +25,7 @@ class ModelOptions:
     dtype: str | None = None  # bfloat16 | float32; None takes config.json's torch_dtype
     max_model_len: int | None = None  # None takes max_position_embeddings
     load_format: str = "safetensors"  # safetensors | random (weights drawn on the device)
-    quantization: str | None = None  # int8: the layers' projections in 8 bits, for architectures that have such layers
+    quantization: str | None = None  # int8 or fp8: the layers' projections in 8 bits, for architectures that have such layers
 
     def __post_init__(self) -> None:
         if self.dtype is not None and self.dtype not in ("bfloat16", "float32"):
@@ -34,8 +34,8 @@ class ModelOptions:
             raise ValueError("max_model_len must be >= 1")
         if self.load_format not in ("safetensors", "random"):
             raise ValueError(f"unknown load_format: {self.load_format}")
-        if self.quantization not in (None, "int8"):
-            raise ValueError(f"unknown quantization: {self.quantization} (int8)")
+        if self.quantization not in (None, "int8", "fp8"):
+            raise ValueError(f"unknown quantization: {self.quantization} (int8, fp8)")
 
 
 ModelConfig = ModelOptions  # the reference's name for it (slipstream/core/config.py:25-57)

@@ -2,12 +2,16 @@
 (slipstream/core/sampling_params.py:8-48).
 
 ``n`` above 1 is rejected: the reference declares it but never forks a sequence.
-``stop_strings`` need a tokenizer in the model folder.
+``stop_strings`` need a tokenizer in the model folder.  ``logprobs`` and ``prompt_logprobs`` (which the reference lacks) ask for the log
+probabilities of the output's and of the prompt's tokens, and for that many of the likeliest tokens beside each.
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+
+
+MAX_TOP_LOGPROBS = 64  # ops/logprobs.py
 
 
 @dataclass(frozen=True)
@@ -22,6 +26,8 @@ class SamplingParams:
     stop_strings: tuple[str, ...] = ()
     ignore_eos: bool = False
     seed: int | None = None
+    logprobs: int | None = None  # None: not told; 0: of the token alone
+    prompt_logprobs: int | None = None
     n: int = 1
     extra: dict[str, object] = field(default_factory=dict, hash=False, compare=False)
 
@@ -34,6 +40,9 @@ class SamplingParams:
             ("top_p", 0.0 < self.top_p <= 1.0, "above 0 and at most 1"),
             ("min_p", 0.0 <= self.min_p <= 1.0, "between 0 and 1"),
             ("repetition_penalty", self.repetition_penalty > 0.0, "positive"),
+            ("logprobs", self.logprobs is None or 0 <= self.logprobs <= MAX_TOP_LOGPROBS, f"None or between 0 and {MAX_TOP_LOGPROBS}"),
+            ("prompt_logprobs", self.prompt_logprobs is None or 0 <= self.prompt_logprobs <= MAX_TOP_LOGPROBS,
+             f"None or between 0 and {MAX_TOP_LOGPROBS}"),
             ("n", self.n == 1, "1: several samples of one prompt are not implemented"),
         )
         for name, ok, wanted in rules:

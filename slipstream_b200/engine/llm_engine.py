@@ -30,6 +30,7 @@ from slipstream_b200 import ops
 from slipstream_b200.sampling.sampler import SampleRow, Sampler
 
 from .context import StepEntry
+from .logprobs import TokenLogprob, read_logprobs
 from .runner import ModelRunner
 from .scheduler import ScheduledSeq, Scheduler, Sequence, SequenceStatus
 
@@ -59,6 +60,8 @@ class RequestOutput:
     output_token_ids: list[int]
     finish_reason: str  # stop | length | abort
     text: str | None = None
+    logprobs: list[TokenLogprob] | None = None  # of the output's tokens, where SamplingParams.logprobs asked for them
+    prompt_logprobs: list[TokenLogprob | None] | None = None  # of the prompt's (None for the first token)
 
 
 @dataclass
@@ -88,6 +91,7 @@ class InFlight:
     tokens_dev: torch.Tensor  # int32 [len(seqs) + 1] on the device: the tokens, then the device error word
     tokens_host: torch.Tensor  # pinned copy, valid once ``ready`` has happened
     ready: torch.cuda.Event
+    logprobs_host: torch.Tensor | None = None  # pinned copy of the tokens' log probabilities, where anybody asked for them
 
 
 def absolute_arrival(ts: float, now: float) -> float:
@@ -143,6 +147,7 @@ class LLMEngine:
         # pinned buffers and events of the steps in flight, made once (a step in flight and the one being launched)
         self._token_ring = [torch.empty(s.max_num_seqs + 1, dtype=torch.int32, pin_memory=True) for _ in range(3)]
         self._event_ring = [torch.cuda.Event() for _ in range(3)]
+        self._logprob_ring: list[torch.Tensor | None] = [None] * 3  # made when first asked for
         self._ring_turn = 0
 
     # ------------------------------------------------------------------ public calls
@@ -258,6 +263,8 @@ class LLMEngine:
         params = request.sampling_params
         if params.stop_strings and self.tokenizer is None:
             raise ValueError("stop_strings need tokenizer.json in the model folder")
+        if max(params.logprobs or 0, params.prompt_logprobs or 0) > vocab:
+            raise ValueError(f"more alternatives asked for than the vocabulary has tokens ({vocab})")
         max_new = capped_new_tokens(len(ids), params.max_tokens, self.max_model_len)
         self._requests_seen += 1
         seed = params.seed if params.seed is not None else (self.config.seed * 1000003 + self._requests_seen)
@@ -294,13 +301,17 @@ class LLMEngine:
         flight.ready.synchronize()
         tokens = flight.tokens_host.tolist()
         self._check_status(tokens.pop(), flight.seqs)
+        told = (read_logprobs(flight.logprobs_host.numpy(), tokens, [s.sampling_params.logprobs for s in flight.seqs])
+                if flight.logprobs_host is not None else [None] * len(tokens))
         now = time.perf_counter()
-        for seq, at, token in zip(flight.seqs, flight.where, tokens):
+        for seq, at, token, logprob in zip(flight.seqs, flight.where, tokens, told):
             if seq in self._zombies:  # stopped one token earlier; this token was computed for nothing
                 self._zombies.remove(seq)
                 self.scheduler.finish(seq)
                 continue
             seq.output_token_ids[at] = int(token)
+            if logprob is not None:
+                seq.logprobs.append(logprob)
             self._mark_emit(seq, now)
             ahead = at + 1 < len(seq.output_token_ids)  # its next token is already being computed
             if self._is_stop(seq, int(token)):
@@ -376,13 +387,20 @@ class LLMEngine:
         turn = self._ring_turn = (self._ring_turn + 1) % len(self._token_ring)
         tokens_host = self._token_ring[turn][: len(todo) + 1]
         tokens_host.copy_(tokens_dev, non_blocking=True)
+        logprobs_host = None
+        packed = self._logprobs(logits, tokens_dev[: len(todo)], todo)
+        if packed is not None:
+            if self._logprob_ring[turn] is None:
+                self._logprob_ring[turn] = torch.empty(self.config.scheduler.max_num_seqs * (3 + 2 * ops.MAX_TOP_LOGPROBS), pin_memory=True)
+            logprobs_host = self._logprob_ring[turn][: packed.numel()].view(packed.shape)
+            logprobs_host.copy_(packed, non_blocking=True)
         ready = self._event_ring[turn]
         ready.record()
         for seq in todo:  # the host's view moves on at once; the token's value follows
             seq.num_computed_tokens += 1
             where.append(len(seq.output_token_ids))
             seq.output_token_ids.append(PENDING)
-        self._inflight = InFlight(todo, where, tokens_dev, tokens_host, ready)
+        self._inflight = InFlight(todo, where, tokens_dev, tokens_host, ready, logprobs_host)
         if prev is not None:
             self._collect(prev)
         st = self.stats
@@ -394,6 +412,22 @@ class LLMEngine:
         st.preemptions = self.scheduler.preemptions
         st.step_time_ms = (time.perf_counter() - started) * 1e3
         return True
+
+    def _logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, seqs: list[Sequence]) -> torch.Tensor | None:
+        """The sampled tokens' log probabilities (`ops.TokenLogprobs.packed`), or None where no request asks for them."""
+        asked = [s.sampling_params.logprobs for s in seqs if s.sampling_params.logprobs is not None]
+        return ops.token_logprobs(logits, tokens, top=max(asked)).packed if asked else None
+
+    def _score_prompts(self, logits: torch.Tensor, rows: list[int], scored: list[tuple[Sequence, int]]) -> None:
+        """Log probabilities of prompt tokens: ``scored`` are (sequence, token), whose distributions are rows ``rows`` of the logits."""
+        device = self.runner.device
+        tokens = [token for _, token in scored]
+        at = torch.tensor([rows, tokens], dtype=torch.int64).to(device)
+        mine = logits if len(rows) == logits.shape[0] else logits.index_select(0, at[0])
+        wanted = [seq.sampling_params.prompt_logprobs for seq, _ in scored]
+        packed = ops.token_logprobs(mine, at[1], top=max(wanted)).packed.cpu().numpy()
+        for (seq, _), told in zip(scored, read_logprobs(packed, tokens, wanted)):
+            seq.prompt_logprobs.append(told)
 
     def _step(self) -> bool:
         """Schedule, run one step-function call, sample, finish.  False when nothing can run."""
@@ -413,6 +447,9 @@ class LLMEngine:
             return False
         entries: list[StepEntry] = []
         sampling: list[ScheduledSeq] = []
+        scored: list[tuple[Sequence, int]] = []  # prompt tokens whose log probabilities this step gives
+        scored_rows: list[int] = []
+        sampled_rows: list[int] = []
         for item in plan.scheduled:
             seq = item.seq
             if seq.num_computed_tokens == 0:
@@ -420,25 +457,40 @@ class LLMEngine:
                 self.runner.reset_state(slot)
                 self.sampler.begin_request(slot, seq.sampling_params,
                                            seq.prompt_token_ids + seq.output_token_ids)
-            want = [item.take - 1] if item.samples else []
-            entries.append(StepEntry(seq.seq_id, seq.tokens_to_feed(item.take), want))
+            want = seq.places_to_score(item.take)
+            scored += [(seq, seq.prompt_token_ids[seq.num_computed_tokens + place + 1]) for place in want]
+            scored_rows += range(len(scored_rows) + len(sampled_rows), len(scored_rows) + len(sampled_rows) + len(want))
             if item.samples:
+                sampled_rows.append(len(scored_rows) + len(sampled_rows))
+                want = want + [item.take - 1]
                 sampling.append(item)
+            entries.append(StepEntry(seq.seq_id, seq.tokens_to_feed(item.take), want))
         decode_tokens = plan.num_decode_tokens
         logits = self.runner.step(entries)
         tokens: list[int] = []
+        told: list[TokenLogprob | None] = [None] * len(sampling)
+        if scored:
+            self._score_prompts(logits, scored_rows, scored)
+            if sampling:
+                logits = logits.index_select(0, torch.tensor(sampled_rows).to(self.runner.device))
         if sampling:
             rows = [SampleRow(i.seq.sampling_params, i.seq.seed, i.seq.num_output_tokens,
                               self.runner.cache.get(i.seq.seq_id).slot) for i in sampling]
             # the step's one device-to-host copy: the tokens and, behind them, the device error word
-            tokens = self.sampler.sample(logits, rows, with_status=True).tolist()
+            tokens_dev = self.sampler.sample(logits, rows, with_status=True)
+            packed = self._logprobs(logits, tokens_dev[: len(rows)], [i.seq for i in sampling])
+            tokens = tokens_dev.tolist()
             self._check_status(tokens.pop(), [i.seq for i in plan.scheduled])
+            if packed is not None:
+                told = read_logprobs(packed.cpu().numpy(), tokens, [i.seq.sampling_params.logprobs for i in sampling])
         for item in plan.scheduled:
             item.seq.num_computed_tokens += item.take
         now = time.perf_counter()
-        for item, token in zip(sampling, tokens):
+        for item, token, logprob in zip(sampling, tokens, told):
             seq = item.seq
             seq.output_token_ids.append(int(token))
+            if logprob is not None:
+                seq.logprobs.append(logprob)
             self._mark_emit(seq, now)
             if self._is_stop(seq, int(token)):
                 seq.status = SequenceStatus.FINISHED_STOPPED
@@ -494,6 +546,9 @@ class LLM:
         outs = []
         for seq in seqs:
             text = engine.tokenizer.decode(seq.output_token_ids) if engine.tokenizer is not None else None
+            asked = seq.sampling_params
             outs.append(RequestOutput(seq.request_id, seq.prompt_token_ids, list(seq.output_token_ids),
-                                      _FINISH.get(seq.status, "abort"), text))
+                                      _FINISH.get(seq.status, "abort"), text,
+                                      None if asked.logprobs is None else list(seq.logprobs),
+                                      None if asked.prompt_logprobs is None else list(seq.prompt_logprobs)))
         return outs

@@ -43,8 +43,8 @@ class ModelRunner:
         ``num_pages``: pages of that size the cache should hold (groups with another page size get as many pages
         as hold the same tokens; a windowed group at most what ``max_num_seqs`` requests can keep of their windows
         when a step feeds up to ``max_step_tokens`` tokens of a request), or one count per cache group, or None
-        to size the pools from the free device memory.  ``quantization`` "int8": the layers' projections run in 8 bits
-        (``parts/int8.py``), their weights rounded here from the checkpoint's."""
+        to size the pools from the free device memory.  ``quantization`` "int8" or "fp8": the layers' projections run in 8 bits
+        (``parts/int8.py``, ``parts/fp8.py``), their weights rounded here from the checkpoint's."""
         ops.require_cuda()
         self.device = torch.device(device)
         if self.device.type == "cuda":

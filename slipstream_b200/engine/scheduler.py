@@ -62,6 +62,10 @@ class Sequence:
     max_new_tokens: int = 16  # output cap under the context window
     seed: int = 0
     preemptions: int = 0
+    # what SamplingParams.logprobs and prompt_logprobs asked for: of every output token that the host knows, and of the prompt's tokens so
+    # far (of the first, which has nothing in front of it, None)
+    logprobs: list = field(default_factory=list)
+    prompt_logprobs: list = field(default_factory=lambda: [None])
 
     @property
     def num_prompt_tokens(self) -> int:
@@ -87,6 +91,14 @@ class Sequence:
     def is_decoding(self) -> bool:
         """Only the last sampled token is missing from the cache."""
         return self.num_output_tokens > 0 and self.num_uncomputed_tokens == 1
+
+    def places_to_score(self, take: int) -> list[int]:
+        """Places of the next ``take`` tokens whose logits give the prompt's next log probabilities, where they are asked for (and not
+        known from before a preemption)."""
+        if self.sampling_params.prompt_logprobs is None:
+            return []
+        first = max(self.num_computed_tokens, len(self.prompt_logprobs) - 1)
+        return [p - self.num_computed_tokens for p in range(first, min(self.num_computed_tokens + take, self.num_prompt_tokens - 1))]
 
     def tokens_to_feed(self, take: int) -> list[int]:
         start = self.num_computed_tokens

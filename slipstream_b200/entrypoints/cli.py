@@ -14,6 +14,7 @@ config.json instead of generating.
 from __future__ import annotations
 
 import argparse
+import dataclasses
 import json
 import sys
 
@@ -24,8 +25,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
     p.add_argument("--max-model-len", type=int, default=None)
     p.add_argument("--load-format", choices=["safetensors", "random"], default="safetensors")
-    p.add_argument("--quantization", choices=["int8"], default=None,
-                   help="run the layers' projections in 8-bit integers (weights rounded at load, activations token by token)")
+    p.add_argument("--quantization", choices=["int8", "fp8"], default=None,
+                   help="run the layers' projections in 8-bit integers, or in 8-bit floats with a scale for each block of 128 "
+                        "(weights rounded at load, activations token by token)")
     p.add_argument("--seed", type=int, default=0, help="engine seed (random weights, unseeded requests)")
     # cache
     p.add_argument("--block-size", type=int, default=16)
@@ -50,6 +52,9 @@ def build_parser() -> argparse.ArgumentParser:
                    help="stop string (needs tokenizer.json); generation ends once the output text holds it; repeatable")
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--sample-seed", type=int, default=None, help="SamplingParams.seed")
+    p.add_argument("--logprobs", type=int, default=None, metavar="N",
+                   help="tell the log probability, rank and entropy of every output token, and the N likeliest tokens beside it")
+    p.add_argument("--prompt-logprobs", type=int, default=None, metavar="N", help="the same for the prompt's tokens")
     # random-weights folder
     p.add_argument("--write-random-model", metavar="CONFIG_JSON", default=None,
                    help="write config.json + model.safetensors with random weights into --model and exit")
@@ -84,7 +89,8 @@ def main(argv: list[str] | None = None) -> int:
         max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
         min_p=args.min_p, repetition_penalty=args.repetition_penalty,
         stop_token_ids=tuple(int(t) for t in args.stop_token_ids.split(",") if t.strip()),
-        stop_strings=tuple(args.stop or ()), ignore_eos=args.ignore_eos, seed=args.sample_seed)
+        stop_strings=tuple(args.stop or ()), ignore_eos=args.ignore_eos, seed=args.sample_seed,
+        logprobs=args.logprobs, prompt_logprobs=args.prompt_logprobs)
     llm = LLM(args.model, dtype=args.dtype, max_model_len=args.max_model_len, block_size=args.block_size,
               num_gpu_blocks=args.num_gpu_blocks, gpu_memory_utilization=args.gpu_memory_utilization,
               max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
@@ -96,8 +102,12 @@ def main(argv: list[str] | None = None) -> int:
     else:
         outs = llm.generate(prompts=args.prompt, sampling_params=params)
     for out in outs:
-        print(json.dumps({"request_id": out.request_id, "output_token_ids": out.output_token_ids,
-                          "finish_reason": out.finish_reason, "text": out.text}))
+        line = {"request_id": out.request_id, "output_token_ids": out.output_token_ids, "finish_reason": out.finish_reason, "text": out.text}
+        for name in ("logprobs", "prompt_logprobs"):
+            told = getattr(out, name)
+            if told is not None:
+                line[name] = [t and dataclasses.asdict(t) for t in told]
+        print(json.dumps(line))
     return 0
 
 

@@ -9,6 +9,7 @@ from .differential import DifferentialAttention
 from .embedding import LMHead, SummedEmbedding, TokenEmbedding
 from .mlp import GELU_TANH, ActivatedFeedForward, GatedFeedForward, SwiGLUFeedForward
 from .experts import RoutedExperts
+from .fp8 import Fp8PagedAttention, Fp8RMSNorm, Fp8SwiGLUFeedForward
 from .int8 import Int8PagedAttention, Int8RMSNorm, Int8SwiGLUFeedForward
 from .norm import GroupRMSNorm, JoiningNorm, NormedBranch, RMSNorm, StreamRounding
 from .state_space import StateSpaceMixer
@@ -26,4 +27,5 @@ __all__ = ["BLOCKS", "EMBEDDINGS", "HEADS", "Embedding", "Head", "FEED_FORWARDS"
            "StateSpaceMixer", "SummedEmbedding", "ActivatedFeedForward", "ConvolvedInput", "GatedRecurrenceMixer",
            "MatrixMemoryMixer", "LatentAttention", "ParallelBlock", "DecayedLinearAttention", "GatedLinearRecurrenceMixer",
            "ParallelMixers", "SandwichBlock", "DifferentialAttention", "GELU_TANH", "JoiningNorm", "NormedBranch",
-           "BandedRotaryEncoding", "Int8PagedAttention", "Int8RMSNorm", "Int8SwiGLUFeedForward"]
+           "BandedRotaryEncoding", "Fp8PagedAttention", "Fp8RMSNorm", "Fp8SwiGLUFeedForward", "Int8PagedAttention", "Int8RMSNorm",
+           "Int8SwiGLUFeedForward"]

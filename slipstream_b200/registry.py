@@ -97,7 +97,7 @@ def _register_builtin() -> None:
     from slipstream_b200.config.sazepel_config import SazepelConfig
     from slipstream_b200.models.sazepel import build_sazepel
 
-    register_architecture("Qwen2ForCausalLM", Qwen2Config, build_qwen2, model_types=("qwen2", "qwen"), quantizations=("int8",))
+    register_architecture("Qwen2ForCausalLM", Qwen2Config, build_qwen2, model_types=("qwen2", "qwen"), quantizations=("int8", "fp8"))
     register_architecture("Fokedra", FokedraConfig, build_fokedra)
     register_architecture("Sarudra", SarudraConfig, build_sarudra)
     register_architecture("Bezutar", BezutarConfig, build_bezutar)
