@@ -653,7 +653,8 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     F8PairCounts* counts = reinterpret_cast<F8PairCounts*>(tmem_slot + 2);
     uint32_t* tops = reinterpret_cast<uint32_t*>(full) + 128;                   // [2][128 tokens][2 parts]
-    unsigned char* runs = reinterpret_cast<unsigned char*>(tops + 4 * F8_BM);  // 1 KB for each epilogue warp
+    float* biases = reinterpret_cast<float*>(tops + 4 * F8_BM);                // [2][256] of a tile's features
+    unsigned char* runs = reinterpret_cast<unsigned char*>(biases + 2 * F8_MAX_BN);  // 1 KB for each epilogue warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();  // 0: the leader
@@ -699,12 +700,17 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const int quarter = warp & 3, part = (warp - 4) >> 2;
         unsigned char* stage = runs + (warp - 4) * 1024;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        int slot = 0, turn = 0;
+        int slot = 0, turn = 0, tile = 0;
         uint32_t parity = 0, there = 0;
         bool ok = true;
 #pragma unroll 1
         for (int t = pair; t < n_tiles; t += n_pairs) {
             const int n0 = (t / n_m) * bn, m0 = (t % n_m) * 2 * F8_BM + rank * F8_BM + quarter * 32, m = m0 + lane;
+            ++tile;
+            if (g.bias) {
+                const int c = threadIdx.x - 128;
+                if (c < bn) biases[(tile & 1) * F8_MAX_BN + c] = n0 + c < g.features ? f8_bias(g, n0 + c) : 0.f;
+            }
             float acc[NC][32];
 #pragma unroll
             for (int i = 0; i < NC; ++i)
@@ -768,13 +774,16 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             // (behind a wait that gave up a warp writes nothing but still comes to the barriers, where the others wait for it)
             // (the flag, not the waits' results: an issuer that gave up has committed what is not formed)
             bool formed = !__shfl_sync(0xffffffffu, *gave_up, 0);
-            if (g.bias && formed) {
+            if (g.bias) {
+                // (two sets: a set is written again two tiles later, behind a barrier that all warps reach when they have read it)
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float* bias = biases + (tile & 1) * F8_MAX_BN;
 #pragma unroll
                 for (int i = 0; i < NC; ++i)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int f = n0 + f8_column<NC, GATED>(part, i) + e;
-                        if (f < g.features) acc[i][e] += f8_bias(g, f);
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(bias + f8_column<NC, GATED>(part, i) + e);
+                        acc[i][e] += v.x; acc[i][e + 1] += v.y; acc[i][e + 2] += v.z; acc[i][e + 3] += v.w;
                     }
             }
             const int of0 = GATED ? n0 / 2 : n0;  // first output feature of the tile
@@ -967,7 +976,7 @@ static int launch_many(const Fp8Call& c, Fp8Args& g) {
         return cudaFuncGetAttributes(&a, gemm_fp8_many_kernel<NC, GATED, T, P>) == cudaSuccess ? a.numRegs : 0;
     }();
     if (registers * F8_MANY_THREADS < 128 * 40 + 256 * 232) return -2008;
-    constexpr int rest = F8_SMEM_REST + 2 * 2 * F8_BM * 4 + 8 * 1024, stage = (F8_BM + bn / 2) * F8_BK;
+    constexpr int rest = F8_SMEM_REST + 2 * 2 * F8_BM * 4 + 2 * F8_MAX_BN * 4 + 8 * 1024, stage = (F8_BM + bn / 2) * F8_BK;
     g.stages = (F8_SMEM_MAX - rest) / stage;
     if (g.stages > 12) g.stages = 12;
     g.slot_columns = NC == 1 ? 64 : NC == 2 ? 128 : 256;

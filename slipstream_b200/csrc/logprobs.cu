@@ -40,12 +40,20 @@ __device__ __forceinline__ float next_above(float z) {
     return __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
 }
 
-constexpr float LOG2_E = 1.4426950408889634f;
-// exp(d) for d <= 0, as 2^(d log2 e); results below 2^-126 are 0 (without that, __expf takes four instructions more).
+// exp(d) for -200 <= d <= 0, as 2^u with u = d log2 e rounded; what was lost, d - u ln 2, comes in behind: p (1 + (d - u ln 2)).
+// Without that p is off by up to half a unit of u, 3e-7 at d = -10; so by what ex2.approx is, about 1e-7.  Results below 2^-126 are 0.
+constexpr float LOG2_E = 1.442695041f, LN_2 = 0.6931471806f;
 __device__ __forceinline__ float exp_of(float d) {
     float p;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(d * LOG2_E));
-    return p;
+    const float u = d * LOG2_E;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(u));
+    return fmaf(p, fmaf(u, -LN_2, d), p);
+}
+// max(d, -200), which keeps a NaN: what is masked counts nothing, and products with it are no NaN.
+__device__ __forceinline__ float bounded(float d) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-200.f));
+    return r;
 }
 
 template <typename T>
@@ -119,7 +127,7 @@ constexpr int NOTHING = -1;
 __device__ __forceinline__ void raise_to(Seen& a, float m, int at) {
     if (m > a.m || (a.at == NOTHING && m == m)) {
         if (a.s > 0.f) {
-            const float d = a.m - m, f = __expf(d);
+            const float d = bounded(a.m - m), f = exp_of(d);
             a.t = f * fmaf(a.s, d, a.t);
             a.s *= f;
         }
@@ -128,9 +136,9 @@ __device__ __forceinline__ void raise_to(Seen& a, float m, int at) {
     }
 }
 __device__ __forceinline__ void add(Seen& a, float z, float m) {
-    const float d = z - m, p = exp_of(d);
+    const float d = bounded(z - m), p = exp_of(d);
     a.s += p;
-    a.t = fmaf(p, fmaxf(d, -200.f), a.t);  // (p is 0 below that; a NaN is in s)
+    a.t = fmaf(p, d, a.t);
 }
 // The same for pairs: two sums each, an instruction for two elements but for the exponentials.
 struct Sums {
@@ -146,18 +154,29 @@ __device__ __forceinline__ float sum_of(unsigned long long v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
     return a + b;
 }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void add2(Sums& a, float z0, float z1, unsigned long long minus_m) {
-    unsigned long long d, u, p;
+    unsigned long long d;
     float d0, d1, u0, u1, p0, p1;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(two(z0, z1)), "l"(minus_m));
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(u) : "l"(d), "l"(two(LOG2_E, LOG2_E)));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
+    d = two(bounded(d0), bounded(d1));
+    const unsigned long long u = mul2(d, two(LOG2_E, LOG2_E));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(u0), "=f"(u1) : "l"(u));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(u0));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(u1));
-    p = two(p0, p1);
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.s) : "l"(p));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a.t) : "l"(p), "l"(two(fmaxf(d0, -200.f), fmaxf(d1, -200.f))));
+    const unsigned long long p = two(p0, p1), q = fma2(p, fma2(u, two(-LN_2, -LN_2), d), p);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.s) : "l"(q));
+    a.t = fma2(q, d, a.t);
 }
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -238,21 +257,14 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         for (int u = 1; u < UNROLL; ++u) m = fmaxf(m, x[u].largest());
         raise_to(a, m, row.index(v, 0));
         const float ref = reference(a.m);
-        if constexpr (G == 8) {  // (the instructions are the work: 1,024 x 151,936 88.4 to 82.7 us)
-            const unsigned long long minus = two(-ref, -ref);
-            Sums sums = {0, 0};
+        const unsigned long long minus = two(-ref, -ref);
+        Sums sums = {0, 0};
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-                for (int e = 0; e < G; e += 2) add2(sums, x[u].at(e), x[u].at(e + 1), minus);
-            a.s += sum_of(sums.s);
-            a.t += sum_of(sums.t);
-        } else {
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-                for (int e = 0; e < G; ++e) add(a, x[u].at(e), ref);
-        }
+            for (int e = 0; e < G; e += 2) add2(sums, x[u].at(e), x[u].at(e + 1), minus);
+        a.s += sum_of(sums.s);
+        a.t += sum_of(sums.t);
         if (m >= z_token) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u)
@@ -272,7 +284,7 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
     __syncthreads();
     const float block_m = warp_max(lane < WARPS ? sh.tops[lane] : -INFINITY);
     {
-        const float d = a.m - block_m, f = a.m == -INFINITY ? 0.f : __expf(d);
+        const float d = bounded(a.m - block_m), f = a.m == -INFINITY ? 0.f : exp_of(d);
         double s = (double)(a.s * f), t = a.m == -INFINITY ? s : (double)(f * fmaf(a.s, d, a.t));
         int n = a.ahead;
 #pragma unroll
@@ -411,9 +423,9 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
                 s = __longlong_as_double((long long)remote(&sh.part.s, lane));
                 t = __longlong_as_double((long long)remote(&sh.part.t, lane));
             }
-            const float high = warp_max(m), d = m - high;
+            const float high = warp_max(m), d = bounded(m - high);
             if (d != 0.f) {  // (a NaN too: of two infinities)
-                const double f = m == -INFINITY ? 0. : (double)__expf(d);
+                const double f = m == -INFINITY ? 0. : (double)exp_of(d);
                 t = m == -INFINITY ? s * 0. : f * (t + s * (double)d);
                 s *= f;
             }
