@@ -236,6 +236,12 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t) {
         c.tokens = tokens; c.features = features; c.K = k; c.gated = gated; c.out_features = columns;
         c.many = plan[0]; c.bn = plan[1]; c.slices = plan[2]; c.per_sm = plan[3];
         c.err = error_word(device); c.stream = c10::cuda::getCurrentCUDAStream().stream();
+        at::Tensor parts;  // (a kernel of the same stream that gets this memory next writes behind those that read it here)
+        if (c.many == 1 && c.slices > 1 && c.slices <= 8 && !gated) {
+            parts = empty(c.slices * tokens, (features + 3) & -4, at::kFloat, *x.values);
+            c.parts = (float*)parts.data_ptr();
+            ++launches;
+        }
         check(product_entry(&c), what);
     }
     return to_fp8 ? pair(std::move(rows.values), std::move(rows.scales)) : THPVariable_Wrap(std::move(out));

@@ -46,6 +46,7 @@ struct Fp8Call {
     int64_t tokens, features, K, gated, out_features, many, bn, slices, per_sm;
     int* err;
     cudaStream_t stream;
+    float* parts;  // many, slices > 1: [slices][tokens][features up to a multiple of 4], on 16 bytes
 };
 
 extern "C" {

@@ -37,6 +37,7 @@ struct Fp8Args {
     const void* bias;  // [features] or null
     void* out;         // [tokens][ldc]
     float* out_scale;  // [out_features / 128][tokens] where the output is e4m3
+    float* parts;      // many tokens, K in slices: [slices][tokens][features up to a multiple of 4]
     int* err;
     int64_t ldc;
     int tokens, features, K;
@@ -162,8 +163,8 @@ __device__ __forceinline__ uint32_t f8_remote(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(p)), "r"(rank));
     return remote;
 }
-// Scales on their way to a thread: four bytes from memory to shared memory, without registers, `FLIGHT` blocks of K ahead of their use (one
-// block ahead, in registers, the loop of the epilogue took as long as a load from L2: 0.6 us a block of K at any tile).  A group a
+// Scales on their way to a thread: four bytes from memory to shared memory, without registers, `FLIGHT` blocks of K ahead of their use, so that
+// the loop of the epilogue, which takes about 0.3 us a block of K, does not wait for memory (about 1 us).  A group a
 // block; what a thread sent for is there for itself when all but the last FLIGHT - 1 groups are through, for its warp behind __syncwarp.
 __device__ __forceinline__ void f8_send_for(float* to, const float* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s_addr(to)), "l"(from) : "memory");
@@ -226,6 +227,12 @@ __device__ __forceinline__ void f8_add2(float (&acc)[2], float r0, float r1, flo
 // barrier of its own; the owner adds the slices' sums in their order.  No block waits for another but for these.
 // Warp 0 (one lane) fetches, warp 1 issues the products, warps 2 to 9 are the epilogue: two of them for each quarter of the lanes,
 // half of the columns each (bn / 2, at most C).
+//
+// Bound by the weights' bytes where they are many (8 x 3,584 x 37,888 gated to fp8 rows: 22.5 us, 6.1 TB/s, of which L2 holds a part), else by
+// what a block of K takes, 0.24 us and 3 ns a token column (a look at a barrier alone takes 150 to 290 cycles): 16 x 18,944 x 3,584,
+// in 4 slices of 37 blocks each, 15.9 us for 10.4 of bytes; 1 x 896 x 1,152 4.0.  Two blocks of K a stage and a slot halve
+// the looks (64 x 18,944 x 3,584 25.4 to 22.1 us) but leave no room for the next kernel's block beside this one's ring (16 x 3,584 x 4,608
+// 6.5 to 8.0), so a stage is one block.
 //
 // Registers: an SM's scheduler has 16,384 for its warps.  Three warps of one block (ten in all) may have 168 each; two blocks on an SM
 // 96, which the sums of up to 64 token columns (gated 32) fit into.
@@ -518,7 +525,13 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 // out and add them up; the products of the next tile's first blocks of K run while they write a tile out.
 //   full[s]       in the leader: the bytes of both blocks' copies;      empty[s]      in each block: the products have read the stage
 //   part_full[b]  in each block: the sums of a block of K are formed;   part_empty[b] in the leader: all 16 epilogue warps have them
-
+//
+// Bound by taking the sums out: 256 x 256 outputs x 128 of K take about 0.53 us, the products alone 0.39 (both at 1.9 GHz; the copies
+// keep up).  4,099 x 3,584 x 37,888 gated: 554 to 572 us in a burst, 620 under the power cap, for 330 us at twice the bfloat16 rate;
+// 2,047 x 3,581 x 4,613 to float32 61.  The tensor pipe is busy for 46 % of 2,048 tokens.
+//
+// Few tiles of a long K (256 x 18,944 x 3,584 has 14 of 256 features, and 74 pairs) are cut into slices of K, each a tile of its own whose sums go
+// to memory in float32 (they stay in L2), and a second kernel adds them up in order: 54 us in one slice, 33 in five.
 //
 // Registers: three warps a scheduler are launched with 168 each; the first four warps (producer, issuer, two that do nothing) hand back
 // all but 40 of theirs, and the epilogue's have 232: 128 sums and 64 columns on their way.
@@ -618,10 +631,10 @@ __device__ __forceinline__ void f8_copy_run(const unsigned char* stage, unsigned
 // (row / 2) % 4, which keeps both directions free of bank conflicts.  P: what is written at a time, which the output's rows start on and
 // are a multiple of.
 template <typename T, typename P>
-__device__ __forceinline__ void f8_write_run(const Fp8Args& g, unsigned char* stage, const uint32_t (&w)[16], int m0, int f) {
+__device__ __forceinline__ void f8_write_run(const Fp8Args& g, void* to, unsigned char* stage, const uint32_t (&w)[16], int m0, int f) {
     const int lane = threadIdx.x & 31, row = lane & 15, size = (int)sizeof(T);
     const int64_t pitch = g.ldc * size;
-    unsigned char* out = (unsigned char*)g.out + m0 * pitch + (int64_t)f * size;
+    unsigned char* out = (unsigned char*)to + m0 * pitch + (int64_t)f * size;
     const int rows = g.tokens - m0, limit = min(64, (g.out_features - f) * size);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -636,12 +649,14 @@ __device__ __forceinline__ void f8_write_run(const Fp8Args& g, unsigned char* st
     }
 }
 
-// T: float, bf16, or (gated) uint8_t, e4m3.
-template <int NC, bool GATED, typename T, typename P>
+// T: float, bf16, or (gated) uint8_t, e4m3.  SPLIT: a tile is one of `slices` parts of K, and its sums go to g.parts, [slices][tokens][ldc] in
+// float32, where fp8_join_kernel takes them from.
+template <int NC, bool GATED, typename T, typename P, bool SPLIT>
 __global__ void __launch_bounds__(F8_MANY_THREADS, 1)
 gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Args g) {
     constexpr int bn = 64 * NC, w_rows = bn / 2, x_bytes = F8_BM * F8_BK, stage_bytes = x_bytes + w_rows * F8_BK;  // this block's halves
     static_assert(GATED ? NC == 4 : sizeof(T) > 1, "");
+    static_assert(!SPLIT || (!GATED && sizeof(T) == 4), "");
     const int stages = g.stages, slots = g.slots;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -659,8 +674,13 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();  // 0: the leader
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-    const int n_m = (g.tokens + 2 * F8_BM - 1) / (2 * F8_BM), n_tiles = n_m * ((g.features + bn - 1) / bn);
-    const int k_iters = (g.K + F8_BK - 1) / F8_BK;
+    const int n_m = (g.tokens + 2 * F8_BM - 1) / (2 * F8_BM), n_out = n_m * ((g.features + bn - 1) / bn), n_tiles = SPLIT ? n_out * g.slices : n_out;
+    const int k_blocks = (g.K + F8_BK - 1) / F8_BK, per = SPLIT ? (k_blocks + g.slices - 1) / g.slices : k_blocks;
+    // of tile t: its slice, the tile of the output, its first block of K and how many there are (no slice is empty: launch_many)
+    const auto slice_of = [&](int t) { return SPLIT ? t / n_out : 0; };
+    const auto out_of = [&](int t) { return SPLIT ? t % n_out : t; };
+    const auto blocks_of = [&](int t) { return SPLIT ? min(per, k_blocks - slice_of(t) * per) : k_blocks; };
+    const int first_k = slice_of(pair) * per;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -671,14 +691,14 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // both blocks' barriers exist before either signals the other's
-    const int first = min(stages, pair < n_tiles ? k_iters : 0);  // stages of the first tile that are fetched ahead
+    const int first = min(stages, pair < n_tiles ? blocks_of(pair) : 0);  // stages of the first tile that are fetched ahead
     const int bytes = 2 * stage_bytes;  // of both blocks
     if (threadIdx.x == 0) {
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
 #pragma unroll 1
         for (int k = 0; k < first; ++k) {
             if (rank == 0) mbar_expect_tx(&full[k], bytes);
-            f8_load_pair(tiles + k * stage_bytes + x_bytes, &map_w, k * F8_BK, (pair / n_m) * bn + rank * w_rows, &full[k]);
+            f8_load_pair(tiles + k * stage_bytes + x_bytes, &map_w, (first_k + k) * F8_BK, (out_of(pair) / n_m) * bn + rank * w_rows, &full[k]);
         }
     }
     pdl_wait();
@@ -688,7 +708,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         pdl_launch_dependents();  // (this warp alone: one call of a block lets the kernel behind go)
     } else if (threadIdx.x == 0) {
 #pragma unroll 1
-        for (int k = 0; k < first; ++k) f8_load_pair(tiles + k * stage_bytes, &map_x, k * F8_BK, (pair % n_m) * 2 * F8_BM + rank * F8_BM, &full[k]);
+        for (int k = 0; k < first; ++k) f8_load_pair(tiles + k * stage_bytes, &map_x, (first_k + k) * F8_BK, (out_of(pair) % n_m) * 2 * F8_BM + rank * F8_BM, &full[k]);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();  // the tensor memory of both blocks has been taken
@@ -705,7 +725,9 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         bool ok = true;
 #pragma unroll 1
         for (int t = pair; t < n_tiles; t += n_pairs) {
-            const int n0 = (t / n_m) * bn, m0 = (t % n_m) * 2 * F8_BM + rank * F8_BM + quarter * 32, m = m0 + lane;
+            const int n0 = (out_of(t) / n_m) * bn, m0 = (out_of(t) % n_m) * 2 * F8_BM + rank * F8_BM + quarter * 32, m = m0 + lane;
+            const int k_iters = blocks_of(t);
+            const int64_t k0 = slice_of(t) * per;
             ++tile;
             if (g.bias) {
                 const int c = threadIdx.x - 128;
@@ -719,12 +741,12 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             // the scales of a block of K: the token's, and those of the chunks' features (no chunk lies in two blocks;
             // a part's chunks lie in one, gated in two)
             constexpr int NW = GATED ? 2 : 1, PER = NC / NW;
-            // Fetched F8_FLIGHT blocks ahead, into registers: one block ahead, the loop took as long as a load from L2.
-            const float* xs = g.x_scale + (int64_t)min(m, g.tokens - 1) * g.x_row;  // (rows behind the last token are not written)
+            // Fetched F8_FLIGHT blocks ahead, into registers: a block of K takes about 0.5 us, a load from memory about 1.
+            const float* xs = g.x_scale + (int64_t)min(m, g.tokens - 1) * g.x_row + k0 * g.x_block;  // (rows behind the last token are not written)
             const float* ws[NW];
 #pragma unroll
             for (int i = 0; i < NW; ++i)
-                ws[i] = g.w_scale + (int64_t)min((n0 + f8_column<NC, GATED>(part, i * PER)) / FP8_BLOCK, (g.features - 1) / FP8_BLOCK) * g.w_row;
+                ws[i] = g.w_scale + (int64_t)min((n0 + f8_column<NC, GATED>(part, i * PER)) / FP8_BLOCK, (g.features - 1) / FP8_BLOCK) * g.w_row + k0 * g.w_block;
             float next_x[F8_FLIGHT], next_w[F8_FLIGHT][NW];
             int fetched = 0;
             const auto fetch_scales = [&](int u) {
@@ -831,6 +853,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 }
             } else {
                 if (!formed) continue;
+                void* to = SPLIT ? (void*)(g.parts + (int64_t)slice_of(t) * g.tokens * g.ldc) : g.out;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) {
                     const int f = of0 + f8_column<NC, GATED>(part, i);
@@ -840,7 +863,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                         for (int h = 0; h < 2; ++h) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(acc[i][16 * h + e]);
-                            f8_write_run<T, P>(g, stage, w, m0, f + 16 * h);
+                            f8_write_run<T, P>(g, to, stage, w, m0, f + 16 * h);
                         }
                     } else {
 #pragma unroll
@@ -848,7 +871,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                             const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i][2 * e], acc[i][2 * e + 1]);
                             w[e] = *reinterpret_cast<const uint32_t*>(&v);
                         }
-                        f8_write_run<T, P>(g, stage, w, m0, f);
+                        f8_write_run<T, P>(g, to, stage, w, m0, f);
                     }
                 }
             }
@@ -864,14 +887,15 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             bool ok = true;
 #pragma unroll 1
             for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-                const int row = x ? (t % n_m) * 2 * F8_BM + rank * F8_BM : (t / n_m) * bn + rank * w_rows;
+                const int row = x ? (out_of(t) % n_m) * 2 * F8_BM + rank * F8_BM : (out_of(t) / n_m) * bn + rank * w_rows;
+                const int k0 = slice_of(t) * per, k_iters = blocks_of(t);
 #pragma unroll 1
                 for (int k = 0; k < k_iters; ++k, ++it) {
                     if (it >= first) {
                         if (!f8_wait(&empty[s], parity, gave_up)) { ok = false; break; }
                         if (elect_one()) {
                             if (x && rank == 0) mbar_expect_tx(&full[s], bytes);
-                            f8_load_pair(to + s * stage_bytes, map, k * F8_BK, row, &full[s]);
+                            f8_load_pair(to + s * stage_bytes, map, (k0 + k) * F8_BK, row, &full[s]);
                         }
                         __syncwarp();
                     }
@@ -887,6 +911,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             bool ok = true;
 #pragma unroll 1
             for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+                const int k_iters = blocks_of(t);
 #pragma unroll 1
                 for (int k = 0; k < k_iters; ++k, ++it) {
                     if (!f8_wait(&full[s], parity, &part_empty[slot], free_parity, gave_up)) { ok = false; break; }
@@ -918,6 +943,39 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
+}
+
+// The parts of K put together: y = sum over the slices, in their order, + bias, rounded once; a warp takes 128 features of a token, a lane
+// four of them.  Where a wait of the product gave up, not all parts are formed (the error word says so), and nothing is written.
+__global__ void __launch_bounds__(256) fp8_join_kernel(const Fp8Args g, int64_t ldp, int64_t units) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= units || (*(volatile int*)g.err & SS_ERR_WAIT_LIMIT)) return;
+    const int lane = threadIdx.x & 31, across = (g.features + 127) / 128, token = (int)(unit / across);
+    const int apart = (g.ldc & 3) == 0 ? 1 : 32, f = (int)(unit % across) * 128 + (apart == 1 ? lane * 4 : lane);
+    if (f >= g.features) return;
+    const int64_t plane = g.tokens * ldp;
+    const float* p = g.parts + token * ldp + f;
+    float v[4] = {};
+    if (apart == 1) {  // (rows of the parts are as long as four elements times some number: those behind the last belong to nobody)
+#pragma unroll 4
+        for (int s = 0; s < g.slices; ++s) {
+            const float4 t = *reinterpret_cast<const float4*>(p + s * plane);
+            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+        }
+    } else {
+        for (int s = 0; s < g.slices; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (f + 32 * e < g.features) v[e] += p[s * plane + 32 * e];
+    }
+    if (g.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (f + e * apart < g.features) v[e] += f8_bias(g, f + e * apart);
+    }
+    f8_store4(g, token, f, apart, v);
 }
 
 // ---------------------------------------------------------------- host side
@@ -962,18 +1020,18 @@ extern "C" int ss_gemm_fp8_resident(int n, int per_sm) {
     return ss_resident_clusters(f8_few_shape, F8_THREADS, per_sm > 1 ? F8_SMEM_SM / per_sm - 1024 : F8_SMEM_MAX, n);
 }
 
-template <int NC, bool GATED, typename T, typename P>
+template <int NC, bool GATED, typename T, typename P, bool SPLIT = false>
 static int launch_many(const Fp8Call& c, Fp8Args& g) {
     CUtensorMap map_x, map_w;
     constexpr int bn = 64 * NC;
     if (int rc = f8_map(&map_x, c.x, g.tokens, g.K, c.ldx, F8_BM)) return rc;
     if (int rc = f8_map(&map_w, c.w, g.features, g.K, c.ldw, bn / 2)) return rc;
     static SsPerDevice opted;
-    if (int rc = ss_opt_in_smem(gemm_fp8_many_kernel<NC, GATED, T, P>, F8_SMEM_MAX, opted)) return rc;
+    if (int rc = ss_opt_in_smem(gemm_fp8_many_kernel<NC, GATED, T, P, SPLIT>, F8_SMEM_MAX, opted)) return rc;
     // what the warps take of the registers is what the block is launched with: a build with fewer would wait for the rest
     static const int registers = [] {
         cudaFuncAttributes a;
-        return cudaFuncGetAttributes(&a, gemm_fp8_many_kernel<NC, GATED, T, P>) == cudaSuccess ? a.numRegs : 0;
+        return cudaFuncGetAttributes(&a, gemm_fp8_many_kernel<NC, GATED, T, P, SPLIT>) == cudaSuccess ? a.numRegs : 0;
     }();
     if (registers * F8_MANY_THREADS < 128 * 40 + 256 * 232) return -2008;
     constexpr int rest = F8_SMEM_REST + 2 * 2 * F8_BM * 4 + 2 * F8_MAX_BN * 4 + 8 * 1024, stage = (F8_BM + bn / 2) * F8_BK;
@@ -981,10 +1039,24 @@ static int launch_many(const Fp8Call& c, Fp8Args& g) {
     if (g.stages > 12) g.stages = 12;
     g.slot_columns = NC == 1 ? 64 : NC == 2 ? 128 : 256;
     g.slots = 512 / g.slot_columns;
-    const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + bn - 1) / bn);
+    const int64_t n_tiles = (int64_t)((g.tokens + 255) / 256) * ((g.features + bn - 1) / bn) * (SPLIT ? g.slices : 1);
     if (n_tiles > INT32_MAX / 2) return -2003;
     const int pairs = (int)(n_tiles < ss_sm_count() / 2 ? n_tiles : ss_sm_count() / 2);
-    ss_launch_cluster_x(gemm_fp8_many_kernel<NC, GATED, T, P>, dim3(2 * pairs), dim3(F8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
+    ss_launch_cluster_x(gemm_fp8_many_kernel<NC, GATED, T, P, SPLIT>, dim3(2 * pairs), dim3(F8_MANY_THREADS), g.stages * stage + rest, c.stream, 2, map_x, map_w, g);
+    return SS_LAUNCH_CHECK();
+}
+
+// K in slices: the product to g.parts, then what puts the parts together.
+template <int NC>
+static int launch_many_split(const Fp8Call& c, Fp8Args& g) {
+    const int k_blocks = (g.K + F8_BK - 1) / F8_BK, per = (k_blocks + g.slices - 1) / g.slices;
+    g.slices = (k_blocks + per - 1) / per;  // that have any K
+    const int64_t ldp = ((int64_t)g.features + 3) & -4, units = (int64_t)g.tokens * ((g.features + 127) / 128), blocks = (units + 7) / 8;
+    if (blocks > INT32_MAX) return -2003;
+    Fp8Args product = g;
+    product.bias = nullptr; product.out = g.parts; product.ldc = ldp; product.out_type = SS_F32; product.out_features = (int)ldp;
+    if (int rc = launch_many<NC, false, float, uint4, true>(c, product)) return rc;
+    ss_launch(fp8_join_kernel, dim3((unsigned)blocks), dim3(256), 0, c.stream, g, ldp, units);
     return SS_LAUNCH_CHECK();
 }
 
@@ -1030,7 +1102,7 @@ static int launch_few(const Fp8Call& c, Fp8Args& g, int per_sm) {
 // gated: w's rows alternate 128 gate and 128 up features; out_features <= features / 2 columns of silu(gate) * up are written.
 // many = 0: bn tokens a tile (a multiple of 16 up to 256, gated 128), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for
 // (2: bn up to 64, gated 32).
-// many = 1: bn features a tile (64, 128 or 256; gated: 256).
+// many = 1: bn features a tile (64, 128 or 256; gated: 256); not gated, of 128 or 256 features: slices 1..8 of K, with `parts` from 2 on.
 extern "C" int ss_gemm_fp8(const Fp8Call* call) {
     const Fp8Call& c = *call;
     if (c.tokens <= 0 || c.features <= 0 || c.out_features <= 0) return 0;
@@ -1040,15 +1112,17 @@ extern "C" int ss_gemm_fp8(const Fp8Call* call) {
     if (c.out_type == F8_OUT_FP8 && c.ldc % 16) return -2005;
     const int bn = (int)c.bn, slices = (int)c.slices, per_sm = (int)c.per_sm;
     if (bn < 16 || bn > F8_MAX_BN || (c.many ? bn != 64 && bn != 128 && bn != 256 : bn % 16) || (c.many && c.gated && bn != 256)
+        || (c.many && (slices < 1 || slices > 8 || (slices > 1 && (c.gated || bn == 64 || !c.parts || ((uintptr_t)c.parts & 15)))))
         || (!c.many && (bn > (c.gated ? 128 : 256) / (per_sm > 1 ? 4 : 1) || slices < 1 || slices > 8 || per_sm < 1 || per_sm > 2
                         || (c.features + F8_BM - 1) / F8_BM > 65535))) return -2006;
     Fp8Args g = {};
     g.x_scale = c.x_scale; g.x_row = c.x_row; g.x_block = c.x_block; g.w_scale = c.w_scale; g.w_row = c.w_row; g.w_block = c.w_block;
-    g.bias = c.bias; g.out = c.out; g.out_scale = c.out_scale; g.err = c.err; g.ldc = c.ldc;
+    g.parts = c.parts; g.bias = c.bias; g.out = c.out; g.out_scale = c.out_scale; g.err = c.err; g.ldc = c.ldc;
     g.tokens = (int)c.tokens; g.features = (int)c.features; g.K = (int)c.K; g.out_features = (int)c.out_features;
     g.out_type = (int)c.out_type; g.bias_f32 = (int)c.bias_f32; g.bn = bn; g.slices = slices;
     if (c.many) {
         if (c.gated) return launch_many_as<4, true>(c, g);
+        if (slices > 1) return bn == 128 ? launch_many_split<2>(c, g) : launch_many_split<4>(c, g);
         return bn == 64 ? launch_many_as<1, false>(c, g) : bn == 128 ? launch_many_as<2, false>(c, g) : launch_many_as<4, false>(c, g);
     }
     if (c.gated)

@@ -118,8 +118,12 @@ __device__ __forceinline__ Place place_of(int i, int groups) {  // the i-th grou
 //
 // A lane takes 16 bytes of a row: a block of 128 is 32 lanes of float32 or 16 of bfloat16, whose largest magnitude is found by
 // shuffles.  A block of threads takes 32 vectors (128 or 256 columns) of each of 32 rows, a warp four rows, all loaded before the first is
-// written; neighbouring blocks take neighbours of the same rows.  The scales of 32 rows stand side by side in memory and are written so
-// (each by the warp that formed it, one at a time: 4,096 x 3,584 18.6 us).
+// written; neighbouring blocks take neighbours of the same rows.  The scales of 32 rows stand side by side in memory and are written so.
+//
+// Bound by instructions as much as by memory: 16 bytes in are 16 values or 8 to take apart, compare, multiply, round and pack.  The largest
+// magnitude of bfloat16 pairs at a time, one division a lane (for the group that it leads) and four rows a warp in flight took 4,096 x 3,584
+// from 18.8 to 11.5 us (6.7 us of bytes; the issue slots are 65 % busy), 2,048 x 18,944 to 25.6 (17.8), 1,531 x 2,051 in float32 from rows that
+// start anywhere to 6.4 (2.4).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS)
 quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
@@ -171,7 +175,7 @@ quantize_rows_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_
 // ---------------------------------------------------------------- weights to fp8
 //
 // A block of threads per 128 x 128 elements, which stay in registers.  Neighbouring blocks take neighbours of the same rows, so that the
-// pieces of a row in memory are read at the same time.
+// pieces of a row in memory are read at the same time.  Bound by memory: 18,944 x 3,584 bfloat16 35.4 us, 5.8 TB/s.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 4 : 3)
 quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scales, int64_t scale_row,
@@ -213,6 +217,8 @@ quantize_blocks_kernel(const T* x, int64_t stride, uint8_t* __restrict__ q, int6
 // 128 (four elements a lane), writes its q at once, and only the scales wait for the row's sum of squares.
 // The squares' sum does not depend on how many rows there are, whatever shape the launch takes for them: a block's sum (a warp's) is
 // formed first, then lane l adds the sums of blocks l, l + 32, ... of the row, then the lanes.
+// Bound by memory, 11 bytes an element with a bfloat16 delta: 4,096 x 3,584 32.0 us (5.1 TB/s; the issue slots are 56 % busy), 4,096 x 8,192 69.5
+// (5.3); few rows by the chain of load, sum, barrier, store: 8 x 3,584 2.2 us.
 __device__ __forceinline__ float squares_of(const float (&v)[4]) {
     return fmaf(v[3], v[3], fmaf(v[2], v[2], fmaf(v[1], v[1], v[0] * v[0])));
 }
@@ -434,7 +440,8 @@ add_rmsnorm_fp8_ring_kernel(const float* residual, const T* delta, float* residu
 //
 // y = q * s, rounded once.  A lane takes eight (bfloat16) or four (float32) elements, side by side where the output's rows start on 16
 // bytes, else 32 apart, so that a warp writes whole pieces of a row either way (1,531 x 2,051 to bfloat16, side by side and one by one:
-// 22.4 us).  Groups are dealt out as in the way there.
+// 22.4 us for 7.9).  Groups are dealt out as in the way there.  Bound by memory: 4,096 x 3,584 to bfloat16 8.4 us (5.2 TB/s), a weight of 18,944 x 3,584
+// 33.0 (6.2).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(ROW_THREADS)
 dequantize_kernel(const uint8_t* q, int64_t q_stride, const float* scales, int64_t scale_row, int64_t scale_block, T* __restrict__ y, int64_t rows,

@@ -136,12 +136,13 @@ def add_rmsnorm_fp8(residual: torch.Tensor, delta: torch.Tensor | None, weight: 
 def fp8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
              resident: tuple[tuple[int, ...], tuple[int, ...]] | None = None) -> tuple[int, int, int, int]:
     """(many, tile, K slices, blocks an SM) of ``x[tokens, k] @ w[features, k].T``: which of the two kernels, the width of its tile
-    (tokens of the first, features of the second), and for the first the slices of K and how many blocks an SM the ring is sized for.
+    (tokens of the first, features of the second), the slices of K, and for the first how many blocks an SM the ring is sized for.
     ``resident``: clusters of 1 to 8 blocks that run at the same time, with the ring sized for one block an SM and for two.
 
     The choice is the cheapest by an estimate in microseconds whose constants are fitted to 2,772 measured products (1 to 512 tokens, the
     projections of the 0.5B, 1.5B and 7B layer sizes, tiles, slices and rings of all sizes): on average 3 % slower than the fastest of
-    them at the same sizes, and at worst 14 %."""
+    them at the same sizes, and at worst 14 %; those of the second kernel with K in slices to 564 more (256 x 18,944 x 3,584: 54 us in
+    one slice, 33 in five)."""
     # what follows depends on the tokens in steps of 16 (their tiles) up to 640 and of 256 beyond: few plans for many counts
     step = 16 if tokens <= 640 else 256
     return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
@@ -198,10 +199,15 @@ def _plan(tokens: int, features: int, k: int, sms: int, gated: bool, resident) -
         for tile in ((256,) if gated else (64, 128, 256)):
             tiles = rows * ((features + tile - 1) // tile)
             pairs = max(1, sms // 2)
-            rounds = (tiles + pairs - 1) // pairs
-            cost = 3.89 + rounds * (blocks * (0.204 + 0.000926 * tile) + 0.138 + 0.0123 * tile)
-            if best is None or cost < best[0]:
-                best = (cost, (1, tile, 1, 1))
+            for slices in (1,) if gated or tile == 64 else range(1, max(1, min(8, blocks // 2)) + 1):
+                if slices > 1 and tiles * slices > 2 * pairs:
+                    break
+                rounds = (tiles * slices + pairs - 1) // pairs
+                cost = 3.89 + rounds * ((blocks + slices - 1) // slices * (0.204 + 0.000926 * tile) + 0.138 + 0.0123 * tile)
+                if slices > 1:  # another launch, the parts written and read again
+                    cost += 3.19 + (0.226 * slices + 0.507) * tokens * features * 4e-6
+                if best is None or cost < best[0]:
+                    best = (cost, (1, tile, slices, 1))
     return best[1]
 
 

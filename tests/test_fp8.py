@@ -19,6 +19,7 @@ def test_plans_are_forms_that_the_kernels_have(sms, resident):
                 many, tile, slices, per = fp8_plan(tokens, features, k, sms, gated, resident)
                 if many:
                     assert tile in (64, 128, 256) and tokens > 32 and (not gated or tile == 256)
+                    assert slices == 1 or (not gated and tile > 64 and 2 <= slices <= min(8, -(-k // 256)) and per == 1)
                 else:
                     assert tile % 16 == 0 and 16 <= tile <= 256 // parts and 1 <= slices <= min(8, -(-k // 128)) and tokens <= 640
                     assert per == 1 or (per == 2 and tile <= 64 // parts)

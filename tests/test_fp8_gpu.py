@@ -236,6 +236,8 @@ def plans(tokens, k, gated):
             for per in (1, 2) if tile <= (32 if gated else 64) else (1,):
                 if slices <= blocks_of(k):
                     out.append((0, tile, slices, per))
+    if not gated:
+        out += [(1, tile, slices, 1) for tile in (128, 256) for slices in (2, 3, 8)]
     return out + [(1, tile, 1, 1) for tile in ((256,) if gated else (64, 128, 256))]
 
 
@@ -288,6 +290,33 @@ def test_linear_twice_gives_the_same_bits():
         first = o.linear_fp8(x, w, None, F32)
         for _ in range(5):
             assert torch.equal(o.linear_fp8(x, w, None, F32), first)
+
+
+def test_products_in_slices_in_graphs_and_on_two_streams():
+    """The parts of K stand in memory of the call's own: two calls at once, and a graph's replays beside calls outside of it, keep to theirs."""
+    o, g = ops(), gen(31)
+    plan = (1, 128, 4, 1)
+    calls = [(fp8_rows(g, 200 + 56 * i, 2000, turned=True), fp8_blocks(g, 900, 2000), normal(g, 900)) for i in range(3)]
+    expected = [o.linear_fp8(x, w, b, BF16, plan=plan) for x, w, b in calls]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [o.linear_fp8(x, w, b, BF16, plan=plan) for x, w, b in calls]
+        graphs.append((graph, outs))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        for stream, (graph, outs) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                again = [o.linear_fp8(x, w, b, BF16, plan=plan) for x, w, b in calls]
+                for out, other in zip(outs, again):
+                    out.copy_(torch.where(out == other, out, torch.nan))
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(outs, expected))
+    o.check_errors(torch.device(DEV))
 
 
 def test_linear_blocks_meet_their_scales():
@@ -531,7 +560,7 @@ def test_two_blocks_share_an_sm_where_the_plan_says_so():
 
 
 @pytest.mark.parametrize("plan", [[0, 16, 1, 1], (0, 16, 1), (0, 16, 1, 1, 1), (0, 16.0, 1, 1), (0, 2 ** 32 + 16, 1, 1), (0, 16, 2 ** 70, 1), (0, -16, 1, 1),
-                                  (-1, 64, 1, 1), 16, "0111", (0, 24, 1, 1), (0, 16, 9, 1), (0, 16, 0, 1), (0, 16, 1, 3), (0, 272, 1, 1), (0, 80, 1, 2), (1, 32, 1, 1), (1, 192, 1, 1), (1, 320, 1, 1)])
+                                  (-1, 64, 1, 1), 16, "0111", (0, 24, 1, 1), (0, 16, 9, 1), (0, 16, 0, 1), (0, 16, 1, 3), (0, 272, 1, 1), (0, 80, 1, 2), (1, 64, 2, 1), (1, 128, 0, 1), (1, 256, 9, 1), (1, 32, 1, 1), (1, 192, 1, 1), (1, 320, 1, 1)])
 def test_plans_that_are_none(plan):
     o = ops()
     rows, w = o.quantize_rows_fp8(torch.ones(4, 64, device=DEV)), o.quantize_blocks_fp8(torch.ones(256, 64, device=DEV))
@@ -612,7 +641,7 @@ def test_refusals():
                  lambda: o.linear_fp8(good, w, torch.zeros(256, device=DEV).half()), lambda: o.linear_fp8(good, w, None, torch.float16), lambda: o.linear_fp8(good, w, None, E4M3),
                  lambda: o.gate_up_swiglu_fp8(good, o.quantize_blocks_fp8(torch.ones(128, 64, device=DEV))), lambda: o.gate_up_swiglu_fp8(good, w, features=129),
                  lambda: o.gate_up_swiglu_fp8(good, w, features=-1), lambda: o.gate_up_swiglu_fp8(good, w, None, torch.float8_e5m2), lambda: o.stack_gate_up_fp8(x, x[:2]),
-                 lambda: o.gate_up_swiglu_fp8(good, w, plan=(1, 128, 1, 1)), lambda: o.gate_up_swiglu_fp8(good, w, plan=(0, 144, 1, 1))):
+                 lambda: o.gate_up_swiglu_fp8(good, w, plan=(1, 128, 1, 1)), lambda: o.gate_up_swiglu_fp8(good, w, plan=(1, 256, 2, 1)), lambda: o.gate_up_swiglu_fp8(good, w, plan=(0, 144, 1, 1))):
         with pytest.raises(err):
             call()
     none = o.quantize_rows_fp8(torch.empty(0, 64, device=DEV))

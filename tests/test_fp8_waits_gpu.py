@@ -26,7 +26,7 @@ class ProductCall(ctypes.Structure):  # Fp8Call
                 ("w_scale", c_void_p), ("w_row", c_int64), ("w_block", c_int64), ("bias", c_void_p), ("bias_f32", c_int64), ("out", c_void_p), ("ldc", c_int64),
                 ("out_type", c_int64), ("out_scale", c_void_p)]
     _fields_ += [(name, c_int64) for name in ("tokens", "features", "K", "gated", "out_features", "many", "bn", "slices", "per_sm")]
-    _fields_ += [("err", c_void_p), ("stream", c_void_p)]
+    _fields_ += [("err", c_void_p), ("stream", c_void_p), ("parts", c_void_p)]
 
 
 @pytest.fixture(scope="module")
@@ -83,10 +83,11 @@ def gives_up(library, tokens, k, features, plan, gated, dtype):
     out_scale = torch.full((-(-columns // 128), tokens), 7.0, device=DEV)
     bias = torch.ones(features, device=DEV)
     many, bn, slices, per_sm = plan
+    parts = torch.empty(slices, tokens, (features + 3) & -4, device=DEV)
     call = ProductCall(x=x.values.data_ptr(), ldx=x.values.stride(0), x_scale=x.scales.data_ptr(), x_row=1, x_block=tokens, w=w.values.data_ptr(),
                        ldw=w.values.stride(0), w_scale=w.scales.data_ptr(), w_row=blocks, w_block=1, bias=bias.data_ptr(), bias_f32=1, out=out.data_ptr(), ldc=pitch,
                        out_type={F32: 0, BF16: 1, E4M3: 2}[dtype], out_scale=out_scale.data_ptr(), tokens=tokens, features=features, K=k, gated=int(gated),
-                       out_features=columns, many=many, bn=bn, slices=slices, per_sm=per_sm)
+                       out_features=columns, many=many, bn=bn, slices=slices, per_sm=per_sm, parts=parts.data_ptr())
     assert ran(library.ss_gemm_fp8, call) == WAIT_LIMIT
     assert (out == 7).all() and (out_scale == 7).all()
     got = ops.gate_up_swiglu_fp8(x, w, bias, dtype, plan=plan) if gated else ops.linear_fp8(x, w, bias, dtype, plan=plan)
@@ -102,6 +103,12 @@ TYPES = [(False, F32), (False, BF16), (True, F32), (True, BF16), (True, E4M3)]
                                              (16, 3584, (0, 16, 4, 2)), (33, 896, (0, 48, 2, 1)), (95, 18944, (0, 96, 5, 1)), (60, 1100, (0, 32, 8, 1))])
 def test_products_of_few_tokens(library, tokens, k, plan, gated, dtype):
     gives_up(library, tokens, k, 1280, plan, gated, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens, k, features, plan", [(256, 18944, 3584, (1, 256, 5, 1)), (100, 300, 1279, (1, 128, 2, 1)), (700, 2000, 5000, (1, 128, 8, 1))])
+def test_products_of_many_tokens_in_slices(library, tokens, k, features, plan, dtype):
+    gives_up(library, tokens, k, features, plan, False, dtype)
 
 
 @pytest.mark.parametrize("gated, dtype", TYPES)
