@@ -14,8 +14,8 @@
 // Bound by memory: a row is read once (and about 5 % of it again for k = 20).  A row has a block of 512 threads, or, where rows are few, a
 // thread-block cluster of up to 8, which put their results together through shared memory.
 // 1,024 rows of 151,936 in float32: 109 us (5.7 TB/s) without alternatives, 134 with 20 (a block loads nothing while
-// it chooses them); in bfloat16 101 us with 20 for 48 of bytes: an exponential, four multiply-adds and two comparisons an
-// element, the issue slots 59 % busy.  One row 5.7 us, with 5 alternatives 9.7: launch, the pass of 8 blocks, the join, the choice.
+// it chooses them; the issue slots are 59 % busy); in bfloat16 101 us with 20 for 48 of bytes, bound by the instructions: an exponential,
+// four multiply-adds and two comparisons an element.  One row 5.7 us, with 5 alternatives 9.7: launch, the pass of 8 blocks, the join, the choice.
 
 #include "common.cuh"
 #include "logprob_calls.h"
