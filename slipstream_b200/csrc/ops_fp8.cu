@@ -559,7 +559,7 @@ inline RingShape ring_shape(const Fp8RowsCall& c) {
     const int64_t bytes = c.width * (4 + (!c.delta ? 0 : c.dtype == SS_BF16 ? 2 : 4));
     if (bytes < 16384 || c.width > 12 * 4 * RING_THREADS || bytes % 16 || (c.delta && c.width * 2 % 16)) return {0, 0};
     for (int blocks = ring_blocks(ring_groups((int)c.width)); blocks >= 2; --blocks) {
-        const int64_t stages = (220 * 1024 / blocks - 3072) / (bytes + 8);
+        const int64_t stages = (220 * 1024 / blocks - 3 * 1024) / (bytes + 8);
         if (stages >= blocks && c.rows >= 4 * (int64_t)blocks * ss_sm_count()) return {blocks, (int)stages};
     }
     return {0, 0};

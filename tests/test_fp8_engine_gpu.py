@@ -97,7 +97,7 @@ def test_logits_are_those_of_the_plain_decoder_that_rounds_alike(model_folders, 
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_steps_replayed_from_graphs_give_the_same_bits(model_folders, dtype):
+def test_steps_replayed_from_graphs(model_folders, dtype):
     """Decode steps and steps with prompt portions, captured (padded to their buckets) and kernel by kernel, with the same plans."""
     from slipstream_b200.engine.runner import ModelRunner
 
