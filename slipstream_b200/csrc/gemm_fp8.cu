@@ -158,6 +158,10 @@ __device__ __forceinline__ void f8_store4(const Fp8Args& g, int token, int f, in
 __device__ __forceinline__ void f8_send(uint32_t to, uint32_t bar, float v) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v), "r"(bar) : "memory");
 }
+// v or-ed into the word at `to`, alike
+__device__ __forceinline__ void f8_send_flag(uint32_t to, uint32_t bar, uint32_t v) {
+    asm volatile("red.async.relaxed.cluster.shared::cluster.mbarrier::complete_tx::bytes.or.b32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar) : "memory");
+}
 __device__ __forceinline__ uint32_t f8_remote(const void* p, uint32_t rank) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(s_addr(p)), "r"(rank));
@@ -257,6 +261,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint64_t* sums_ready = part_empty + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_ready + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* unformed = gave_up + 1;  // of the cluster's sums that were sent here some are not formed
     float* factors = reinterpret_cast<float*>(full) + 128;  // of the eight warps, behind the barriers
     // [senders][own columns][FL]: of a cluster's block behind the factors; alone ([columns][FL]) over the ring, when all its stages have been used
     float* sums = n_sl > 1 ? factors + 8 * f8_few_floats(MT, C) : reinterpret_cast<float*>(tiles);
@@ -278,10 +283,10 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < slots; ++s) { mbar_init(&part_full[s], 1); mbar_init(&part_empty[s], 8); }
         mbar_init(sums_ready, 1);
-        *gave_up = 0;
+        *gave_up = *unformed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (n_sl > 1) mbar_expect_tx(sums_ready, (uint32_t)(senders * mine * FL * 4));
+        if (n_sl > 1) mbar_expect_tx(sums_ready, (uint32_t)(senders * (mine * FL + 8) * 4));  // (and a flag of each warp)
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
         const uint64_t once = l2_evict_first_policy();
         for (int it = 0; it < ahead; ++it) {
@@ -453,7 +458,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         } else {
             if (k_iters > 0) {
                 // a warp that gave up sends what it has: the bytes that the owners count always arrive, so that none of them leaves with
-                // sums on their way to it (what they write is wrong then; the error word says so)
+                // sums on their way to it; its flag, which they count too, tells them to write none of it
                 const int some = live / n_sl, more = live % n_sl;  // block r owns some (+ 1 where r < more) columns
                 int owner = c0 % n_sl, at = c0 / n_sl;             // of column c: block c % slices, its column c / slices
 #pragma unroll
@@ -465,9 +470,10 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                         for (int m = 0; m < MT; ++m) f8_send(to + m * F8_BM * 4, bar, acc[m][c]);
                         if (++owner == n_sl) { owner = 0; ++at; }
                     }
+                if (lane < n_sl) f8_send_flag(f8_remote((const void*)unformed, lane), f8_remote(sums_ready, lane), !ok);
             }
             if (!mbar_wait(sums_ready, 0, gave_up)) mbar_drain(sums_ready, 0);
-            ok = !*gave_up;
+            ok = !*gave_up && !*unformed;
         }
         // a warp takes a token column at a time, a lane four features (gated: pairs) of it
         const int n_sum = n_sl > 1 ? senders : 1;

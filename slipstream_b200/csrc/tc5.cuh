@@ -4,7 +4,11 @@
 #include "common.cuh"
 
 #define WAIT_LIMIT (1u << 20)
-// Polls after which a wait gives up.  A build may set 0: every wait gives up at once, which shows what a kernel does then.
+// Polls after which a wait gives up.  A build may set 0: every wait gives up at once, which shows what a kernel does then.  With
+// SOME_WAITS_GIVE_UP only those of some blocks do: of a second block along z (a second slice of K), and of blocks 2 and 3 along x (a pair).
+#ifdef SOME_WAITS_GIVE_UP
+#define WAIT_POLLS (blockIdx.z == 1 || blockIdx.x >> 1 == 1 ? 0u : WAIT_LIMIT)
+#endif
 #ifndef WAIT_POLLS
 #define WAIT_POLLS WAIT_LIMIT
 #endif
