@@ -178,6 +178,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     uint64_t* sums_ready = acc_ready + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_ready + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* unformed = gave_up + 1;  // of the cluster's sums that were added here some are not formed
     float* xs_s = reinterpret_cast<float*>(full) + 64;  // [256], behind the barriers
     // [own columns][128]: of a cluster's block behind the scales; alone over the ring, when all its stages have been used
     int* sums = n_sl > 1 ? reinterpret_cast<int*>(xs_s + I8_MAX_BN) : reinterpret_cast<int*>(tiles);
@@ -199,10 +200,10 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(acc_ready, 1);
         mbar_init(sums_ready, 1);
-        *gave_up = 0;
+        *gave_up = *unformed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (n_sl > 1) mbar_expect_tx(sums_ready, (uint32_t)(senders * mine * I8_BM * 4));
+        if (n_sl > 1) mbar_expect_tx(sums_ready, (uint32_t)(senders * (mine * I8_BM + 4) * 4));  // (and a flag of each warp)
         // the weights do not depend on the kernels in front: their first tiles are on the way before those are through
         const uint64_t once = l2_evict_first_policy();
         for (int it = 0; it < ahead; ++it) {
@@ -311,7 +312,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 int owner = 0, at = 0;  // of column c: block c % slices, its column c / slices
                 for (int c = 0; c < live; c += 16) {
                     // a warp that gave up sends zeros: the bytes that the owners count always arrive, so that none of them leaves with
-                    // sums on their way to it (what they write is wrong then; the error word says so)
+                    // sums on their way to it; its flag, which they count too, tells them to write none of it
                     uint32_t r[16] = {};
                     if (ok) tmem_ld16(acc + c, r);
 #pragma unroll
@@ -321,9 +322,10 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                         if (++owner == n_sl) { owner = 0; ++at; }
                     }
                 }
+                if (lane < n_sl) i8_add_remote(i8_remote((const void*)unformed, lane), i8_remote(sums_ready, lane), !ok);
             }
             if (!mbar_wait(sums_ready, 0, gave_up)) i8_drain(sums_ready);
-            ok = !*gave_up;
+            ok = !*gave_up && !*unformed;
         }
         // a warp takes a token column (gated: each of its halves one) at a time, a lane four features of it
         for (int i = g.gated ? 2 * quarter + half : quarter; ok && i < mine; i += g.gated ? 8 : 4) {
