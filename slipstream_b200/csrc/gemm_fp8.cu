@@ -656,7 +656,9 @@ __device__ __forceinline__ void f8_write_run(const Fp8Args& g, void* to, unsigne
 }
 
 // T: float, bf16, or (gated) uint8_t, e4m3.  SPLIT: a tile is one of `slices` parts of K, and its sums go to g.parts, [slices][tokens][ldc] in
-// float32, where fp8_join_kernel takes them from.
+// float32, where fp8_join_kernel takes them from.  Behind a wait that gave up F8_UNFORMED stands there in their place: a NaN that no
+// arithmetic gives (results that are NaN have the bits 0x7fffffff).
+#define F8_UNFORMED 0x7fc0beefu
 template <int NC, bool GATED, typename T, typename P, bool SPLIT>
 __global__ void __launch_bounds__(F8_MANY_THREADS, 1)
 gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Args g) {
@@ -858,7 +860,13 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     }
                 }
             } else {
-                if (!formed) continue;
+                if (!formed) {
+                    if constexpr (!SPLIT) continue;
+#pragma unroll
+                    for (int i = 0; i < NC; ++i)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) acc[i][e] = __uint_as_float(F8_UNFORMED);
+                }
                 void* to = SPLIT ? (void*)(g.parts + (int64_t)slice_of(t) * g.tokens * g.ldc) : g.out;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) {
@@ -952,30 +960,36 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 }
 
 // The parts of K put together: y = sum over the slices, in their order, + bias, rounded once; a warp takes 128 features of a token, a lane
-// four of them.  Where a wait of the product gave up, not all parts are formed (the error word says so), and nothing is written.
+// four of them.  Where a wait of this product gave up, its parts say which sums are not formed, and nothing is written there.
 __global__ void __launch_bounds__(256) fp8_join_kernel(const Fp8Args g, int64_t ldp, int64_t units) {
     pdl_wait();
     pdl_launch_dependents();
     const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (unit >= units || (*(volatile int*)g.err & SS_ERR_WAIT_LIMIT)) return;
+    if (unit >= units) return;
     const int lane = threadIdx.x & 31, across = (g.features + 127) / 128, token = (int)(unit / across);
     const int apart = (g.ldc & 3) == 0 ? 1 : 32, f = (int)(unit % across) * 128 + (apart == 1 ? lane * 4 : lane);
     if (f >= g.features) return;
     const int64_t plane = g.tokens * ldp;
     const float* p = g.parts + token * ldp + f;
     float v[4] = {};
+    bool formed = true;
+    const auto add = [&](int e, float part) {
+        formed = formed && __float_as_uint(part) != F8_UNFORMED;
+        v[e] += part;
+    };
     if (apart == 1) {  // (rows of the parts are as long as four elements times some number: those behind the last belong to nobody)
 #pragma unroll 4
         for (int s = 0; s < g.slices; ++s) {
             const float4 t = *reinterpret_cast<const float4*>(p + s * plane);
-            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+            add(0, t.x); add(1, t.y); add(2, t.z); add(3, t.w);
         }
     } else {
         for (int s = 0; s < g.slices; ++s)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (f + 32 * e < g.features) v[e] += p[s * plane + 32 * e];
+                if (f + 32 * e < g.features) add(e, p[s * plane + 32 * e]);
     }
+    if (!formed) return;
     if (g.bias) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)

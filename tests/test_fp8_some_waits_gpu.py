@@ -19,8 +19,9 @@ def library():
     return ctypes.CDLL(str(compile_library("slipstream_fp8", FP8_SOURCES, {"SOME_WAITS_GIVE_UP": 1})))
 
 
-def products(library, tokens, k, features, plan, gated, dtype):
-    """(what the build leaves in an output of sevens, its scales, what the ordinary one makes of the same operands, its scales)"""
+def products(library, tokens, k, features, plan, gated, dtype, word=0):
+    """(what the build leaves in an output of sevens, its scales, what the ordinary one makes of the same operands, its scales)
+    ``word``: an error that stands in the error word already; the build is then the ordinary one."""
     from slipstream_b200 import ops
 
     blocks, gen = -(-k // 128), torch.Generator(device=DEV).manual_seed(tokens + k)
@@ -41,7 +42,13 @@ def products(library, tokens, k, features, plan, gated, dtype):
                        ldw=w.values.stride(0), w_scale=w.scales.data_ptr(), w_row=blocks, w_block=1, out=out.data_ptr(), ldc=pitch,
                        out_type={F32: 0, BF16: 1, E4M3: 2}[dtype], out_scale=out_scale.data_ptr(), tokens=tokens, features=features, K=k, gated=int(gated),
                        out_features=columns, many=many, bn=bn, slices=slices, per_sm=per_sm, parts=parts.data_ptr())
-    assert ran(library.ss_gemm_fp8, call) == WAIT_LIMIT
+    if word:
+        err = torch.full((1,), word, dtype=torch.int32, device=DEV)
+        call.err, call.stream = err.data_ptr(), torch.cuda.current_stream().cuda_stream
+        assert library.ss_gemm_fp8(ctypes.byref(call)) == 0
+        assert int(err.item()) == word
+    else:
+        assert ran(library.ss_gemm_fp8, call) == WAIT_LIMIT
     whole = ops.gate_up_swiglu_fp8(x, w, None, dtype, plan=plan) if gated else ops.linear_fp8(x, w, None, dtype, plan=plan)
     ops.check_errors(torch.device(DEV))
     if dtype == E4M3:
@@ -67,3 +74,34 @@ def test_tiles_of_few_tokens(library, tokens, k, tile, gated, dtype):
     assert (out[lost] == 7).all() and torch.equal(out[~lost], whole[~lost])
     if dtype == E4M3:
         assert (scale[:, lost] == 7).all() and torch.equal(scale[:, ~lost], whole_scale[:, ~lost])
+
+
+SLICED = [(256, 18944, 3584, (1, 256, 5, 1)), (100, 300, 1279, (1, 128, 2, 1)), (700, 2000, 5000, (1, 128, 8, 1))]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens, k, features, plan", SLICED)
+def test_a_pair_of_many_tokens_in_slices(library, tokens, k, features, plan, dtype):
+    """A pair of blocks gives up: tiles of which it forms a part are left as they are, the others are right."""
+    out, _, whole, _ = products(library, tokens, k, features, plan, False, dtype)
+    _, tile, slices, _ = plan
+    blocks = -(-k // 128)
+    slices = -(-blocks // -(-blocks // slices))  # (that have any K)
+    down = -(-tokens // 256)
+    tiles = down * -(-features // tile)
+    pairs = min(tiles * slices, torch.cuda.get_device_properties(DEV).multi_processor_count // 2)
+    lost = torch.zeros(tokens, features, dtype=torch.bool, device=DEV)
+    for t in range(1, tiles * slices, pairs):
+        m, f = t % tiles % down * 256, t % tiles // down * tile
+        lost[m: m + 256, f: f + tile] = True
+    assert lost.any() and (out[lost] == 7).all() and torch.equal(out[~lost], whole[~lost])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens, k, features, plan", SLICED)
+def test_an_error_of_another_call(tokens, k, features, plan, dtype):
+    """A wait of another call gave up, and nobody has read the error word yet: this call's result is whole all the same."""
+    from slipstream_b200.ops.functions import fp8_library
+
+    out, _, whole, _ = products(fp8_library(), tokens, k, features, plan, False, dtype, word=WAIT_LIMIT)
+    assert torch.equal(out, whole)
