@@ -203,6 +203,17 @@ struct alignas(16) Shared {  // (every array starts on 16 bytes)
     int n_found, n_chosen;
 };
 
+// How many of 2 * pairs keys (on 16 bytes, in shared memory) are above `own`: two a read, the same ones for all threads of a warp.
+__device__ __forceinline__ int keys_above(const Key* keys, int pairs, Key own) {
+    int n = 0;
+#pragma unroll 8
+    for (int j = 0; j < pairs; ++j) {
+        const ulonglong2 k = reinterpret_cast<const ulonglong2*>(keys)[j];
+        n += (k.x > own) + (k.y > own);
+    }
+    return n;
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(THREADS, 3)
 token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int wide, float* __restrict__ out, int vocabulary, int top, int blocks, int* err) {
@@ -315,17 +326,10 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         if (lane % per_group == 0) sh.groups[tid / per_group] = group;
         if (tid == 0) sh.bound = 0;  // fewer than `top` groups have elements: all of them count
         __syncthreads();
-        // the place of each group's largest element among them, two at a time of what all threads of a warp look at together
+        // the place of each group's largest element among them
         if (tid < groups) {
-            const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(sh.groups);
             const Key own = sh.groups[tid];
-            int place = 0;
-#pragma unroll 8
-            for (int j = 0; j < groups / 2; ++j) {
-                const ulonglong2 k = pairs[j];
-                place += (k.x > own) + (k.y > own);
-            }
-            if (own && place == top - 1) sh.bound = own;
+            if (own && keys_above(sh.groups, groups / 2, own) == top - 1) sh.bound = own;
         }
         __syncthreads();
         const Key limit = sh.bound;
@@ -370,11 +374,11 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
         const int n = sh.n_found;
         if (tid < top) sh.best[tid] = 0;
         if (n <= CANDIDATES) {
+            if (tid == 0 && n % 2) sh.found[n] = 0;  // (CANDIDATES is even: there is room)
             __syncthreads();
             if (tid < n) {
                 const Key own = sh.found[tid];
-                int place = 0;
-                for (int j = 0; j < n; ++j) place += sh.found[j] > own;
+                const int place = keys_above(sh.found, (n + 1) / 2, own);
                 if (place < top) sh.best[place] = own;
             }
         } else {
@@ -458,7 +462,7 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
             if (blocks == 1) {
                 if (tid < top) write(tid, sh.best[tid]);
             } else {
-                // (up to 8 * 64 = 512 keys, in `found`)
+                // (up to 8 * 64 = 512 keys, in `found`; an even number of blocks, so an even number of keys)
                 const int all = blocks * top;
                 Key own = 0;
                 if (tid < all) {
@@ -468,8 +472,9 @@ token_logprobs_kernel(const T* logits, int64_t stride, const void* tokens, int w
                 }
                 __syncthreads();
                 if (tid < all) {
-                    int place = 0;
-                    for (int j = 0; j < all; ++j) place += sh.found[j] > own || (!own && !sh.found[j] && j < tid);
+                    int place = keys_above(sh.found, all / 2, own);
+                    if (!own)  // (no alternative: behind those that are, in some order)
+                        for (int j = 0; j < tid; ++j) place += !sh.found[j];
                     if (place < top) write(place, own);
                 }
             }
