@@ -240,9 +240,9 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t) {
         if (c.many == 1 && c.slices > 1 && c.slices <= 8 && !gated) {
             parts = empty(c.slices * tokens, (features + 3) & -4, at::kFloat, *x.values);
             c.parts = (float*)parts.data_ptr();
-            ++launches;
         }
         check(product_entry(&c), what);
+        if (c.parts) ++launches;  // (the kernel that puts the parts together)
     }
     return to_fp8 ? pair(std::move(rows.values), std::move(rows.scales)) : THPVariable_Wrap(std::move(out));
     CALL_END
