@@ -100,7 +100,6 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t) {
     const bool blocks = args[1] == Py_True;
     if (k < 1) refuse("rows without elements have no scale");
     check_size(n, k);
-    if (blocks && blocks_of(k) > 65535) refuse("weights are rounded up to " + std::to_string(65535 * BLOCK) + " elements wide, not " + std::to_string(k));
     if (k > 1 && x.stride(1) != 1) refuse("the rows of x must be contiguous, got strides " + say(x.strides()));
     OnDevice here(x);
     New r = empty_fp8(n, k, blocks, x);
