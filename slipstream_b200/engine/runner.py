@@ -29,8 +29,15 @@ from slipstream_b200.weights.random_init import random_weights_on_device
 
 from .context import StepContext, StepEntry, StepInputError, plan_step, to_device
 from .graphs import BUCKETS, DecodeGraph, MixedGraph, bucket_for, mixed_bucket
+from .scheduler import MAX_SCORED_TOKENS
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+
+
+def page_bytes(free: int, utilization: float, logits: int) -> int:
+    """Bytes for pages, of ``free``: nine tenths of what ``utilization`` grants, and at least a tenth beside what
+    the logits of scored prompts take (``logits``) is left for activations."""
+    return max(0, min(int(free * utilization * 0.9), int(free * 0.9) - logits))
 
 
 class ModelRunner:
@@ -72,6 +79,8 @@ class ModelRunner:
         layouts = self.model.group_layouts
         page_sizes = [layout.spec.page_size or page_size for layout in layouts]
         step_tokens = max_step_tokens or self.max_model_len
+        # logits that captured steps with logits per token keep, all together: a step for which there is no room runs kernel by kernel
+        self.max_graph_logits_bytes = torch.cuda.get_device_properties(self.device).total_memory // 32
         if isinstance(num_pages, (list, tuple)):
             pools = [int(n) for n in num_pages]
         else:
@@ -80,8 +89,8 @@ class ModelRunner:
                 torch.cuda.empty_cache()
                 free, _total = torch.cuda.mem_get_info(self.device)
                 per_token = [PagedStore.bytes_per_token(layout, self.runtime.dtype) for layout in layouts]
-                # leave room for activations of the largest step beside the pages
-                tokens = tokens_that_fit(layouts, page_sizes, per_token, int(free * gpu_memory_utilization * 0.9),
+                # leave room for activations of the largest step beside the pages, and for the logits of scored prompts
+                tokens = tokens_that_fit(layouts, page_sizes, per_token, page_bytes(free, gpu_memory_utilization, self.scored_bytes(max_num_seqs, step_tokens)),
                                          max_num_seqs, self.max_model_len, step_tokens)
             else:
                 tokens = int(num_pages) * page_size
@@ -110,6 +119,12 @@ class ModelRunner:
         self._mixed_graphs: dict[tuple, "MixedGraph | int"] = {}
         self.mixed_graph_after = 6  # steps of a bucket that run kernel by kernel before it is captured
         self.max_mixed_graphs = 24
+
+    def scored_bytes(self, max_num_seqs: int, step_tokens: int) -> int:
+        """Bytes of float32 logits, at most, of a step that scores prompts (a row for each scored token, and one a request twice:
+        those that are sampled from are put together) and of the captured steps that do."""
+        rows = min(MAX_SCORED_TOKENS, step_tokens) + 2 * max_num_seqs
+        return rows * self.config.vocab_size * 4 + self.max_graph_logits_bytes
 
     # ------------------------------------------------------------------ requests
     def admit(self, request_id: object) -> None:
@@ -183,7 +198,11 @@ class ModelRunner:
         if seen < self.mixed_graph_after:
             self._mixed_graphs[key] = seen + 1
             return None
-        if sum(isinstance(g, MixedGraph) for g in self._mixed_graphs.values()) >= self.max_mixed_graphs:
+        captured = [g for g in self._mixed_graphs.values() if isinstance(g, MixedGraph)]
+        if len(captured) >= self.max_mixed_graphs:
+            return None
+        if per_token and (sizes[0] * self.config.vocab_size * 4
+                          + sum(g.logits.numel() * 4 for g in captured if g.n_logits > g.n_requests)) > self.max_graph_logits_bytes:
             return None
         graph = self._mixed_graphs[key] = MixedGraph(self, sizes[0], sizes[1], sizes[0] if per_token else sizes[1], variants)
         return graph

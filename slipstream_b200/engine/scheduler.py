@@ -24,6 +24,9 @@ When pages run out:
     the FRONT of the waiting queue and later replays prompt + outputs
     (:169-177, :253-268); if there is nobody else to preempt, the request skips
     this step and keeps what it has (:255-257).
+
+A step scores at most ``MAX_SCORED_TOKENS`` prompt tokens (``SamplingParams.prompt_logprobs``), since
+each of them takes a row of logits: portions are cut there, and a prompt that is to be scored waits for a later step.
 """
 
 from __future__ import annotations
@@ -35,6 +38,9 @@ from dataclasses import dataclass, field
 from slipstream_b200.cache import AllocStatus, CacheManager
 from slipstream_b200.config.engine_config import SchedulerConfig
 from slipstream_b200.config.sampling_params import SamplingParams
+
+
+MAX_SCORED_TOKENS = 1024  # of a step: 0.6 GB of logits at a vocabulary of 151,936, and enough rows to fill the products of a step
 
 
 class SequenceStatus(enum.IntEnum):
@@ -97,8 +103,17 @@ class Sequence:
         known from before a preemption)."""
         if self.sampling_params.prompt_logprobs is None:
             return []
-        first = max(self.num_computed_tokens, len(self.prompt_logprobs) - 1)
-        return [p - self.num_computed_tokens for p in range(first, min(self.num_computed_tokens + take, self.num_prompt_tokens - 1))]
+        return [p - self.num_computed_tokens for p in range(self._first_to_score, min(self.num_computed_tokens + take, self.num_prompt_tokens - 1))]
+
+    @property
+    def _first_to_score(self) -> int:
+        return max(self.num_computed_tokens, len(self.prompt_logprobs) - 1)
+
+    def take_scoring(self, take: int, limit: int) -> int:
+        """The part of the next ``take`` tokens that scores at most ``limit`` of the prompt's."""
+        if self.sampling_params.prompt_logprobs is None or self._first_to_score + limit >= self.num_prompt_tokens - 1:
+            return take
+        return min(take, self._first_to_score + limit - self.num_computed_tokens)
 
     def tokens_to_feed(self, take: int) -> list[int]:
         start = self.num_computed_tokens
@@ -167,6 +182,7 @@ class Scheduler:
         aborted: list[Sequence] = []
         protected: set[int] = set()
         tokens = 0
+        to_score = MAX_SCORED_TOKENS
 
         def try_take(seq: Sequence, take: int) -> bool:
             """Reserve pages for ``take`` more tokens of a running sequence, preempting if needed."""
@@ -195,10 +211,11 @@ class Scheduler:
         for seq in list(self.running):
             if seq not in self.running or seq.is_decoding or seq.seq_id in protected:
                 continue
-            take = min(seq.num_uncomputed_tokens, budget - tokens, chunk)
+            take = seq.take_scoring(min(seq.num_uncomputed_tokens, budget - tokens, chunk), to_score)
             if take <= 0:
                 continue
-            try_take(seq, take)
+            if try_take(seq, take):
+                to_score -= len(seq.places_to_score(take))
 
         # 3. admit waiting sequences, first come first served
         for seq in sorted(self.waiting, key=lambda s: (s.arrival_ts, s.seq_id)):
@@ -206,7 +223,9 @@ class Scheduler:
                 break
             if seq in preempted:
                 continue  # it lost its pages in this very step
-            take = min(seq.num_uncomputed_tokens, budget - tokens, chunk)
+            take = seq.take_scoring(min(seq.num_uncomputed_tokens, budget - tokens, chunk), to_score)
+            if take <= 0:
+                continue  # its turn to score comes in a later step: rows of logits, unlike pages, come anew with every step
             total = seq.num_prompt_tokens + seq.max_new_tokens
             status = self.cache.can_admit(total, take, chunk)
             if status is AllocStatus.NEVER:
@@ -224,6 +243,7 @@ class Scheduler:
             scheduled.append(ScheduledSeq(seq, take))
             protected.add(seq.seq_id)
             tokens += take
+            to_score -= len(seq.places_to_score(take))
 
         assert tokens <= budget, "token budget exceeded"
         return SchedulerOutput(scheduled, tokens, preempted, aborted)
