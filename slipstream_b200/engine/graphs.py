@@ -363,7 +363,8 @@ class MixedGraph:
             tiles[i, 0, : req.size] = req
             tiles[i, 1, : req.size] = first
 
-    def run(self, plan: HostPlan) -> torch.Tensor:
+    def run(self, plan: HostPlan, keep: bool = True) -> torch.Tensor:
+        """``keep`` False returns a view of the static logits buffer, valid until the next replay."""
         i = self.turn
         self.turn ^= 1
         if self.used[i]:
@@ -374,7 +375,8 @@ class MixedGraph:
         self.used[i] = True
         self.graph.replay()
         ops.count_launches(self.kernels)
-        return self.logits[: plan.logit_rows.size].clone()
+        logits = self.logits[: plan.logit_rows.size]
+        return logits.clone() if keep else logits
 
     @property
     def h2d_bytes(self) -> int:

@@ -466,7 +466,7 @@ class LLMEngine:
                 sampling.append(item)
             entries.append(StepEntry(seq.seq_id, seq.tokens_to_feed(item.take), want))
         decode_tokens = plan.num_decode_tokens
-        logits = self.runner.step(entries)
+        logits = self.runner.step(entries, keep=False)  # (read by kernels of this step alone)
         tokens: list[int] = []
         told: list[TokenLogprob | None] = [None] * len(sampling)
         if scored:

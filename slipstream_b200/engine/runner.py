@@ -143,7 +143,8 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ the step function
     @torch.inference_mode()
-    def step(self, entries: list[StepEntry]) -> torch.Tensor:
+    def step(self, entries: list[StepEntry], keep: bool = True) -> torch.Tensor:
+        """Run the entries' tokens; float32 logits of the wanted rows.  ``keep`` False: they may be a view that is valid until the next step."""
         for e in entries:
             if e.request_id not in self.cache:
                 self.admit(e.request_id)
@@ -154,10 +155,10 @@ class ModelRunner:
         if bucket is not None:
             graph = self._decode_graph(bucket, plan)
             self.last_h2d_bytes = graph.h2d_bytes
-            logits = graph.run(plan)
+            logits = graph.run(plan, keep=keep)
         elif mixed is not None:
             self.last_h2d_bytes = mixed.h2d_bytes
-            logits = mixed.run(plan)
+            logits = mixed.run(plan, keep=keep)
         else:
             ctx = to_device(plan, self.device)
             self.last_h2d_bytes = ctx.extras["host_buffer"].numel() * 4

@@ -64,3 +64,29 @@ def test_logits_of_captured_steps_are_bounded(folder):
             assert a.output_token_ids == b.output_token_ids
             # (a step padded to its bucket may sum in another order: bfloat16 logits of this model are off by less than 0.1)
             assert all(abs(x.logprob - y.logprob) < 0.2 for x, y in zip(a.prompt_logprobs[1:], b.prompt_logprobs[1:]))
+
+
+def test_replayed_steps_are_scored_where_their_logits_lie(folder):
+    """A replayed step hands the engine a view of its logits; who calls the runner gets a copy unless it says otherwise."""
+    from slipstream_b200 import LLM
+    from slipstream_b200.engine.context import StepEntry
+    from slipstream_b200.engine.graphs import MixedGraph
+
+    llm = LLM(folder, dtype="bfloat16", num_gpu_blocks=1024, max_num_seqs=32, prefill_chunk_size=64)
+    runner = llm.engine.runner
+    runner.mixed_graph_after = 0
+    step, seen = runner.step, []
+    runner.step = lambda entries, **more: seen.append(step(entries, **more)) or seen[-1]
+    first = scored(llm)
+    own = {g.logits.data_ptr() for g in runner._mixed_graphs.values() if isinstance(g, MixedGraph)}
+    assert own & {t.data_ptr() for t in seen}
+    runner.step = step
+    results = {}
+    for keep in (True, False):
+        entries = [StepEntry(f"r{keep}", prompts()[0][:64], list(range(64)))]
+        results[keep] = runner.step(entries, keep=keep)
+        runner.release(f"r{keep}")
+    graphs = [g for g in runner._mixed_graphs.values() if isinstance(g, MixedGraph)]
+    assert results[True].data_ptr() not in {g.logits.data_ptr() for g in graphs}
+    assert results[False].data_ptr() in {g.logits.data_ptr() for g in graphs} and torch.equal(results[True], results[False])
+    assert all(a.output_token_ids == b.output_token_ids for a, b in zip(first, scored(llm)))
