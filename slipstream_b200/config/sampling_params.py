@@ -9,9 +9,13 @@ probabilities of the output's and of the prompt's tokens, and for that many of t
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-
+from numbers import Integral
 
 MAX_TOP_LOGPROBS = 64  # ops/logprobs.py
+
+
+def _alternatives(n: object) -> bool:
+    return n is None or isinstance(n, Integral) and not isinstance(n, bool) and 0 <= n <= MAX_TOP_LOGPROBS
 
 
 @dataclass(frozen=True)
@@ -40,9 +44,8 @@ class SamplingParams:
             ("top_p", 0.0 < self.top_p <= 1.0, "above 0 and at most 1"),
             ("min_p", 0.0 <= self.min_p <= 1.0, "between 0 and 1"),
             ("repetition_penalty", self.repetition_penalty > 0.0, "positive"),
-            ("logprobs", self.logprobs is None or 0 <= self.logprobs <= MAX_TOP_LOGPROBS, f"None or between 0 and {MAX_TOP_LOGPROBS}"),
-            ("prompt_logprobs", self.prompt_logprobs is None or 0 <= self.prompt_logprobs <= MAX_TOP_LOGPROBS,
-             f"None or between 0 and {MAX_TOP_LOGPROBS}"),
+            ("logprobs", _alternatives(self.logprobs), f"None or a whole number between 0 and {MAX_TOP_LOGPROBS}"),
+            ("prompt_logprobs", _alternatives(self.prompt_logprobs), f"None or a whole number between 0 and {MAX_TOP_LOGPROBS}"),
             ("n", self.n == 1, "1: several samples of one prompt are not implemented"),
         )
         for name, ok, wanted in rules:

@@ -89,3 +89,15 @@ def test_bytes_for_pages():
     assert page_bytes(170 * gb, 1.0, 7 * gb) == int(170 * gb * 0.9) - 7 * gb
     assert page_bytes(20 * gb, 0.9, 2 * gb) == 16 * gb
     assert page_bytes(gb, 0.9, 2 * gb) == 0
+
+
+@pytest.mark.parametrize("name", ["logprobs", "prompt_logprobs"])
+def test_alternatives_are_whole_numbers(name):
+    """A number that is none would otherwise be found out in the middle of a step, beside other requests."""
+    import numpy as np
+
+    for bad in (1.5, 2.0, True, "3", float("nan"), -1, 65):
+        with pytest.raises(ValueError, match=name):
+            SamplingParams(**{name: bad})
+    for good in (None, 0, 64, np.int64(5)):
+        assert getattr(SamplingParams(**{name: good}), name) == good
