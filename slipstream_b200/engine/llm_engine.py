@@ -138,6 +138,10 @@ class LLMEngine:
         # the host comes to know them (slipstream/engine/llm_engine.py:89-90,577-598)
         self.last_ttft_s: list[float] = []
         self.last_itl_s: list[float] = []
+        # what the requests of the last generate, generate_batch or stream asked to be told of their tokens, one list a request (None
+        # where nothing was asked for); a stream's lists grow with it
+        self.last_logprobs: list[list[TokenLogprob] | None] = []
+        self.last_prompt_logprobs: list[list[TokenLogprob | None] | None] = []
         self._started_at: dict[int, float] = {}
         self._last_emit: dict[int, float] = {}
         self._requests_seen = 0
@@ -152,12 +156,13 @@ class LLMEngine:
 
     # ------------------------------------------------------------------ public calls
     def generate(self, request: Request) -> list[int]:
-        """Blocking generation of one request; returns the output token ids only."""
+        """Blocking generation of one request; returns the output token ids only (``last_logprobs``: what else was asked for)."""
         return self.generate_batch([request])[0]
 
     def stream(self, request: Request) -> Iterator[int]:
         """Token iterator with the same tokens as ``generate``."""
         seq = self._make_sequence(request)
+        self._tell_of([seq])
         self._started_at[seq.seq_id] = time.perf_counter()
         self.scheduler.add_seq(seq)
         emitted = 0
@@ -194,6 +199,7 @@ class LLMEngine:
         if inject not in ("all", "arrival"):
             raise ValueError("inject must be 'all' or 'arrival'")
         seqs = [self._make_sequence(r) for r in requests]
+        self._tell_of(seqs)
         wall, perf = time.time(), time.perf_counter()
         self.last_ttft_s.clear()
         self.last_itl_s.clear()
@@ -251,6 +257,10 @@ class LLMEngine:
         return list(self.tokenizer.encode(request.prompt, add_special_tokens=False).ids)
 
     # ------------------------------------------------------------------ internals
+    def _tell_of(self, seqs: list[Sequence]) -> None:
+        self.last_logprobs = [None if s.sampling_params.logprobs is None else s.logprobs for s in seqs]
+        self.last_prompt_logprobs = [None if s.sampling_params.prompt_logprobs is None else s.prompt_logprobs for s in seqs]
+
     def _make_sequence(self, request: Request) -> Sequence:
         ids = self.tokenize(request)
         if not ids:
@@ -476,7 +486,7 @@ class LLMEngine:
         if sampling:
             rows = [SampleRow(i.seq.sampling_params, i.seq.seed, i.seq.num_output_tokens,
                               self.runner.cache.get(i.seq.seq_id).slot) for i in sampling]
-            # the step's one device-to-host copy: the tokens and, behind them, the device error word
+            # the tokens and, behind them, the device error word in one device-to-host copy; log probabilities, where asked for, in another
             tokens_dev = self.sampler.sample(logits, rows, with_status=True)
             packed = self._logprobs(logits, tokens_dev[: len(rows)], [i.seq for i in sampling])
             tokens = tokens_dev.tolist()
