@@ -532,12 +532,14 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 //   full[s]       in the leader: the bytes of both blocks' copies;      empty[s]      in each block: the products have read the stage
 //   part_full[b]  in each block: the sums of a block of K are formed;   part_empty[b] in the leader: all 16 epilogue warps have them
 //
-// Bound by taking the sums out: 256 x 256 outputs x 128 of K take about 0.53 us, the products alone 0.39 (both at 1.9 GHz; the copies
-// keep up).  4,099 x 3,584 x 37,888 gated: 554 to 572 us in a burst, 620 under the power cap, for 330 us at twice the bfloat16 rate;
-// 2,047 x 3,581 x 4,613 to float32 61.  The tensor pipe is busy for 46 % of 2,048 tokens.
+// 256 x 256 outputs x 128 of K take about 0.53 us, the products alone 0.39 (both at 1.9 GHz; the copies keep up), the tensor pipe 0.27.
+// Two slots of 256 columns fill the tensor memory, so a period is half of a slot's way round: products, a look at the barrier, the sums
+// taken out, their release, another look.  Neither the tensor pipe nor the issue slots (43 % busy) are at a limit; what each part of that
+// way takes has not been measured apart.  4,099 x 3,584 x 37,888 gated: 554 to 572 us in a burst, 620 under the power cap, for 330 us at twice the bfloat16 rate;
+// 2,047 x 3,581 x 4,613 to float32 60.  The tensor pipe is busy for 46 % of 2,048 tokens.
 //
 // Few tiles of a long K (256 x 18,944 x 3,584 has 14 of 256 features, and 74 pairs) are cut into slices of K, each a tile of its own whose sums go
-// to memory in float32 (they stay in L2), and a second kernel adds them up in order: 54 us in one slice, 33 in five.
+// to memory in float32 (they stay in L2), and a second kernel adds them up in order: 54 us in one slice, 31 in five.
 //
 // Registers: three warps a scheduler are launched with 168 each; the first four warps (producer, issuer, two that do nothing) hand back
 // all but 40 of theirs, and the epilogue's have 232: 128 sums and 64 columns on their way.
@@ -1120,7 +1122,7 @@ static int launch_few(const Fp8Call& c, Fp8Args& g, int per_sm) {
 
 // Row strides are multiples of 16 bytes and bases stand on 16 bytes.
 // gated: w's rows alternate 128 gate and 128 up features; out_features <= features / 2 columns of silu(gate) * up are written.
-// many = 0: bn tokens a tile (a multiple of 16 up to 256, gated 128), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for
+// many = 0: bn tokens a tile (a multiple of 16 up to 256, gated 128; ops/fp8.py's own plans go up to 128, gated 64), slices 1..8 of K, `per_sm` blocks an SM that the ring is sized for
 // (2: bn up to 64, gated 32).
 // many = 1: bn features a tile (64, 128 or 256; gated: 256); not gated, of 128 or 256 features: slices 1..8 of K, with `parts` from 2 on.
 extern "C" int ss_gemm_fp8(const Fp8Call* call) {

@@ -140,9 +140,9 @@ def fp8_plan(tokens: int, features: int, k: int, sms: int, gated: bool = False,
     ``resident``: clusters of 1 to 8 blocks that run at the same time, with the ring sized for one block an SM and for two.
 
     The choice is the cheapest by an estimate in microseconds whose constants are fitted to 2,772 measured products (1 to 512 tokens, the
-    projections of the 0.5B, 1.5B and 7B layer sizes, tiles, slices and rings of all sizes): on average 3 % slower than the fastest of
-    them at the same sizes, and at worst 14 %; those of the second kernel with K in slices to 564 more (256 x 18,944 x 3,584: 54 us in
-    one slice, 33 in five)."""
+    projections of the 0.5B, 1.5B and 7B layer sizes, tiles, slices and rings of all sizes): on average 2 % slower than the fastest of
+    them at the same sizes, and at worst 16 % (48 tokens of 1,536 x 8,960 gated); those of the second kernel with K in slices to 564 more (256 x 18,944 x 3,584: 54 us in
+    one slice, 31 in five)."""
     # what follows depends on the tokens in steps of 16 (their tiles) up to 640 and of 256 beyond: few plans for many counts
     step = 16 if tokens <= 640 else 256
     return _plan((tokens + step - 1) // step * step, features, k, sms, gated, resident)
