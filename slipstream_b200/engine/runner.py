@@ -35,9 +35,9 @@ _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
 def page_bytes(free: int, utilization: float, logits: int) -> int:
-    """Bytes for pages, of ``free``: nine tenths of what ``utilization`` grants, and at least a tenth beside what
-    the logits of scored prompts take (``logits``) is left for activations."""
-    return max(0, min(int(free * utilization * 0.9), int(free * 0.9) - logits))
+    """Bytes for pages, of ``free``: nine tenths of what ``utilization`` grants, so that a tenth is left for activations, and beside
+    it what the logits of scored prompts take (``logits``; a quarter of ``free`` at most, for a device that is nearly full)."""
+    return min(int(free * utilization * 0.9), int(free * 0.9) - min(logits, free // 4))
 
 
 class ModelRunner:
@@ -80,7 +80,7 @@ class ModelRunner:
         page_sizes = [layout.spec.page_size or page_size for layout in layouts]
         step_tokens = max_step_tokens or self.max_model_len
         # logits that captured steps with logits per token keep, all together: a step for which there is no room runs kernel by kernel
-        self.max_graph_logits_bytes = torch.cuda.get_device_properties(self.device).total_memory // 32
+        self.max_graph_logits_bytes = torch.cuda.mem_get_info(self.device)[0] // 32
         if isinstance(num_pages, (list, tuple)):
             pools = [int(n) for n in num_pages]
         else:

@@ -88,7 +88,7 @@ def test_bytes_for_pages():
     assert page_bytes(170 * gb, 0.9, 7 * gb) == int(170 * gb * 0.9 * 0.9)
     assert page_bytes(170 * gb, 1.0, 7 * gb) == int(170 * gb * 0.9) - 7 * gb
     assert page_bytes(20 * gb, 0.9, 2 * gb) == 16 * gb
-    assert page_bytes(gb, 0.9, 2 * gb) == 0
+    assert page_bytes(gb, 0.9, 2 * gb) == int(0.9 * gb) - gb // 4
 
 
 @pytest.mark.parametrize("name", ["logprobs", "prompt_logprobs"])
